@@ -453,6 +453,77 @@ int nl_embedding_bwd(void* stream, int batch, int seq, int D, int vocab, const i
                      const nl_bf16* dx, float* dtok, float* dpos, int accumulate_pos, void* ws,
                      size_t ws_bytes);
 
+/* ======================================================================== */
+/* 8-bit floating point with a scale for each block of 128                    */
+/* ======================================================================== */
+/*
+ * An operand of rows x K values: q, e4m3 bytes (OCP: 448 is the largest, 0x7f and 0xff NaN)
+ * with the K axis contiguous in whole blocks of 128 (row stride ldq >= K rounded
+ * up to 128; the bytes past K of the last block are zero), and scale, one e8m0
+ * byte s for each block of 128 along K and each `group` rows (group 1 or 128;
+ * row r's scales are row r / group, lds bytes apart):
+ *     value[r][k] = q[r][k] * 2^(scale[r / group][k / 128] - 127).
+ * q needs 16-byte aligned rows; scale rows that are a multiple of 4 bytes and
+ * start on 4 bytes are read four blocks at a time.
+ */
+
+/* Quantises x[rows][cols] (fp32 or bf16, row stride ldx, any alignment of its
+ * type; 16-byte aligned rows are read 8 elements at a time). A block's scale is
+ * 2^e with e the least integer such that its largest finite |x| <= 448 * 2^e
+ * (not below 2^-127; 1 for a block without a finite value other than zero), and
+ * q = x / 2^e to nearest even; a value that is not finite becomes NaN.
+ *   q, scale:    x itself, blocks along the columns (q NULL: not wanted);
+ *   qt, scale_t: the transpose, cols x rows, blocks along the rows (qt NULL: not
+ *                wanted). With group 128 both have the same 128 x 128 blocks.
+ * Padding bytes of q and qt inside their last blocks are written as zero;
+ * padding of the scale rows is not written. One launch, one read of x. */
+int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t ldx,
+                    int group, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                    uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst);
+
+/* C[M][N] = A . B^T for A of M x K and B of N x K values as above, summed in
+ * fp32, written as fp32 or bf16 (to nearest even). C: 16-byte aligned, ldc a
+ * multiple of 8. K == 0 writes zeros. Rows of A and B are below 8 MiB. A small C
+ * with a long K is split over K into fp32 partials in the caller's workspace
+ * (nl_gemm_fp8_ws_bytes(); 0: none), summed in a fixed order; a NULL or smaller
+ * workspace just disables the split. */
+size_t nl_gemm_fp8_ws_bytes(int M, int N, int K);
+int nl_gemm_fp8(void* stream, int M, int N, int K,
+                const uint8_t* A, int64_t lda, const uint8_t* scale_a, int64_t ldsa, int group_a,
+                const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b,
+                void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes);
+
+/* ======================================================================== */
+/* Distillation from a teacher's top logits                                   */
+/* ======================================================================== */
+/*
+ * For each row of logits[M][V] (bf16, row stride ld): its k largest values,
+ * largest first, equal ones by the lower id, and lse = log sum_v exp(logit_v / T).
+ *   values[M][k] bf16 (the logits as stored), ids[M][k], lse[M].
+ * NaN counts as larger than any number and -0 as equal to 0; a row with a NaN
+ * has lse NaN. 1 <= k <= min(V, NL_TOP_MAX_K), T > 0 and finite. */
+#define NL_TOP_MAX_K 256
+int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k, float temperature,
+                  nl_bf16* values, int32_t* ids, float* lse);
+
+/* The distillation loss of a student's logits z[M][V] against k entries a row
+ * of a teacher's: ids[M][k] (int32, or int64 with ids_64), values[M][k] (the
+ * teacher's logits, bf16 or fp32), lse[M] the teacher's logsumexp at T, or NULL.
+ *     p_j = exp(values_j / T - lse)        with lse NULL: softmax of the row's k values / T
+ *     log q_v = z_v / T - log sum_u exp(z_u / T)
+ *     loss[m] = T^2 sum_j p_j (log p_j - log q_{id_j})
+ *     dlogits[m][v] = scale * T * (S q_v - sum_{j: id_j = v} p_j),   S = sum_j p_j
+ * so that dlogits is the gradient of scale * sum_m loss[m]. An entry with a
+ * negative id is padding and left out; entries may name an id more than once
+ * (their p add up). A row whose p are all zero, padding alone for instance, has
+ * loss 0 and a zero gradient whatever its logits are. An id >= V, or a NaN in a
+ * row that has entries, makes that row's loss and gradient NaN.
+ * dlogits NULL: the loss alone. dlogits may alias logits (the same address and
+ * stride), which it then overwrites. 1 <= k <= NL_TOP_MAX_K. */
+int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k, const void* ids,
+                       int ids_64, const void* values, int values_dtype, const float* lse, float temperature,
+                       float* loss, float scale, nl_bf16* dlogits, int64_t ld_dlogits);
+
 #ifdef __cplusplus
 }
 #endif

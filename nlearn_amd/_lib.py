@@ -90,6 +90,11 @@ _SIGNATURES = {
     "nl_embedding_fwd": [_P, _I, _I, _I, _I, _P, _P, _P, _P],
     "nl_embedding_bwd_ws_bytes": [_I, _I, _I, _I],
     "nl_embedding_bwd": [_P, _I, _I, _I, _I, _P, _P, _P, _P, _I, _P, ctypes.c_size_t],
+    "nl_quantize_fp8": [_P, _I64, _I64, _P, _I, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64],
+    "nl_gemm_fp8_ws_bytes": [_I, _I, _I],
+    "nl_gemm_fp8": [_P, _I, _I, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I, _I64, _P, ctypes.c_size_t],
+    "nl_top_logits": [_P, _I, _I, _P, _I64, _I, _F, _P, _P, _P],
+    "nl_distill_fwd_bwd": [_P, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _F, _P, _F, _P, _I64],
 }
 _RESTYPES = {
     "nl_strerror": ctypes.c_char_p,
@@ -103,6 +108,7 @@ _RESTYPES = {
     "nl_lce_ws_bytes": ctypes.c_size_t,
     "nl_global_norm_ws_bytes": ctypes.c_size_t,
     "nl_embedding_bwd_ws_bytes": ctypes.c_size_t,
+    "nl_gemm_fp8_ws_bytes": ctypes.c_size_t,
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -169,6 +175,18 @@ def stream_of(t) -> int:
     if index < 0:
         return torch.cuda.current_stream(t.device).cuda_stream
     return torch._C._cuda_getCurrentRawStream(index)
+
+
+def call_on(t, name: str, *args) -> None:
+    """``call(name, stream, *args)`` on the current stream of the tensor ``t``'s
+    device, with that device current for the launch."""
+    import torch
+
+    index = t.get_device()
+    if index < 0 or index == torch._C._cuda_getDevice():
+        return call(name, stream_of(t), *args)
+    with torch.cuda.device(index):
+        return call(name, stream_of(t), *args)
 
 
 def ws_bytes(batch: int, heads: int, seq: int) -> int:

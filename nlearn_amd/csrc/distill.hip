@@ -1,0 +1,530 @@
+// distill.hip — distillation from a teacher's top logits, for gfx950.
+//
+//   top:   the k largest of x[m, :], ties to the lowest index, and
+//          lse[m] = log sum_v exp(x[m, v] / T)
+//   loss:  p_j = exp(v_j / T - lse_t)  (or the softmax of the row's v_j / T)
+//          loss[m] = T^2 sum_j p_j (log p_j - log q[id_j]),  q = softmax(z[m] / T)
+//          dz[m, v] = scale T (S q_v - sum_{j: id_j = v} p_j),  S = sum_j p_j
+//
+// Both are bound by HBM: a row of logits is read once into registers by one
+// workgroup (as the cross-entropy does), and every pass over it runs from there.
+// Rows that no workgroup's registers hold are read twice.
+#include "common.h"
+
+namespace nl {
+namespace {
+
+constexpr int kMaxK = NL_TOP_MAX_K;
+
+// 2^x for x of any size with the error of a small argument: the integer part goes
+// into the exponent exactly. 0 at -inf, NaN at NaN.
+__device__ __forceinline__ float exp2_split(double x) {
+  if (x < -300.0) return 0.f;
+  if (x > 300.0) return INFINITY;
+  const double n = rint(x);
+  return ldexpf(fast_exp2((float)(x - n)), (int)n);
+}
+
+// A row of V bf16 values held by a workgroup of NT threads: 8-element vectors in
+// NVEC registers sets per thread (0: left in memory and read again), and at most
+// one loose element (before the first or behind the last 16-byte boundary).
+template <int NT, int NVEC>
+struct Row {
+  const uint16_t* p;
+  const u32x4* body;
+  int V, head, nbody, eidx;
+  u32x4 v[NVEC ? NVEC : 1];
+  float xe;  // the loose element
+
+  __device__ __forceinline__ void load(const uint16_t* row, int n, int tid) {
+    p = row;
+    V = n;
+    const int mis = (int)(((uintptr_t)row & 15) >> 1);
+    head = min(mis ? 8 - mis : 0, V);
+    nbody = (V - head) >> 3;
+    const int tail = (V - head) & 7;
+    body = reinterpret_cast<const u32x4*>(row + head);
+#pragma unroll
+    for (int j = 0; j < NVEC; ++j)
+      if (j * NT + tid < nbody) v[j] = __builtin_nontemporal_load(body + j * NT + tid);
+    eidx = -1;
+    if (tid < head) eidx = tid;
+    else if (tid >= 8 && tid < 8 + tail) eidx = head + nbody * 8 + (tid - 8);
+    xe = eidx >= 0 ? bf16_to_f32(row[eidx]) : 0.f;
+  }
+  // keeps the row packed between passes (unpacked floats would take twice the registers)
+  __device__ __forceinline__ void fence() {
+#pragma unroll
+    for (int j = 0; j < NVEC; ++j) asm volatile("" : "+v"(v[j]));
+  }
+  // f(vector, index of its first element / 8 in the body) for this thread's vectors
+  template <class F>
+  __device__ __forceinline__ void vectors(int tid, F f) {
+    if constexpr (NVEC > 0) {
+#pragma unroll
+      for (int j = 0; j < NVEC; ++j)
+        if (j * NT + tid < nbody) f(v[j], j * NT + tid);
+    } else {
+      for (int i = tid; i < nbody; i += NT) f(body[i], i);
+    }
+  }
+};
+
+template <int NT>
+struct RowSums {
+  float m[NT / kWave], s[NT / kWave];
+};
+
+// (X, S) over the workgroup's row: X = max x and S = sum 2^((x - X) c); xmax is the
+// thread's own max. A NaN makes S NaN; an infinity without one makes both infinite.
+__device__ __forceinline__ float finite_or_0(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
+__device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, float c) {
+  const float mn = fmaxf(m, m2);
+  const float at = finite_or_0(mn);
+  s = s * fast_exp2((m - at) * c) + s2 * fast_exp2((m2 - at) * c);
+  m = mn;
+}
+
+// x c itself would overflow: masks of the type's lowest value stand alone in a row
+__device__ __forceinline__ bool too_large(float m, float c) { return fabsf(m) * c > 1e37f; }
+
+template <int NT, int NVEC>
+__device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, RowSums<NT>& sm, float& X, float& S,
+                                         float& xmax) {
+  float m = r.eidx >= 0 ? r.xe : -INFINITY;
+  float s;
+  if constexpr (NVEC > 0) {
+    r.vectors(tid, [&](const u32x4& v, int) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m = fmaxf(m, fmaxf(bf16_lo(v[q]), bf16_hi(v[q])));
+    });
+    r.fence();
+    auto sum = [&](auto f) __attribute__((always_inline)) {
+      s = r.eidx >= 0 ? fast_exp2(f(r.xe)) : 0.f;
+      r.vectors(tid, [&](const u32x4& v, int) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          s += fast_exp2(f(bf16_lo(v[q])));
+          s += fast_exp2(f(bf16_hi(v[q])));
+        }
+      });
+    };
+    const float at = finite_or_0(m);
+    if (!too_large(at, c)) {
+      // one fma an element against the rounded at * c, whose rounding comes off the sum
+      const float off = at * c;
+      sum([&](float x) { return __builtin_fmaf(x, c, -off); });
+      s *= fast_exp2(__builtin_fmaf(-at, c, off));
+    } else {
+      sum([&](float x) { return (x - at) * c; });
+    }
+    r.fence();
+  } else {
+    // one read: the running maximum moves once per vector at most
+    float at = finite_or_0(m);
+    s = r.eidx >= 0 ? fast_exp2((r.xe - at) * c) : 0.f;
+    r.vectors(tid, [&](const u32x4& v, int) {
+      float mv = -INFINITY;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) mv = fmaxf(mv, fmaxf(bf16_lo(v[q]), bf16_hi(v[q])));
+      if (mv > m) {
+        const float to = finite_or_0(mv);
+        s *= s == 0.f ? 1.f : fast_exp2((at - to) * c);  // (a sum of 0 has no reference yet)
+        m = mv;
+        at = to;
+      }
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        s += fast_exp2((bf16_lo(v[q]) - at) * c);
+        s += fast_exp2((bf16_hi(v[q]) - at) * c);
+      }
+    });
+  }
+  xmax = m;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const float m2 = __shfl_xor(m, o, kWave);
+    const float s2 = __shfl_xor(s, o, kWave);
+    combine(m, s, m2, s2, c);
+  }
+  if constexpr (NT > kWave) {
+    if ((tid & (kWave - 1)) == 0) {
+      sm.m[tid / kWave] = m;
+      sm.s[tid / kWave] = s;
+    }
+    __syncthreads();
+    m = sm.m[0];
+    s = sm.s[0];
+#pragma unroll
+    for (int w = 1; w < NT / kWave; ++w) combine(m, s, sm.m[w], sm.s[w], c);
+  }
+  X = m;
+  S = s;
+}
+
+// ===========================================================================
+// The k largest
+// ===========================================================================
+//
+// The k-th largest of the threads' maxima is a bound that at least k elements
+// reach and, with elements in no particular order, hardly more do: those go to
+// LDS as (key, index) and their rank among each other is their place. Rows with
+// more candidates than fit (ties, mostly) find the k-th (key, index) bit by bit,
+// counting over the row.
+
+constexpr int kCand = 1024;
+
+// bf16 bits as an ordered 16-bit number: -0 as 0, every NaN above infinity
+__device__ __forceinline__ uint32_t order16(uint32_t h) {
+  if ((h & 0x7fff) > 0x7f80) return 0xffffu;
+  if (h == 0x8000) h = 0;
+  return (h & 0x8000) ? (~h & 0xffff) : (h | 0x8000);
+}
+
+template <int NT>
+__device__ __forceinline__ int block_count(int n, int tid, int* sm) {
+  n = (int)wave_sum((float)n);  // counts stay below 2^24 (V < 2^24)
+  if constexpr (NT > kWave) {
+    __syncthreads();
+    if ((tid & (kWave - 1)) == 0) sm[tid / kWave] = n;
+    __syncthreads();
+    n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) n += sm[w];
+  }
+  return n;
+}
+
+template <int NT, int NVEC>
+__global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restrict__ logits, int64_t ld, int k,
+                                                 float c, uint16_t* __restrict__ values, int32_t* __restrict__ ids,
+                                                 float* __restrict__ lse) {
+  __shared__ RowSums<NT> sums;
+  __shared__ uint32_t tmax[NT];
+  __shared__ unsigned long long cand[kCand];
+  __shared__ int count;
+  __shared__ int cnt[NT / kWave];
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  Row<NT, NVEC> r;
+  r.load(logits + row * ld, V, tid);
+  float X, S, xm;
+  row_sums<NT, NVEC>(r, c, tid, sums, X, S, xm);
+  if (tid == 0) {
+    lse[row] = (float)(((double)X * c + log2((double)S)) * 0.69314718055994530942);
+    count = 0;
+  }
+  // the bound: largest T16 with k thread maxima at or above it (0 if there are fewer threads)
+  tmax[tid] = order16(__float_as_uint(xm) >> 16);
+  __syncthreads();
+  uint32_t mine[NT / kWave];
+#pragma unroll
+  for (int w = 0; w < NT / kWave; ++w) mine[w] = tmax[w * kWave + lane];
+  uint32_t bound = 0;
+#pragma unroll
+  for (int b = 15; b >= 0; --b) {
+    const uint32_t t = bound | (1u << b);
+    int n = 0;
+#pragma unroll
+    for (int w = 0; w < NT / kWave; ++w) n += __popcll(__ballot(mine[w] >= t));
+    if (n >= k) bound = t;
+  }
+  const uint32_t row_bits = bound & 0x8000 ? bound & 0x7fff : ~bound & 0xffff;
+  const float fb = bound <= 0x7f ? -INFINITY : bf16_to_f32((uint16_t)row_bits);  // order16(-inf) = 0x7f
+  auto each = [&](auto f) __attribute__((always_inline)) {  // f(bits, index) over this thread's elements
+    if (r.eidx >= 0) f(__float_as_uint(r.xe) >> 16, r.eidx);
+    r.vectors(tid, [&](const u32x4& v, int i) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        f(v[q] & 0xffffu, r.head + i * 8 + 2 * q);
+        f(v[q] >> 16, r.head + i * 8 + 2 * q + 1);
+      }
+    });
+  };
+  // a NaN is no less than anything
+  each([&](uint32_t h, int i) {
+    if (!(__uint_as_float(h << 16) < fb)) {
+      const int at = atomicAdd(&count, 1);
+      if (at < kCand)
+        cand[at] = ((unsigned long long)order16(h) << 48) | ((unsigned long long)(uint32_t)(~i) << 16) | h;
+    }
+  });
+  __syncthreads();
+  int n = count;
+  if (n > kCand) {
+    // the k-th largest key, then the index up to which its equals are in
+    uint32_t key = 0;
+    for (int b = 15; b >= 0; --b) {
+      const uint32_t t = key | (1u << b);
+      int m = 0;
+      each([&](uint32_t h, int) { m += order16(h) >= t; });
+      if (block_count<NT>(m, tid, cnt) >= k) key = t;
+    }
+    int above = 0;
+    each([&](uint32_t h, int) { above += order16(h) > key; });
+    const int want = k - block_count<NT>(above, tid, cnt);  // >= 1 of the equal ones
+    int lim = 0;                                            // largest index with fewer than `want` equals below it
+    for (int b = 30; b >= 0; --b) {
+      const int t = lim | (1 << b);
+      if (t >= V) continue;
+      int m = 0;
+      each([&](uint32_t h, int i) { m += order16(h) == key && i < t; });
+      if (block_count<NT>(m, tid, cnt) < want) lim = t;
+    }
+    __syncthreads();
+    if (tid == 0) count = 0;
+    __syncthreads();
+    each([&](uint32_t h, int i) {
+      const uint32_t o = order16(h);
+      if (o > key || (o == key && i <= lim))
+        cand[atomicAdd(&count, 1)] = ((unsigned long long)o << 48) | ((unsigned long long)(uint32_t)(~i) << 16) | h;
+    });
+    __syncthreads();
+    n = count;  // k
+  }
+  for (int i = tid; i < n; i += NT) {
+    const unsigned long long me = cand[i];
+    int rank = 0;
+    for (int j = 0; j < n; ++j) rank += cand[j] > me;
+    if (rank < k) {
+      values[row * k + rank] = (uint16_t)me;
+      ids[row * k + rank] = (int32_t)~(uint32_t)(me >> 16);
+    }
+  }
+}
+
+// ===========================================================================
+// The loss and its gradient
+// ===========================================================================
+
+struct DistillArgs {
+  int V, k;
+  const uint16_t* z;
+  int64_t ld;
+  const void* ids;
+  int ids_64;
+  const void* values;
+  int values_f32;
+  const float* lse;  // null: softmax over the row's entries
+  double cd;         // log2(e) / T
+  float c;           // the same in 32 bits: the temperature that the student's row is taken at
+  float t2ln2;       // T^2 ln 2
+  float grad;        // scale T
+  float* loss;
+  uint16_t* dz;      // may be z itself
+  int64_t ldd;
+  int same_phase;    // rows of dz start at the same offset from 16 bytes as those of z
+};
+
+template <int NT, int NVEC, bool kGrad>
+__global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
+  __shared__ RowSums<NT> sums;
+  __shared__ int sid[kMaxK];     // -1: padding
+  __shared__ float sp[kMaxK];    // p_j
+  __shared__ float sz[kMaxK];    // z[id_j]
+  __shared__ double slp[kMaxK];  // log2 p_j
+  __shared__ float sS;
+  const int64_t row = blockIdx.x;
+  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const uint16_t* zrow = a.z + row * a.ld;
+  Row<NT, NVEC> r;
+  r.load(zrow, a.V, tid);
+  // The first wave takes the teacher's entries, up to 4 a lane. They count in 64
+  // bits: the loss is a difference of logarithms that may nearly cancel.
+  if (tid < kWave) {
+    double lp[kMaxK / kWave];
+    bool bad = false;
+    double mx = -INFINITY;
+    const double sub = a.lse ? (double)a.lse[row] * 1.4426950408889634074 : 0.0;
+#pragma unroll
+    for (int e = 0; e < kMaxK / kWave; ++e) {
+      const int j = e * kWave + lane;
+      lp[e] = -INFINITY;
+      if (j >= a.k) continue;
+      const int64_t at = row * a.k + j;
+      const int64_t id = a.ids_64 ? reinterpret_cast<const int64_t*>(a.ids)[at]
+                                  : (int64_t)reinterpret_cast<const int32_t*>(a.ids)[at];
+      sid[j] = id < 0 ? -1 : (id < a.V ? (int)id : -2);
+      float z = 0.f;
+      if (id >= 0) {
+        const float v = a.values_f32 ? reinterpret_cast<const float*>(a.values)[at]
+                                     : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]);
+        lp[e] = (double)v * a.cd - sub;
+        if (id < a.V) z = bf16_to_f32(zrow[id]);
+        else lp[e] = __builtin_nan("");
+        bad |= lp[e] != lp[e];
+        mx = fmax(mx, lp[e]);
+      }
+      sz[j] = z;
+    }
+    if (!a.lse) {
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) mx = fmax(mx, __shfl_xor(mx, o, kWave));
+      const double at = mx == -INFINITY ? 0.0 : mx;
+      float s = 0.f;
+#pragma unroll
+      for (int e = 0; e < kMaxK / kWave; ++e) s += exp2_split(lp[e] - at);
+      s = wave_sum(s);
+      const double l = s == 0.f ? 0.0 : at + log2((double)s);
+#pragma unroll
+      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] -= l;
+    }
+    float S = 0.f;
+#pragma unroll
+    for (int e = 0; e < kMaxK / kWave; ++e) {
+      const int j = e * kWave + lane;
+      const float p = exp2_split(lp[e]);
+      S += p;
+      if (j < a.k) {
+        sp[j] = p;
+        slp[j] = lp[e];
+      }
+    }
+    S = wave_sum(S);
+    if (__ballot(bad)) S = __builtin_nanf("");
+    if (lane == 0) sS = S;
+  }
+  float X, S, xm;
+  row_sums<NT, NVEC>(r, a.c, tid, sums, X, S, xm);
+  if constexpr (NT == kWave) __syncthreads();
+  const float mass = sS;
+  const bool none = mass == 0.f;  // no entry, or none with any weight
+  if (tid < kWave) {
+    const double l2 = (double)X * a.c + log2((double)S);
+    double sum = 0.0;
+    for (int j = lane; j < a.k; j += kWave) {
+      const float p = sp[j];
+      if (p != 0.f) sum += (double)p * (slp[j] - ((double)sz[j] * (double)a.c - l2));
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
+    if (lane == 0) a.loss[row] = none ? 0.f : (mass != mass ? mass : (float)(sum * (double)a.t2ln2));
+  }
+  if constexpr (kGrad) {
+    uint16_t* drow = a.dz + row * a.ldd;
+    const float w = mass * a.grad;
+    const bool large = too_large(finite_or_0(X), a.c);
+    const float lS = fast_log2(S);
+    const float nb = -(X * a.c + lS);
+    auto grad = [&](float x) __attribute__((always_inline)) {
+      return fast_exp2(large ? (x - X) * a.c - lS : __builtin_fmaf(x, a.c, nb)) * w;
+    };
+    if (none) {  // whatever the row holds
+      r.vectors(tid, [&](const u32x4&, int i) {
+        if (a.same_phase) {
+          reinterpret_cast<u32x4*>(drow + r.head)[i] = u32x4{0, 0, 0, 0};
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) drow[r.head + i * 8 + e] = 0;
+        }
+      });
+      if (r.eidx >= 0) drow[r.eidx] = 0;
+      return;
+    }
+    r.vectors(tid, [&](const u32x4& v, int i) {
+      u32x4 o;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(grad(bf16_lo(v[q])), grad(bf16_hi(v[q])));
+      if (a.same_phase) {
+        __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(drow + r.head) + i);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) drow[r.head + i * 8 + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
+      }
+    });
+    if (r.eidx >= 0) drow[r.eidx] = f32_to_bf16(grad(r.xe));
+    // The k entries again, with their p taken off before the one rounding: the
+    // first of equal ids adds up all of them, in order.
+    __syncthreads();
+    for (int j = tid; j < a.k; j += NT) {
+      const int id = sid[j];
+      if (id < 0) continue;
+      float p = 0.f;
+      bool first = true;
+      for (int i = 0; i < a.k; ++i)
+        if (sid[i] == id) {
+          first &= i >= j;
+          p += sp[i];
+        }
+      if (first) drow[id] = f32_to_bf16(grad(sz[j]) - p * a.grad);
+    }
+  }
+}
+
+// Threads and vectors per thread for a row of V elements. A workgroup holds 8 NT
+// NVEC of them (less up to 7 before the first vector).
+#define NL_ROW_SIZES(X) X(64, 1) X(256, 1) X(256, 2) X(512, 2) X(512, 4) X(512, 7) X(512, 10) X(512, 13) X(1024, 9) X(1024, 13)
+
+void launch_top(hipStream_t st, int M, int V, const uint16_t* x, int64_t ld, int k, float c, uint16_t* values,
+                int32_t* ids, float* lse) {
+#define NL_TOP(NT, NV)                                                                                           \
+  if (V / 8 <= NT * NV) {                                                                                        \
+    hipLaunchKernelGGL((top_kernel<NT, NV>), dim3(M), dim3(NT), 0, st, V, x, ld, k, c, values, ids, lse);       \
+    return;                                                                                                      \
+  }
+  NL_ROW_SIZES(NL_TOP)
+#undef NL_TOP
+  hipLaunchKernelGGL((top_kernel<1024, 0>), dim3(M), dim3(1024), 0, st, V, x, ld, k, c, values, ids, lse);
+}
+
+template <bool kGrad>
+void launch_distill(hipStream_t st, int M, const DistillArgs& a) {
+#define NL_DISTILL(NT, NV)                                                                     \
+  if (a.V / 8 <= NT * NV) {                                                                    \
+    hipLaunchKernelGGL((distill_kernel<NT, NV, kGrad>), dim3(M), dim3(NT), 0, st, a);          \
+    return;                                                                                    \
+  }
+  NL_ROW_SIZES(NL_DISTILL)
+#undef NL_DISTILL
+  hipLaunchKernelGGL((distill_kernel<1024, 0, kGrad>), dim3(M), dim3(1024), 0, st, a);
+}
+
+int check_rows(const char* what, int M, int V, const void* logits, int64_t ld, int k, float t) {
+  const std::string w(what);
+  if (M < 0 || V <= 0 || V >= (1 << 24)) return nl_set_error(NL_EINVAL, w + ": need M >= 0 and 0 < V < 2^24");
+  if (k < 1 || k > kMaxK) return nl_set_error(NL_EINVAL, w + ": need 1 <= k <= NL_TOP_MAX_K");
+  if (!(t > 0.f) || t == INFINITY || !(kLog2e / t < INFINITY) || !(t * t < INFINITY) || kLog2e / t < 1e-30f)
+    return nl_set_error(NL_EINVAL, w + ": the temperature must be positive and finite");
+  if (M > 0 && !logits) return nl_set_error(NL_EINVAL, w + ": null logits");
+  if (M > 1 && ld < V) return nl_set_error(NL_EINVAL, w + ": ld < V");
+  if ((uintptr_t)logits & 1) return nl_set_error(NL_EALIGN, w + ": logits not 2-byte aligned");
+  return NL_OK;
+}
+
+}  // namespace
+}  // namespace nl
+
+using namespace nl;
+
+extern "C" int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k, float temperature,
+                             nl_bf16* values, int32_t* ids, float* lse) {
+  if (int rc = check_rows("top_logits", M, V, logits, ld, k, temperature)) return rc;
+  if (k > V) return nl_set_error(NL_EINVAL, "top_logits: k > V");
+  if (M == 0) return NL_OK;
+  if (!values || !ids || !lse) return nl_set_error(NL_EINVAL, "top_logits: null output");
+  launch_top((hipStream_t)stream, M, V, logits, ld, k, kLog2e / temperature, values, ids, lse);
+  return nl_check_launch("nl_top_logits");
+}
+
+extern "C" int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k,
+                                  const void* ids, int ids_64, const void* values, int values_dtype, const float* lse,
+                                  float temperature, float* loss, float scale, nl_bf16* dlogits, int64_t ld_dlogits) {
+  if (int rc = check_rows("distill", M, V, logits, ld, k, temperature)) return rc;
+  if (values_dtype != NL_DTYPE_F32 && values_dtype != NL_DTYPE_BF16)
+    return nl_set_error(NL_EINVAL, "distill: values are fp32 or bf16");
+  if (M == 0) return NL_OK;
+  if (!ids || !values || !loss) return nl_set_error(NL_EINVAL, "distill: null pointer");
+  if (dlogits) {
+    if (M > 1 && ld_dlogits < V) return nl_set_error(NL_EINVAL, "distill: ld_dlogits < V");
+    if ((uintptr_t)dlogits & 1) return nl_set_error(NL_EALIGN, "distill: dlogits not 2-byte aligned");
+    if ((const void*)dlogits == (const void*)logits && M > 1 && ld_dlogits != ld)
+      return nl_set_error(NL_EINVAL, "distill: dlogits over the logits need ld_dlogits == ld");
+  }
+  DistillArgs a{V, k, logits, ld, ids, ids_64 != 0, values, values_dtype == NL_DTYPE_F32, lse,
+                1.4426950408889634074 / temperature, kLog2e / temperature,
+                temperature * temperature * kLn2, scale * temperature, loss, dlogits, ld_dlogits,
+                (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0 && (M == 1 || (ld - ld_dlogits) % 8 == 0)};
+  if (dlogits) launch_distill<true>((hipStream_t)stream, M, a);
+  else launch_distill<false>((hipStream_t)stream, M, a);
+  return nl_check_launch("nl_distill_fwd_bwd");
+}

@@ -1,0 +1,239 @@
+"""nlearn_amd.kernels.fp8 — products in 8-bit floating point with a scale for each block of 128.
+
+* ``quantize_fp8(x)`` / ``quantize_fp8_both(x)``: a matrix to e4m3 values with one
+  power-of-two scale for each block of 128 along the summed axis, per row
+  (``group=1``: activations, gradients) or per 128 rows (``group=128``: weights).
+* ``gemm_fp8(a, b)``: a . b^T of two such operands, fp32 sums, bf16 or fp32 out.
+* ``linear_fp8(x, W)``: ``linear(x, W)`` with all three products in 8 bits: y = x W,
+  dX = dY W^T and dW = X^T dY, every operand quantised along the axis that its
+  product sums over. ``fp8_weight(W)`` lays a frozen weight out once.
+
+A block's scale is the least 2^e with max|x| <= 448 * 2^e. A power of two leaves
+one rounding per value (to e4m3, half a step being 2^-4 of the value) and is
+applied by the matrix unit itself. The reference has no 8-bit path: this stands
+beside ``linear`` (gemm.py:93-115), in whose place it can be called.
+"""
+from __future__ import annotations
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _lib
+from . import wgrad
+from .gemm import _BF16, _F32, _check_device, _ld, _rows_disjoint, grad_buffer, padded_empty
+
+_E4M3 = torch.float8_e4m3fn
+_E8M0 = torch.float8_e8m0fnu
+BLOCK = 128
+
+
+def _blocks(n: int) -> int:
+    return (n + BLOCK - 1) // BLOCK
+
+
+class Fp8Blocks:
+    """A matrix of ``shape`` = (rows, K) in 8 bits, quantised along K.
+
+    q:     float8_e4m3fn [rows, K rounded up to 128], unit column stride, 16-byte
+           aligned rows; the columns past K are zero.
+    scale: float8_e8m0fnu [ceil(rows / group), blocks of K], unit column stride.
+    value[r, k] = q[r, k] * scale[r // group, k // 128].
+    """
+
+    __slots__ = ("q", "scale", "shape", "group")
+
+    def __init__(self, q: torch.Tensor, scale: torch.Tensor, shape, group: int = 1):
+        rows, K = (int(n) for n in shape)
+        if group not in (1, BLOCK):
+            raise ValueError(f"Fp8Blocks: a scale holds for 1 or {BLOCK} rows, not {group}")
+        kb = _blocks(K)
+        if q.dtype != _E4M3 or tuple(q.shape) != (rows, kb * BLOCK):
+            raise ValueError(f"Fp8Blocks: q must be float8_e4m3fn of shape {(rows, kb * BLOCK)}, "
+                             f"got {q.dtype} {tuple(q.shape)}")
+        if scale.dtype != _E8M0 or tuple(scale.shape) != ((rows + group - 1) // group, kb):
+            raise ValueError(f"Fp8Blocks: scale must be float8_e8m0fnu of shape {((rows + group - 1) // group, kb)}, "
+                             f"got {scale.dtype} {tuple(scale.shape)}")
+        for name, t in (("q", q), ("scale", scale)):
+            if t.numel() and ((t.stride(1) != 1 and t.shape[1] > 1) or not _rows_disjoint(t)):
+                raise ValueError(f"Fp8Blocks: {name} needs a unit column stride and rows of their own")
+        if scale.device != q.device:
+            raise ValueError("Fp8Blocks: q and scale are on different devices")
+        if q.numel() and (q.data_ptr() % 16 or (rows > 1 and q.stride(0) % 16)):
+            raise ValueError("Fp8Blocks: q needs 16-byte aligned rows")
+        self.q, self.scale, self.shape, self.group = q, scale, (rows, K), group
+
+    @classmethod
+    def empty(cls, rows: int, K: int, group: int, device) -> "Fp8Blocks":
+        kb, sr = _blocks(K), (rows + group - 1) // group
+        b = cls.__new__(cls)
+        b.q = torch.empty((rows, kb * BLOCK), dtype=_E4M3, device=device)
+        # scale rows padded to whole dwords: the product reads four blocks at a time
+        ld = (kb + 3) // 4 * 4
+        s = torch.empty((sr, ld), dtype=_E8M0, device=device)
+        b.scale = s if ld == kb else s[:, :kb]
+        b.shape, b.group = (rows, K), group
+        return b
+
+    def _abi(self):
+        """(q, ldq, scale, lds) as the C entry points take them."""
+        return self.q.data_ptr(), _row_stride(self.q), self.scale.data_ptr(), _row_stride(self.scale)
+
+    def dequantize(self) -> torch.Tensor:
+        """The fp32 values (a plain torch expression, for checks and inspection)."""
+        rows, K = self.shape
+        s = self.scale.float().repeat_interleave(self.group, 0)[:rows]
+        return (self.q.float().view(rows, -1, BLOCK) * s[:, :, None]).view(rows, -1)[:, :K]
+
+
+def _row_stride(t: torch.Tensor) -> int:
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _source(x: torch.Tensor):
+    """x as the quantiser reads it (fp32 or bf16, unit column stride, rows of their own) and its row stride."""
+    if x.dim() != 2:
+        raise ValueError(f"quantize_fp8: expected a 2-D tensor, got shape {tuple(x.shape)}")
+    _check_device(x)
+    x = x.detach()
+    if x.dtype not in (_BF16, _F32):
+        raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {x.dtype}")
+    if (x.shape[1] > 1 and x.stride(1) != 1) or not _rows_disjoint(x):
+        x = x.contiguous()
+    return x, _row_stride(x)
+
+
+def _quantize(x, group: int, along: bool, across: bool):
+    if group not in (1, BLOCK):
+        raise ValueError(f"quantize_fp8: a scale holds for 1 or {BLOCK} rows, not {group}")
+    x, ldx = _source(x)
+    rows, cols = x.shape
+    a = Fp8Blocks.empty(rows, cols, group, x.device) if along else None
+    t = Fp8Blocks.empty(cols, rows, group, x.device) if across else None
+    none = (None, 0, None, 0)
+    if rows and cols:
+        _lib.call_on(x, "nl_quantize_fp8", rows, cols, x.data_ptr(),
+                  _lib.NL_DTYPE_F32 if x.dtype is _F32 else _lib.NL_DTYPE_BF16, ldx, group,
+                  *(a._abi() if along else none), *(t._abi() if across else none))
+    return a, t
+
+
+def quantize_fp8(x: torch.Tensor, group: int = 1, transpose: bool = False) -> Fp8Blocks:
+    """x (R, C), bf16 or fp32, quantised along its columns; with ``transpose`` x^T
+    (C, R), quantised along the rows of x. One scale for each block of 128 and
+    each ``group`` rows of the result. Values that are not finite become NaN and
+    have no part in the scales."""
+    a, t = _quantize(x, group, not transpose, transpose)
+    return t if transpose else a
+
+
+def quantize_fp8_both(x: torch.Tensor, group: int = 1):
+    """(quantize_fp8(x), quantize_fp8(x, transpose=True)) from one read of x."""
+    return _quantize(x, group, True, True)
+
+
+def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:
+    """The workspace gemm_fp8 would allocate for this product (or None)."""
+    wsb = int(_lib.load().nl_gemm_fp8_ws_bytes(a.shape[0], b.shape[0], a.shape[1]))
+    return torch.empty(wsb // 4, dtype=_F32, device=a.q.device) if wsb else None
+
+
+def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | None = None,
+             ws: torch.Tensor | None = None) -> torch.Tensor:
+    """a (M, K) . b (N, K)^T -> (M, N), summed in fp32, on the current stream.
+    ws: as ``gemm_fp8_ws`` gives it (allocated here if None)."""
+    (M, K), (N, Kb) = a.shape, b.shape
+    if K != Kb:
+        raise ValueError(f"gemm_fp8: inner dimensions differ ({K} vs {Kb})")
+    _check_device(a.q, b.q)
+    if a.q.device != b.q.device:
+        raise ValueError(f"gemm_fp8: operands on {a.q.device} and {b.q.device}")
+    if out is None:
+        if out_dtype not in (_F32, _BF16):
+            raise ValueError("gemm_fp8: output must be float32 or bfloat16")
+        out = padded_empty(M, N, out_dtype, a.q.device)
+    elif out.dtype not in (_F32, _BF16) or tuple(out.shape) != (M, N) or out.device != a.q.device:
+        raise ValueError(f"gemm_fp8: output must be float32 or bfloat16 of shape {(M, N)} on {a.q.device}")
+    if M == 0 or N == 0:
+        return out
+    if ws is None:
+        ws = gemm_fp8_ws(a, b)
+    qa, lda, sa, ldsa = a._abi()
+    qb, ldb, sb, ldsb = b._abi()
+    _lib.call_on(a.q, "nl_gemm_fp8", M, N, K, qa, lda, sa, ldsa, a.group, qb, ldb, sb, ldsb, b.group,
+              out.data_ptr(), _lib.NL_DTYPE_F32 if out.dtype is _F32 else _lib.NL_DTYPE_BF16, _ld(out),
+              ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
+    return out
+
+
+class Fp8Weight:
+    """A weight W (K, N) in 8 bits with a scale for each 128 x 128 block, laid out
+    for both products that read it: ``fwd`` is W^T (N, K), ``bwd`` W (K, N), the
+    same values."""
+
+    __slots__ = ("fwd", "bwd", "shape")
+
+    def __init__(self, fwd: Fp8Blocks, bwd: Fp8Blocks):
+        if fwd.shape != bwd.shape[::-1]:
+            raise ValueError(f"Fp8Weight: {fwd.shape} is not the transpose of {bwd.shape}")
+        self.fwd, self.bwd, self.shape = fwd, bwd, bwd.shape
+
+
+def fp8_weight(W: torch.Tensor) -> Fp8Weight:
+    """W (K, N) quantised once, for a weight that stays as it is (a frozen teacher's)."""
+    bwd, fwd = quantize_fp8_both(W, group=BLOCK)
+    return Fp8Weight(fwd, bwd)
+
+
+class _LinearFp8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x2, W, frozen):
+        need_dx, need_dW = ctx.needs_input_grad[:2]
+        if frozen is None:
+            bwd, fwd = _quantize(W, BLOCK, need_dx, True)
+        else:
+            bwd, fwd = frozen.bwd, frozen.fwd
+        xq, xt = _quantize(x2, 1, True, need_dW)
+        ctx.save_for_backward(W)
+        ctx.x_dtype = x2.dtype
+        ctx.bwd = bwd if need_dx else None  # W for dX, X^T for dW: 8 bits each
+        ctx.xt = xt
+        return gemm_fp8(xq, fwd, x2.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        (W,) = ctx.saved_tensors
+        need_dx, need_dW = ctx.needs_input_grad[:2]
+        if dy.dtype not in (_BF16, _F32):
+            dy = dy.to(_F32)
+        dyq, dyt = _quantize(dy, 1, need_dx, need_dW)
+        dx = gemm_fp8(dyq, ctx.bwd, ctx.x_dtype) if need_dx else None      # dY . W^T
+        dW = None
+        if need_dW:
+            mg = grad_buffer(W)
+            if mg is not None:
+                xt, ws = ctx.xt, gemm_fp8_ws(ctx.xt, dyt)                  # X^T . dY -> main_grad
+                wgrad.fork(lambda: gemm_fp8(xt, dyt, out=mg, ws=ws), xt, dyt, mg, ws)
+            else:
+                dW = gemm_fp8(ctx.xt, dyt, W.dtype)
+        return dx, dW, None
+
+
+def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
+    """x[..., K] @ W[K, N] -> [..., N] in x's dtype, with 8-bit products.
+
+    W: an fp32 or bf16 weight, quantised here, or an ``Fp8Weight`` (frozen: it gets
+    no gradient). The gradients are those of the product of the quantised
+    operands, with dY quantised too and the rounding taken as the identity."""
+    if x.dim() < 2:
+        raise ValueError("linear_fp8: x needs >= 2 dims")
+    frozen = W if isinstance(W, Fp8Weight) else None
+    if frozen is None and W.dim() != 2:
+        raise ValueError("linear_fp8: W needs exactly 2 dims")
+    if x.shape[-1] != W.shape[0]:
+        raise ValueError(f"linear_fp8: x has {x.shape[-1]} features, W has {W.shape[0]} rows")
+    if x.dtype not in (_BF16, _F32):
+        raise ValueError(f"linear_fp8: x must be bfloat16 or float32, got {x.dtype}")
+    lead = x.shape[:-1]
+    y = _LinearFp8.apply(x.reshape(-1, x.shape[-1]), W if frozen is None else None, frozen)
+    return y.reshape(*lead, W.shape[1])
