@@ -18,6 +18,8 @@
 // result, but not the sum that an fp32 result stands for. A product with an fp32
 // result therefore widens its operands to bf16 in registers (exact, with the
 // scale) and takes v_mfma_f32_32x32x16_bf16, whose sums are fp32, at half the rate.
+#include <type_traits>
+
 #include "common.h"
 
 namespace nl {
@@ -297,7 +299,40 @@ __device__ __forceinline__ void widen(const u32x4& v, float scale, bf16x8 out[2]
   out[1] = as_bf16x8(u32x4{w[4], w[5], w[6], w[7]});
 }
 
-__device__ __forceinline__ int swz8(int r) { return (r ^ (r >> 3)) & 7; }
+// Slot of 16-byte chunk c of row r: c ^ swz(r). 16 consecutive rows at one chunk (a
+// fragment read) fall on all 64 banks, and rows 16 apart share the swizzle.
+__device__ __forceinline__ int swz(int r) { return (r & 7) ^ ((r >> 3) & 1); }
+
+// A lane's fragment: 16 bytes to widen, or the 32 that an 8-bit MFMA takes.
+template <bool kWide>
+struct FragOf {
+  typedef u32x4 type;
+};
+template <>
+struct FragOf<false> {
+  typedef i32x8 type;
+};
+template <bool kWide>
+__device__ __forceinline__ typename FragOf<kWide>::type read_frag(const uint8_t* p, const int* off) {
+  const u32x4 lo = *reinterpret_cast<const u32x4*>(p + off[0]);
+  if constexpr (kWide) {
+    return lo;
+  } else {
+    const u32x4 hi = *reinterpret_cast<const u32x4*>(p + off[1]);
+    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+  }
+}
+
+// One MFMA, then its share of the R fragment reads of the next step.
+template <int M, int NM, int R>
+__device__ __forceinline__ void sched_f8() {
+  if constexpr (M < NM) {
+    __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+    constexpr int lo = M * R / NM, hi = (M + 1) * R / NM;
+    if constexpr (hi > lo) __builtin_amdgcn_sched_group_barrier(0x100, hi - lo, 0);
+    sched_f8<M + 1, NM, R>();
+  }
+}
 
 template <int BM, int BN, int WTM, int WTN, typename OutT>
 __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 1 : 2) void gemm_f8_kernel(
@@ -307,6 +342,9 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   constexpr int STAGE = (BM + BN) * kB;
   constexpr int IA = BM / 8 / NWV, IB = BN / 8 / NWV;  // DMA instructions (8 rows each) per wave and stage
   static_assert(IA * 8 * NWV == BM && IB * 8 * NWV == BN, "a stage splits into whole DMA instructions");
+  constexpr bool kWide = sizeof(OutT) == 4;            // widened to bf16 for fp32 sums
+  constexpr int NS = kWide ? 4 : 2;                    // fragment steps of a stage: 16 or 32 bytes of k a lane
+  constexpr int CH = kWide ? 1 : 2;                    // 16-byte chunks of a fragment
   __shared__ __attribute__((aligned(16))) uint8_t st0[STAGE];
   __shared__ __attribute__((aligned(16))) uint8_t st1[STAGE];
 
@@ -337,22 +375,25 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   // Descriptors start at the tile's first row (64-bit base), so 32-bit offsets
   // reach any matrix; rows past the last one read as zero.
   const int ra_rows = min(g.M - m0, BM), rb_rows = min(g.N - n0, BN);
-  const __amdgpu_buffer_rsrc_t ra =
-      make_rsrc(g.A + (int64_t)m0 * g.lda, (uint32_t)((int64_t)(ra_rows - 1) * g.lda + g.Kp));
-  const __amdgpu_buffer_rsrc_t rb =
-      make_rsrc(g.B + (int64_t)n0 * g.ldb, (uint32_t)((int64_t)(rb_rows - 1) * g.ldb + g.Kp));
+  const uint8_t* pa = g.A + (int64_t)m0 * g.lda;
+  const uint8_t* pb = g.B + (int64_t)n0 * g.ldb;
+  const uint32_t ba = (uint32_t)((int64_t)(ra_rows - 1) * g.lda + g.Kp);
+  const uint32_t bb = (uint32_t)((int64_t)(rb_rows - 1) * g.ldb + g.Kp);
   uint32_t va[IA], vb[IB];
 #pragma unroll
   for (int i = 0; i < IA; ++i) {
     const int r = (i * NWV + wave) * 8 + (lane >> 3);
-    va[i] = (uint32_t)((int64_t)r * g.lda) + (((lane & 7) ^ swz8(r)) << 4);
+    va[i] = (uint32_t)((int64_t)r * g.lda) + (((lane & 7) ^ swz(r)) << 4);
   }
 #pragma unroll
   for (int i = 0; i < IB; ++i) {
     const int r = (i * NWV + wave) * 8 + (lane >> 3);
-    vb[i] = (uint32_t)((int64_t)r * g.ldb) + (((lane & 7) ^ swz8(r)) << 4);
+    vb[i] = (uint32_t)((int64_t)r * g.ldb) + (((lane & 7) ^ swz(r)) << 4);
   }
   auto issue = [&](uint8_t* sb, int kt) __attribute__((always_inline)) {
+    // behind the last stage an empty descriptor reads nothing: a branch here would let
+    // the compiler move the MFMAs before it to the ones behind it
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(pa, kt < nkb ? ba : 0), rb = make_rsrc(pb, kt < nkb ? bb : 0);
     const uint32_t soff = (uint32_t)(kb0 + kt) * kB;
 #pragma unroll
     for (int i = 0; i < IA; ++i) dma16(ra, sb + (i * NWV + wave) * 1024, va[i], soff);
@@ -360,48 +401,43 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     for (int i = 0; i < IB; ++i) dma16(rb, sb + BM * kB + (i * NWV + wave) * 1024, vb[i], soff);
   };
 
-  // scale rows of this lane's fragments, four blocks to a dword
-  const uint8_t* psa[FM];
-  const uint8_t* psb[FN];
+  // scale rows of this lane's fragments (byte offsets from the tile's first), four blocks to a dword
+  const uint8_t* psa = g.sa + (int64_t)(m0 >> g.sha) * g.ldsa + kb0;
+  const uint8_t* psb = g.sb + (int64_t)(n0 >> g.shb) * g.ldsb + kb0;
+  uint32_t osa[FM], osb[FN];
   const int frow = lane & 31;
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int m = min(m0 + wm * WTM + i * 32 + frow, g.M - 1);
-    psa[i] = g.sa + (int64_t)(m >> g.sha) * g.ldsa + kb0;
-  }
+  for (int i = 0; i < FM; ++i)
+    osa[i] = (uint32_t)((min(wm * WTM + i * 32 + frow, ra_rows - 1) >> g.sha) * g.ldsa);
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int n = min(n0 + wn * WTN + j * 32 + frow, g.N - 1);
-    psb[j] = g.sb + (int64_t)(n >> g.shb) * g.ldsb + kb0;
-  }
+  for (int j = 0; j < FN; ++j)
+    osb[j] = (uint32_t)((min(wn * WTN + j * 32 + frow, rb_rows - 1) >> g.shb) * g.ldsb);
   uint32_t sca[FM], scb[FN], nca[FM], ncb[FN];
   auto load_scales = [&](int q) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < FM; ++i) nca[i] = scales4(psa[i], q, nkb, g.dwa);
+    for (int i = 0; i < FM; ++i) nca[i] = scales4(psa + osa[i], q, nkb, g.dwa);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) ncb[j] = scales4(psb[j], q, nkb, g.dwb);
+    for (int j = 0; j < FN; ++j) ncb[j] = scales4(psb + osb[j], q, nkb, g.dwb);
   };
 
-  int offa[FM], offb[FN], swa[FM], swb[FN];
+  // fragment (i, step t): row i * 32 + frow, chunks of step t; one offset per step and chunk
+  int offa[NS][CH], offb[NS][CH];
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
-    const int r = wm * WTM + i * 32 + frow;
-    offa[i] = r * kB;
-    swa[i] = swz8(r);
-  }
+  for (int t = 0; t < NS; ++t)
 #pragma unroll
-  for (int j = 0; j < FN; ++j) {
-    const int r = wn * WTN + j * 32 + frow;
-    offb[j] = BM * kB + r * kB;
-    swb[j] = swz8(r);
-  }
-  auto chunk = [&](const uint8_t* sb, int off, int sw, int c) __attribute__((always_inline)) {
-    return *reinterpret_cast<const u32x4*>(sb + off + ((c ^ sw) << 4));
-  };
-  auto frag = [&](const uint8_t* sb, int off, int sw, int ks) __attribute__((always_inline)) {
-    const int c = ks * 4 + (lane >> 5) * 2;
-    const u32x4 lo = chunk(sb, off, sw, c), hi = chunk(sb, off, sw, c + 1);
-    return i32x8{(int)lo[0], (int)lo[1], (int)lo[2], (int)lo[3], (int)hi[0], (int)hi[1], (int)hi[2], (int)hi[3]};
+    for (int h = 0; h < CH; ++h) {
+      const int c = (t * 2 + (lane >> 5)) * CH + h;
+      const int o = frow * kB + ((c ^ swz(frow)) << 4);
+      offa[t][h] = wm * WTM * kB + o;
+      offb[t][h] = (BM + wn * WTN) * kB + o;
+    }
+  using Frag = typename FragOf<kWide>::type;
+  Frag fa[2][FM], fb[2][FN];
+  auto read = [&](const uint8_t* sb, int t, int into) __attribute__((always_inline)) {
+#pragma unroll
+    for (int j = 0; j < FN; ++j) fb[into][j] = read_frag<kWide>(sb + j * 32 * kB, offb[t]);
+#pragma unroll
+    for (int i = 0; i < FM; ++i) fa[into][i] = read_frag<kWide>(sb + i * 32 * kB, offa[t]);
   };
 
   f32x16 acc[FM][FN];
@@ -411,70 +447,86 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     for (int j = 0; j < FN; ++j)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-
-  auto step = [&](uint8_t* cur, uint8_t* nxt, int kt) __attribute__((always_inline)) {
-    wait_vm<0>();
-    __syncthreads();
-    if ((kt & 3) == 0) {
+  auto compute = [&](int in, auto pos) __attribute__((always_inline)) {
+    constexpr int P = decltype(pos)::value;  // the block's byte in the scale dwords
+    if constexpr (kWide) {
+      bf16x8 b[FN][2];
 #pragma unroll
-      for (int i = 0; i < FM; ++i) sca[i] = nca[i];
+      for (int j = 0; j < FN; ++j) widen(fb[in][j], __uint_as_float((scb[j] >> (8 * P) & 0xff) << 23), b[j]);
 #pragma unroll
-      for (int j = 0; j < FN; ++j) scb[j] = ncb[j];
-      if (kt + 4 < nkb) load_scales((kt >> 2) + 1);
-    }
-    if (kt + 1 < nkb) issue(nxt, kt + 1);
-    if constexpr (sizeof(OutT) == 4) {
-      // 16 bytes of a row make two fragments of 8 bf16, scaled on the way (exact)
-      float fa[FM], fb[FN];
-#pragma unroll
-      for (int i = 0; i < FM; ++i) fa[i] = __uint_as_float((sca[i] & 0xff) << 23);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) fb[j] = __uint_as_float((scb[j] & 0xff) << 23);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        bf16x8 a[FM][2], b[FN][2];
-#pragma unroll
-        for (int i = 0; i < FM; ++i) widen(chunk(cur, offa[i], swa[i], 2 * c + (lane >> 5)), fa[i], a[i]);
-#pragma unroll
-        for (int j = 0; j < FN; ++j) widen(chunk(cur, offb[j], swb[j], 2 * c + (lane >> 5)), fb[j], b[j]);
+      for (int i = 0; i < FM; ++i) {
+        bf16x8 a[2];
+        widen(fa[in][i], __uint_as_float((sca[i] >> (8 * P) & 0xff) << 23), a);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int i = 0; i < FM; ++i)
-#pragma unroll
-            for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j][h], a[i][h], acc[i][j]);
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j][h], a[h], acc[i][j]);
       }
     } else {
-    i32x8 af[2][FM], bf[2][FN];
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks) {
-#pragma unroll
-      for (int i = 0; i < FM; ++i) af[ks][i] = frag(cur, offa[i], swa[i], ks);
-#pragma unroll
-      for (int j = 0; j < FN; ++j) bf[ks][j] = frag(cur, offb[j], swb[j], ks);
-    }
-#pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(bf[ks][j], af[ks][i], acc[i][j], 0, 0, 0,
-                                                                     (int)scb[j], 0, (int)sca[i]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[in][j], fa[in][i], acc[i][j], 0, 0, P,
+                                                                     (int)scb[j], P, (int)sca[i]);
     }
-#pragma unroll
-    for (int i = 0; i < FM; ++i) sca[i] >>= 8;
-#pragma unroll
-    for (int j = 0; j < FN; ++j) scb[j] >>= 8;
   };
+
+  // Stage kt: every step reads the next one's fragments while its MFMAs run. The
+  // last step's fragments are in registers when the workgroup meets, so the stage's
+  // buffer is free for stage kt + 2 and the first fragments of kt + 1 (whose DMA has
+  // had a whole stage to land) are read under the last step's MFMAs.
+  auto stage = [&](int kt, auto pos) __attribute__((always_inline)) {
+    uint8_t* cur = decltype(pos)::value % 2 == 0 ? st0 : st1;
+    uint8_t* nxt = decltype(pos)::value % 2 == 0 ? st1 : st0;
+#pragma unroll
+    for (int t = 0; t < NS; ++t) {
+      if (t + 1 < NS) {
+        read(cur, t + 1, (t + 1) & 1);
+      } else {
+        wait_vm<0>();
+        __syncthreads();
+        issue(cur, kt + 2);
+        read(nxt, 0, 0);  // (behind the last stage: not used)
+      }
+      compute(t & 1, pos);
+      if constexpr (!kWide) sched_f8<0, FM * FN, (FM + FN) * CH>();
+    }
+  };
+  using P0 = std::integral_constant<int, 0>;
+  using P1 = std::integral_constant<int, 1>;
+  using P2 = std::integral_constant<int, 2>;
+  using P3 = std::integral_constant<int, 3>;
+  auto next_scales = [&](int kt) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sca[i] = nca[i];
+#pragma unroll
+    for (int j = 0; j < FN; ++j) scb[j] = ncb[j];
+    load_scales(min((kt >> 2) + 1, (nkb - 1) >> 2));
+  };
+  int kt = 0;
   if (nkb > 0) {
     load_scales(0);
     issue(st0, 0);
-  }
-  for (int kt = 0; kt < nkb; kt += 2) {
-    step(st0, st1, kt);
-    if (kt + 1 >= nkb) break;
-    step(st1, st0, kt + 1);
+    issue(st1, 1);
+    wait_vm<IA + IB>();
+    __syncthreads();
+    read(st0, 0, 0);
+    for (; kt + 4 <= nkb; kt += 4) {
+      next_scales(kt);
+      stage(kt, P0{});
+      stage(kt + 1, P1{});
+      stage(kt + 2, P2{});
+      stage(kt + 3, P3{});
+    }
+    if (kt < nkb) {
+      next_scales(kt);
+      stage(kt, P0{});
+      if (kt + 1 < nkb) {
+        stage(kt + 1, P1{});
+        if (kt + 2 < nkb) stage(kt + 2, P2{});
+      }
+    }
   }
 
   const int g4 = (lane >> 5) * 4;
@@ -501,6 +553,7 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   __syncthreads();
   constexpr int PITCH = WTN * (int)sizeof(OutT), CPR = PITCH / 16, EPC = 16 / (int)sizeof(OutT), RPI = 64 / CPR;
   static_assert(NWV * 32 * PITCH <= STAGE, "the slabs fit the first stage");
+  static_assert(CPR <= 64, "a row is one instruction's pieces at most");
   uint8_t* wl = st0 + wave * 32 * PITCH;
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
@@ -591,7 +644,7 @@ template <typename OutT>
 void launch_f8(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
   const dim3 grid((unsigned)(p.tiles * p.splits));
   if (p.huge)
-    hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 64, OutT>), grid, dim3(512), 0, st, g);
+    hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT>), grid, dim3(256), 0, st, g);
   else
     hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT>), grid, dim3(256), 0, st, g);
   if (p.splits > 1)
