@@ -21,6 +21,19 @@ int nl_check_launch(const char* what) {
   return NL_OK;
 }
 
+// Compute units of the current device (cached per device).
+int nl::cu_count() {
+  static int cached[64] = {0};
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+  if (!cached[dev]) {
+    int n = 0;
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached[dev] = n;
+  }
+  return cached[dev];
+}
+
 extern "C" const char* nl_strerror(int status) {
   switch (status) {
     case NL_OK: return "ok";

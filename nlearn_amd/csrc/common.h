@@ -176,3 +176,6 @@ __device__ __forceinline__ void transpose8x8_b16(const u32x4 in[8], u32x4 out[8]
 // ---------------------------------------------------------------------------
 int nl_set_error(int code, const std::string& msg);
 int nl_check_launch(const char* what);
+namespace nl {
+int cu_count();  // compute units of the current device (256 where there is none)
+}

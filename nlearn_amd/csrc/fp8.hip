@@ -261,29 +261,34 @@ struct GemmF8Args {
   const uint8_t* sa;
   int64_t ldsa;
   int sha;  // log2 of the rows per scale: 0 or 7
-  int dwa;  // scale rows are whole, aligned dwords
   const uint8_t* B;
   int64_t ldb;
   const uint8_t* sb;
   int64_t ldsb;
-  int shb, dwb;
+  int shb;
+  int dw;  // scale rows of both are whole, aligned dwords
   void* C;
   int64_t ldc;
   float* ws;     // split partials [splits][M][ldw], or null
   int64_t ldw;
   int tiles;     // output tiles
+  int items;     // tiles * splits
   int kb_chunk;  // blocks per split (a multiple of 4 when there is more than one)
 };
 
-// Scale bytes 4q .. 4q+3 of one row (nkb of them there): one dword where rows
-// start on 4 bytes and are padded to whole dwords, else byte by byte.
-__device__ __forceinline__ uint32_t scales4(const uint8_t* p, int q, int nkb, int dw) {
-  if (dw) return reinterpret_cast<const uint32_t*>(p)[q];
-  uint32_t v = 0;
+// Four scale bytes of one row from byte `off` (n of them there): one dword where
+// rows are whole, aligned dwords, else byte by byte.
+template <bool kDw>
+__device__ __forceinline__ uint32_t scales4(__amdgpu_buffer_rsrc_t rs, uint32_t off, int n) {
+  if constexpr (kDw) {
+    return __builtin_amdgcn_raw_buffer_load_b32(rs, off, 0, 0);
+  } else {
+    uint32_t v = 0;
 #pragma unroll
-  for (int b = 0; b < 4; ++b)
-    if (4 * q + b < nkb) v |= (uint32_t)p[4 * q + b] << (8 * b);
-  return v;
+    for (int b = 0; b < 4; ++b)
+      v |= (uint32_t)__builtin_amdgcn_raw_buffer_load_b8(rs, b < n ? off + b : 0xffffffffu, 0, 0) << (8 * b);
+    return v;
+  }
 }
 
 // 16 e4m3 bytes times a power of two (given as the float it is) to two fragments
@@ -334,7 +339,56 @@ __device__ __forceinline__ void sched_f8() {
   }
 }
 
-template <int BM, int BN, int WTM, int WTN, typename OutT>
+// A workgroup (one per CU with 256 x 256 tiles, two with 128 x 128) walks its items
+// (a tile's share of K) without a pause in the operand stream: an item's last two
+// stages start the DMA of the next item's first two, and its stores drain while the
+// next item's first stages compute.
+struct F8Item {
+  int m0, n0, split, kb0, nkb;  // nkb: blocks of K
+  const uint8_t *a, *b, *sa, *sb;
+  uint32_t ba, bb, bsa, bsb;    // bytes in reach of each (0: no such item)
+};
+
+// the same on every lane, and known to be
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = (uint64_t)p;
+  return reinterpret_cast<const uint8_t*>((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
+template <int BM, int BN>
+__device__ __forceinline__ F8Item f8_item(const GemmF8Args& g, int item) {
+  F8Item t;
+  const int tiles_n = (g.N + BN - 1) / BN;
+  const int tiles_m = (g.M + BM - 1) / BM;
+  item = uniform(item);
+  t.split = item / g.tiles;
+  const int tile = item - t.split * g.tiles;
+  constexpr int GM = 8;  // tile rows that neighbours share a column of B over
+  const int in_group = GM * tiles_n;
+  const int first_m = (tile / in_group) * GM;
+  const int gsize = min(tiles_m - first_m, GM);
+  t.m0 = (first_m + (tile % in_group) % gsize) * BM;
+  t.n0 = ((tile % in_group) / gsize) * BN;
+  t.kb0 = t.split * g.kb_chunk;
+  t.nkb = min(g.Kp / kB, t.kb0 + g.kb_chunk) - t.kb0;
+  // Descriptors start at the item's first row (64-bit base), so 32-bit offsets reach
+  // any matrix; rows past the last one read as zero.
+  const int ra = min(g.M - t.m0, BM), rb = min(g.N - t.n0, BN);
+  t.a = g.A + (int64_t)t.m0 * g.lda;
+  t.b = g.B + (int64_t)t.n0 * g.ldb;
+  t.sa = g.sa + (int64_t)(t.m0 >> g.sha) * g.ldsa + t.kb0;
+  t.sb = g.sb + (int64_t)(t.n0 >> g.shb) * g.ldsb + t.kb0;
+  t.ba = (uint32_t)((int64_t)(ra - 1) * g.lda + g.Kp);
+  t.bb = (uint32_t)((int64_t)(rb - 1) * g.ldb + g.Kp);
+  // whole dwords of scales where rows hold them (the last one may end in padding)
+  t.bsa = (uint32_t)(((ra - 1) >> g.sha) * g.ldsa + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
+  t.bsb = (uint32_t)(((rb - 1) >> g.shb) * g.ldsb + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
+  return t;
+}
+
+// kDw: scale rows are whole, aligned dwords. Else a scale dword is four byte loads.
+template <int BM, int BN, int WTM, int WTN, typename OutT, bool kDw>
 __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 1 : 2) void gemm_f8_kernel(
     GemmF8Args g) {
   constexpr int WNW = BN / WTN, NWV = (BM / WTM) * WNW;
@@ -345,40 +399,26 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   constexpr bool kWide = sizeof(OutT) == 4;            // widened to bf16 for fp32 sums
   constexpr int NS = kWide ? 4 : 2;                    // fragment steps of a stage: 16 or 32 bytes of k a lane
   constexpr int CH = kWide ? 1 : 2;                    // 16-byte chunks of a fragment
+  constexpr int PITCH = 2 * WTN;                       // bytes of a slab row: WTN bf16 or half as many fp32
+  // Each stage is an LDS object of its own: the compiler then knows that the DMA into
+  // one does not alias the reads of the other.
   __shared__ __attribute__((aligned(16))) uint8_t st0[STAGE];
   __shared__ __attribute__((aligned(16))) uint8_t st1[STAGE];
+  __shared__ __attribute__((aligned(16))) uint8_t slabs[NWV * 32 * PITCH];
 
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WNW, wn = wave % WNW;
 
-  // each XCD takes a contiguous run of tiles, in groups of 8 tile rows
-  int bid = blockIdx.x;
-  {
-    const int nwg = gridDim.x, per = nwg / 8;
-    if (bid < per * 8) bid = (bid % 8) * per + bid / 8;
-  }
-  const int tiles_n = (g.N + BN - 1) / BN;
-  const int tiles_m = (g.M + BM - 1) / BM;
-  const int split = bid / g.tiles;
-  const int tile = bid - split * g.tiles;
-  constexpr int GM = 8;
-  const int in_group = GM * tiles_n;
-  const int first_m = (tile / in_group) * GM;
-  const int gsize = min(tiles_m - first_m, GM);
-  const int tm = first_m + (tile % in_group) % gsize;
-  const int tn = (tile % in_group) / gsize;
-  const int m0 = tm * BM, n0 = tn * BN;
-  const int kb0 = split * g.kb_chunk;
-  const int nkb = min(g.Kp / kB, kb0 + g.kb_chunk) - kb0;  // blocks of this split
+  // Items of this workgroup: each XCD takes a contiguous run of them (neighbours share
+  // rows of A and B in its L2), its workgroups take turns within it.
+  const int nx = gridDim.x >= 8 ? 8 : 1;
+  const int xcd = blockIdx.x % nx, turn = blockIdx.x / nx;
+  const int wgs = (gridDim.x - xcd + nx - 1) / nx;
+  const int last = (int)((int64_t)g.items * (xcd + 1) / nx);
+  int item = (int)((int64_t)g.items * xcd / nx) + turn;
+  if (item >= last) return;
 
-  // Descriptors start at the tile's first row (64-bit base), so 32-bit offsets
-  // reach any matrix; rows past the last one read as zero.
-  const int ra_rows = min(g.M - m0, BM), rb_rows = min(g.N - n0, BN);
-  const uint8_t* pa = g.A + (int64_t)m0 * g.lda;
-  const uint8_t* pb = g.B + (int64_t)n0 * g.ldb;
-  const uint32_t ba = (uint32_t)((int64_t)(ra_rows - 1) * g.lda + g.Kp);
-  const uint32_t bb = (uint32_t)((int64_t)(rb_rows - 1) * g.ldb + g.Kp);
   uint32_t va[IA], vb[IB];
 #pragma unroll
   for (int i = 0; i < IA; ++i) {
@@ -390,34 +430,42 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     const int r = (i * NWV + wave) * 8 + (lane >> 3);
     vb[i] = (uint32_t)((int64_t)r * g.ldb) + (((lane & 7) ^ swz(r)) << 4);
   }
-  auto issue = [&](uint8_t* sb, int kt) __attribute__((always_inline)) {
-    // behind the last stage an empty descriptor reads nothing: a branch here would let
-    // the compiler move the MFMAs before it to the ones behind it
-    const __amdgpu_buffer_rsrc_t ra = make_rsrc(pa, kt < nkb ? ba : 0), rb = make_rsrc(pb, kt < nkb ? bb : 0);
-    const uint32_t soff = (uint32_t)(kb0 + kt) * kB;
+  // the DMA of an item's stage kt; behind its last block an empty descriptor gives zeros
+  auto issue = [&](uint8_t* sb, const F8Item& t, int kt) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(uniform(t.a), uniform(kt < t.nkb ? t.ba : 0));
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(uniform(t.b), uniform(kt < t.nkb ? t.bb : 0));
+    const uint32_t soff = uniform((t.kb0 + kt) * kB);
 #pragma unroll
     for (int i = 0; i < IA; ++i) dma16(ra, sb + (i * NWV + wave) * 1024, va[i], soff);
 #pragma unroll
     for (int i = 0; i < IB; ++i) dma16(rb, sb + BM * kB + (i * NWV + wave) * 1024, vb[i], soff);
   };
 
-  // scale rows of this lane's fragments (byte offsets from the tile's first), four blocks to a dword
-  const uint8_t* psa = g.sa + (int64_t)(m0 >> g.sha) * g.ldsa + kb0;
-  const uint8_t* psb = g.sb + (int64_t)(n0 >> g.shb) * g.ldsb + kb0;
-  uint32_t osa[FM], osb[FN];
+  // Scale bytes of this lane's rows, four blocks to a dword; rows and blocks that are
+  // not there read as 0 (2^-127, against values of zero).
   const int frow = lane & 31;
+  uint32_t osa[FM], osb[FN];
 #pragma unroll
-  for (int i = 0; i < FM; ++i)
-    osa[i] = (uint32_t)((min(wm * WTM + i * 32 + frow, ra_rows - 1) >> g.sha) * g.ldsa);
+  for (int i = 0; i < FM; ++i) osa[i] = (uint32_t)(((wm * WTM + i * 32 + frow) >> g.sha) * g.ldsa);
 #pragma unroll
-  for (int j = 0; j < FN; ++j)
-    osb[j] = (uint32_t)((min(wn * WTN + j * 32 + frow, rb_rows - 1) >> g.shb) * g.ldsb);
+  for (int j = 0; j < FN; ++j) osb[j] = (uint32_t)(((wn * WTN + j * 32 + frow) >> g.shb) * g.ldsb);
   uint32_t sca[FM], scb[FN], nca[FM], ncb[FN];
-  auto load_scales = [&](int q) __attribute__((always_inline)) {
+  auto load_scales = [&](const F8Item& t, int q) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t ra = make_rsrc(uniform(t.sa), uniform(t.bsa));
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(uniform(t.sb), uniform(t.bsb));
 #pragma unroll
-    for (int i = 0; i < FM; ++i) nca[i] = scales4(psa + osa[i], q, nkb, g.dwa);
+    for (int i = 0; i < FM; ++i) nca[i] = scales4<kDw>(ra, osa[i] + 4 * q, t.nkb - 4 * q);
 #pragma unroll
-    for (int j = 0; j < FN; ++j) ncb[j] = scales4(psb + osb[j], q, nkb, g.dwb);
+    for (int j = 0; j < FN; ++j) ncb[j] = scales4<kDw>(rb, osb[j] + 4 * q, t.nkb - 4 * q);
+  };
+  // n: the blocks that the set holds. What stands behind them in the last dword is not
+  // a scale, and could be a NaN.
+  auto take_scales = [&](int n) __attribute__((always_inline)) {
+    const uint32_t there = n >= 4 ? ~0u : (1u << (8 * n)) - 1u;
+#pragma unroll
+    for (int i = 0; i < FM; ++i) sca[i] = nca[i] & there;
+#pragma unroll
+    for (int j = 0; j < FN; ++j) scb[j] = ncb[j] & there;
   };
 
   // fragment (i, step t): row i * 32 + frow, chunks of step t; one offset per step and chunk
@@ -441,14 +489,12 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   };
 
   f32x16 acc[FM][FN];
-#pragma unroll
-  for (int i = 0; i < FM; ++i)
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
-  auto compute = [&](int in, auto pos) __attribute__((always_inline)) {
+  auto compute = [&](int in, auto pos, auto first) __attribute__((always_inline)) {
     constexpr int P = decltype(pos)::value;  // the block's byte in the scale dwords
+    constexpr bool kFirst = decltype(first)::value;
+    f32x16 zero;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero[r] = 0.f;
     if constexpr (kWide) {
       bf16x8 b[FN][2];
 #pragma unroll
@@ -460,36 +506,49 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
-          for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j][h], a[h], acc[i][j]);
+          for (int j = 0; j < FN; ++j) acc[i][j] = mfma32(b[j][h], a[h], kFirst && h == 0 ? zero : acc[i][j]);
       }
     } else {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
         for (int j = 0; j < FN; ++j)
-          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[in][j], fa[in][i], acc[i][j], 0, 0, P,
-                                                                     (int)scb[j], P, (int)sca[i]);
+          acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+              fb[in][j], fa[in][i], kFirst ? zero : acc[i][j], 0, 0, P, (int)scb[j], P, (int)sca[i]);
     }
   };
 
   // Stage kt: every step reads the next one's fragments while its MFMAs run. The
   // last step's fragments are in registers when the workgroup meets, so the stage's
-  // buffer is free for stage kt + 2 and the first fragments of kt + 1 (whose DMA has
-  // had a whole stage to land) are read under the last step's MFMAs.
-  auto stage = [&](int kt, auto pos) __attribute__((always_inline)) {
-    uint8_t* cur = decltype(pos)::value % 2 == 0 ? st0 : st1;
-    uint8_t* nxt = decltype(pos)::value % 2 == 0 ? st1 : st0;
+  // buffer is free for the stage after next (its own item's or the next one's), and
+  // the first fragments of the next stage, whose DMA has had a whole stage to land,
+  // are read under the last step's MFMAs. (No branch stands between MFMAs: the
+  // compiler would move those before it to the ones behind it.)
+  F8Item cur = f8_item<BM, BN>(g, item), nxt = cur;
+  int stages = 0;  // of the current item: an even number, the last one of zeros with an odd one of blocks
+  auto stage = [&](int kt, auto pos, auto first, auto wait) __attribute__((always_inline)) {
+    uint8_t* here = decltype(pos)::value % 2 == 0 ? st0 : st1;
+    uint8_t* there = decltype(pos)::value % 2 == 0 ? st1 : st0;
 #pragma unroll
     for (int t = 0; t < NS; ++t) {
       if (t + 1 < NS) {
-        read(cur, t + 1, (t + 1) & 1);
+        read(here, t + 1, (t + 1) & 1);
       } else {
-        wait_vm<0>();
+        wait_vm<decltype(wait)::value>();
         __syncthreads();
-        issue(cur, kt + 2);
-        read(nxt, 0, 0);  // (behind the last stage: not used)
+        const bool own = kt + 2 < stages;
+        F8Item ahead = cur;
+        ahead.a = own ? cur.a : nxt.a;
+        ahead.b = own ? cur.b : nxt.b;
+        ahead.ba = own ? cur.ba : nxt.ba;
+        ahead.bb = own ? cur.bb : nxt.bb;
+        ahead.kb0 = own ? cur.kb0 : nxt.kb0;
+        ahead.nkb = own ? cur.nkb : nxt.nkb;
+        issue(here, ahead, own ? kt + 2 : kt + 2 - stages);
+        read(there, 0, 0);
       }
-      compute(t & 1, pos);
+      if (t == 0) compute(0, pos, first);
+      else compute(t & 1, pos, std::false_type{});
       if constexpr (!kWide) sched_f8<0, FM * FN, (FM + FN) * CH>();
     }
   };
@@ -497,96 +556,158 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   using P1 = std::integral_constant<int, 1>;
   using P2 = std::integral_constant<int, 2>;
   using P3 = std::integral_constant<int, 3>;
-  auto next_scales = [&](int kt) __attribute__((always_inline)) {
-#pragma unroll
-    for (int i = 0; i < FM; ++i) sca[i] = nca[i];
-#pragma unroll
-    for (int j = 0; j < FN; ++j) scb[j] = ncb[j];
-    load_scales(min((kt >> 2) + 1, (nkb - 1) >> 2));
+  using No = std::false_type;
+  // the scales of the four blocks behind kt's, or the next item's first
+  auto scales_ahead = [&](int kt) __attribute__((always_inline)) {
+    const bool own = kt + 4 < cur.nkb;
+    F8Item t = cur;
+    t.sa = own ? cur.sa : nxt.sa;
+    t.sb = own ? cur.sb : nxt.sb;
+    t.bsa = own ? cur.bsa : nxt.bsa;
+    t.bsb = own ? cur.bsb : nxt.bsb;
+    t.nkb = own ? cur.nkb : nxt.nkb;
+    load_scales(t, own ? (kt >> 2) + 1 : 0);
   };
-  int kt = 0;
-  if (nkb > 0) {
-    load_scales(0);
-    issue(st0, 0);
-    issue(st1, 1);
-    wait_vm<IA + IB>();
-    __syncthreads();
-    read(st0, 0, 0);
-    for (; kt + 4 <= nkb; kt += 4) {
-      next_scales(kt);
-      stage(kt, P0{});
-      stage(kt + 1, P1{});
-      stage(kt + 2, P2{});
-      stage(kt + 3, P3{});
-    }
-    if (kt < nkb) {
-      next_scales(kt);
-      stage(kt, P0{});
-      if (kt + 1 < nkb) {
-        stage(kt + 1, P1{});
-        if (kt + 2 < nkb) stage(kt + 2, P2{});
-      }
-    }
-  }
+  constexpr int kScales = (FM + FN) * (kDw ? 1 : 4);       // loads of one set of scales
+  constexpr int kStores = FM * (sizeof(OutT) / 2) * PITCH / 32;  // stores of a whole tile, 64 lanes of 16 bytes each
 
-  const int g4 = (lane >> 5) * 4;
-  if (g.ws) {
-    float* W = g.ws + (int64_t)split * g.M * g.ldw;
-#pragma unroll
-    for (int i = 0; i < FM; ++i) {
-      const int m = m0 + wm * WTM + i * 32 + frow;
-      if (m >= g.M) continue;
-#pragma unroll
-      for (int j = 0; j < FN; ++j)
-#pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          const int n = n0 + wn * WTN + j * 32 + q * 8 + g4;
-          if (n < g.N)
-            *reinterpret_cast<f32x4*>(W + (int64_t)m * g.ldw + n) =
-                f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
-        }
-    }
-    return;
-  }
-  // Each wave passes 32 rows at a time through its own LDS slab and stores rows
-  // in 16-byte pieces (a lane's own results are pieces of 32 different rows).
+  load_scales(cur, 0);
+  issue(st0, cur, 0);
+  issue(st1, cur, 1);
+  wait_vm<0>();  // both: the first stage's wait counts on the stores of an item before it
   __syncthreads();
-  constexpr int PITCH = WTN * (int)sizeof(OutT), CPR = PITCH / 16, EPC = 16 / (int)sizeof(OutT), RPI = 64 / CPR;
-  static_assert(NWV * 32 * PITCH <= STAGE, "the slabs fit the first stage");
-  static_assert(CPR <= 64, "a row is one instruction's pieces at most");
-  uint8_t* wl = st0 + wave * 32 * PITCH;
-#pragma unroll
-  for (int i = 0; i < FM; ++i) {
-#pragma unroll
-    for (int j = 0; j < FN; ++j)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int cb = (j * 32 + q * 8 + g4) * (int)sizeof(OutT);
-        uint8_t* at = wl + frow * PITCH + (((cb >> 4) ^ (frow & (CPR - 1))) << 4) + (cb & 15);
-        const float x0 = acc[i][j][4 * q], x1 = acc[i][j][4 * q + 1], x2 = acc[i][j][4 * q + 2],
-                    x3 = acc[i][j][4 * q + 3];
-        if constexpr (sizeof(OutT) == 2) *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
-        else *reinterpret_cast<f32x4*>(at) = f32x4{x0, x1, x2, x3};
+  take_scales(cur.nkb);
+  read(st0, 0, 0);
+  for (;;) {
+    const int next = item + wgs;
+    if (next < last) {
+      nxt = f8_item<BM, BN>(g, next);
+    } else {
+      nxt.nkb = 0;
+      nxt.bsa = nxt.bsb = 0;
+    }
+    stages = (cur.nkb + 1) & ~1;
+    // Behind this stage's DMA lie the last item's stores and this set of scales (a tile
+    // at an edge has waited for its stores itself).
+    scales_ahead(0);
+    stage(0, P0{}, std::true_type{}, std::integral_constant<int, (kScales + kStores < 63 ? kScales + kStores : 63)>{});
+    stage(1, P1{}, No{}, P0{});
+    if (stages > 2) {
+      stage(2, P2{}, No{}, P0{});
+      stage(3, P3{}, No{}, P0{});
+      int kt = 4;
+      for (; kt + 4 <= stages; kt += 4) {
+        take_scales(cur.nkb - kt);
+        scales_ahead(kt);
+        stage(kt, P0{}, No{}, P0{});
+        stage(kt + 1, P1{}, No{}, P0{});
+        stage(kt + 2, P2{}, No{}, P0{});
+        stage(kt + 3, P3{}, No{}, P0{});
       }
-#pragma unroll
-    for (int it = 0; it < 32 / RPI; ++it) {
-      const int r = it * RPI + lane / CPR, ch = lane % CPR;
-      const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
-      const int m = m0 + wm * WTM + i * 32 + r;
-      const int n = n0 + wn * WTN + ch * EPC;
-      if (m >= g.M || n >= g.N) continue;
-      OutT* dst = reinterpret_cast<OutT*>(g.C) + (int64_t)m * g.ldc + n;
-      if (n + EPC <= g.N) {
-        __builtin_nontemporal_store(val, reinterpret_cast<u32x4*>(dst));
-      } else {
-#pragma unroll
-        for (int k = 0; k < EPC; ++k) {
-          if (n + k >= g.N) break;
-          if constexpr (sizeof(OutT) == 2) dst[k] = (OutT)(val[k >> 1] >> (16 * (k & 1)));
-          else dst[k] = __uint_as_float(val[k]);
-        }
+      if (kt < stages) {
+        take_scales(cur.nkb - kt);
+        scales_ahead(kt);
+        stage(kt, P0{}, No{}, P0{});
+        stage(kt + 1, P1{}, No{}, P0{});
       }
     }
+    take_scales(nxt.nkb);  // landed by the last stage's wait: nothing of the next item waits for the stores below
+
+    // Each wave passes 32 rows of PITCH bytes at a time through its own LDS slab and
+    // stores rows in 16-byte pieces (a lane's own results are pieces of 32 rows).
+    uint8_t* wl = slabs + wave * 32 * PITCH;
+    // (hidden from the compiler, which would keep every address of the stores across
+    // the loop over items, in registers that the fragments need)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int fr = ln & 31, g4 = (ln >> 5) * 4;
+    const bool whole = cur.m0 + BM <= g.M && cur.n0 + BN <= g.N;
+    auto put = [&]() __attribute__((always_inline)) {
+      using T = OutT;
+      constexpr int SC = PITCH / (int)sizeof(T);                 // columns of a slab
+      constexpr int CPR = PITCH / 16, EPC = 16 / (int)sizeof(T), RPI = 64 / CPR;
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int c0 = 0; c0 < WTN; c0 += SC) {
+#pragma unroll
+          for (int j = c0 / 32; j < (c0 + SC) / 32; ++j) {
+            asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const int cb = (j * 32 - c0 + q * 8 + g4) * (int)sizeof(T);
+              uint8_t* at = wl + fr * PITCH + (((cb >> 4) ^ (fr & (CPR - 1))) << 4) + (cb & 15);
+              const float x0 = acc[i][j][4 * q], x1 = acc[i][j][4 * q + 1], x2 = acc[i][j][4 * q + 2],
+                          x3 = acc[i][j][4 * q + 3];
+              if constexpr (sizeof(T) == 2)
+                *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
+              else
+                *reinterpret_cast<f32x4*>(at) = f32x4{x0, x1, x2, x3};
+            }
+          }
+          const int r0 = ln / CPR, ch = ln % CPR;
+          if (whole) {
+            // rows behind one another from a 64-bit base, 32-bit offsets within the tile
+            const int mrow = wm * WTM + i * 32, ncol = wn * WTN + c0;
+            const __amdgpu_buffer_rsrc_t rc =
+                make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
+                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), 0xffffffffu);
+            const uint32_t vo = (uint32_t)((r0 * g.ldc + ch * EPC) * (int64_t)sizeof(T));
+#pragma unroll
+            for (int it = 0; it < 32 / RPI; ++it) {
+              const int r = it * RPI + r0;
+              const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  val, rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
+            }
+          } else {
+#pragma unroll 1
+            for (int it = 0; it < 32 / RPI; ++it) {
+              const int r = it * RPI + r0;
+              const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
+              const int m = cur.m0 + wm * WTM + i * 32 + r;
+              const int n = cur.n0 + wn * WTN + c0 + ch * EPC;
+              if (m >= g.M || n >= g.N) continue;
+              T* dst = reinterpret_cast<T*>(g.C) + (int64_t)m * g.ldc + n;
+              if (n + EPC <= g.N) {
+                *reinterpret_cast<u32x4*>(dst) = val;
+              } else {
+#pragma unroll
+                for (int k = 0; k < EPC; ++k) {
+                  if (n + k >= g.N) break;
+                  if constexpr (sizeof(T) == 2) dst[k] = (T)(val[k >> 1] >> (16 * (k & 1)));
+                  else dst[k] = __uint_as_float(val[k]);
+                }
+              }
+            }
+          }
+        }
+    };
+    if (g.ws) {
+      float* W = g.ws + (int64_t)cur.split * g.M * g.ldw;
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int m = cur.m0 + wm * WTM + i * 32 + fr;
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          asm volatile("" : "+v"(acc[i][j]));
+          if (m >= g.M) continue;
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const int n = cur.n0 + wn * WTN + j * 32 + q * 8 + g4;
+            if (n < g.N)
+              *reinterpret_cast<f32x4*>(W + (int64_t)m * g.ldw + n) =
+                  f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+          }
+        }
+      }
+    } else {
+      put();
+    }
+    if (g.ws || !whole || next >= last) wait_vm<0>();  // (no DMA is in flight when the workgroup ends)
+    if (next >= last) break;
+    item = next;
+    cur = nxt;
   }
 }
 
@@ -642,11 +763,16 @@ int64_t f8_ldw(int N) { return ((int64_t)N + 3) / 4 * 4; }
 
 template <typename OutT>
 void launch_f8(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
-  const dim3 grid((unsigned)(p.tiles * p.splits));
-  if (p.huge)
-    hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT>), grid, dim3(256), 0, st, g);
-  else
-    hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT>), grid, dim3(256), 0, st, g);
+  const int cus = cu_count();
+  if (p.huge) {
+    const dim3 grid((unsigned)std::min(g.items, cus));
+    if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT, true>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT, false>), grid, dim3(256), 0, st, g);
+  } else {
+    const dim3 grid((unsigned)std::min(g.items, 2 * cus));
+    if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT, true>), grid, dim3(256), 0, st, g);
+    else hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT, false>), grid, dim3(256), 0, st, g);
+  }
   if (p.splits > 1)
     hipLaunchKernelGGL((f8_reduce_kernel<OutT>),
                        dim3((unsigned)((g.N + 255) / 256), (unsigned)std::min<int64_t>(((int64_t)g.M + 3) / 4, 65535)),
@@ -732,15 +858,17 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
   if (((uintptr_t)C & 15) || ldc % 8) return nl_set_error(NL_EALIGN, "gemm_fp8: C needs 16-byte aligned rows");
   const int64_t Kp = ((int64_t)K + kB - 1) / kB * kB;
   // 256 rows of a tile are addressed with 31-bit offsets
-  if (lda > INT32_MAX / 256 || ldb > INT32_MAX / 256 || Kp > INT32_MAX / 256)
+  if (ldc > INT32_MAX / 256 / 4) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of C of 2 million elements and more");
+  if (lda > INT32_MAX / 256 || ldb > INT32_MAX / 256 || ldsa > INT32_MAX / 256 || ldsb > INT32_MAX / 256)
     return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of 8 MiB and more");
   F8Plan p = f8_plan(M, N, K);
   if (p.tiles < 0 || (int64_t)p.tiles * p.splits > INT32_MAX) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: too many tiles");
-  auto dwords = [](const void* s, int64_t ld) { return (int)(ld % 4 == 0 && ((uintptr_t)s & 3) == 0); };
+  auto dwords = [](const void* s, int64_t ld) { return ld % 4 == 0 && ((uintptr_t)s & 3) == 0; };
   GemmF8Args g{M, N, K, (int)Kp,
-               A, lda, scale_a, ldsa, group_a == kB ? 7 : 0, dwords(scale_a, ldsa),
-               B, ldb, scale_b, ldsb, group_b == kB ? 7 : 0, dwords(scale_b, ldsb),
-               C, ldc, nullptr, f8_ldw(N), p.tiles, p.kb_chunk};
+               A, lda, scale_a, ldsa, group_a == kB ? 7 : 0,
+               B, ldb, scale_b, ldsb, group_b == kB ? 7 : 0,
+               dwords(scale_a, ldsa) && dwords(scale_b, ldsb) ? 1 : 0,
+               C, ldc, nullptr, f8_ldw(N), p.tiles, 0, p.kb_chunk};
   if (p.splits > 1) {
     if (ws && ws_bytes >= nl_gemm_fp8_ws_bytes(M, N, K)) {
       if ((uintptr_t)ws & 15) return nl_set_error(NL_EALIGN, "gemm_fp8: workspace not 16-byte aligned");
@@ -750,6 +878,7 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
       g.kb_chunk = (int)(Kp / kB);
     }
   }
+  g.items = p.tiles * p.splits;
   if (c_dtype == NL_DTYPE_F32) launch_f8<float>((hipStream_t)stream, p, g);
   else launch_f8<uint16_t>((hipStream_t)stream, p, g);
   return nl_check_launch("nl_gemm_fp8");
