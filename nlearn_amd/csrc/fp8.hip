@@ -328,14 +328,17 @@ __device__ __forceinline__ typename FragOf<kWide>::type read_frag(const uint8_t*
   }
 }
 
-// One MFMA, then its share of the R fragment reads of the next step.
-template <int M, int NM, int R>
+// One MFMA, then its share of the R fragment reads of the next step and of the D
+// DMA instructions of a stage.
+template <int M, int NM, int R, int D>
 __device__ __forceinline__ void sched_f8() {
   if constexpr (M < NM) {
     __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
     constexpr int lo = M * R / NM, hi = (M + 1) * R / NM;
     if constexpr (hi > lo) __builtin_amdgcn_sched_group_barrier(0x100, hi - lo, 0);
-    sched_f8<M + 1, NM, R>();
+    constexpr int dlo = M * D / NM, dhi = (M + 1) * D / NM;
+    if constexpr (dhi > dlo) __builtin_amdgcn_sched_group_barrier(0x010, dhi - dlo, 0);
+    sched_f8<M + 1, NM, R, D>();
   }
 }
 
@@ -549,7 +552,11 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
       }
       if (t == 0) compute(0, pos, first);
       else compute(t & 1, pos, std::false_type{});
-      if constexpr (!kWide) sched_f8<0, FM * FN, (FM + FN) * CH>();
+      if constexpr (!kWide) {
+        if (t + 1 < NS) sched_f8<0, FM * FN, (FM + FN) * CH, 0>();
+        else sched_f8<0, FM * FN, (FM + FN) * CH, IA + IB>();
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
   using P0 = std::integral_constant<int, 0>;
