@@ -34,6 +34,7 @@ struct Row {
   const u32x4* body;
   int V, head, nbody, eidx;
   u32x4 v[NVEC ? NVEC : 1];
+  float top[NVEC ? NVEC : 1];  // largest of each vector (NaN apart), where row_sums is asked for it
   float xe;  // the loose element
 
   __device__ __forceinline__ void load(const uint16_t* row, int n, int tid) {
@@ -57,15 +58,15 @@ struct Row {
 #pragma unroll
     for (int j = 0; j < NVEC; ++j) asm volatile("" : "+v"(v[j]));
   }
-  // f(vector, index of its first element / 8 in the body) for this thread's vectors
+  // f(vector, index of its first element / 8 in the body, j) for this thread's vectors
   template <class F>
   __device__ __forceinline__ void vectors(int tid, F f) {
     if constexpr (NVEC > 0) {
 #pragma unroll
       for (int j = 0; j < NVEC; ++j)
-        if (j * NT + tid < nbody) f(v[j], j * NT + tid);
+        if (j * NT + tid < nbody) f(v[j], j * NT + tid, j);
     } else {
-      for (int i = tid; i < nbody; i += NT) f(body[i], i);
+      for (int i = tid; i < nbody; i += NT) f(body[i], i, 0);
     }
   }
 };
@@ -75,8 +76,7 @@ struct RowSums {
   float m[NT / kWave], s[NT / kWave];
 };
 
-// (X, S) over the workgroup's row: X = max x and S = sum 2^((x - X) c); xmax is the
-// thread's own max. A NaN makes S NaN; an infinity without one makes both infinite.
+// (X, S) over the workgroup's row: X = max x and S = sum 2^((x - X) c). A NaN makes S NaN; an infinity without one makes both infinite.
 __device__ __forceinline__ float finite_or_0(float m) { return fabsf(m) == INFINITY ? 0.f : m; }
 __device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, float c) {
   const float mn = fmaxf(m, m2);
@@ -88,20 +88,29 @@ __device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, 
 // x c itself would overflow: masks of the type's lowest value stand alone in a row
 __device__ __forceinline__ bool too_large(float m, float c) { return fabsf(m) * c > 1e37f; }
 
-template <int NT, int NVEC>
+// per_wave(thread's max) runs on every wave ahead of the workgroup's barrier.
+__device__ __forceinline__ float max8(const u32x4& v) {
+  float m = fmaxf(bf16_lo(v[0]), bf16_hi(v[0]));
+#pragma unroll
+  for (int q = 1; q < 4; ++q) m = fmaxf(m, fmaxf(bf16_lo(v[q]), bf16_hi(v[q])));
+  return m;
+}
+
+template <bool kTops = false, int NT, int NVEC, class F>
 __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, RowSums<NT>& sm, float& X, float& S,
-                                         float& xmax) {
+                                         F per_wave) {
   float m = r.eidx >= 0 ? r.xe : -INFINITY;
   float s;
   if constexpr (NVEC > 0) {
-    r.vectors(tid, [&](const u32x4& v, int) {
-#pragma unroll
-      for (int q = 0; q < 4; ++q) m = fmaxf(m, fmaxf(bf16_lo(v[q]), bf16_hi(v[q])));
+    r.vectors(tid, [&](const u32x4& v, int, int j) {
+      const float t = max8(v);
+      if constexpr (kTops) r.top[j] = t;
+      m = fmaxf(m, t);
     });
     r.fence();
     auto sum = [&](auto f) __attribute__((always_inline)) {
       s = r.eidx >= 0 ? fast_exp2(f(r.xe)) : 0.f;
-      r.vectors(tid, [&](const u32x4& v, int) {
+      r.vectors(tid, [&](const u32x4& v, int, int) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           s += fast_exp2(f(bf16_lo(v[q])));
@@ -123,10 +132,8 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
     // one read: the running maximum moves once per vector at most
     float at = finite_or_0(m);
     s = r.eidx >= 0 ? fast_exp2((r.xe - at) * c) : 0.f;
-    r.vectors(tid, [&](const u32x4& v, int) {
-      float mv = -INFINITY;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) mv = fmaxf(mv, fmaxf(bf16_lo(v[q]), bf16_hi(v[q])));
+    r.vectors(tid, [&](const u32x4& v, int, int) {
+      const float mv = max8(v);
       if (mv > m) {
         const float to = finite_or_0(mv);
         s *= s == 0.f ? 1.f : fast_exp2((at - to) * c);  // (a sum of 0 has no reference yet)
@@ -140,7 +147,7 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
       }
     });
   }
-  xmax = m;
+  per_wave(m);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float m2 = __shfl_xor(m, o, kWave);
@@ -166,19 +173,28 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
 // The k largest
 // ===========================================================================
 //
-// The k-th largest of the threads' maxima is a bound that at least k elements
-// reach and, with elements in no particular order, hardly more do: those go to
-// LDS as (key, index) and their rank among each other is their place. Rows with
-// more candidates than fit (ties, mostly) find the k-th (key, index) bit by bit,
-// counting over the row.
-
-constexpr int kCand = 1024;
+// Each wave finds the j-th largest of its lanes' maxima, j = ceil(k / waves): at least
+// j of its elements reach that, so at least k of the row's reach the least of the
+// waves' bounds, and with elements in no particular order hardly twice as many do.
+// (Where j is a large part of the 64 lanes, and a row is short, the waves count over
+// all their elements instead.) Those go to LDS as (key, index), a list for each wave,
+// and their rank among each other is their place. A row with more of them than fit
+// (ties, mostly), or with a NaN, goes over the row in memory again.
 
 // bf16 bits as an ordered 16-bit number: -0 as 0, every NaN above infinity
 __device__ __forceinline__ uint32_t order16(uint32_t h) {
   if ((h & 0x7fff) > 0x7f80) return 0xffffu;
   if (h == 0x8000) h = 0;
   return (h & 0x8000) ? (~h & 0xffff) : (h | 0x8000);
+}
+// the number that has this order (-inf below all of them)
+__device__ __forceinline__ float from_order16(uint32_t o) {
+  return o <= 0x7f ? -INFINITY : bf16_to_f32((uint16_t)(o & 0x8000 ? o & 0x7fff : ~o & 0xffff));
+}
+
+// larger key first, then the lower index; the low 16 bits carry the value
+__device__ __forceinline__ unsigned long long entry(uint32_t h, int i) {
+  return ((unsigned long long)order16(h) << 48) | ((unsigned long long)(uint32_t)(~i) << 16) | h;
 }
 
 template <int NT>
@@ -195,102 +211,178 @@ __device__ __forceinline__ int block_count(int n, int tid, int* sm) {
   return n;
 }
 
+// The k largest of the row in memory into cand, exactly k of them. `key`: an order
+// that at least k elements reach.
+template <int NT>
+__device__ __noinline__ void select_in_memory(const uint16_t* row, int V, int k, uint32_t key, int tid, int* cnt,
+                                              int* count, unsigned long long* cand) {
+  Row<NT, 0> r;
+  r.load(row, V, tid);
+  auto above = [&](uint32_t t) {  // elements with a larger order than t
+    int m = r.eidx >= 0 && order16(__float_as_uint(r.xe) >> 16) > t;
+#pragma unroll 4
+    for (int i = tid; i < r.nbody; i += NT) {
+      const u32x4 v = r.body[i];
+#pragma unroll
+      for (int q = 0; q < 4; ++q) m += (order16(v[q] & 0xffffu) > t) + (order16(v[q] >> 16) > t);
+    }
+    return block_count<NT>(m, tid, cnt);
+  };
+  // the k-th largest key: the bound itself where ties are what there is too much of
+  int more = above(key);
+  if (more >= k) {
+    key = 0;
+#pragma unroll 1
+    for (int b = 15; b >= 0; --b)
+      if (above((key | (1u << b)) - 1) >= k) key |= 1u << b;
+    more = above(key);
+  }
+  // its equals in the order of their indices: each thread counts a stretch of the row
+  const int len = (V + NT - 1) / NT, i0 = min(tid * len, V), i1 = min(i0 + len, V);
+  int eq = 0;
+#pragma unroll 4
+  for (int i = i0; i < i1; ++i) eq += order16(row[i]) == key;
+  int before = eq;  // inclusive over the wave's lanes
+#pragma unroll
+  for (int o = 1; o < kWave; o <<= 1) {
+    const int up = __shfl_up(before, o, kWave);
+    if ((tid & (kWave - 1)) >= o) before += up;
+  }
+  __syncthreads();
+  if ((tid & (kWave - 1)) == kWave - 1) cnt[tid / kWave] = before;
+  if (tid == 0) *count = 0;
+  __syncthreads();
+  before -= eq;
+  for (int w = 0; w < tid / kWave; ++w) before += cnt[w];
+  const int want = k - more;  // >= 1 of the equals
+#pragma unroll 1
+  for (int i = i0; i < i1; ++i) {
+    const uint32_t h = row[i], o = order16(h);
+    if (o > key) cand[want + atomicAdd(count, 1)] = entry(h, i);
+    else if (o == key && before < want) cand[before++] = entry(h, i);
+  }
+  __syncthreads();
+}
+
 template <int NT, int NVEC>
 __global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restrict__ logits, int64_t ld, int k,
                                                  float c, uint16_t* __restrict__ values, int32_t* __restrict__ ids,
                                                  float* __restrict__ lse) {
+  constexpr int NW = NT / kWave;
+  constexpr int kCand = NW == 1 ? 512 : 1024;            // candidates that are ranked
+  constexpr int CAP = NW == 1 ? kCand : 2 * kCand / NW;  // and that a wave's list holds
   __shared__ RowSums<NT> sums;
-  __shared__ uint32_t tmax[NT];
-  __shared__ unsigned long long cand[kCand];
+  __shared__ uint32_t bounds[NW];
+  __shared__ unsigned long long list[NW == 1 ? 1 : NW][NW == 1 ? 1 : CAP];
+  __shared__ __attribute__((aligned(16))) unsigned long long cand[kCand];
   __shared__ int count;
-  __shared__ int cnt[NT / kWave];
+  __shared__ int cnt[NW];
   const int64_t row = blockIdx.x;
-  const int tid = threadIdx.x, lane = tid & (kWave - 1);
+  const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
+  const uint16_t* xrow = logits + row * ld;
   Row<NT, NVEC> r;
-  r.load(logits + row * ld, V, tid);
-  float X, S, xm;
-  row_sums<NT, NVEC>(r, c, tid, sums, X, S, xm);
-  if (tid == 0) {
-    lse[row] = (float)(((double)X * c + log2((double)S)) * 0.69314718055994530942);
-    count = 0;
-  }
-  // the bound: largest T16 with k thread maxima at or above it (0 if there are fewer threads)
-  tmax[tid] = order16(__float_as_uint(xm) >> 16);
-  __syncthreads();
-  uint32_t mine[NT / kWave];
+  r.load(xrow, V, tid);
+  float X, S;
+  row_sums<true>(r, c, tid, sums, X, S, [&](float m) __attribute__((always_inline)) {
+    const int want = (k + NW - 1) / NW;
+    uint32_t bound = 0;
+    if (NVEC > 0 && NVEC * NT <= 512 && want > 16) {
+#pragma unroll 1
+      for (int b = 15; b >= 0; --b) {
+        const float t = from_order16(bound | (1u << b));
+        int n = __popcll(__ballot(r.eidx >= 0 && r.xe >= t));
+        r.vectors(tid, [&](const u32x4& v, int, int) {
 #pragma unroll
-  for (int w = 0; w < NT / kWave; ++w) mine[w] = tmax[w * kWave + lane];
-  uint32_t bound = 0;
+          for (int q = 0; q < 4; ++q) n += __popcll(__ballot(bf16_lo(v[q]) >= t)) + __popcll(__ballot(bf16_hi(v[q]) >= t));
+        });
+        // (a lane without the vector counts nothing: take the largest, lane 0 has every one)
+        if (__builtin_amdgcn_readfirstlane(n) >= want) bound |= 1u << b;
+      }
+    } else {
+      const uint32_t mine = order16(__float_as_uint(m) >> 16);
 #pragma unroll
-  for (int b = 15; b >= 0; --b) {
-    const uint32_t t = bound | (1u << b);
-    int n = 0;
+      for (int b = 15; b >= 0; --b)
+        if (__popcll(__ballot(mine >= (bound | (1u << b)))) >= want) bound |= 1u << b;
+    }
+    if (lane == 0) bounds[wave] = bound;
+  });
+  if constexpr (NT == kWave) __syncthreads();
+  uint32_t bound = bounds[0];
 #pragma unroll
-    for (int w = 0; w < NT / kWave; ++w) n += __popcll(__ballot(mine[w] >= t));
-    if (n >= k) bound = t;
-  }
-  const uint32_t row_bits = bound & 0x8000 ? bound & 0x7fff : ~bound & 0xffff;
-  const float fb = bound <= 0x7f ? -INFINITY : bf16_to_f32((uint16_t)row_bits);  // order16(-inf) = 0x7f
-  auto each = [&](auto f) __attribute__((always_inline)) {  // f(bits, index) over this thread's elements
-    if (r.eidx >= 0) f(__float_as_uint(r.xe) >> 16, r.eidx);
-    r.vectors(tid, [&](const u32x4& v, int i) {
+  for (int w = 1; w < NW; ++w) bound = min(bound, bounds[w]);
+  bound = __builtin_amdgcn_readfirstlane(bound);
+  const float fb = from_order16(bound);
+  int n = 0;  // of this wave's list
+  auto offer = [&](bool has, uint32_t h, int i) __attribute__((always_inline)) {
+    const bool in = has && __uint_as_float(h << 16) >= fb;
+    const unsigned long long mask = __ballot(in);
+    if (mask == 0) return;
+    const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+    if (in && at < CAP) (NW == 1 ? cand : list[wave])[at] = entry(h, i);
+    n += __popcll(mask);
+  };
+  if (S == S) {
+    offer(r.eidx >= 0, __float_as_uint(r.xe) >> 16, r.eidx);
+    auto vec = [&](bool has, const u32x4& v, int i) __attribute__((always_inline)) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        f(v[q] & 0xffffu, r.head + i * 8 + 2 * q);
-        f(v[q] >> 16, r.head + i * 8 + 2 * q + 1);
+        offer(has, v[q] & 0xffffu, r.head + i * 8 + 2 * q);
+        offer(has, v[q] >> 16, r.head + i * 8 + 2 * q + 1);
       }
-    });
-  };
-  // a NaN is no less than anything
-  each([&](uint32_t h, int i) {
-    if (!(__uint_as_float(h << 16) < fb)) {
-      const int at = atomicAdd(&count, 1);
-      if (at < kCand)
-        cand[at] = ((unsigned long long)order16(h) << 48) | ((unsigned long long)(uint32_t)(~i) << 16) | h;
+    };
+    if constexpr (NVEC > 0) {
+#pragma unroll
+      for (int j = 0; j < NVEC; ++j) {
+        const bool has = j * NT + tid < r.nbody && r.top[j] >= fb;
+        if (__ballot(has)) vec(has, r.v[j], j * NT + tid);
+      }
+    } else {
+      for (int i0 = wave * kWave; i0 < r.nbody; i0 += NT) {
+        const int i = i0 + lane;
+        u32x4 v = {0, 0, 0, 0};
+        if (i < r.nbody) v = r.body[i];
+        const bool has = i < r.nbody && max8(v) >= fb;
+        if (__ballot(has)) vec(has, v, i);
+      }
     }
-  });
-  __syncthreads();
-  int n = count;
-  if (n > kCand) {
-    // the k-th largest key, then the index up to which its equals are in
-    uint32_t key = 0;
-    for (int b = 15; b >= 0; --b) {
-      const uint32_t t = key | (1u << b);
-      int m = 0;
-      each([&](uint32_t h, int) { m += order16(h) >= t; });
-      if (block_count<NT>(m, tid, cnt) >= k) key = t;
-    }
-    int above = 0;
-    each([&](uint32_t h, int) { above += order16(h) > key; });
-    const int want = k - block_count<NT>(above, tid, cnt);  // >= 1 of the equal ones
-    int lim = 0;                                            // largest index with fewer than `want` equals below it
-    for (int b = 30; b >= 0; --b) {
-      const int t = lim | (1 << b);
-      if (t >= V) continue;
-      int m = 0;
-      each([&](uint32_t h, int i) { m += order16(h) == key && i < t; });
-      if (block_count<NT>(m, tid, cnt) < want) lim = t;
-    }
-    __syncthreads();
-    if (tid == 0) count = 0;
-    __syncthreads();
-    each([&](uint32_t h, int i) {
-      const uint32_t o = order16(h);
-      if (o > key || (o == key && i <= lim))
-        cand[atomicAdd(&count, 1)] = ((unsigned long long)o << 48) | ((unsigned long long)(uint32_t)(~i) << 16) | h;
-    });
-    __syncthreads();
-    n = count;  // k
+  } else {
+    n = CAP + 1;
   }
-  for (int i = tid; i < n; i += NT) {
+  if (lane == 0) cnt[wave] = n;
+  __syncthreads();
+  int total = 0, before = 0;
+  bool fits = true;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int m = cnt[w];
+    if (w < wave) before += m;
+    total += m;
+    fits &= m <= CAP;
+  }
+  if (fits && total <= kCand) {
+    if constexpr (NW > 1) {
+      for (int i = lane; i < n; i += kWave) cand[before + i] = list[wave][i];
+      __syncthreads();
+    }
+  } else {
+    select_in_memory<NT>(xrow, V, k, S == S ? bound : 0, tid, cnt, &count, cand);
+    total = k;
+  }
+  // rank of each candidate, by as many threads as there are for one
+  int per = 1;
+  while (per < 16 && total * per * 2 <= NT) per *= 2;
+  for (int i = tid / per; i < total; i += NT / per) {
     const unsigned long long me = cand[i];
     int rank = 0;
-    for (int j = 0; j < n; ++j) rank += cand[j] > me;
-    if (rank < k) {
+#pragma unroll 4
+    for (int j = tid % per; j < total; j += per) rank += cand[j] > me;
+    for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o, kWave);
+    if (tid % per == 0 && rank < k) {
       values[row * k + rank] = (uint16_t)me;
       ids[row * k + rank] = (int32_t)~(uint32_t)(me >> 16);
     }
   }
+  if (tid == NT - 1) lse[row] = (float)(((double)X * c + log2((double)S)) * 0.69314718055994530942);
 }
 
 // ===========================================================================
@@ -384,8 +476,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     if (__ballot(bad)) S = __builtin_nanf("");
     if (lane == 0) sS = S;
   }
-  float X, S, xm;
-  row_sums<NT, NVEC>(r, a.c, tid, sums, X, S, xm);
+  float X, S;
+  row_sums(r, a.c, tid, sums, X, S, [](float) {});
   if constexpr (NT == kWave) __syncthreads();
   const float mass = sS;
   const bool none = mass == 0.f;  // no entry, or none with any weight
@@ -410,7 +502,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       return fast_exp2(large ? (x - X) * a.c - lS : __builtin_fmaf(x, a.c, nb)) * w;
     };
     if (none) {  // whatever the row holds
-      r.vectors(tid, [&](const u32x4&, int i) {
+      r.vectors(tid, [&](const u32x4&, int i, int) {
         if (a.same_phase) {
           reinterpret_cast<u32x4*>(drow + r.head)[i] = u32x4{0, 0, 0, 0};
         } else {
@@ -421,7 +513,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       if (r.eidx >= 0) drow[r.eidx] = 0;
       return;
     }
-    r.vectors(tid, [&](const u32x4& v, int i) {
+    r.vectors(tid, [&](const u32x4& v, int i, int) {
       u32x4 o;
 #pragma unroll
       for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(grad(bf16_lo(v[q])), grad(bf16_hi(v[q])));
@@ -453,7 +545,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 
 // Threads and vectors per thread for a row of V elements. A workgroup holds 8 NT
 // NVEC of them (less up to 7 before the first vector).
-#define NL_ROW_SIZES(X) X(64, 1) X(256, 1) X(256, 2) X(512, 2) X(512, 4) X(512, 7) X(512, 10) X(512, 13) X(1024, 9) X(1024, 13)
+#define NL_ROW_SIZES(X) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(512, 2) X(512, 4) X(512, 7) X(512, 10) X(512, 13) X(1024, 9) X(1024, 13)
 
 void launch_top(hipStream_t st, int M, int V, const uint16_t* x, int64_t ld, int k, float c, uint16_t* values,
                 int32_t* ids, float* lse) {
