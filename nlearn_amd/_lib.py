@@ -153,7 +153,7 @@ def set_probe(probe) -> None:
 
 def call(name: str, *args) -> None:
     """Invoke an ``nl_*`` status-returning entry point; raise NlError on failure."""
-    lib = load()
+    lib = _lib if _lib is not None else load()
     ctx = _probe(name, args) if _probe is not None else None
     if ctx is None:
         rc = getattr(lib, name)(*args)
@@ -177,16 +177,24 @@ def stream_of(t) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
+_cuda = None  # (torch.cuda, current device, current raw stream of a device), looked up once
+
+
 def call_on(t, name: str, *args) -> None:
     """``call(name, stream, *args)`` on the current stream of the tensor ``t``'s
     device, with that device current for the launch."""
-    import torch
+    global _cuda
+    if _cuda is None:
+        import torch
 
+        _cuda = (torch.cuda, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
     index = t.get_device()
-    if index < 0 or index == torch._C._cuda_getDevice():
+    if index < 0:
         return call(name, stream_of(t), *args)
-    with torch.cuda.device(index):
-        return call(name, stream_of(t), *args)
+    if index == _cuda[1]():
+        return call(name, _cuda[2](index), *args)
+    with _cuda[0].device(index):
+        return call(name, _cuda[2](index), *args)
 
 
 def ws_bytes(batch: int, heads: int, seq: int) -> int:

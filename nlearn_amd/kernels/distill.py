@@ -23,17 +23,23 @@ MAX_K = 256  # NL_TOP_MAX_K
 
 
 def _rows(what: str, logits: torch.Tensor) -> torch.Tensor:
-    if logits.dim() < 1 or logits.dtype != _BF16:
+    dim = logits.dim()
+    if dim < 1 or logits.dtype is not _BF16:
         raise ValueError(f"{what}: logits must be bfloat16 with the vocabulary as last dimension")
     V = logits.shape[-1]
     if V < 1:
         raise ValueError(f"{what}: an empty vocabulary")
-    x = logits.reshape(-1, V)
-    if x.stride(-1) != 1 and V > 1:
+    x = logits if dim == 2 else logits.reshape(-1, V)
+    s0, s1 = x.stride()
+    if s1 != 1 and V > 1:
         raise ValueError(f"{what}: logits need a unit stride along the vocabulary")
-    if x.shape[0] > 1 and x.stride(0) < V:  # rows sharing memory (a broadcast view)
+    if s0 < V and x.shape[0] > 1:  # rows sharing memory (a broadcast view)
         x = x.contiguous()
     return x
+
+
+def _dense(t: torch.Tensor, k: int) -> torch.Tensor:
+    return t if t.dim() == 2 and t.is_contiguous() else t.reshape(-1, k).contiguous()
 
 
 def _temperature(what: str, t) -> float:
@@ -50,7 +56,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
 
     exp(values / temperature - lse) are the row's probabilities. NaN counts as
     larger than any number. 1 <= k <= min(V, 256). Not differentiable."""
-    x = _rows("top_logits", logits.detach())
+    x = _rows("top_logits", logits)
     T = _temperature("top_logits", temperature)
     M, V = x.shape
     if not 1 <= k <= min(V, MAX_K):
@@ -117,10 +123,10 @@ def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch
     x = _rows("distill_cross_entropy", logits)
     T = _temperature("distill_cross_entropy", temperature)
     M, V = x.shape
-    lead = tuple(logits.shape[:-1])
-    if ids.dim() < 1 or tuple(ids.shape[:-1]) != lead or tuple(values.shape) != tuple(ids.shape):
+    lead = logits.shape[:-1]
+    if ids.dim() < 1 or ids.shape[:-1] != lead or values.shape != ids.shape:
         raise ValueError(f"distill_cross_entropy: ids {tuple(ids.shape)} and values {tuple(values.shape)} must both be "
-                         f"{lead} + (k,)")
+                         f"{tuple(lead)} + (k,)")
     k = ids.shape[-1]
     if not 1 <= k <= MAX_K:
         raise ValueError(f"distill_cross_entropy: need 1 <= k <= {MAX_K}, got {k}")
@@ -131,13 +137,15 @@ def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch
     if values.requires_grad or (lse is not None and lse.requires_grad):
         raise ValueError("distill_cross_entropy: the teacher gets no gradient (detach values and lse)")
     if lse is not None:
-        if lse.dtype != _F32 or tuple(lse.shape) != lead:
-            raise ValueError(f"distill_cross_entropy: lse must be float32 of shape {lead}")
-        lse = lse.reshape(-1).contiguous()
+        if lse.dtype is not _F32 or lse.shape != lead:
+            raise ValueError(f"distill_cross_entropy: lse must be float32 of shape {tuple(lead)}")
+        if lse.dim() != 1 or not lse.is_contiguous():
+            lse = lse.reshape(-1).contiguous()
     if inplace and x.data_ptr() != logits.data_ptr():
         raise ValueError("distill_cross_entropy: inplace needs logits whose rows can be written where they are")
-    ids, values = ids.reshape(-1, k).contiguous(), values.reshape(-1, k).contiguous()
-    _check_device(x, ids, values, *(() if lse is None else (lse,)))
-    if any(t.device != x.device for t in (ids, values) + (() if lse is None else (lse,))):
+    ids, values = _dense(ids, k), _dense(values, k)
+    _check_device(x, ids, values)
+    dev = x.get_device()
+    if ids.get_device() != dev or values.get_device() != dev or (lse is not None and lse.get_device() != dev):
         raise ValueError("distill_cross_entropy: all tensors must be on the logits' device")
     return _Distill.apply(x, ids, values, lse, T, bool(inplace))

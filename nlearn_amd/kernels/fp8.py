@@ -20,15 +20,12 @@ from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import wgrad
-from .gemm import _BF16, _F32, _check_device, _ld, _rows_disjoint, grad_buffer, padded_empty
+from .gemm import _BF16, _F32, _check_device, _ld, grad_buffer, padded_empty
 
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
+_NONE = (None, 0, None, 0)  # an output that is not wanted
 BLOCK = 128
-
-
-def _blocks(n: int) -> int:
-    return (n + BLOCK - 1) // BLOCK
 
 
 class Fp8Blocks:
@@ -43,28 +40,29 @@ class Fp8Blocks:
     __slots__ = ("q", "scale", "shape", "group")
 
     def __init__(self, q: torch.Tensor, scale: torch.Tensor, shape, group: int = 1):
-        rows, K = (int(n) for n in shape)
-        if group not in (1, BLOCK):
+        rows, K = shape
+        if group != 1 and group != BLOCK:
             raise ValueError(f"Fp8Blocks: a scale holds for 1 or {BLOCK} rows, not {group}")
-        kb = _blocks(K)
-        if q.dtype != _E4M3 or tuple(q.shape) != (rows, kb * BLOCK):
+        kb, sr = (K + BLOCK - 1) // BLOCK, rows if group == 1 else (rows + BLOCK - 1) // BLOCK
+        if q.dtype is not _E4M3 or q.shape != (rows, kb * BLOCK):
             raise ValueError(f"Fp8Blocks: q must be float8_e4m3fn of shape {(rows, kb * BLOCK)}, "
                              f"got {q.dtype} {tuple(q.shape)}")
-        if scale.dtype != _E8M0 or tuple(scale.shape) != ((rows + group - 1) // group, kb):
-            raise ValueError(f"Fp8Blocks: scale must be float8_e8m0fnu of shape {((rows + group - 1) // group, kb)}, "
+        if scale.dtype is not _E8M0 or scale.shape != (sr, kb):
+            raise ValueError(f"Fp8Blocks: scale must be float8_e8m0fnu of shape {(sr, kb)}, "
                              f"got {scale.dtype} {tuple(scale.shape)}")
-        for name, t in (("q", q), ("scale", scale)):
-            if t.numel() and ((t.stride(1) != 1 and t.shape[1] > 1) or not _rows_disjoint(t)):
-                raise ValueError(f"Fp8Blocks: {name} needs a unit column stride and rows of their own")
-        if scale.device != q.device:
+        if scale.get_device() != q.get_device():
             raise ValueError("Fp8Blocks: q and scale are on different devices")
-        if q.numel() and (q.data_ptr() % 16 or (rows > 1 and q.stride(0) % 16)):
-            raise ValueError("Fp8Blocks: q needs 16-byte aligned rows")
+        if rows and K:
+            (q0, q1), (s0, s1) = q.stride(), scale.stride()
+            if q1 != 1 or (rows > 1 and q0 < kb * BLOCK) or (kb > 1 and s1 != 1) or (sr > 1 and s0 < kb):
+                raise ValueError("Fp8Blocks: q and scale need a unit column stride and rows of their own")
+            if q.data_ptr() % 16 or (rows > 1 and q0 % 16):
+                raise ValueError("Fp8Blocks: q needs 16-byte aligned rows")
         self.q, self.scale, self.shape, self.group = q, scale, (rows, K), group
 
     @classmethod
     def empty(cls, rows: int, K: int, group: int, device) -> "Fp8Blocks":
-        kb, sr = _blocks(K), (rows + group - 1) // group
+        kb, sr = (K + BLOCK - 1) // BLOCK, (rows + group - 1) // group
         b = cls.__new__(cls)
         b.q = torch.empty((rows, kb * BLOCK), dtype=_E4M3, device=device)
         # scale rows padded to whole dwords: the product reads four blocks at a time
@@ -89,31 +87,26 @@ def _row_stride(t: torch.Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _source(x: torch.Tensor):
-    """x as the quantiser reads it (fp32 or bf16, unit column stride, rows of their own) and its row stride."""
+def _quantize(x, group: int, along: bool, across: bool):
+    """(x in 8 bits or None, x^T in 8 bits or None), one launch."""
+    if group != 1 and group != BLOCK:
+        raise ValueError(f"quantize_fp8: a scale holds for 1 or {BLOCK} rows, not {group}")
     if x.dim() != 2:
         raise ValueError(f"quantize_fp8: expected a 2-D tensor, got shape {tuple(x.shape)}")
-    _check_device(x)
-    x = x.detach()
-    if x.dtype not in (_BF16, _F32):
+    f32 = x.dtype is _F32
+    if not f32 and x.dtype is not _BF16:
         raise ValueError(f"quantize_fp8: x must be bfloat16 or float32, got {x.dtype}")
-    if (x.shape[1] > 1 and x.stride(1) != 1) or not _rows_disjoint(x):
-        x = x.contiguous()
-    return x, _row_stride(x)
-
-
-def _quantize(x, group: int, along: bool, across: bool):
-    if group not in (1, BLOCK):
-        raise ValueError(f"quantize_fp8: a scale holds for 1 or {BLOCK} rows, not {group}")
-    x, ldx = _source(x)
-    rows, cols = x.shape
-    a = Fp8Blocks.empty(rows, cols, group, x.device) if along else None
-    t = Fp8Blocks.empty(cols, rows, group, x.device) if across else None
-    none = (None, 0, None, 0)
+    _check_device(x)
+    (rows, cols), (s0, s1) = x.shape, x.stride()
+    if (cols > 1 and s1 != 1) or (rows > 1 and s0 < cols):  # a transposed view, rows that share memory
+        x = x.detach().contiguous()
+        s0 = cols
+    dev = x.device
+    a = Fp8Blocks.empty(rows, cols, group, dev) if along else None
+    t = Fp8Blocks.empty(cols, rows, group, dev) if across else None
     if rows and cols:
-        _lib.call_on(x, "nl_quantize_fp8", rows, cols, x.data_ptr(),
-                  _lib.NL_DTYPE_F32 if x.dtype is _F32 else _lib.NL_DTYPE_BF16, ldx, group,
-                  *(a._abi() if along else none), *(t._abi() if across else none))
+        _lib.call_on(x, "nl_quantize_fp8", rows, cols, x.data_ptr(), 0 if f32 else 1, s0 if rows > 1 else cols, group,
+                     *(a._abi() if along else _NONE), *(t._abi() if across else _NONE))
     return a, t
 
 
@@ -145,10 +138,10 @@ def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | No
     if K != Kb:
         raise ValueError(f"gemm_fp8: inner dimensions differ ({K} vs {Kb})")
     _check_device(a.q, b.q)
-    if a.q.device != b.q.device:
+    if a.q.get_device() != b.q.get_device():
         raise ValueError(f"gemm_fp8: operands on {a.q.device} and {b.q.device}")
     if out is None:
-        if out_dtype not in (_F32, _BF16):
+        if out_dtype is not _F32 and out_dtype is not _BF16:
             raise ValueError("gemm_fp8: output must be float32 or bfloat16")
         out = padded_empty(M, N, out_dtype, a.q.device)
     elif out.dtype not in (_F32, _BF16) or tuple(out.shape) != (M, N) or out.device != a.q.device:
