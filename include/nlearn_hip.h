@@ -493,6 +493,25 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
                 const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b,
                 void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes);
 
+/* y[M][N] = x[M][K] . W[K][N] with both operands quantised first (x in blocks of 1 x
+ * 128 along K, W of 128 x 128), and its gradients from dy[M][N]: dx = dy . W^T (dy in
+ * blocks along N) and dW = x^T . dy (x^T and dy^T in blocks along M), each the product
+ * of the quantised operands. x, W, dy are fp32 or bf16 as nl_quantize_fp8 takes them,
+ * the results fp32 or bf16 as nl_gemm_fp8 writes them. M, K, N > 0.
+ * The forward leaves what the wanted gradients (need_dx, need_dw) read of x and W in
+ * `saved`, in 8 bits; the backward gets the same need_dx, need_dw and, for a gradient
+ * that is not wanted, NULL. One call launches 3 (forward) to 5 kernels; the workspaces
+ * are not needed behind them. saved and ws: 16-byte aligned, of the sizes given here. */
+size_t nl_linear_fp8_saved_bytes(int M, int K, int N, int need_dx, int need_dw);
+size_t nl_linear_fp8_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw);
+int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
+                      const void* W, int w_dtype, int64_t ldw, void* y, int y_dtype, int64_t ldy,
+                      int need_dx, int need_dw, void* saved, size_t saved_bytes, void* ws, size_t ws_bytes);
+int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
+                      const void* saved, size_t saved_bytes, int need_dx, int need_dw,
+                      void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw,
+                      void* ws, size_t ws_bytes);
+
 /* ======================================================================== */
 /* Distillation from a teacher's top logits                                   */
 /* ======================================================================== */
@@ -518,11 +537,12 @@ int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, int64_t ld,
  * (their p add up). A row whose p are all zero, padding alone for instance, has
  * loss 0 and a zero gradient whatever its logits are. An id >= V, or a NaN in a
  * row that has entries, makes that row's loss and gradient NaN.
+ * mean (may be NULL): the mean of the rows' losses, summed as nl_mean_f32 does it.
  * dlogits NULL: the loss alone. dlogits may alias logits (the same address and
  * stride), which it then overwrites. 1 <= k <= NL_TOP_MAX_K. */
 int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k, const void* ids,
                        int ids_64, const void* values, int values_dtype, const float* lse, float temperature,
-                       float* loss, float scale, nl_bf16* dlogits, int64_t ld_dlogits);
+                       float* loss, float* mean, float scale, nl_bf16* dlogits, int64_t ld_dlogits);
 
 #ifdef __cplusplus
 }

@@ -94,7 +94,13 @@ _SIGNATURES = {
     "nl_gemm_fp8_ws_bytes": [_I, _I, _I],
     "nl_gemm_fp8": [_P, _I, _I, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I, _I64, _P, ctypes.c_size_t],
     "nl_top_logits": [_P, _I, _I, _P, _I64, _I, _F, _P, _P, _P],
-    "nl_distill_fwd_bwd": [_P, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _F, _P, _F, _P, _I64],
+    "nl_linear_fp8_saved_bytes": [_I, _I, _I, _I, _I],
+    "nl_linear_fp8_ws_bytes": [_I, _I, _I, _I, _I, _I],
+    "nl_linear_fp8_fwd": [_P, _I, _I, _I, _P, _I, _I64, _P, _I, _I64, _P, _I, _I64, _I, _I, _P, ctypes.c_size_t, _P,
+                          ctypes.c_size_t],
+    "nl_linear_fp8_bwd": [_P, _I, _I, _I, _P, _I, _I64, _P, ctypes.c_size_t, _I, _I, _P, _I, _I64, _P, _I, _I64, _P,
+                          ctypes.c_size_t],
+    "nl_distill_fwd_bwd": [_P, _I, _I, _P, _I64, _I, _P, _I, _P, _I, _P, _F, _P, _P, _F, _P, _I64],
 }
 _RESTYPES = {
     "nl_strerror": ctypes.c_char_p,
@@ -109,6 +115,8 @@ _RESTYPES = {
     "nl_global_norm_ws_bytes": ctypes.c_size_t,
     "nl_embedding_bwd_ws_bytes": ctypes.c_size_t,
     "nl_gemm_fp8_ws_bytes": ctypes.c_size_t,
+    "nl_linear_fp8_saved_bytes": ctypes.c_size_t,
+    "nl_linear_fp8_ws_bytes": ctypes.c_size_t,
 }
 
 EXPORTED = tuple(_SIGNATURES)
@@ -177,24 +185,42 @@ def stream_of(t) -> int:
     return torch._C._cuda_getCurrentRawStream(index)
 
 
-_cuda = None  # (torch.cuda, current device, current raw stream of a device), looked up once
+_cuda = None   # (torch.cuda, current device, current raw stream of a device), looked up once
+_held = None   # the library through calls that keep Python's lock
+
+
+def _load_held():
+    """The library loaded for ``call_on``: a launch returns in a few microseconds,
+    less than handing Python's lock over and back costs on autograd's thread."""
+    global _cuda, _held
+    import torch
+
+    load()
+    _cuda = (torch.cuda, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    held = ctypes.PyDLL(str(LIB_PATH))
+    for name, argtypes in _SIGNATURES.items():
+        fn = getattr(held, name)
+        fn.argtypes = argtypes
+        fn.restype = _RESTYPES.get(name, ctypes.c_int)
+    _held = held
 
 
 def call_on(t, name: str, *args) -> None:
     """``call(name, stream, *args)`` on the current stream of the tensor ``t``'s
     device, with that device current for the launch."""
-    global _cuda
-    if _cuda is None:
-        import torch
-
-        _cuda = (torch.cuda, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
+    if _held is None:
+        _load_held()
     index = t.get_device()
-    if index < 0:
+    if index < 0 or _probe is not None:
         return call(name, stream_of(t), *args)
     if index == _cuda[1]():
-        return call(name, _cuda[2](index), *args)
-    with _cuda[0].device(index):
-        return call(name, _cuda[2](index), *args)
+        rc = getattr(_held, name)(_cuda[2](index), *args)
+    else:
+        with _cuda[0].device(index):
+            rc = getattr(_held, name)(_cuda[2](index), *args)
+    if rc != NL_OK:
+        msg = _held.nl_last_error().decode() or _held.nl_strerror(rc).decode()
+        raise NlError(name, rc, msg)
 
 
 def ws_bytes(batch: int, heads: int, seq: int) -> int:

@@ -600,11 +600,12 @@ extern "C" int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, 
 
 extern "C" int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k,
                                   const void* ids, int ids_64, const void* values, int values_dtype, const float* lse,
-                                  float temperature, float* loss, float scale, nl_bf16* dlogits, int64_t ld_dlogits) {
+                                  float temperature, float* loss, float* mean, float scale, nl_bf16* dlogits,
+                                  int64_t ld_dlogits) {
   if (int rc = check_rows("distill", M, V, logits, ld, k, temperature)) return rc;
   if (values_dtype != NL_DTYPE_F32 && values_dtype != NL_DTYPE_BF16)
     return nl_set_error(NL_EINVAL, "distill: values are fp32 or bf16");
-  if (M == 0) return NL_OK;
+  if (M == 0) return mean ? nl_mean_f32(stream, loss, 0, mean) : NL_OK;
   if (!ids || !values || !loss) return nl_set_error(NL_EINVAL, "distill: null pointer");
   if (dlogits) {
     if (M > 1 && ld_dlogits < V) return nl_set_error(NL_EINVAL, "distill: ld_dlogits < V");
@@ -618,5 +619,6 @@ extern "C" int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* log
                 (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0 && (M == 1 || (ld - ld_dlogits) % 8 == 0)};
   if (dlogits) launch_distill<true>((hipStream_t)stream, M, a);
   else launch_distill<false>((hipStream_t)stream, M, a);
-  return nl_check_launch("nl_distill_fwd_bwd");
+  if (int rc = nl_check_launch("nl_distill_fwd_bwd")) return rc;
+  return mean ? nl_mean_f32(stream, loss, M, mean) : NL_OK;
 }

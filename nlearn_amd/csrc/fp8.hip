@@ -890,3 +890,123 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
   else launch_f8<uint16_t>((hipStream_t)stream, p, g);
   return nl_check_launch("nl_gemm_fp8");
 }
+
+// ===========================================================================
+// linear and its gradients in one call each
+// ===========================================================================
+namespace nl {
+namespace {
+
+// A quantised operand inside a byte buffer: values, then scale rows of whole dwords.
+struct Part {
+  int64_t rows, cols;  // cols: the summed axis
+  int group;
+  int64_t at = 0, sat = 0;
+  int64_t ld() const { return (cols + kB - 1) / kB * kB; }
+  int64_t lds() const { return ((cols + kB - 1) / kB + 3) / 4 * 4; }
+  // places it at `end` (a multiple of 16) and returns the end behind it
+  int64_t place(int64_t end) {
+    at = end;
+    sat = at + rows * ld();
+    return (sat + (rows + group - 1) / group * lds() + 15) / 16 * 16;
+  }
+};
+
+struct LinearParts {
+  Part wb, xt;      // kept for the gradients: W (K, N), X^T (K, M)
+  Part x, wf;       // of the forward: X (M, K), W^T (N, K)
+  Part dy, dyt;     // of the backward: dY (M, N), dY^T (N, M)
+  int64_t saved, fwd, bwd;
+  size_t ws_fwd, ws_dx, ws_dw;
+};
+
+LinearParts linear_parts(int M, int K, int N, bool dx, bool dw) {
+  LinearParts p{};
+  p.wb = {K, N, kB};
+  p.xt = {K, M, 1};
+  p.x = {M, K, 1};
+  p.wf = {N, K, kB};
+  p.dy = {M, N, 1};
+  p.dyt = {N, M, 1};
+  if (dx) p.saved = p.wb.place(p.saved);
+  if (dw) p.saved = p.xt.place(p.saved);
+  p.fwd = p.wf.place(p.x.place(0));
+  if (dx) p.bwd = p.dy.place(p.bwd);
+  if (dw) p.bwd = p.dyt.place(p.bwd);
+  p.ws_fwd = nl_gemm_fp8_ws_bytes(M, N, K);
+  p.ws_dx = dx ? nl_gemm_fp8_ws_bytes(M, K, N) : 0;
+  p.ws_dw = dw ? nl_gemm_fp8_ws_bytes(K, N, M) : 0;
+  return p;
+}
+
+int quantize_into(void* st, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* buf,
+                  const Part* a, uint8_t* tbuf, const Part* t) {
+  return nl_quantize_fp8(st, rows, cols, x, dtype, ldx, a ? a->group : t->group, a ? buf + a->at : nullptr,
+                         a ? a->ld() : 0, a ? buf + a->sat : nullptr, a ? a->lds() : 0, t ? tbuf + t->at : nullptr,
+                         t ? t->ld() : 0, t ? tbuf + t->sat : nullptr, t ? t->lds() : 0);
+}
+
+int product(void* st, const uint8_t* abuf, const Part& a, const uint8_t* bbuf, const Part& b, void* C, int dtype,
+            int64_t ldc, void* ws, size_t wsb) {
+  return nl_gemm_fp8(st, (int)a.rows, (int)b.rows, (int)a.cols, abuf + a.at, a.ld(), abuf + a.sat, a.lds(), a.group,
+                     bbuf + b.at, b.ld(), bbuf + b.sat, b.lds(), b.group, C, dtype, ldc, wsb ? ws : nullptr, wsb);
+}
+
+int check_linear(const char* what, int M, int K, int N, const void* buf, size_t have, int64_t want, const char* name) {
+  if (M < 0 || K < 0 || N < 0) return nl_set_error(NL_EINVAL, std::string(what) + ": need M, K, N >= 0");
+  if (want > 0 && (!buf || have < (size_t)want))
+    return nl_set_error(NL_EINVAL, std::string(what) + ": " + name + " too small");
+  if ((uintptr_t)buf & 15) return nl_set_error(NL_EALIGN, std::string(what) + ": " + name + " not 16-byte aligned");
+  return NL_OK;
+}
+
+}  // namespace
+}  // namespace nl
+
+extern "C" size_t nl_linear_fp8_saved_bytes(int M, int K, int N, int need_dx, int need_dw) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  return (size_t)linear_parts(M, K, N, need_dx != 0, need_dw != 0).saved;
+}
+
+extern "C" size_t nl_linear_fp8_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw) {
+  if (M <= 0 || K <= 0 || N <= 0) return 0;
+  const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
+  return backward ? (size_t)p.bwd + std::max(p.ws_dx, p.ws_dw) : (size_t)p.fwd + p.ws_fwd;
+}
+
+extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
+                                 const void* W, int w_dtype, int64_t ldw, void* y, int y_dtype, int64_t ldy,
+                                 int need_dx, int need_dw, void* saved, size_t saved_bytes, void* ws,
+                                 size_t ws_bytes) {
+  if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_fwd: need M, K, N > 0");
+  const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
+  if (int rc = check_linear("linear_fp8_fwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
+  if (int rc = check_linear("linear_fp8_fwd", M, K, N, ws, ws_bytes, p.fwd + (int64_t)p.ws_fwd, "workspace")) return rc;
+  uint8_t *sv = (uint8_t*)saved, *b = (uint8_t*)ws;
+  if (int rc = quantize_into(stream, W, w_dtype, ldw, K, N, sv, need_dx ? &p.wb : nullptr, b, &p.wf)) return rc;
+  if (int rc = quantize_into(stream, x, x_dtype, ldx, M, K, b, &p.x, sv, need_dw ? &p.xt : nullptr)) return rc;
+  return product(stream, b, p.x, b, p.wf, y, y_dtype, ldy, b + p.fwd, p.ws_fwd);
+}
+
+extern "C" int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
+                                 const void* saved, size_t saved_bytes, int need_dx, int need_dw, void* dx,
+                                 int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws,
+                                 size_t ws_bytes) {
+  if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_bwd: need M, K, N > 0");
+  if (!need_dx && !need_dw) return NL_OK;
+  const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
+  if (int rc = check_linear("linear_fp8_bwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
+  if (int rc = check_linear("linear_fp8_bwd", M, K, N, ws, ws_bytes, p.bwd + (int64_t)std::max(p.ws_dx, p.ws_dw),
+                            "workspace"))
+    return rc;
+  const uint8_t* sv = (const uint8_t*)saved;
+  uint8_t* b = (uint8_t*)ws;
+  if (int rc = quantize_into(stream, dy, dy_dtype, lddy, M, N, b, need_dx ? &p.dy : nullptr, b,
+                             need_dw ? &p.dyt : nullptr))
+    return rc;
+  if (need_dx)
+    if (int rc = product(stream, b, p.dy, sv, p.wb, dx, dx_dtype, lddx, b + p.bwd, p.ws_dx)) return rc;
+  if (need_dw)
+    if (int rc = product(stream, sv, p.xt, b, p.dyt, dW, dw_dtype, lddw, b + p.bwd, p.ws_dw)) return rc;
+  return NL_OK;
+}

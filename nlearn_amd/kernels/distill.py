@@ -76,6 +76,7 @@ class _Distill(torch.autograd.Function):
     def forward(ctx, x, ids, values, lse, T, inplace):
         M, V = x.shape
         loss_rows = torch.empty(M, dtype=_F32, device=x.device)
+        loss = torch.empty((), dtype=_F32, device=x.device)
         d = None
         if ctx.needs_input_grad[0]:
             # rows of the gradient start at the same offsets from 16 bytes as the logits'
@@ -83,11 +84,9 @@ class _Distill(torch.autograd.Function):
         _lib.call_on(x, "nl_distill_fwd_bwd", M, V, x.data_ptr(), _ld(x), ids.shape[1], ids.data_ptr(),
                   int(ids.dtype is torch.int64), values.data_ptr(),
                   _lib.NL_DTYPE_F32 if values.dtype is _F32 else _lib.NL_DTYPE_BF16,
-                  lse.data_ptr() if lse is not None else None, T, loss_rows.data_ptr(), 1.0 / max(M, 1),
+                  lse.data_ptr() if lse is not None else None, T, loss_rows.data_ptr(), loss.data_ptr(), 1.0 / max(M, 1),
                   d.data_ptr() if d is not None else None, _ld(d) if d is not None else 0)
         ctx.d = d
-        loss = torch.empty((), dtype=_F32, device=x.device)
-        _lib.call_on(x, "nl_mean_f32", loss_rows.data_ptr(), M, loss.data_ptr())
         return loss
 
     @staticmethod

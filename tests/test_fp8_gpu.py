@@ -285,7 +285,12 @@ def test_linear_forward_and_gradients(dev, lead, K, N, wdtype):
     W = (torch.from_numpy(_matrix(rng, K, N)).to(dev) * 0.05).to(getattr(torch, wdtype)).requires_grad_(True)
     dy = torch.from_numpy(_matrix(rng, M, N)).to(dev).to(torch.bfloat16).reshape(*lead, N)
     y = linear_fp8(x, W)
+    # each gradient alone is the same as with the other
+    (gx,) = torch.autograd.grad(linear_fp8(x, W.detach()), x, dy)
+    (gW,) = torch.autograd.grad(linear_fp8(x.detach(), W), W, dy)
+    assert torch.equal(linear_fp8(x.detach(), W.detach()), y)
     y.backward(dy)
+    assert torch.equal(gx, x.grad) and torch.equal(gW, W.grad)
     assert y.dtype == torch.bfloat16 and x.grad.dtype == torch.bfloat16 and W.grad.dtype == W.dtype
     x2, dy2 = x.detach().reshape(M, K), dy.reshape(M, N)
     Wq = _quantised(W, 128)
