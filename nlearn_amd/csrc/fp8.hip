@@ -552,11 +552,13 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
       }
       if (t == 0) compute(0, pos, first);
       else compute(t & 1, pos, std::false_type{});
-      if constexpr (!kWide) {
+      if constexpr (kWide) {
+        if (t + 1 == NS) sched_f8<0, 2 * FM * FN, 0, IA + IB>();
+      } else {
         if (t + 1 < NS) sched_f8<0, FM * FN, (FM + FN) * CH, 0>();
         else sched_f8<0, FM * FN, (FM + FN) * CH, IA + IB>();
-        __builtin_amdgcn_sched_barrier(0);
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   using P0 = std::integral_constant<int, 0>;
@@ -758,7 +760,7 @@ F8Plan f8_plan(int M, int N, int K) {
   p.huge = tiles(256) >= 256;
   const int64_t t = tiles(p.huge ? 256 : 128);
   int64_t s = 1;
-  if (!p.huge && t < 256) s = std::max<int64_t>(1, std::min<int64_t>(512 / t, kb / 4));
+  if (!p.huge && t < 256) s = std::max<int64_t>(1, std::min<int64_t>(256 / t, kb / 4));
   const int64_t chunk = s > 1 ? ((kb + s - 1) / s + 3) / 4 * 4 : std::max<int64_t>(kb, 1);
   p.splits = (int)std::max<int64_t>(1, (kb + chunk - 1) / chunk);
   p.kb_chunk = (int)chunk;
