@@ -432,7 +432,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     for (int e = 0; e < kMaxK / kWave; ++e) {
       const int j = e * kWave + lane;
       lp[e] = -INFINITY;
-      if (j >= a.k) continue;
+      if (e * kWave >= a.k || j >= a.k) continue;
       const int64_t at = row * a.k + j;
       const int64_t id = a.ids_64 ? reinterpret_cast<const int64_t*>(a.ids)[at]
                                   : (int64_t)reinterpret_cast<const int32_t*>(a.ids)[at];
@@ -455,7 +455,8 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       const double at = mx == -INFINITY ? 0.0 : mx;
       float s = 0.f;
 #pragma unroll
-      for (int e = 0; e < kMaxK / kWave; ++e) s += exp2_split(lp[e] - at);
+      for (int e = 0; e < kMaxK / kWave; ++e)
+        if (e * kWave < a.k) s += exp2_split(lp[e] - at);
       s = wave_sum(s);
       const double l = s == 0.f ? 0.0 : at + log2((double)s);
 #pragma unroll
@@ -465,6 +466,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 #pragma unroll
     for (int e = 0; e < kMaxK / kWave; ++e) {
       const int j = e * kWave + lane;
+      if (e * kWave >= a.k) continue;
       const float p = exp2_split(lp[e]);
       S += p;
       if (j < a.k) {
@@ -481,6 +483,55 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   if constexpr (NT == kWave) __syncthreads();
   const float mass = sS;
   const bool none = mass == 0.f;  // no entry, or none with any weight
+  if constexpr (kGrad) {
+    uint16_t* drow = a.dz + row * a.ldd;
+    const float w = mass * a.grad;
+    const float lS = fast_log2(S);
+    const float nb = -(X * a.c + lS);
+    const bool large = too_large(finite_or_0(X), a.c);
+    auto write = [&](auto f) __attribute__((always_inline)) {
+      r.vectors(tid, [&](const u32x4& v, int i, int) {
+        u32x4 o;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(f(bf16_lo(v[q])), f(bf16_hi(v[q])));
+        if (a.same_phase) {
+          __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(drow + r.head) + i);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) drow[r.head + i * 8 + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
+        }
+      });
+      if (r.eidx >= 0) drow[r.eidx] = f32_to_bf16(f(r.xe));
+    };
+    auto at = [&](float x) __attribute__((always_inline)) { return fast_exp2(__builtin_fmaf(x, a.c, nb)) * w; };
+    auto at_large = [&](float x) __attribute__((always_inline)) { return fast_exp2((x - X) * a.c - lS) * w; };
+    if (none) write([](float) { return 0.f; });  // whatever the row holds
+    else if (!large) write(at);
+    else write(at_large);
+    if (!none) {
+      // The k entries again, with their p taken off before the one rounding: the first
+      // of equal ids adds up all of them, in a fixed order. A few threads share an entry.
+      __syncthreads();
+      int per = 1;
+      while (per < 16 && a.k * per * 2 <= NT) per *= 2;
+      for (int j = tid / per; j < a.k; j += NT / per) {
+        const int id = sid[j];
+        float p = 0.f;
+        int lead = a.k;
+        for (int i = tid % per; i < a.k; i += per)
+          if (sid[i] == id) {
+            lead = min(lead, i);
+            p += sp[i];
+          }
+        for (int o = 1; o < per; o <<= 1) {
+          lead = min(lead, __shfl_xor(lead, o, kWave));
+          p += __shfl_xor(p, o, kWave);
+        }
+        if (tid % per == 0 && id >= 0 && lead == j)
+          drow[id] = f32_to_bf16((large ? at_large(sz[j]) : at(sz[j])) - p * a.grad);
+      }
+    }
+  }
   if (tid < kWave) {
     const double l2 = (double)X * a.c + log2((double)S);
     double sum = 0.0;
@@ -491,55 +542,6 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);
     if (lane == 0) a.loss[row] = none ? 0.f : (mass != mass ? mass : (float)(sum * (double)a.t2ln2));
-  }
-  if constexpr (kGrad) {
-    uint16_t* drow = a.dz + row * a.ldd;
-    const float w = mass * a.grad;
-    const bool large = too_large(finite_or_0(X), a.c);
-    const float lS = fast_log2(S);
-    const float nb = -(X * a.c + lS);
-    auto grad = [&](float x) __attribute__((always_inline)) {
-      return fast_exp2(large ? (x - X) * a.c - lS : __builtin_fmaf(x, a.c, nb)) * w;
-    };
-    if (none) {  // whatever the row holds
-      r.vectors(tid, [&](const u32x4&, int i, int) {
-        if (a.same_phase) {
-          reinterpret_cast<u32x4*>(drow + r.head)[i] = u32x4{0, 0, 0, 0};
-        } else {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) drow[r.head + i * 8 + e] = 0;
-        }
-      });
-      if (r.eidx >= 0) drow[r.eidx] = 0;
-      return;
-    }
-    r.vectors(tid, [&](const u32x4& v, int i, int) {
-      u32x4 o;
-#pragma unroll
-      for (int q = 0; q < 4; ++q) o[q] = pack_bf16x2(grad(bf16_lo(v[q])), grad(bf16_hi(v[q])));
-      if (a.same_phase) {
-        __builtin_nontemporal_store(o, reinterpret_cast<u32x4*>(drow + r.head) + i);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) drow[r.head + i * 8 + e] = (uint16_t)(o[e >> 1] >> (16 * (e & 1)));
-      }
-    });
-    if (r.eidx >= 0) drow[r.eidx] = f32_to_bf16(grad(r.xe));
-    // The k entries again, with their p taken off before the one rounding: the
-    // first of equal ids adds up all of them, in order.
-    __syncthreads();
-    for (int j = tid; j < a.k; j += NT) {
-      const int id = sid[j];
-      if (id < 0) continue;
-      float p = 0.f;
-      bool first = true;
-      for (int i = 0; i < a.k; ++i)
-        if (sid[i] == id) {
-          first &= i >= j;
-          p += sp[i];
-        }
-      if (first) drow[id] = f32_to_bf16(grad(sz[j]) - p * a.grad);
-    }
   }
 }
 
