@@ -273,7 +273,9 @@ __global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restri
   constexpr int CAP = NW == 1 ? kCand : 2 * kCand / NW;  // and that a wave's list holds
   __shared__ RowSums<NT> sums;
   __shared__ uint32_t bounds[NW];
-  __shared__ unsigned long long list[NW == 1 ? 1 : NW][NW == 1 ? 1 : CAP];
+  __shared__ __attribute__((aligned(16))) unsigned long long list[NW][CAP];
+  __shared__ __attribute__((aligned(16))) u32x4 held[NW][kWave];  // vectors with a candidate, and where they stand
+  __shared__ int held_at[NW][kWave];
   __shared__ __attribute__((aligned(16))) unsigned long long cand[kCand];
   __shared__ int count;
   __shared__ int cnt[NW];
@@ -318,66 +320,119 @@ __global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restri
     const unsigned long long mask = __ballot(in);
     if (mask == 0) return;
     const int at = n + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
-    if (in && at < CAP) (NW == 1 ? cand : list[wave])[at] = entry(h, i);
+    if (in && at < CAP) list[wave][at] = entry(h, i);
     n += __popcll(mask);
   };
   if (S == S) {
     offer(r.eidx >= 0, __float_as_uint(r.xe) >> 16, r.eidx);
-    auto vec = [&](bool has, const u32x4& v, int i) __attribute__((always_inline)) {
+    // Vectors that hold a candidate are few: they are gathered, one a lane, and looked
+    // through together.
+    int waiting = 0;
+    auto look = [&]() __attribute__((always_inline)) {
+      const bool has = lane < waiting;
+      u32x4 v = {0, 0, 0, 0};
+      int i = 0;
+      __builtin_amdgcn_wave_barrier();
+      if (has) {
+        v = held[wave][lane];
+        i = held_at[wave][lane];
+      }
+      __builtin_amdgcn_wave_barrier();
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        offer(has, v[q] & 0xffffu, r.head + i * 8 + 2 * q);
-        offer(has, v[q] >> 16, r.head + i * 8 + 2 * q + 1);
+        offer(has, v[q] & 0xffffu, i + 2 * q);
+        offer(has, v[q] >> 16, i + 2 * q + 1);
       }
+      waiting = 0;
+    };
+    auto hold = [&](bool has, const u32x4& v, int i) __attribute__((always_inline)) {
+      const unsigned long long mask = __ballot(has);
+      if (mask == 0) return;
+      const int more = __popcll(mask);
+      if (waiting + more > kWave) look();
+      if (has) {
+        const int at =
+            waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0));
+        held[wave][at] = v;
+        held_at[wave][at] = r.head + i * 8;
+      }
+      waiting += more;
     };
     if constexpr (NVEC > 0) {
 #pragma unroll
-      for (int j = 0; j < NVEC; ++j) {
-        const bool has = j * NT + tid < r.nbody && r.top[j] >= fb;
-        if (__ballot(has)) vec(has, r.v[j], j * NT + tid);
-      }
+      for (int j = 0; j < NVEC; ++j)
+        hold(j * NT + tid < r.nbody && r.top[j] >= fb, r.v[j], j * NT + tid);
     } else {
       for (int i0 = wave * kWave; i0 < r.nbody; i0 += NT) {
         const int i = i0 + lane;
         u32x4 v = {0, 0, 0, 0};
         if (i < r.nbody) v = r.body[i];
-        const bool has = i < r.nbody && max8(v) >= fb;
-        if (__ballot(has)) vec(has, v, i);
+        hold(i < r.nbody && max8(v) >= fb, v, i);
       }
     }
+    look();
   } else {
     n = CAP + 1;
   }
   if (lane == 0) cnt[wave] = n;
   __syncthreads();
-  int total = 0, before = 0;
-  bool fits = true;
+  int total = 0, before = 0, most = 0;
 #pragma unroll
   for (int w = 0; w < NW; ++w) {
     const int m = cnt[w];
     if (w < wave) before += m;
     total += m;
-    fits &= m <= CAP;
+    most = max(most, m);
   }
-  if (fits && total <= kCand) {
+  if (most <= CAP && total <= kCand) {
+    // each wave sorts its list by counting; then a candidate's rank is its place there
+    // and, by bisection, the number of larger ones in every other list
+    for (int i = lane; i < n; i += kWave) {
+      const unsigned long long me = list[wave][i];
+      int at = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) at += list[wave][j] > me;
+      if (NW > 1) {
+        cand[before + at] = me;
+      } else if (at < k) {
+        values[row * k + at] = (uint16_t)me;
+        ids[row * k + at] = (int32_t)~(uint32_t)(me >> 16);
+      }
+    }
     if constexpr (NW > 1) {
-      for (int i = lane; i < n; i += kWave) cand[before + i] = list[wave][i];
       __syncthreads();
+      int half = 1;
+      while (half * 2 <= most) half *= 2;
+      for (int i = tid; i < total; i += NT) {
+        const unsigned long long me = cand[i];
+        int at[NW];
+#pragma unroll
+        for (int w = 0; w < NW; ++w) at[w] = 0;
+        for (int step = half; step > 0; step >>= 1) {
+          int off = 0;
+#pragma unroll
+          for (int w = 0; w < NW; ++w) {
+            const int m = cnt[w], to = at[w] + step;
+            if (to <= m && cand[off + to - 1] > me) at[w] = to;
+            off += m;
+          }
+        }
+        int rank = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) rank += at[w];
+        if (rank < k) {
+          values[row * k + rank] = (uint16_t)me;
+          ids[row * k + rank] = (int32_t)~(uint32_t)(me >> 16);
+        }
+      }
     }
   } else {
     select_in_memory<NT>(xrow, V, k, S == S ? bound : 0, tid, cnt, &count, cand);
-    total = k;
-  }
-  // rank of each candidate, by as many threads as there are for one
-  int per = 1;
-  while (per < 16 && total * per * 2 <= NT) per *= 2;
-  for (int i = tid / per; i < total; i += NT / per) {
-    const unsigned long long me = cand[i];
-    int rank = 0;
+    for (int i = tid; i < k; i += NT) {
+      const unsigned long long me = cand[i];
+      int rank = 0;
 #pragma unroll 4
-    for (int j = tid % per; j < total; j += per) rank += cand[j] > me;
-    for (int o = 1; o < per; o <<= 1) rank += __shfl_xor(rank, o, kWave);
-    if (tid % per == 0 && rank < k) {
+      for (int j = 0; j < k; ++j) rank += cand[j] > me;
       values[row * k + rank] = (uint16_t)me;
       ids[row * k + rank] = (int32_t)~(uint32_t)(me >> 16);
     }
