@@ -604,6 +604,15 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
 // NVEC of them (less up to 7 before the first vector).
 #define NL_ROW_SIZES(X) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(512, 2) X(512, 4) X(512, 7) X(512, 10) X(512, 13) X(1024, 9) X(1024, 13)
 
+// threads of a row's workgroup
+int row_threads(int V) {
+#define NL_THREADS(NT, NV) \
+  if (V / 8 <= NT * NV) return NT;
+  NL_ROW_SIZES(NL_THREADS)
+#undef NL_THREADS
+  return 1024;
+}
+
 void launch_top(hipStream_t st, int M, int V, const uint16_t* x, int64_t ld, int k, float c, uint16_t* values,
                 int32_t* ids, float* lse) {
 #define NL_TOP(NT, NV)                                                                                           \
@@ -634,6 +643,8 @@ int check_rows(const char* what, int M, int V, const void* logits, int64_t ld, i
   if (k < 1 || k > kMaxK) return nl_set_error(NL_EINVAL, w + ": need 1 <= k <= NL_TOP_MAX_K");
   if (!(t > 0.f) || t == INFINITY || !(kLog2e / t < INFINITY) || !(t * t < INFINITY) || kLog2e / t < 1e-30f)
     return nl_set_error(NL_EINVAL, w + ": the temperature must be positive and finite");
+  if ((int64_t)M * row_threads(V) >= (int64_t)1 << 32)  // the threads of one launch
+    return nl_set_error(NL_EUNSUPPORTED, w + ": too many rows");
   if (M > 0 && !logits) return nl_set_error(NL_EINVAL, w + ": null logits");
   if (M > 1 && ld < V) return nl_set_error(NL_EINVAL, w + ": ld < V");
   if ((uintptr_t)logits & 1) return nl_set_error(NL_EALIGN, w + ": logits not 2-byte aligned");

@@ -148,12 +148,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
 // l = tid % 16 columns 8l .. 8l+7, so a thread has the 8 bytes of a column that
 // lie together in the transpose.
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a) {
+__global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
   __shared__ uint32_t colmax[16][kB];
   __shared__ uint8_t colbyte[kB];
   __shared__ __attribute__((aligned(16))) u32x2 tile[kB * 16];  // [column][8-row slot ^ (column / 8)]
   const int tid = threadIdx.x, l = tid & 15, g = tid >> 4;
-  const int64_t r0 = (int64_t)blockIdx.y * kB, c0 = (int64_t)blockIdx.x * kB;
+  const uint32_t by = blockIdx.x / cb, bx = blockIdx.x - by * cb;
+  const int64_t r0 = (int64_t)by * kB, c0 = (int64_t)bx * kB;
   const int64_t cl = c0 + l * 8;
   float v[8][8];
 #pragma unroll
@@ -209,9 +210,9 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a) {
       for (int j = 0; j < 8; ++j) w[j] = q_in(v[i][j], inv);
       *reinterpret_cast<u32x2*>(a.q + r * a.ldq + cl) =
           u32x2{pack_e4m3x4(w[0], w[1], w[2], w[3]), pack_e4m3x4(w[4], w[5], w[6], w[7])};
-      if (l == 0 && a.group == 1) a.s[r * a.lds + blockIdx.x] = (uint8_t)byte;
+      if (l == 0 && a.group == 1) a.s[r * a.lds + bx] = (uint8_t)byte;
     }
-    if (a.group != 1 && tid == 0) a.s[(int64_t)blockIdx.y * a.lds + blockIdx.x] = (uint8_t)one;
+    if (a.group != 1 && tid == 0) a.s[(int64_t)by * a.lds + bx] = (uint8_t)one;
   }
   if (!a.qt) return;
 #pragma unroll
@@ -233,9 +234,9 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a) {
     *reinterpret_cast<u32x4*>(a.qt + (c0 + c) * a.ldqt + r0 + h * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
   }
   if (a.group == 1) {
-    if (tid < kB && c0 + tid < a.cols) a.st[(c0 + tid) * a.ldst + blockIdx.y] = colbyte[tid];
+    if (tid < kB && c0 + tid < a.cols) a.st[(c0 + tid) * a.ldst + by] = colbyte[tid];
   } else if (tid == 0) {
-    a.st[(int64_t)blockIdx.x * a.ldst + blockIdx.y] = (uint8_t)one;
+    a.st[(int64_t)bx * a.ldst + by] = (uint8_t)one;
   }
 }
 
@@ -830,7 +831,8 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
   hipStream_t st = (hipStream_t)stream;
   if (!qt && group == 1) {
     const int64_t blocks = rows * cb;
-    if (blocks > INT32_MAX) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: more than 2^31 blocks");
+    // a launch has fewer than 2^32 threads: 16 a block of 128 here, 256 a tile below
+    if (blocks >= (int64_t)1 << 28) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^28 blocks and more");
     const dim3 grid((unsigned)((blocks + 15) / 16));
     if (esz == 2)
       hipLaunchKernelGGL((quantize_rows_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
@@ -838,12 +840,12 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
       hipLaunchKernelGGL((quantize_rows_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     return nl_check_launch("nl_quantize_fp8");
   }
-  if (rb > 65535) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: more than 65535 blocks of rows");
-  const dim3 grid((unsigned)cb, (unsigned)rb);
+  if (rb * cb >= (int64_t)1 << 24) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^24 tiles of 128 x 128 and more");
+  const dim3 grid((unsigned)(rb * cb));
   if (esz == 2)
-    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)cb);
   else
-    hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)cb);
   return nl_check_launch("nl_quantize_fp8");
 }
 

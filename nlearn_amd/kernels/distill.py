@@ -73,12 +73,12 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
 
 class _Distill(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, ids, values, lse, T, inplace):
+    def forward(ctx, x, ids, values, lse, T, inplace, need):
         M, V = x.shape
         loss_rows = torch.empty(M, dtype=_F32, device=x.device)
         loss = torch.empty((), dtype=_F32, device=x.device)
         d = None
-        if ctx.needs_input_grad[0]:
+        if need:
             # rows of the gradient start at the same offsets from 16 bytes as the logits'
             d = x if inplace else torch.empty((M, V + (_ld(x) - V) % 8), dtype=_BF16, device=x.device)[:, :V]
         _lib.call_on(x, "nl_distill_fwd_bwd", M, V, x.data_ptr(), _ld(x), ids.shape[1], ids.data_ptr(),
@@ -98,7 +98,7 @@ class _Distill(torch.autograd.Function):
                                "backward pass; call the loss again")
         g = g.to(_F32)
         _lib.call_on(d, "nl_scale_bf16_by_device_scalar", d.data_ptr(), d.shape[0], d.shape[1], _ld(d), g.data_ptr())
-        return d, None, None, None, None, None
+        return d, None, None, None, None, None, None
 
 
 def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch.Tensor,
@@ -117,8 +117,9 @@ def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch
     without any weight adds 0 to the mean and has a zero gradient. An id >= V, or
     a NaN, makes its row's loss and gradient NaN. 1 <= k <= 256.
 
-    The gradient of the logits is formed by the same pass over them;
-    ``inplace=True`` writes it over ``logits`` (when nothing else reads them)."""
+    Where logits need a gradient it is formed by the same pass over them (and handed
+    out by one backward pass); ``inplace=True`` writes it over ``logits`` (when nothing
+    else reads them)."""
     x = _rows("distill_cross_entropy", logits)
     T = _temperature("distill_cross_entropy", temperature)
     M, V = x.shape
@@ -147,4 +148,4 @@ def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch
     dev = x.get_device()
     if ids.get_device() != dev or values.get_device() != dev or (lse is not None and lse.get_device() != dev):
         raise ValueError("distill_cross_entropy: all tensors must be on the logits' device")
-    return _Distill.apply(x, ids, values, lse, T, bool(inplace))
+    return _Distill.apply(x, ids, values, lse, T, bool(inplace), x.requires_grad and torch.is_grad_enabled())

@@ -119,7 +119,7 @@ def quantize_fp8(x: torch.Tensor, group: int = 1, transpose: bool = False) -> Fp
     """x (R, C), bf16 or fp32, quantised along its columns; with ``transpose`` x^T
     (C, R), quantised along the rows of x. One scale for each block of 128 and
     each ``group`` rows of the result. Values that are not finite become NaN and
-    have no part in the scales."""
+    have no part in the scales. Not differentiable (``linear_fp8`` is)."""
     a, t = _quantize(x, group, not transpose, transpose)
     return t if transpose else a
 
@@ -204,8 +204,8 @@ class _LinearFp8(torch.autograd.Function):
     product is what it costs (15 us against 55 for a forward pass call by call)."""
 
     @staticmethod
-    def forward(ctx, x2, W):
-        need_dx, need_dW = ctx.needs_input_grad
+    def forward(ctx, x2, W, need_dx, need_dW):
+        ctx.need = need_dx, need_dW
         (M, K), N = x2.shape, W.shape[1]
         ctx.save_for_backward(W)
         ctx.sizes = (M, K, N, x2.dtype)
@@ -225,7 +225,7 @@ class _LinearFp8(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dy):
         (W,) = ctx.saved_tensors
-        need_dx, need_dW = ctx.needs_input_grad
+        need_dx, need_dW = ctx.need
         M, K, N, x_dtype = ctx.sizes
         mg = grad_buffer(W) if need_dW else None
         dev = dy.device
@@ -235,7 +235,7 @@ class _LinearFp8(torch.autograd.Function):
             for t in (dx, dW):
                 if t is not None:
                     t.zero_()
-            return dx, dW if mg is None else None
+            return dx, dW if mg is None else None, None, None
         dy, lddy = _rows(dy if dy.dtype in (_BF16, _F32) else dy.to(_F32))
         saved_bytes, _, wsb = _linear_bytes(M, K, N, need_dx, need_dW)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
@@ -243,7 +243,7 @@ class _LinearFp8(torch.autograd.Function):
                      need_dx, need_dW,
                      *((dx.data_ptr(), _code(dx), _ld(dx)) if need_dx else (None, 0, 0)),
                      *((dW.data_ptr(), _code(dW), _ld(dW)) if need_dW else (None, 0, 0)), ws.data_ptr(), wsb)
-        return dx, dW if mg is None else None
+        return dx, dW if mg is None else None, None, None
 
 
 class _LinearFp8Frozen(torch.autograd.Function):
@@ -285,5 +285,6 @@ def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
         _check_device(x2, W)
         if x2.get_device() != W.get_device():
             raise ValueError(f"linear_fp8: x on {x.device}, W on {W.device}")
-        y = _LinearFp8.apply(x2, W)
+        grads = torch.is_grad_enabled()
+        y = _LinearFp8.apply(x2, W, grads and x2.requires_grad, grads and W.requires_grad)
     return y if x.dim() == 2 else y.reshape(*lead, W.shape[1])
