@@ -33,10 +33,12 @@ typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8;
 // Quantisation
 // ===========================================================================
 
-// |x| as ordered bits, 0 for a value that is not finite (it has no part in the scale).
+// |x| as ordered bits, and with 0 for a value that is not finite (it has no part in the scale).
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
 __device__ __forceinline__ uint32_t finite_abs_bits(float x) {
-  const uint32_t u = __float_as_uint(x) & 0x7fffffffu;
-  return u < 0x7f800000u ? u : 0u;
+  const uint32_t u = abs_bits(x);
+  return u < kInfBits ? u : 0u;
 }
 
 // The e8m0 byte (e + 127) of a block whose largest |x| has these bits: with |x| =
@@ -51,10 +53,7 @@ __device__ __forceinline__ int scale_byte(uint32_t amax) {
 // wherever e4m3 keeps anything of it.
 __device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-// Four scaled values to four e4m3 bytes; a value that is not finite becomes NaN.
-__device__ __forceinline__ float q_in(float x, float inv) {
-  return (__float_as_uint(x) & 0x7fffffffu) < 0x7f800000u ? x * inv : __builtin_nanf("");
-}
+// Four scaled values to four e4m3 bytes (an infinity or a NaN gives NaN).
 __device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
   int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
   return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
@@ -133,33 +132,46 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
   load8<T>(a, row, c0, v);
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, finite_abs_bits(v[i]));
+  for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
+  if (m >= kInfBits) {  // look again for what is finite
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, finite_abs_bits(v[i]));
+  }
   const int byte = scale_byte(max16(m));
   const float inv = inv_scale(byte);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = q_in(v[i], inv);
   *reinterpret_cast<u32x2*>(a.q + (int64_t)row * a.ldq + c0) =
-      u32x2{pack_e4m3x4(v[0], v[1], v[2], v[3]), pack_e4m3x4(v[4], v[5], v[6], v[7])};
+      u32x2{pack_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
+            pack_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
   if (l == 0) a.s[(int64_t)row * a.lds + b] = (uint8_t)byte;
 }
 
+// max over the lanes l, l + 16, l + 32, l + 48
+__device__ __forceinline__ uint32_t max_rows(uint32_t v) {
+  const auto r16 = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+  v = max((uint32_t)r16[0], (uint32_t)r16[1]);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+  return max((uint32_t)r32[0], (uint32_t)r32[1]);
+}
+
 // A 128 x 128 tile per workgroup: read once, written along the rows and, through
-// LDS, along the columns. Lane group g = tid / 16 holds rows 8g .. 8g+7, lane
-// l = tid % 16 columns 8l .. 8l+7, so a thread has the 8 bytes of a column that
-// lie together in the transpose.
+// LDS, along the columns. Lane group g = tid / 16 holds rows 4g .. 4g+3, lane
+// l = tid % 16 columns 8l .. 8l+7, so a thread has 4 bytes of a column that lie
+// together in the transpose. Column c's dword g is at slot g ^ 4 (c / 8 % 8): 16-byte
+// pieces stay whole, and 8 lanes' columns fall on different banks.
 template <typename T>
-__global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
-  __shared__ uint32_t colmax[16][kB];
+__global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
+  __shared__ uint32_t colmax[8][kB];
   __shared__ uint8_t colbyte[kB];
-  __shared__ __attribute__((aligned(16))) u32x2 tile[kB * 16];  // [column][8-row slot ^ (column / 8)]
+  __shared__ __attribute__((aligned(16))) uint32_t tile[kB * 32];
   const int tid = threadIdx.x, l = tid & 15, g = tid >> 4;
   const uint32_t by = blockIdx.x / cb, bx = blockIdx.x - by * cb;
   const int64_t r0 = (int64_t)by * kB, c0 = (int64_t)bx * kB;
   const int64_t cl = c0 + l * 8;
-  float v[8][8];
+  float v[4][8];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int64_t r = r0 + g * 8 + i;
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = r0 + g * 4 + i;
     if (r < a.rows) {
       load8<T>(a, r, cl, v[i]);
     } else {
@@ -167,25 +179,35 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a, uint32_
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     }
   }
-  uint32_t rm[8], cm[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  uint32_t rm[4], cm[8];
+  auto maxima = [&](auto bits) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    rm[i] = 0;
+    for (int j = 0; j < 8; ++j) cm[j] = 0;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t u = finite_abs_bits(v[i][j]);
-      rm[i] = max(rm[i], u);
-      cm[j] = max(cm[j], u);
+    for (int i = 0; i < 4; ++i) {
+      rm[i] = 0;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t u = bits(v[i][j]);
+        rm[i] = max(rm[i], u);
+        cm[j] = max(cm[j], u);
+      }
     }
-  }
+  };
+  maxima([](float x) { return abs_bits(x); });
+  if (max(max(rm[0], rm[1]), max(rm[2], rm[3])) >= kInfBits)  // look again for what is finite
+    maxima([](float x) { return finite_abs_bits(x); });
   if (a.group != 1 || a.qt) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) colmax[g][l * 8 + j] = cm[j];
+    for (int j = 0; j < 8; ++j) {
+      const uint32_t m = max_rows(cm[j]);
+      if ((tid & 63) < 16) colmax[tid >> 6][l * 8 + j] = m;
+    }
     __syncthreads();
     if (tid < kB) {
       uint32_t m = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) m = max(m, colmax[i][tid]);
+      for (int i = 0; i < 8; ++i) m = max(m, colmax[i][tid]);
       if (a.group == 1) colbyte[tid] = (uint8_t)scale_byte(m);
       else colmax[0][tid] = m;  // this thread alone read column tid
     }
@@ -200,16 +222,15 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a, uint32_
   }
   if (a.q) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t r = r0 + g * 8 + i;
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + g * 4 + i;
       const int byte = a.group != 1 ? one : scale_byte(max16(rm[i]));
       if (r >= a.rows) continue;
       const float inv = inv_scale(byte);
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = q_in(v[i][j], inv);
+      const float* w = v[i];
       *reinterpret_cast<u32x2*>(a.q + r * a.ldq + cl) =
-          u32x2{pack_e4m3x4(w[0], w[1], w[2], w[3]), pack_e4m3x4(w[4], w[5], w[6], w[7])};
+          u32x2{pack_e4m3x4(w[0] * inv, w[1] * inv, w[2] * inv, w[3] * inv),
+                pack_e4m3x4(w[4] * inv, w[5] * inv, w[6] * inv, w[7] * inv)};
       if (l == 0 && a.group == 1) a.s[r * a.lds + bx] = (uint8_t)byte;
     }
     if (a.group != 1 && tid == 0) a.s[(int64_t)by * a.lds + bx] = (uint8_t)one;
@@ -219,19 +240,16 @@ __global__ __launch_bounds__(256) void quantize_tile_kernel(QuantArgs a, uint32_
   for (int j = 0; j < 8; ++j) {
     const int c = l * 8 + j;
     const float inv = inv_scale(a.group != 1 ? one : colbyte[c]);
-    float w[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) w[i] = q_in(v[i][j], inv);
-    tile[c * 16 + (g ^ l)] = u32x2{pack_e4m3x4(w[0], w[1], w[2], w[3]), pack_e4m3x4(w[4], w[5], w[6], w[7])};
+    tile[c * 32 + (g ^ ((l & 7) << 2))] = pack_e4m3x4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
   }
   __syncthreads();
   // 8 lanes write a column's 128 bytes, 16 a lane
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int c = it * 32 + (tid >> 3), h = tid & 7;
+  for (int it = 0; it < 2; ++it) {
+    const int c = it * 64 + (tid >> 3), h = tid & 7;
     if (c0 + c >= a.cols) continue;
-    const u32x2 lo = tile[c * 16 + ((2 * h) ^ (c >> 3))], hi = tile[c * 16 + ((2 * h + 1) ^ (c >> 3))];
-    *reinterpret_cast<u32x4*>(a.qt + (c0 + c) * a.ldqt + r0 + h * 16) = u32x4{lo[0], lo[1], hi[0], hi[1]};
+    *reinterpret_cast<u32x4*>(a.qt + (c0 + c) * a.ldqt + r0 + h * 16) =
+        *reinterpret_cast<const u32x4*>(tile + c * 32 + ((h ^ ((c >> 3) & 7)) << 2));
   }
   if (a.group == 1) {
     if (tid < kB && c0 + tid < a.cols) a.st[(c0 + tid) * a.ldst + by] = colbyte[tid];
@@ -831,7 +849,7 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
   hipStream_t st = (hipStream_t)stream;
   if (!qt && group == 1) {
     const int64_t blocks = rows * cb;
-    // a launch has fewer than 2^32 threads: 16 a block of 128 here, 256 a tile below
+    // a launch has fewer than 2^32 threads: 16 a block of 128 here, 512 a tile below
     if (blocks >= (int64_t)1 << 28) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^28 blocks and more");
     const dim3 grid((unsigned)((blocks + 15) / 16));
     if (esz == 2)
@@ -840,12 +858,12 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
       hipLaunchKernelGGL((quantize_rows_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     return nl_check_launch("nl_quantize_fp8");
   }
-  if (rb * cb >= (int64_t)1 << 24) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^24 tiles of 128 x 128 and more");
+  if (rb * cb >= (int64_t)1 << 23) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
   const dim3 grid((unsigned)(rb * cb));
   if (esz == 2)
-    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)cb);
+    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   else
-    hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)cb);
+    hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   return nl_check_launch("nl_quantize_fp8");
 }
 
