@@ -160,7 +160,9 @@ def test_c_abi_refusals_and_sizes():
                    (dict(ldc=1 << 21), U)):
         assert gemm(**kw) == rc, kw
     assert L.nl_gemm_fp8_ws_bytes(8192, 8192, 8192) == 0 and L.nl_gemm_fp8_ws_bytes(0, 4, 4) == 0
-    assert L.nl_gemm_fp8_ws_bytes(512, 512, 16384) == 16 * 512 * 512 * 4
+    # a small output with a long sum is split: whole fp32 partials, at least 2 of them
+    n = L.nl_gemm_fp8_ws_bytes(512, 512, 16384)
+    assert n % (512 * 512 * 4) == 0 and n >= 2 * 512 * 512 * 4
     # linear: sizes, workspaces
     assert L.nl_linear_fp8_saved_bytes(4, 130, 200, 0, 0) == 0
     # W (130 rows of 256 bytes, 2 rows of 4 scale bytes), X^T (130 rows of 128 bytes and 4 scale bytes)
