@@ -8,7 +8,9 @@
 //
 // Both are bound by HBM: a row of logits is read once into registers by one
 // workgroup (as the cross-entropy does), and every pass over it runs from there.
-// Rows that no workgroup's registers hold are read twice.
+// Rows that no workgroup's registers hold (beyond 106503 logits) are read twice.
+// Measured at 16384 x 50257, k = 64: the loss with its gradient 642 us (5.1 TB/s; a copy
+// reaches 4.7), the loss alone 328 us (5.0 TB/s), the top logits 406 us (4.1 TB/s).
 #include "common.h"
 
 namespace nl {
@@ -180,6 +182,9 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
 // all their elements instead.) Those go to LDS as (key, index), a list for each wave,
 // and their rank among each other is their place. A row with more of them than fit
 // (ties, mostly), or with a NaN, goes over the row in memory again.
+// At 16384 x 50257: 391 us for k = 1, 406 for 64, 564 for 256, of which the sums of the
+// row take 328. (Every candidate ranked against all others, and each vector looked
+// through where it was found: 397, 482 and 1112 us.)
 
 // bf16 bits as an ordered 16-bit number: -0 as 0, every NaN above infinity
 __device__ __forceinline__ uint32_t order16(uint32_t h) {
@@ -600,8 +605,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   }
 }
 
-// Threads and vectors per thread for a row of V elements. A workgroup holds 8 NT
-// NVEC of them (less up to 7 before the first vector).
+// Threads and vectors per thread for a row of V elements (a workgroup holds 8 NT NVEC
+// of them, less up to 7 before the first vector): the fewest threads whose registers
+// hold the row, so that several rows share a CU and one's loads pass under another's
+// sums. Rows of up to 2055 logits take one wave and no barrier (16384 x 500, k = 64:
+// 44 us, with 4 waves 330); 1024 threads for 50257 logits took 844 us where 512 took 482.
 #define NL_ROW_SIZES(X) X(64, 1) X(64, 2) X(64, 4) X(256, 2) X(512, 2) X(512, 4) X(512, 7) X(512, 10) X(512, 13) X(1024, 9) X(1024, 13)
 
 // threads of a row's workgroup

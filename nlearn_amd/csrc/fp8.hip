@@ -120,7 +120,8 @@ __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c
   }
 }
 
-// One row's block of 128 per 16 lanes, 8 elements a lane: one read, one write.
+// One row's block of 128 per 16 lanes, 8 elements a lane: one read, one write. Bound
+// by HBM: 16384 x 2048 bf16 17.8 us, 8192 x 8192 32.5 us (5.7 and 6.2 TB/s).
 template <typename T>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_t blocks, uint32_t kb) {
   const uint32_t id = blockIdx.x * 16u + (threadIdx.x >> 4);
@@ -159,6 +160,9 @@ __device__ __forceinline__ uint32_t max_rows(uint32_t v) {
 // l = tid % 16 columns 8l .. 8l+7, so a thread has 4 bytes of a column that lie
 // together in the transpose. Column c's dword g is at slot g ^ 4 (c / 8 % 8): 16-byte
 // pieces stay whole, and 8 lanes' columns fall on different banks.
+// Bound by HBM: 16384 x 2048 bf16 28.9 us (4.65 TB/s, where a copy reaches 4.66), an
+// fp32 weight of 512 x 50257 28.7 us; with 256 threads of twice the elements, each
+// looked at twice for values that are not finite, they took 33.1 and 31.9 us.
 template <typename T>
 __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
   __shared__ uint32_t colmax[8][kB];
@@ -271,7 +275,18 @@ __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_
 //     and the scale holds for all 128.
 //   * The lane's scale bytes of four K steps come as one dword per 32 rows.
 //   * Operands are swapped (B as src A), so a lane ends up with 4 consecutive
-//     columns; rows leave through LDS in whole 16-byte pieces.
+//     columns; rows leave through LDS in whole 16-byte pieces (stored from the lanes
+//     as they are, in pieces of 32 bytes a row, 16384 x 50257 x 512 took 672 us for 515).
+//   * 256 x 256 tiles run 4 waves of 128 x 128, one a SIMD: 256 accumulator registers
+//     and two sets of fragments (128) in the 512 it has, and two thirds of the LDS
+//     reads of 8 waves of 128 x 64, which with the DMA's writes would take as long as
+//     the MFMAs.
+// Measured: 8192^3 to bf16 410 us, 2.68 PFLOP/s (a library's product with one scale a
+// tensor 3.03): the MFMAs are busy 71% of the cycles, at the 1.57 GHz that the part
+// holds under them; the rest is the meeting of the waves at each stage and the tiles'
+// stores. To fp32 (widened) 735 us, 1.50 PFLOP/s. 16384 x 50257 x 512, four stages a
+// tile: 484 to 500 us by card, of which some 343 without the tiles' stores and conversions: 1.65 GB go out
+// in the bursts between K loops that the next tile's first two stages hide in part.
 
 struct GemmF8Args {
   int M, N, K, Kp;
@@ -370,6 +385,10 @@ struct F8Item {
   const uint8_t *a, *b, *sa, *sb;
   uint32_t ba, bb, bsa, bsb;    // bytes in reach of each (0: no such item)
 };
+
+// the bytes that a descriptor of a tile reaches, and an offset past them, for stores that
+// are dropped: 16 bytes from there do not pass 2^32 either
+constexpr uint32_t kNowhere = 0xfffffff0u;
 
 // the same on every lane, and known to be
 __device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
@@ -652,7 +671,7 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     asm volatile("" : "+v"(ln));
     const int fr = ln & 31, g4 = (ln >> 5) * 4;
     const bool whole = cur.m0 + BM <= g.M && cur.n0 + BN <= g.N;
-    auto put = [&]() __attribute__((always_inline)) {
+    auto put = [&](auto inside) __attribute__((always_inline)) {
       using T = OutT;
       constexpr int SC = PITCH / (int)sizeof(T);                 // columns of a slab
       constexpr int CPR = PITCH / 16, EPC = 16 / (int)sizeof(T), RPI = 64 / CPR;
@@ -676,12 +695,12 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
             }
           }
           const int r0 = ln / CPR, ch = ln % CPR;
-          if (whole) {
+          if constexpr (decltype(inside)::value) {
             // rows behind one another from a 64-bit base, 32-bit offsets within the tile
             const int mrow = wm * WTM + i * 32, ncol = wn * WTN + c0;
             const __amdgpu_buffer_rsrc_t rc =
                 make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
-                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), 0xffffffffu);
+                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), kNowhere);
             const uint32_t vo = (uint32_t)((r0 * g.ldc + ch * EPC) * (int64_t)sizeof(T));
 #pragma unroll
             for (int it = 0; it < 32 / RPI; ++it) {
@@ -691,22 +710,27 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
                   val, rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
             }
           } else {
+            // rows and columns past the matrix get an offset out of every range, and a
+            // piece that N cuts goes element by element: no lane branches here either
+            const int mrow = cur.m0 + wm * WTM + i * 32, n = cur.n0 + wn * WTN + c0 + ch * EPC;
+            const __amdgpu_buffer_rsrc_t rc =
+                make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
+                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), kNowhere);
 #pragma unroll 1
             for (int it = 0; it < 32 / RPI; ++it) {
               const int r = it * RPI + r0;
               const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
-              const int m = cur.m0 + wm * WTM + i * 32 + r;
-              const int n = cur.n0 + wn * WTN + c0 + ch * EPC;
-              if (m >= g.M || n >= g.N) continue;
-              T* dst = reinterpret_cast<T*>(g.C) + (int64_t)m * g.ldc + n;
-              if (n + EPC <= g.N) {
-                *reinterpret_cast<u32x4*>(dst) = val;
-              } else {
+              const bool in = mrow + r < g.M;
+              const uint32_t off = (uint32_t)(((wm * WTM + i * 32 + r) * g.ldc + wn * WTN + c0 + ch * EPC) * (int64_t)sizeof(T));
+              __builtin_amdgcn_raw_buffer_store_b128(val, rc, in && n + EPC <= g.N ? off : kNowhere, 0, 0);
+              if (g.N % EPC != 0) {
 #pragma unroll
-                for (int k = 0; k < EPC; ++k) {
-                  if (n + k >= g.N) break;
-                  if constexpr (sizeof(T) == 2) dst[k] = (T)(val[k >> 1] >> (16 * (k & 1)));
-                  else dst[k] = __uint_as_float(val[k]);
+                for (int k = 0; k < EPC - 1; ++k) {
+                  const uint32_t at = in && n + EPC > g.N && n + k < g.N ? off + k * (uint32_t)sizeof(T) : kNowhere;
+                  if constexpr (sizeof(T) == 2)
+                    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(val[k >> 1] >> (16 * (k & 1))), rc, at, 0, 0);
+                  else
+                    __builtin_amdgcn_raw_buffer_store_b32(val[k], rc, at, 0, 0);
                 }
               }
             }
@@ -714,27 +738,35 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
         }
     };
     if (g.ws) {
-      float* W = g.ws + (int64_t)cur.split * g.M * g.ldw;
+      const __amdgpu_buffer_rsrc_t rw =
+          make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.ws + ((int64_t)cur.split * g.M + cur.m0) * g.ldw + cur.n0)),
+                    kNowhere);
 #pragma unroll
       for (int i = 0; i < FM; ++i) {
-        const int m = cur.m0 + wm * WTM + i * 32 + fr;
+        const int m = wm * WTM + i * 32 + fr;
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           asm volatile("" : "+v"(acc[i][j]));
-          if (m >= g.M) continue;
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            const int n = cur.n0 + wn * WTN + j * 32 + q * 8 + g4;
-            if (n < g.N)
-              *reinterpret_cast<f32x4*>(W + (int64_t)m * g.ldw + n) =
-                  f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+            const int n = wn * WTN + j * 32 + q * 8 + g4;
+            const u32x4 v = __builtin_bit_cast(
+                u32x4, f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]});
+            __builtin_amdgcn_raw_buffer_store_b128(
+                v, rw, cur.m0 + m < g.M && cur.n0 + n < g.N ? (uint32_t)((m * g.ldw + n) * 4) : kNowhere, 0, 0);
           }
         }
       }
+      wait_vm<0>();
+    } else if (whole) {
+      // no branch among these stores: the compiler counts them where it lets the next
+      // stage's reads pass, and would count none of those it is not sure of
+      put(std::true_type{});
     } else {
-      put();
+      put(std::false_type{});
+      wait_vm<0>();
     }
-    if (g.ws || !whole || next >= last) wait_vm<0>();  // (no DMA is in flight when the workgroup ends)
+    if (next >= last) wait_vm<0>();  // no DMA is in flight when the workgroup ends
     if (next >= last) break;
     item = next;
     cur = nxt;
@@ -778,6 +810,9 @@ F8Plan f8_plan(int M, int N, int K) {
   const int64_t kb = ((int64_t)K + kB - 1) / kB;
   auto tiles = [&](int t) { return (((int64_t)M + t - 1) / t) * (((int64_t)N + t - 1) / t); };
   F8Plan p;
+  // 256 x 256 tiles where there is one for every CU (4096^3 55.8 us against 70.1 with 128 x
+  // 128); with 128 of them half the CUs stand idle (16384 x 512 x 2048 26.5 against 22.8,
+  // 4096 x 2048 x 2048 25.5 against 19.9).
   p.huge = tiles(256) >= 256;
   const int64_t t = tiles(p.huge ? 256 : 128);
   // A split of K shortens the walk over it (0.39 us a block with a bf16 result, 0.69 with
@@ -786,7 +821,7 @@ F8Plan f8_plan(int M, int N, int K) {
   // 512 x 2048 9.8, 14.4 in 2, 18.8 in 4; 8 x 4096 x 4096 16.0, 8.2 in 8.
   int64_t s = 1, best_s = 1;
   double best = 0.5 * (double)kb;
-  if (!p.huge)
+  if (!p.huge && N <= 1 << 20)  // (a tile's rows of partials within 32-bit offsets)
     for (s = 2; s * t <= 256 && s * 4 <= kb; ++s) {
       const int64_t chunk = ((kb + s - 1) / s + 3) / 4 * 4;
       const double us = 0.5 * (double)chunk + 3.0 + 2.6e-6 * (double)M * (double)N * (double)s;
