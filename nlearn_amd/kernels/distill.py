@@ -33,6 +33,8 @@ def _rows(what: str, logits: torch.Tensor) -> torch.Tensor:
     s0, s1 = x.stride()
     if s1 != 1 and V > 1:
         raise ValueError(f"{what}: logits need a unit stride along the vocabulary")
+    if max(x.shape) >= 1 << 31:  # the kernels count rows and logits in 32 bits
+        raise ValueError(f"{what}: sizes must be less than 2^31, got {tuple(x.shape)}")
     if s0 < V and x.shape[0] > 1:  # rows sharing memory (a broadcast view)
         x = x.contiguous()
     return x
@@ -67,7 +69,7 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     ids = torch.empty((*lead, k), dtype=torch.int32, device=x.device)
     lse = torch.empty(lead, dtype=_F32, device=x.device)
     _lib.call_on(x, "nl_top_logits", M, V, x.data_ptr(), _ld(x), int(k), T, values.data_ptr(),
-              ids.data_ptr(), lse.data_ptr())
+                 ids.data_ptr(), lse.data_ptr())
     return values, ids, lse
 
 
@@ -82,10 +84,10 @@ class _Distill(torch.autograd.Function):
             # rows of the gradient start at the same offsets from 16 bytes as the logits'
             d = x if inplace else torch.empty((M, V + (_ld(x) - V) % 8), dtype=_BF16, device=x.device)[:, :V]
         _lib.call_on(x, "nl_distill_fwd_bwd", M, V, x.data_ptr(), _ld(x), ids.shape[1], ids.data_ptr(),
-                  int(ids.dtype is torch.int64), values.data_ptr(),
-                  _lib.NL_DTYPE_F32 if values.dtype is _F32 else _lib.NL_DTYPE_BF16,
-                  lse.data_ptr() if lse is not None else None, T, loss_rows.data_ptr(), loss.data_ptr(), 1.0 / max(M, 1),
-                  d.data_ptr() if d is not None else None, _ld(d) if d is not None else 0)
+                     int(ids.dtype is torch.int64), values.data_ptr(),
+                     _lib.NL_DTYPE_F32 if values.dtype is _F32 else _lib.NL_DTYPE_BF16,
+                     lse.data_ptr() if lse is not None else None, T, loss_rows.data_ptr(), loss.data_ptr(), 1.0 / max(M, 1),
+                     d.data_ptr() if d is not None else None, _ld(d) if d is not None else 0)
         ctx.d = d
         return loss
 

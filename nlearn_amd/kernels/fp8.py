@@ -21,12 +21,17 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .gemm import _BF16, _F32, _check_device, _ld, grad_buffer, padded_empty
+from .gemm import _BF16, _F32, _aligned, _check_device, _ld, grad_buffer, padded_empty
 
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 _NONE = (None, 0, None, 0)  # an output that is not wanted
 BLOCK = 128
+
+
+def _check_sizes(what: str, *sizes: int) -> None:
+    if max(sizes) >= 1 << 31:  # the products count in 32 bits
+        raise ValueError(f"{what}: sizes must be less than 2^31, got {sizes}")
 
 
 def _code(t: torch.Tensor) -> int:
@@ -138,10 +143,12 @@ def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:
 def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | None = None,
              ws: torch.Tensor | None = None) -> torch.Tensor:
     """a (M, K) . b (N, K)^T -> (M, N), summed in fp32, on the current stream.
-    ws: as ``gemm_fp8_ws`` gives it (allocated here if None)."""
+    out: fp32 or bf16 with 16-byte aligned rows. ws: as ``gemm_fp8_ws`` gives it
+    (allocated here if None; too small a one is not used and K is summed in one piece)."""
     (M, K), (N, Kb) = a.shape, b.shape
     if K != Kb:
         raise ValueError(f"gemm_fp8: inner dimensions differ ({K} vs {Kb})")
+    _check_sizes("gemm_fp8", M, N, K)
     _check_device(a.q, b.q)
     if a.q.get_device() != b.q.get_device():
         raise ValueError(f"gemm_fp8: operands on {a.q.device} and {b.q.device}")
@@ -155,11 +162,13 @@ def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | No
         return out
     if ws is None:
         ws = gemm_fp8_ws(a, b)
+    elif ws.get_device() != a.q.get_device() or not ws.is_contiguous():
+        raise ValueError(f"gemm_fp8: the workspace must be contiguous and on {a.q.device}")
     qa, lda, sa, ldsa = a._abi()
     qb, ldb, sb, ldsb = b._abi()
     _lib.call_on(a.q, "nl_gemm_fp8", M, N, K, qa, lda, sa, ldsa, a.group, qb, ldb, sb, ldsb, b.group,
-              out.data_ptr(), _lib.NL_DTYPE_F32 if out.dtype is _F32 else _lib.NL_DTYPE_BF16, _ld(out),
-              ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
+                 out.data_ptr(), _lib.NL_DTYPE_F32 if out.dtype is _F32 else _lib.NL_DTYPE_BF16, _ld(out),
+                 ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
     return out
 
 
@@ -230,9 +239,11 @@ class _LinearFp8(torch.autograd.Function):
         mg = grad_buffer(W) if need_dW else None
         dev = dy.device
         dx = padded_empty(M, K, x_dtype, dev) if need_dx else None                  # dY . W^T
-        dW = (padded_empty(K, N, W.dtype, dev) if mg is None else mg) if need_dW else None  # X^T . dY
+        # X^T . dY, straight into main_grad where its rows are aligned for the product's stores
+        direct = mg is not None and mg.dtype in (_BF16, _F32) and _aligned(mg)
+        dW = (mg if direct else padded_empty(K, N, W.dtype if mg is None else _F32, dev)) if need_dW else None
         if M == 0 or K == 0 or N == 0:
-            for t in (dx, dW):
+            for t in (dx, mg if mg is not None else dW):
                 if t is not None:
                     t.zero_()
             return dx, dW if mg is None else None, None, None
@@ -243,7 +254,11 @@ class _LinearFp8(torch.autograd.Function):
                      need_dx, need_dW,
                      *((dx.data_ptr(), _code(dx), _ld(dx)) if need_dx else (None, 0, 0)),
                      *((dW.data_ptr(), _code(dW), _ld(dW)) if need_dW else (None, 0, 0)), ws.data_ptr(), wsb)
-        return dx, dW if mg is None else None, None, None
+        if mg is None:
+            return dx, dW, None, None
+        if not direct:
+            mg.copy_(dW)
+        return dx, None, None, None
 
 
 class _LinearFp8Frozen(torch.autograd.Function):
@@ -277,6 +292,7 @@ def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
         raise ValueError(f"linear_fp8: x must be bfloat16 or float32, got {x.dtype}")
     lead = x.shape[:-1]
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+    _check_sizes("linear_fp8", *x2.shape, W.shape[1])
     if frozen is not None:
         y = _LinearFp8Frozen.apply(x2, frozen)
     else:

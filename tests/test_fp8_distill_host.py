@@ -199,3 +199,21 @@ def test_c_abi_refusals_and_sizes():
                    (dict(loss=None), E), (dict(ldd=99), E), (dict(d=4097), A), (dict(d=256, ldd=104), E), (dict(T=0.0), E),
                    (dict(ld=50), E), (dict(z=None), E), (dict(V=0), E)):
         assert dist(**kw) == rc, kw
+
+
+def test_sizes_past_32_bits_are_refused():
+    """The kernels count rows in 32 bits: more of them raise, and are not cut to their low bits."""
+    import torch
+    from nlearn_amd.kernels import distill, fp8
+
+    n = (1 << 32) + 8
+    blocks = fp8.Fp8Blocks.empty(n, 0, 1, "cpu")
+    with pytest.raises(ValueError, match=r"2\^31"):
+        fp8.gemm_fp8(blocks, fp8.Fp8Blocks.empty(4, 0, 1, "cpu"))
+    x = torch.zeros((1, 8), dtype=torch.bfloat16).expand(n, 8)
+    with pytest.raises(ValueError, match=r"2\^31"):
+        fp8.linear_fp8(x, torch.zeros((8, 8)))
+    with pytest.raises(ValueError, match=r"2\^31"):
+        distill.top_logits(x, 3)
+    with pytest.raises(ValueError, match=r"2\^31"):
+        distill.distill_cross_entropy(x, torch.zeros((1, 3), dtype=torch.int32).expand(n, 3), torch.zeros((1, 3)).expand(n, 3))

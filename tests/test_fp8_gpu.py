@@ -388,3 +388,36 @@ def test_product_in_a_graph_and_on_two_streams(dev):
     torch.cuda.synchronize()
     for i, y in enumerate(got):
         assert torch.equal(y, want[i % 4])
+
+
+@pytest.mark.parametrize("K,N", [(64, 50), (130, 7)])
+def test_linear_main_grad_of_odd_rows(dev, K, N):
+    """A main_grad laid out like a contiguous weight has rows off 16 bytes: it gets the same gradient, and
+    its neighbours in the flat buffer nothing."""
+    import torch
+    from nlearn_amd.kernels.fp8 import linear_fp8
+
+    rng = _rng(31, K, N)
+    x = torch.from_numpy(_matrix(rng, 200, K)).to(dev).to(torch.bfloat16)
+    dy = torch.from_numpy(_matrix(rng, 200, N)).to(dev).to(torch.bfloat16)
+    W = torch.from_numpy(_matrix(rng, K, N)).to(dev).requires_grad_(True)
+    linear_fp8(x, W).backward(dy)
+    want, W.grad = W.grad.clone(), None
+    for lead in (0, 3):
+        flat = torch.full((lead + K * N + 5,), float("nan"), device=dev)
+        W.main_grad = flat[lead:lead + K * N].view(K, N)
+        linear_fp8(x, W).backward(dy)
+        assert W.grad is None and torch.equal(W.main_grad, want)
+        assert torch.isnan(flat[:lead]).all() and torch.isnan(flat[lead + K * N:]).all()
+
+
+def test_gemm_workspace_elsewhere_is_refused(dev):
+    import torch
+    from nlearn_amd.kernels.fp8 import gemm_fp8, quantize_fp8
+
+    a = quantize_fp8(torch.ones((8, 4096), device=dev))
+    b = quantize_fp8(torch.ones((64, 4096), device=dev))
+    for ws in (torch.empty(1 << 16), torch.empty((256, 512), device=dev)[:, :256]):
+        with pytest.raises(ValueError, match="workspace"):
+            gemm_fp8(a, b, ws=ws)
+    assert torch.equal(gemm_fp8(a, b, ws=torch.empty(4, device=dev)), gemm_fp8(a, b))
