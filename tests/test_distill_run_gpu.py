@@ -135,3 +135,43 @@ def test_side_stream_and_two_calls_at_once(dev):
     torch.cuda.synchronize()
     for n, outs in enumerate(got):
         assert all(torch.equal(a, b) for a, b in zip(outs, want[n % 2]))
+
+
+def test_training_step_in_a_graph(dev):
+    """Two 8-bit layers, the loss and all gradients captured once and replayed on new batches; the weights'
+    gradients go to buffers, of which the head's has rows off 16 bytes."""
+    import torch
+    from nlearn_amd.kernels.distill import distill_cross_entropy
+    from nlearn_amd.kernels.fp8 import linear_fp8
+
+    g = torch.Generator(device=dev).manual_seed(8)
+    M, D, V, k = 70, 256, 301, 9
+    W1, W2 = ((torch.randn(s, generator=g, device=dev) / 16).requires_grad_(True) for s in ((D, D), (D, V)))
+    sets = [(torch.randn((M, D), generator=g, device=dev).to(torch.bfloat16),
+             torch.randint(0, V, (M, k), generator=g, device=dev, dtype=torch.int32),
+             torch.randn((M, k), generator=g, device=dev)) for _ in range(3)]
+
+    def step(x, i, v):
+        for W in (W1, W2):
+            W.main_grad.fill_(float("nan"))
+        loss = distill_cross_entropy(linear_fp8(linear_fp8(x, W1), W2), i, v, None, 2.0, inplace=True)
+        loss.backward()
+        return loss.detach()
+
+    for W in (W1, W2):
+        W.main_grad = torch.empty(tuple(W.shape), device=dev)
+    want = [(step(*s).clone(), W1.main_grad.clone(), W2.main_grad.clone()) for s in sets]
+    bufs = [t.clone() for t in sets[0]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = step(*bufs)
+    for _ in range(2):
+        for s, ref in zip(sets, want):
+            for b, t in zip(bufs, s):
+                b.copy_(t)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip((loss, W1.main_grad, W2.main_grad), ref))
+            assert torch.isfinite(W2.main_grad).all() and W1.grad is None and W2.grad is None
+            step(*sets[1])
