@@ -284,9 +284,11 @@ __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_
 // Measured: 8192^3 to bf16 410 us, 2.68 PFLOP/s (a library's product with one scale a
 // tensor 3.03): the MFMAs are busy 71% of the cycles, at the 1.57 GHz that the part
 // holds under them; the rest is the meeting of the waves at each stage and the tiles'
-// stores. To fp32 (widened) 735 us, 1.50 PFLOP/s. 16384 x 50257 x 512, four stages a
-// tile: 484 to 500 us by card, of which some 343 without the tiles' stores and conversions: 1.65 GB go out
-// in the bursts between K loops that the next tile's first two stages hide in part.
+// stores. To fp32 (widened) 727 us, 1.51 PFLOP/s. 16384 x 50257 x 512, four stages a
+// tile: 480 to 489 us by card, 387 without its stores: 1.65 GB go out in the bursts
+// between K loops that the next tile's first two stages hide in part. The stores pass
+// the caches by (not so, 16384 x 50257 x 512 took 569 us for 489, and the products of a
+// 16384 x 512 x 2048 layer with its gradients 137 us for 132).
 
 struct GemmF8Args {
   int M, N, K, Kp;
@@ -702,13 +704,18 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
                 make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
                                   ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), kNowhere);
             const uint32_t vo = (uint32_t)((r0 * g.ldc + ch * EPC) * (int64_t)sizeof(T));
+            // (all of a slab's reads before its first store: the compiler takes a store for
+            // one that could change what a later read finds)
+            u32x4 val[32 / RPI];
 #pragma unroll
             for (int it = 0; it < 32 / RPI; ++it) {
               const int r = it * RPI + r0;
-              const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
-              __builtin_amdgcn_raw_buffer_store_b128(
-                  val, rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
+              val[it] = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
             }
+#pragma unroll
+            for (int it = 0; it < 32 / RPI; ++it)
+              __builtin_amdgcn_raw_buffer_store_b128(
+                  val[it], rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
           } else {
             // rows and columns past the matrix get an offset out of every range, and a
             // piece that N cuts goes element by element: no lane branches here either
