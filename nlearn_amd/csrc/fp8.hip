@@ -285,7 +285,7 @@ __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_
 // tensor 3.03): the MFMAs are busy 71% of the cycles, at the 1.57 GHz that the part
 // holds under them; the rest is the meeting of the waves at each stage and the tiles'
 // stores. To fp32 (widened) 727 us, 1.51 PFLOP/s. 16384 x 50257 x 512, four stages a
-// tile: 480 to 489 us by card, 387 without its stores: 1.65 GB go out in the bursts
+// tile: 466 to 491 us by card, some 100 fewer without its stores: 1.65 GB go out in bursts
 // between K loops that the next tile's first two stages hide in part. The stores pass
 // the caches by (not so, 16384 x 50257 x 512 took 569 us for 489, and the products of a
 // 16384 x 512 x 2048 layer with its gradients 137 us for 132).
@@ -673,76 +673,80 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     asm volatile("" : "+v"(ln));
     const int fr = ln & 31, g4 = (ln >> 5) * 4;
     const bool whole = cur.m0 + BM <= g.M && cur.n0 + BN <= g.N;
-    auto put = [&](auto inside) __attribute__((always_inline)) {
-      using T = OutT;
-      constexpr int SC = PITCH / (int)sizeof(T);                 // columns of a slab
-      constexpr int CPR = PITCH / 16, EPC = 16 / (int)sizeof(T), RPI = 64 / CPR;
+    using T = OutT;
+    constexpr int SC = PITCH / (int)sizeof(T);                 // columns of a slab
+    constexpr int CPR = PITCH / 16, EPC = 16 / (int)sizeof(T), RPI = 64 / CPR;
+    constexpr int kSlabs = FM * WTN / SC, kPieces = SC / 8, kReads = 32 / RPI;
+    const int r0 = ln / CPR, ch = ln % CPR;
+    // piece p of slab s: this lane's 4 columns of 8
+    auto piece = [&](int s, int p) __attribute__((always_inline)) {
+      const int i = s / (WTN / SC), j = s % (WTN / SC) * (SC / 32) + p / 4, q = p % 4;
+      if (q == 0) asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
+      const int cb = (p * 8 + g4) * (int)sizeof(T);
+      uint8_t* at = wl + fr * PITCH + (((cb >> 4) ^ (fr & (CPR - 1))) << 4) + (cb & 15);
+      const float x0 = acc[i][j][4 * q], x1 = acc[i][j][4 * q + 1], x2 = acc[i][j][4 * q + 2], x3 = acc[i][j][4 * q + 3];
+      if constexpr (sizeof(T) == 2) *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
+      else *reinterpret_cast<f32x4*>(at) = f32x4{x0, x1, x2, x3};
+    };
+    auto slab_row = [&](int it) __attribute__((always_inline)) {
+      const int r = it * RPI + r0;
+      return *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
+    };
+    const __amdgpu_buffer_rsrc_t rc =
+        make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) + ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)),
+                  kNowhere);
+    auto put_whole = [&]() __attribute__((always_inline)) {
+      // rows behind one another from a 64-bit base, 32-bit offsets within the tile
+      const uint32_t vo = (uint32_t)((r0 * g.ldc + ch * EPC) * (int64_t)sizeof(T));
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int p = 0; p < kPieces; ++p) piece(0, p);
 #pragma unroll
-        for (int c0 = 0; c0 < WTN; c0 += SC) {
+      for (int s = 0; s < kSlabs; ++s) {
+        // All of a slab's reads before its first store (the compiler takes a store for one
+        // that could change what a later read finds), the next slab's pieces between the
+        // stores, which leave 64 bytes a cycle.
+        u32x4 val[kReads];
 #pragma unroll
-          for (int j = c0 / 32; j < (c0 + SC) / 32; ++j) {
-            asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
+        for (int it = 0; it < kReads; ++it) val[it] = slab_row(it);
+        const int mrow = wm * WTM + s / (WTN / SC) * 32, ncol = wn * WTN + s % (WTN / SC) * SC;
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              const int cb = (j * 32 - c0 + q * 8 + g4) * (int)sizeof(T);
-              uint8_t* at = wl + fr * PITCH + (((cb >> 4) ^ (fr & (CPR - 1))) << 4) + (cb & 15);
-              const float x0 = acc[i][j][4 * q], x1 = acc[i][j][4 * q + 1], x2 = acc[i][j][4 * q + 2],
-                          x3 = acc[i][j][4 * q + 3];
-              if constexpr (sizeof(T) == 2)
-                *reinterpret_cast<u32x2*>(at) = u32x2{pack_bf16x2(x0, x1), pack_bf16x2(x2, x3)};
-              else
-                *reinterpret_cast<f32x4*>(at) = f32x4{x0, x1, x2, x3};
-            }
+        for (int it = 0; it < kReads; ++it) {
+          __builtin_amdgcn_raw_buffer_store_b128(
+              val[it], rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
+          if (s + 1 < kSlabs) {
+#pragma unroll
+            for (int p = it * kPieces / kReads; p < (it + 1) * kPieces / kReads; ++p) piece(s + 1, p);
           }
-          const int r0 = ln / CPR, ch = ln % CPR;
-          if constexpr (decltype(inside)::value) {
-            // rows behind one another from a 64-bit base, 32-bit offsets within the tile
-            const int mrow = wm * WTM + i * 32, ncol = wn * WTN + c0;
-            const __amdgpu_buffer_rsrc_t rc =
-                make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
-                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), kNowhere);
-            const uint32_t vo = (uint32_t)((r0 * g.ldc + ch * EPC) * (int64_t)sizeof(T));
-            // (all of a slab's reads before its first store: the compiler takes a store for
-            // one that could change what a later read finds)
-            u32x4 val[32 / RPI];
+        }
+      }
+    };
+    auto put_edge = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int it = 0; it < 32 / RPI; ++it) {
-              const int r = it * RPI + r0;
-              val[it] = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
-            }
+      for (int s = 0; s < kSlabs; ++s) {
 #pragma unroll
-            for (int it = 0; it < 32 / RPI; ++it)
-              __builtin_amdgcn_raw_buffer_store_b128(
-                  val[it], rc, vo, uniform((int)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T))), 2 /* nt */);
-          } else {
-            // rows and columns past the matrix get an offset out of every range, and a
-            // piece that N cuts goes element by element: no lane branches here either
-            const int mrow = cur.m0 + wm * WTM + i * 32, n = cur.n0 + wn * WTN + c0 + ch * EPC;
-            const __amdgpu_buffer_rsrc_t rc =
-                make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) +
-                                  ((int64_t)cur.m0 * g.ldc + cur.n0) * (int64_t)sizeof(T)), kNowhere);
+        for (int p = 0; p < kPieces; ++p) piece(s, p);
+        // rows and columns past the matrix get an offset out of every range, and a piece
+        // that N cuts goes element by element: no lane branches here either
+        const int mrow = wm * WTM + s / (WTN / SC) * 32 + r0, ncol = wn * WTN + s % (WTN / SC) * SC + ch * EPC;
+        const int n = cur.n0 + ncol;
 #pragma unroll 1
-            for (int it = 0; it < 32 / RPI; ++it) {
-              const int r = it * RPI + r0;
-              const u32x4 val = *reinterpret_cast<const u32x4*>(wl + r * PITCH + ((ch ^ (r & (CPR - 1))) << 4));
-              const bool in = mrow + r < g.M;
-              const uint32_t off = (uint32_t)(((wm * WTM + i * 32 + r) * g.ldc + wn * WTN + c0 + ch * EPC) * (int64_t)sizeof(T));
-              __builtin_amdgcn_raw_buffer_store_b128(val, rc, in && n + EPC <= g.N ? off : kNowhere, 0, 0);
-              if (g.N % EPC != 0) {
+        for (int it = 0; it < kReads; ++it) {
+          const u32x4 val = slab_row(it);
+          const bool in = cur.m0 + mrow + it * RPI < g.M;
+          const uint32_t off = (uint32_t)(((mrow + it * RPI) * g.ldc + ncol) * (int64_t)sizeof(T));
+          __builtin_amdgcn_raw_buffer_store_b128(val, rc, in && n + EPC <= g.N ? off : kNowhere, 0, 0);
+          if (g.N % EPC != 0) {
 #pragma unroll
-                for (int k = 0; k < EPC - 1; ++k) {
-                  const uint32_t at = in && n + EPC > g.N && n + k < g.N ? off + k * (uint32_t)sizeof(T) : kNowhere;
-                  if constexpr (sizeof(T) == 2)
-                    __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(val[k >> 1] >> (16 * (k & 1))), rc, at, 0, 0);
-                  else
-                    __builtin_amdgcn_raw_buffer_store_b32(val[k], rc, at, 0, 0);
-                }
-              }
+            for (int k = 0; k < EPC - 1; ++k) {
+              const uint32_t at = in && n + EPC > g.N && n + k < g.N ? off + k * (uint32_t)sizeof(T) : kNowhere;
+              if constexpr (sizeof(T) == 2)
+                __builtin_amdgcn_raw_buffer_store_b16((uint16_t)(val[k >> 1] >> (16 * (k & 1))), rc, at, 0, 0);
+              else
+                __builtin_amdgcn_raw_buffer_store_b32(val[k], rc, at, 0, 0);
             }
           }
         }
+      }
     };
     if (g.ws) {
       const __amdgpu_buffer_rsrc_t rw =
@@ -768,9 +772,9 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     } else if (whole) {
       // no branch among these stores: the compiler counts them where it lets the next
       // stage's reads pass, and would count none of those it is not sure of
-      put(std::true_type{});
+      put_whole();
     } else {
-      put(std::false_type{});
+      put_edge();
       wait_vm<0>();
     }
     if (next >= last) wait_vm<0>();  // no DMA is in flight when the workgroup ends
