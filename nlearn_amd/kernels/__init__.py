@@ -1,1 +1,1 @@
-"""HIP kernels behind nlearn's ``nlearn.kernels`` entry points (gemm, cross_entropy)."""
+"""HIP kernels behind nlearn's ``nlearn.kernels`` entry points (gemm, cross_entropy), and beside them fp8 and distill."""
