@@ -162,14 +162,21 @@ __device__ __forceinline__ uint32_t max_rows(uint32_t v) {
 // pieces stay whole, and 8 lanes' columns fall on different banks.
 // Bound by HBM: 16384 x 2048 bf16 28.9 us (4.65 TB/s, where a copy reaches 4.66), an
 // fp32 weight of 512 x 50257 28.7 us; with 256 threads of twice the elements, each
-// looked at twice for values that are not finite, they took 33.1 and 31.9 us.
+// looked at twice for values that are not finite, they took 33.1 and 31.9 us. A layer's x
+// and W go in one launch: 777 x 1000 x 333 forward 22.3 us, in two 26.7; 16384 x 2048 x 512
+// 48.2 and 52.5.
+struct QuantTile {
+  uint32_t tile[kB * 32];
+  uint32_t colmax[8][kB];
+  uint8_t colbyte[kB];
+};
 template <typename T>
-__global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
-  __shared__ uint32_t colmax[8][kB];
-  __shared__ uint8_t colbyte[kB];
-  __shared__ __attribute__((aligned(16))) uint32_t tile[kB * 32];
+__device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block, uint32_t cb, QuantTile& sm) {
+  auto& tile = sm.tile;
+  auto& colmax = sm.colmax;
+  auto& colbyte = sm.colbyte;
   const int tid = threadIdx.x, l = tid & 15, g = tid >> 4;
-  const uint32_t by = blockIdx.x / cb, bx = blockIdx.x - by * cb;
+  const uint32_t by = block / cb, bx = block - by * cb;
   const int64_t r0 = (int64_t)by * kB, c0 = (int64_t)bx * kB;
   const int64_t cl = c0 + l * 8;
   float v[4][8];
@@ -260,6 +267,21 @@ __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_
   } else if (tid == 0) {
     a.st[(int64_t)bx * a.ldst + by] = (uint8_t)one;
   }
+}
+
+template <typename T>
+__global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
+  __shared__ __attribute__((aligned(16))) QuantTile sm;
+  quantize_tile<T>(a, blockIdx.x, cb, sm);
+}
+
+// Two matrices in one launch, the first one's tiles (na of them) before the second's.
+template <typename TA, typename TB>
+__global__ __launch_bounds__(512) void quantize_two_kernel(QuantArgs a, uint32_t cba, uint32_t na, QuantArgs b,
+                                                           uint32_t cbb) {
+  __shared__ __attribute__((aligned(16))) QuantTile sm;
+  if (blockIdx.x < na) quantize_tile<TA>(a, blockIdx.x, cba, sm);
+  else quantize_tile<TB>(b, blockIdx.x - na, cbb, sm);
 }
 
 // ===========================================================================
@@ -885,9 +907,12 @@ int check_operand(const char* what, int64_t rows, int64_t K, const void* q, int6
 
 using namespace nl;
 
-extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t ldx,
-                               int group, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, uint8_t* qt,
-                               int64_t ldqt, uint8_t* scale_t, int64_t ldst) {
+namespace nl {
+namespace {
+
+// The checks of nl_quantize_fp8, and its kernel's arguments (rows or cols 0: nothing to do).
+int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t ldx, int group, uint8_t* q, int64_t ldq,
+               uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, QuantArgs* out) {
   if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > INT32_MAX)
     return nl_set_error(NL_EINVAL, "quantize_fp8: need 0 <= rows, cols < 2^31");
   if (x_dtype != NL_DTYPE_F32 && x_dtype != NL_DTYPE_BF16)
@@ -902,28 +927,69 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
   if (!x) return nl_set_error(NL_EINVAL, "quantize_fp8: null x");
   if (rows > 1 && ldx < cols) return nl_set_error(NL_EINVAL, "quantize_fp8: ldx < cols");
   if ((uintptr_t)x % esz) return nl_set_error(NL_EALIGN, "quantize_fp8: x is not aligned to its type");
-  const int64_t rb = (rows + kB - 1) / kB, cb = (cols + kB - 1) / kB;
-  QuantArgs a{rows, cols, x, ldx, (((uintptr_t)x & 15) == 0 && (rows == 1 || ldx * esz % 16 == 0)) ? 1 : 0, group,
-              q, ldq, scale, lds, qt, ldqt, scale_t, ldst};
-  hipStream_t st = (hipStream_t)stream;
-  if (!qt && group == 1) {
-    const int64_t blocks = rows * cb;
-    // a launch has fewer than 2^32 threads: 16 a block of 128 here, 512 a tile below
-    if (blocks >= (int64_t)1 << 28) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^28 blocks and more");
+  *out = QuantArgs{rows, cols, x, ldx, (((uintptr_t)x & 15) == 0 && (rows == 1 || ldx * esz % 16 == 0)) ? 1 : 0, group,
+                   q, ldq, scale, lds, qt, ldqt, scale_t, ldst};
+  return NL_OK;
+}
+
+int64_t blocks_of(int64_t n) { return (n + kB - 1) / kB; }
+// a launch has fewer than 2^32 threads: 16 a block of 128 by rows, 512 a tile
+constexpr int64_t kMaxBlocks = (int64_t)1 << 28, kMaxTiles = (int64_t)1 << 23;
+
+int quantize_one(hipStream_t st, const QuantArgs& a, int dtype) {
+  const int64_t rb = blocks_of(a.rows), cb = blocks_of(a.cols);
+  if (!a.qt && a.group == 1) {
+    const int64_t blocks = a.rows * cb;
+    if (blocks >= kMaxBlocks) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^28 blocks and more");
     const dim3 grid((unsigned)((blocks + 15) / 16));
-    if (esz == 2)
+    if (dtype == NL_DTYPE_BF16)
       hipLaunchKernelGGL((quantize_rows_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     else
       hipLaunchKernelGGL((quantize_rows_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     return nl_check_launch("nl_quantize_fp8");
   }
-  if (rb * cb >= (int64_t)1 << 23) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
+  if (rb * cb >= kMaxTiles) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
   const dim3 grid((unsigned)(rb * cb));
-  if (esz == 2)
+  if (dtype == NL_DTYPE_BF16)
     hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   else
     hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   return nl_check_launch("nl_quantize_fp8");
+}
+
+// Two matrices in one launch where both go by tiles (and there is room for the grid).
+int quantize_two(hipStream_t st, const QuantArgs& a, int a_dtype, const QuantArgs& b, int b_dtype) {
+  const int64_t ca = blocks_of(a.cols), cb = blocks_of(b.cols);
+  const int64_t na = blocks_of(a.rows) * ca, nb = blocks_of(b.rows) * cb;
+  if ((!a.qt && a.group == 1) || (!b.qt && b.group == 1) || na + nb >= kMaxTiles) {
+    if (int rc = quantize_one(st, a, a_dtype)) return rc;
+    return quantize_one(st, b, b_dtype);
+  }
+  const dim3 grid((unsigned)(na + nb));
+#define NL_QUANT_TWO(TA, TB)                                                                                  \
+  hipLaunchKernelGGL((quantize_two_kernel<TA, TB>), grid, dim3(512), 0, st, a, (uint32_t)ca, (uint32_t)na, b, \
+                     (uint32_t)cb)
+  if (a_dtype == NL_DTYPE_BF16) {
+    if (b_dtype == NL_DTYPE_BF16) NL_QUANT_TWO(uint16_t, uint16_t);
+    else NL_QUANT_TWO(uint16_t, float);
+  } else {
+    if (b_dtype == NL_DTYPE_BF16) NL_QUANT_TWO(float, uint16_t);
+    else NL_QUANT_TWO(float, float);
+  }
+#undef NL_QUANT_TWO
+  return nl_check_launch("nl_quantize_fp8");
+}
+
+}  // namespace
+}  // namespace nl
+
+extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t ldx,
+                               int group, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, uint8_t* qt,
+                               int64_t ldqt, uint8_t* scale_t, int64_t ldst) {
+  QuantArgs a;
+  if (int rc = quant_args(rows, cols, x, x_dtype, ldx, group, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, &a))
+    return rc;
+  return rows == 0 || cols == 0 ? NL_OK : quantize_one((hipStream_t)stream, a, x_dtype);
 }
 
 extern "C" size_t nl_gemm_fp8_ws_bytes(int M, int N, int K) {
@@ -1020,11 +1086,11 @@ LinearParts linear_parts(int M, int K, int N, bool dx, bool dw) {
   return p;
 }
 
-int quantize_into(void* st, const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* buf,
-                  const Part* a, uint8_t* tbuf, const Part* t) {
-  return nl_quantize_fp8(st, rows, cols, x, dtype, ldx, a ? a->group : t->group, a ? buf + a->at : nullptr,
-                         a ? a->ld() : 0, a ? buf + a->sat : nullptr, a ? a->lds() : 0, t ? tbuf + t->at : nullptr,
-                         t ? t->ld() : 0, t ? tbuf + t->sat : nullptr, t ? t->lds() : 0);
+int part_args(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols, uint8_t* buf, const Part* a,
+              uint8_t* tbuf, const Part* t, QuantArgs* out) {
+  return quant_args(rows, cols, x, dtype, ldx, a ? a->group : t->group, a ? buf + a->at : nullptr, a ? a->ld() : 0,
+                    a ? buf + a->sat : nullptr, a ? a->lds() : 0, t ? tbuf + t->at : nullptr, t ? t->ld() : 0,
+                    t ? tbuf + t->sat : nullptr, t ? t->lds() : 0, out);
 }
 
 int product(void* st, const uint8_t* abuf, const Part& a, const uint8_t* bbuf, const Part& b, void* C, int dtype,
@@ -1064,8 +1130,10 @@ extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* 
   if (int rc = check_linear("linear_fp8_fwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
   if (int rc = check_linear("linear_fp8_fwd", M, K, N, ws, ws_bytes, p.fwd + (int64_t)p.ws_fwd, "workspace")) return rc;
   uint8_t *sv = (uint8_t*)saved, *b = (uint8_t*)ws;
-  if (int rc = quantize_into(stream, W, w_dtype, ldw, K, N, sv, need_dx ? &p.wb : nullptr, b, &p.wf)) return rc;
-  if (int rc = quantize_into(stream, x, x_dtype, ldx, M, K, b, &p.x, sv, need_dw ? &p.xt : nullptr)) return rc;
+  QuantArgs qw, qx;
+  if (int rc = part_args(W, w_dtype, ldw, K, N, sv, need_dx ? &p.wb : nullptr, b, &p.wf, &qw)) return rc;
+  if (int rc = part_args(x, x_dtype, ldx, M, K, b, &p.x, sv, need_dw ? &p.xt : nullptr, &qx)) return rc;
+  if (int rc = quantize_two((hipStream_t)stream, qx, x_dtype, qw, w_dtype)) return rc;
   return product(stream, b, p.x, b, p.wf, y, y_dtype, ldy, b + p.fwd, p.ws_fwd);
 }
 
@@ -1082,9 +1150,10 @@ extern "C" int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* 
     return rc;
   const uint8_t* sv = (const uint8_t*)saved;
   uint8_t* b = (uint8_t*)ws;
-  if (int rc = quantize_into(stream, dy, dy_dtype, lddy, M, N, b, need_dx ? &p.dy : nullptr, b,
-                             need_dw ? &p.dyt : nullptr))
+  QuantArgs qdy;
+  if (int rc = part_args(dy, dy_dtype, lddy, M, N, b, need_dx ? &p.dy : nullptr, b, need_dw ? &p.dyt : nullptr, &qdy))
     return rc;
+  if (int rc = quantize_one((hipStream_t)stream, qdy, dy_dtype)) return rc;
   if (need_dx)
     if (int rc = product(stream, b, p.dy, sv, p.wb, dx, dx_dtype, lddx, b + p.bwd, p.ws_dx)) return rc;
   if (need_dw)

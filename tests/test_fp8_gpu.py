@@ -421,3 +421,25 @@ def test_gemm_workspace_elsewhere_is_refused(dev):
         with pytest.raises(ValueError, match="workspace"):
             gemm_fp8(a, b, ws=ws)
     assert torch.equal(gemm_fp8(a, b, ws=torch.empty(4, device=dev)), gemm_fp8(a, b))
+
+
+@pytest.mark.parametrize("wdtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("xdtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("M,K,N", [(1, 130, 5), (300, 257, 129), (128, 128, 128)])
+def test_linear_is_its_parts(dev, M, K, N, xdtype, wdtype):
+    """linear_fp8 quantises x and W in one launch: bit for bit what the operators give one by one."""
+    import torch
+    from nlearn_amd.kernels.fp8 import gemm_fp8, linear_fp8, quantize_fp8_both
+
+    rng = _rng(41, M, K, N)
+    x = torch.from_numpy(_matrix(rng, M, K)).to(dev).to(getattr(torch, xdtype)).requires_grad_(True)
+    W = torch.from_numpy(_matrix(rng, K, N)).to(dev).to(getattr(torch, wdtype)).requires_grad_(True)
+    dy = torch.from_numpy(_matrix(rng, M, N)).to(dev).to(getattr(torch, xdtype))
+    y = linear_fp8(x, W)
+    y.backward(dy)
+    qx, qxt = quantize_fp8_both(x.detach())
+    wb, wf = quantize_fp8_both(W.detach(), group=128)
+    qd, qdt = quantize_fp8_both(dy)
+    assert torch.equal(y, gemm_fp8(qx, wf, x.dtype))
+    assert torch.equal(x.grad, gemm_fp8(qd, wb, x.dtype))
+    assert torch.equal(W.grad, gemm_fp8(qxt, qdt, W.dtype))
