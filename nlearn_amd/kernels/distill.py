@@ -82,7 +82,7 @@ class _Distill(torch.autograd.Function):
         d = None
         if need:
             # rows of the gradient start at the same offsets from 16 bytes as the logits'
-            d = x if inplace else torch.empty((M, V + (_ld(x) - V) % 8), dtype=_BF16, device=x.device)[:, :V]
+            d = x if inplace else torch.empty_strided((M, V), (V + (_ld(x) - V) % 8, 1), dtype=_BF16, device=x.device)
         _lib.call_on(x, "nl_distill_fwd_bwd", M, V, x.data_ptr(), _ld(x), ids.shape[1], ids.data_ptr(),
                      int(ids.dtype is torch.int64), values.data_ptr(),
                      _lib.NL_DTYPE_F32 if values.dtype is _F32 else _lib.NL_DTYPE_BF16,

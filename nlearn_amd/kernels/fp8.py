@@ -21,7 +21,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .gemm import _BF16, _F32, _aligned, _check_device, _ld, grad_buffer, padded_empty
+from .gemm import _BF16, _F32, _aligned, _check_device, _ld, grad_buffer, padded_ld
 
 _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
@@ -32,6 +32,11 @@ BLOCK = 128
 def _check_sizes(what: str, *sizes: int) -> None:
     if max(sizes) >= 1 << 31:  # the products count in 32 bits
         raise ValueError(f"{what}: sizes must be less than 2^31, got {sizes}")
+
+
+def _result(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """An empty result with the row stride of ``padded_empty``, in one call of torch."""
+    return torch.empty_strided((rows, cols), (padded_ld(cols), 1), dtype=dtype, device=device)
 
 
 def _code(t: torch.Tensor) -> int:
@@ -155,7 +160,7 @@ def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | No
     if out is None:
         if out_dtype is not _F32 and out_dtype is not _BF16:
             raise ValueError("gemm_fp8: output must be float32 or bfloat16")
-        out = padded_empty(M, N, out_dtype, a.q.device)
+        out = _result(M, N, out_dtype, a.q.device)
     elif out.dtype not in (_F32, _BF16) or tuple(out.shape) != (M, N) or out.device != a.q.device:
         raise ValueError(f"gemm_fp8: output must be float32 or bfloat16 of shape {(M, N)} on {a.q.device}")
     if M == 0 or N == 0:
@@ -218,7 +223,7 @@ class _LinearFp8(torch.autograd.Function):
         (M, K), N = x2.shape, W.shape[1]
         ctx.save_for_backward(W)
         ctx.sizes = (M, K, N, x2.dtype)
-        y = padded_empty(M, N, x2.dtype, x2.device)
+        y = _result(M, N, x2.dtype, x2.device)
         if M == 0 or K == 0 or N == 0:
             return y.zero_()
         saved_bytes, wsb, _ = _linear_bytes(M, K, N, need_dx, need_dW)
@@ -238,10 +243,16 @@ class _LinearFp8(torch.autograd.Function):
         M, K, N, x_dtype = ctx.sizes
         mg = grad_buffer(W) if need_dW else None
         dev = dy.device
-        dx = padded_empty(M, K, x_dtype, dev) if need_dx else None                  # dY . W^T
+        dx = _result(M, K, x_dtype, dev) if need_dx else None                  # dY . W^T
         # X^T . dY, straight into main_grad where its rows are aligned for the product's stores
         direct = mg is not None and mg.dtype in (_BF16, _F32) and _aligned(mg)
-        dW = (mg if direct else padded_empty(K, N, W.dtype if mg is None else _F32, dev)) if need_dW else None
+        dW = None
+        if direct:
+            dW = mg
+        elif mg is None and need_dW and W.is_contiguous() and N % 8 == 0:
+            dW = torch.empty_like(W)  # laid out like W: autograd keeps it as W.grad without a copy
+        elif need_dW:
+            dW = _result(K, N, W.dtype if mg is None else _F32, dev)
         if M == 0 or K == 0 or N == 0:
             for t in (dx, mg if mg is not None else dW):
                 if t is not None:
