@@ -87,10 +87,11 @@ __device__ __forceinline__ void combine(float& m, float& s, float m2, float s2, 
   m = mn;
 }
 
-// x c itself would overflow: masks of the type's lowest value stand alone in a row
-__device__ __forceinline__ bool too_large(float m, float c) { return fabsf(m) * c > 1e37f; }
+// Sums over a row take 2^(x c - off) with off = m c rounded, one fma an element, and multiply by
+// 2^(off - m c) at the end. That rounding is at most 2^-24 |m| c, so 1/16 up to here; beyond it
+// (masks of a large finite value) the factor would soon leave fp32, and (x - m) c is formed instead.
+__device__ __forceinline__ bool is_far(float m, float c) { return !(fabsf(m) * c <= 1048576.f); }
 
-// per_wave(thread's max) runs on every wave ahead of the workgroup's barrier.
 __device__ __forceinline__ float max8(const u32x4& v) {
   float m = fmaxf(bf16_lo(v[0]), bf16_hi(v[0]));
 #pragma unroll
@@ -98,6 +99,7 @@ __device__ __forceinline__ float max8(const u32x4& v) {
   return m;
 }
 
+// per_wave(thread's max) runs on every wave ahead of the workgroup's barrier.
 template <bool kTops = false, int NT, int NVEC, class F>
 __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, RowSums<NT>& sm, float& X, float& S,
                                          F per_wave) {
@@ -121,8 +123,7 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
       });
     };
     const float at = finite_or_0(m);
-    if (!too_large(at, c)) {
-      // one fma an element against the rounded at * c, whose rounding comes off the sum
+    if (!is_far(at, c)) {
       const float off = at * c;
       sum([&](float x) { return __builtin_fmaf(x, c, -off); });
       s *= fast_exp2(__builtin_fmaf(-at, c, off));
@@ -548,7 +549,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     const float w = mass * a.grad;
     const float lS = fast_log2(S);
     const float nb = -(X * a.c + lS);
-    const bool large = too_large(finite_or_0(X), a.c);
+    const bool large = fabsf(finite_or_0(X)) * a.c > 1e37f;
     auto write = [&](auto f) __attribute__((always_inline)) {
       r.vectors(tid, [&](const u32x4& v, int i, int) {
         u32x4 o;

@@ -1,0 +1,127 @@
+"""top_logits and the distillation loss on logits of large finite values: masks of -1e4 to the type's
+lowest beside ordinary logits and alone, and rows far from zero.
+
+With e = (x - X) / T, X the row's maximum, u = 2^-24 and S = sum exp(e), the bounds are:
+  S        4 roundings of an exponent (the rounded 1/T two, the difference, the product; a further one of
+           each reference a partial sum moves to is part of them) cost 4 |e| u of a term, and the mean of
+           |e| under the weights exp(e) / S is at most log V < 18; two roundings of each exp2, 132 of the
+           sums: (72 + 4 + 132) u < 2^8 u = 2^-16.
+  lse      2^-16, u |lse| for its own rounding, and 2 u |X| / T where 1/T is rounded.
+  loss     T^2 times: S_t 2^-16 for the student's sum (S_t = sum p), 2^-22 p |e| of each entry, and
+           2^-21 sum p |gap| for p itself.
+  dlogits  half a step of bf16 (2^-8 of the value); q is off by 2^-16 and, where it is above 2^-126,
+           by 4 |e| u < 2^-15: 2^-14 of S_t q + p.
+"""
+import numpy as np
+import pytest
+
+from oracle import distill_fp8 as orc
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+MASKS = [-1e4, -1e9, -1e10, -1e20, -1e30, -3.3895313892515355e38]  # the last: bf16's lowest
+ROWS = [700, 9000, 50257, 120000]  # one wave, several, the model's, streamed
+
+
+def _normal(rng, M, V):
+    import torch
+
+    return torch.from_numpy((rng.standard_normal((M, V)) * 2).astype(np.float32)).to(torch.bfloat16)
+
+
+def _beside(rng, V):
+    """Rows with masks over a tail, a head, a stretch within, and all but three logits."""
+    x = _normal(rng, 4 * len(MASKS), V)
+    for n, a in enumerate(MASKS):
+        x[4 * n, V - V // 3:] = a
+        x[4 * n + 1, :V // 2] = a
+        x[4 * n + 2, V // 7:V // 2] = a
+        keep = x[4 * n + 3, [0, V // 2, V - 1]].clone()
+        x[4 * n + 3] = a
+        x[4 * n + 3, [0, V // 2, V - 1]] = keep
+    return x
+
+
+def _entries(rng, x, k, T):
+    """A teacher near the student's logits: its k largest and its logsumexp."""
+    import torch
+
+    t = x.double() + torch.from_numpy(rng.standard_normal(tuple(x.shape)))
+    v, i = torch.topk(t, k, 1)
+    return i.int(), v.float(), torch.logsumexp(t / T, 1).float()
+
+
+def _distill(x, ids, v, lse, T, dev):
+    """Losses by row and the gradient of their mean, from the C entry point."""
+    import torch
+    from nlearn_amd import _lib
+
+    M, V = x.shape
+    z, i, w, l = x.to(dev), ids.to(dev), v.to(dev), None if lse is None else lse.to(dev)
+    loss, d = torch.empty(M, device=dev), torch.empty_like(z)
+    _lib.call("nl_distill_fwd_bwd", _lib.stream_of(z), M, V, z.data_ptr(), V, ids.shape[1], i.data_ptr(), 0,
+              w.data_ptr(), _lib.NL_DTYPE_F32, None if l is None else l.data_ptr(), T, loss.data_ptr(), None, 1.0 / M,
+              d.data_ptr(), V)
+    return loss.double().cpu().numpy(), d.double().cpu().numpy()
+
+
+def _from_max(x):
+    """x less the row's maximum, in float64: the loss and its gradient are the same, and no sum of a
+    large value and a logarithm is formed."""
+    x = x.double().numpy()
+    with np.errstate(invalid="ignore"):
+        return x - x.max(1, keepdims=True)
+
+
+def _check_loss(got, x, ids, v, lse, T):
+    z, i = _from_max(x), ids.numpy()
+    want, _, mass, spread = orc.distill(z, i, v.double().numpy(), None if lse is None else lse.double().numpy(), T, 1.0)
+    on = i >= 0
+    with np.errstate(divide="ignore"):
+        w = np.where(on, v.double().numpy() / T, -np.inf)
+        p = np.exp(w - (orc.lse(w) if lse is None else lse.double().numpy())[:, None])
+    e = np.where(p > 0, np.abs(np.take_along_axis(z, np.where(on, i, 0), 1)) / T, 0)
+    lim = T * T * (2.0 ** -16 * mass + 2.0 ** -22 * (p * e).sum(1) + 2.0 ** -21 * spread) + U * np.abs(want)
+    assert (np.abs(got - want) <= lim).all(), (got, want, lim)
+
+
+def _check_gradient(got, x, ids, v, lse, T):
+    z, i = _from_max(x), ids.numpy()
+    M = x.shape[0]
+    _, d, mass, _ = orc.distill(z, i, v.double().numpy(), None if lse is None else lse.double().numpy(), T, 1.0 / M)
+    entry = np.zeros(x.shape, bool)
+    for m in range(M):
+        entry[m, i[m][i[m] >= 0]] = True
+    # S_t q + p <= |d| M / T, and 2 S_t more at the entries
+    both = np.abs(d) + np.where(entry, 2 * mass[:, None], 0) * T / M
+    bad = ~(np.abs(got - d) <= 1.01 * 2.0 ** -8 * np.abs(d) + 2.0 ** -14 * both + 1e-38)
+    assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[0], got[bad][0], d[bad][0])
+
+
+@pytest.mark.parametrize("T", [1.0, 2.0 ** -7, 1024.0])
+@pytest.mark.parametrize("V", ROWS)
+def test_top_logits_beside_masks(dev, V, T):
+    import torch
+    from nlearn_amd.kernels.distill import top_logits
+
+    x = _beside(np.random.default_rng(V), V)
+    values, ids, lse = top_logits(x.to(dev), 8, T)
+    want = orc.top(x.double().numpy(), 8, T)
+    np.testing.assert_array_equal(ids.cpu().numpy(), want[0])
+    assert torch.equal(values.cpu(), x.gather(1, ids.cpu().long()))
+    top = x.double().numpy().max(1)
+    lim = 2.0 ** -16 + U * np.abs(want[1]) + 2 * U * np.abs(top) / T
+    assert (np.abs(lse.double().cpu().numpy() - want[1]) <= lim).all()
+
+
+@pytest.mark.parametrize("T", [1.0, 1024.0])
+@pytest.mark.parametrize("V", ROWS)
+def test_loss_and_gradient_beside_masks(dev, V, T):
+    rng = np.random.default_rng(V + 1)
+    x = _beside(rng, V)
+    ids, v, lse = _entries(rng, x, 3, T)
+    for l in (lse, None):
+        loss, d = _distill(x, ids, v, l, T, dev)
+        _check_loss(loss, x, ids, v, l, T)
+        _check_gradient(d, x, ids, v, l, T)
