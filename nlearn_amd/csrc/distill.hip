@@ -546,10 +546,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   const bool none = mass == 0.f;  // no entry, or none with any weight
   if constexpr (kGrad) {
     uint16_t* drow = a.dz + row * a.ldd;
-    const float w = mass * a.grad;
-    const float lS = fast_log2(S);
-    const float nb = -(X * a.c + lS);
-    const bool large = fabsf(finite_or_0(X)) * a.c > 1e37f;
+    // q_v S_t scale T, in the two forms that the sums take (an infinite X has but the second)
+    const bool far = is_far(X, a.c);
+    const float off = X * a.c;
+    const float w = mass * a.grad / S;
+    const float wn = w * fast_exp2(__builtin_fmaf(-X, a.c, off));
     auto write = [&](auto f) __attribute__((always_inline)) {
       r.vectors(tid, [&](const u32x4& v, int i, int) {
         u32x4 o;
@@ -564,11 +565,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       });
       if (r.eidx >= 0) drow[r.eidx] = f32_to_bf16(f(r.xe));
     };
-    auto at = [&](float x) __attribute__((always_inline)) { return fast_exp2(__builtin_fmaf(x, a.c, nb)) * w; };
-    auto at_large = [&](float x) __attribute__((always_inline)) { return fast_exp2((x - X) * a.c - lS) * w; };
+    auto near_x = [&](float x) __attribute__((always_inline)) { return fast_exp2(__builtin_fmaf(x, a.c, -off)) * wn; };
+    auto far_x = [&](float x) __attribute__((always_inline)) { return fast_exp2((x - X) * a.c) * w; };
     if (none) write([](float) { return 0.f; });  // whatever the row holds
-    else if (!large) write(at);
-    else write(at_large);
+    else if (!far) write(near_x);
+    else write(far_x);
     if (!none) {
       // The k entries again, with their p taken off before the one rounding: the first
       // of equal ids adds up all of them, in a fixed order. A few threads share an entry.
@@ -589,7 +590,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
           p += __shfl_xor(p, o, kWave);
         }
         if (tid % per == 0 && id >= 0 && lead == j)
-          drow[id] = f32_to_bf16((large ? at_large(sz[j]) : at(sz[j])) - p * a.grad);
+          drow[id] = f32_to_bf16((far ? far_x(sz[j]) : near_x(sz[j])) - p * a.grad);
       }
     }
   }

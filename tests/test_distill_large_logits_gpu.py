@@ -9,8 +9,9 @@ With e = (x - X) / T, X the row's maximum, u = 2^-24 and S = sum exp(e), the bou
   lse      2^-16, u |lse| for its own rounding, and 2 u |X| / T where 1/T is rounded.
   loss     T^2 times: S_t 2^-16 for the student's sum (S_t = sum p), 2^-22 p |e| of each entry, and
            2^-21 sum p |gap| for p itself.
-  dlogits  half a step of bf16 (2^-8 of the value); q is off by 2^-16 and, where it is above 2^-126,
-           by 4 |e| u < 2^-15: 2^-14 of S_t q + p.
+  dlogits  half a step of bf16 (2^-8 of the value); q is off by 2^-16 and, where exp(e) is above 2^-126,
+           by 4 |e| u < 2^-15: 2^-14 of S_t q + p. An exp(e) below 2^-126 is flushed to 0: q = exp(e) / S,
+           S >= 1, so 2^-126 T S_t / M of the gradient, and 1e-38 for a bf16 below its own normal range.
 """
 import numpy as np
 import pytest
@@ -95,7 +96,8 @@ def _check_gradient(got, x, ids, v, lse, T):
         entry[m, i[m][i[m] >= 0]] = True
     # S_t q + p <= |d| M / T, and 2 S_t more at the entries
     both = np.abs(d) + np.where(entry, 2 * mass[:, None], 0) * T / M
-    bad = ~(np.abs(got - d) <= 1.01 * 2.0 ** -8 * np.abs(d) + 2.0 ** -14 * both + 1e-38)
+    bad = ~(np.abs(got - d) <= 1.01 * 2.0 ** -8 * np.abs(d) + 2.0 ** -14 * both + 2.0 ** -126 * mass[:, None] * T / M
+            + 1e-38)
     assert not bad.any(), (int(bad.sum()), np.argwhere(bad)[0], got[bad][0], d[bad][0])
 
 
@@ -125,3 +127,45 @@ def test_loss_and_gradient_beside_masks(dev, V, T):
         loss, d = _distill(x, ids, v, l, T, dev)
         _check_loss(loss, x, ids, v, l, T)
         _check_gradient(d, x, ids, v, l, T)
+
+
+def _far(rng, V):
+    """Rows of one value (a mask that leaves nothing among them), and rows about a value far from zero."""
+    import torch
+
+    one = MASKS + [3e4, -1e6, 1e6, -1e7, 1e10, 1e30]
+    about = [(1e3, 16.0), (-3e4, 512.0), (1e6, 2.0 ** 14), (-1e10, 2.0 ** 28)]  # some bf16 steps wide
+    x = torch.empty((len(one) + len(about), V), dtype=torch.bfloat16)
+    for m, a in enumerate(one):
+        x[m] = a
+    for m, (a, s) in enumerate(about):
+        x[len(one) + m] = (a + s * torch.from_numpy(rng.standard_normal(V))).to(torch.bfloat16)
+    return x
+
+
+def _teacher(rng, M, V, k):
+    """Entries of a teacher of its own: distinct ids, the largest logits among the row's and their sums."""
+    import torch
+
+    ids = np.stack([rng.permutation(V)[:k] for _ in range(M)]).astype(np.int32)
+    v = rng.standard_normal((M, k))
+    lse = orc.lse(v) + 0.5
+    return torch.from_numpy(ids), torch.from_numpy(v.astype(np.float32)), torch.from_numpy(lse.astype(np.float32))
+
+
+TEMPERATURES = [1.0, float(np.float32(1e-3)), 2.0 ** -7, 1024.0]
+
+
+@pytest.mark.parametrize("T", TEMPERATURES)
+@pytest.mark.parametrize("V", ROWS)
+def test_gradient_far_from_zero(dev, V, T):
+    rng = np.random.default_rng(V + 2)
+    x = _far(rng, V)
+    ids, v, lse = _teacher(rng, x.shape[0], V, 4)
+    v = v * T  # p as at T = 1, whatever the temperature
+    for l in (lse, None):
+        _check_gradient(_distill(x, ids, v, l, T, dev)[1], x, ids, v, l, T)
+    # the masks of a batch beside ordinary logits, at every temperature
+    y = _beside(rng, V)
+    ids, v, lse = _entries(rng, y, 3, T)
+    _check_gradient(_distill(y, ids, v, lse, T, dev)[1], y, ids, v, lse, T)
