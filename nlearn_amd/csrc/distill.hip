@@ -519,9 +519,10 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       for (int e = 0; e < kMaxK / kWave; ++e)
         if (e * kWave < a.k) s += exp2_split(lp[e] - at);
       s = wave_sum(s);
-      const double l = s == 0.f ? 0.0 : at + log2((double)s);
+      // (the largest comes off first: beside a value of 1e17 the logarithm would be lost)
+      const double l = s == 0.f ? 0.0 : log2((double)s);
 #pragma unroll
-      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] -= l;
+      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] = (lp[e] - at) - l;
     }
     float S = 0.f;
 #pragma unroll
@@ -595,11 +596,11 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
     }
   }
   if (tid < kWave) {
-    const double l2 = (double)X * a.c + log2((double)S);
+    const double l2 = log2((double)S);  // of the sum against X, which comes off each logit first
     double sum = 0.0;
     for (int j = lane; j < a.k; j += kWave) {
       const float p = sp[j];
-      if (p != 0.f) sum += (double)p * (slp[j] - ((double)sz[j] * (double)a.c - l2));
+      if (p != 0.f) sum += (double)p * (slp[j] - (((double)sz[j] - (double)X) * (double)a.c - l2));
     }
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o, kWave);

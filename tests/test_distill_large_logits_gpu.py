@@ -169,3 +169,28 @@ def test_gradient_far_from_zero(dev, V, T):
     y = _beside(rng, V)
     ids, v, lse = _entries(rng, y, 3, T)
     _check_gradient(_distill(y, ids, v, lse, T, dev)[1], y, ids, v, lse, T)
+
+
+@pytest.mark.parametrize("T", TEMPERATURES)
+@pytest.mark.parametrize("V", ROWS)
+def test_loss_far_from_zero(dev, V, T):
+    import torch
+
+    rng = np.random.default_rng(V + 3)
+    x = _far(rng, V)
+    ids, v, lse = _teacher(rng, x.shape[0], V, 4)
+    v = v * T
+    for l in (lse, None):
+        _check_loss(_distill(x, ids, v, l, T, dev)[0], x, ids, v, l, T)
+    y = _beside(rng, V)
+    yi, yv, yl = _entries(rng, y, 3, T)
+    for l in (yl, None):
+        _check_loss(_distill(y, yi, yv, l, T, dev)[0], y, yi, yv, l, T)
+    # a teacher far from zero too: the softmax of its entries is that of their distances
+    far = torch.tensor(MASKS, dtype=torch.float64).repeat(3)[:x.shape[0], None].float()
+    w = torch.where(torch.arange(4) < 3, far, far * 2)
+    z = _normal(rng, x.shape[0], V)
+    loss, d = _distill(z, ids, w, None, T, dev)
+    shifted = (w.double() - far.double()).clamp(min=-1e38).float()
+    _check_loss(loss, z, ids, shifted, None, T)
+    _check_gradient(d, z, ids, shifted, None, T)
