@@ -272,8 +272,8 @@ __device__ __noinline__ void select_in_memory(const uint16_t* row, int V, int k,
 
 template <int NT, int NVEC>
 __global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restrict__ logits, int64_t ld, int k,
-                                                 float c, uint16_t* __restrict__ values, int32_t* __restrict__ ids,
-                                                 float* __restrict__ lse) {
+                                                 float c, double inv_t, uint16_t* __restrict__ values,
+                                                 int32_t* __restrict__ ids, float* __restrict__ lse) {
   constexpr int NW = NT / kWave;
   constexpr int kCand = NW == 1 ? 512 : 1024;            // candidates that are ranked
   constexpr int CAP = NW == 1 ? kCand : 2 * kCand / NW;  // and that a wave's list holds
@@ -443,7 +443,8 @@ __global__ __launch_bounds__(NT) void top_kernel(int V, const uint16_t* __restri
       ids[row * k + rank] = (int32_t)~(uint32_t)(me >> 16);
     }
   }
-  if (tid == NT - 1) lse[row] = (float)(((double)X * c + log2((double)S)) * 0.69314718055994530942);
+  // X / T in 64 bits: c's rounding would be as much as the logarithm where X / T is large
+  if (tid == NT - 1) lse[row] = (float)((double)X * inv_t + log2((double)S) * 0.69314718055994530942);
 }
 
 // ===========================================================================
@@ -624,16 +625,18 @@ int row_threads(int V) {
   return 1024;
 }
 
-void launch_top(hipStream_t st, int M, int V, const uint16_t* x, int64_t ld, int k, float c, uint16_t* values,
+void launch_top(hipStream_t st, int M, int V, const uint16_t* x, int64_t ld, int k, float t, uint16_t* values,
                 int32_t* ids, float* lse) {
+  const float c = kLog2e / t;
+  const double inv_t = 1.0 / t;
 #define NL_TOP(NT, NV)                                                                                           \
   if (V / 8 <= NT * NV) {                                                                                        \
-    hipLaunchKernelGGL((top_kernel<NT, NV>), dim3(M), dim3(NT), 0, st, V, x, ld, k, c, values, ids, lse);       \
+    hipLaunchKernelGGL((top_kernel<NT, NV>), dim3(M), dim3(NT), 0, st, V, x, ld, k, c, inv_t, values, ids, lse); \
     return;                                                                                                      \
   }
   NL_ROW_SIZES(NL_TOP)
 #undef NL_TOP
-  hipLaunchKernelGGL((top_kernel<1024, 0>), dim3(M), dim3(1024), 0, st, V, x, ld, k, c, values, ids, lse);
+  hipLaunchKernelGGL((top_kernel<1024, 0>), dim3(M), dim3(1024), 0, st, V, x, ld, k, c, inv_t, values, ids, lse);
 }
 
 template <bool kGrad>
@@ -673,7 +676,7 @@ extern "C" int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, 
   if (k > V) return nl_set_error(NL_EINVAL, "top_logits: k > V");
   if (M == 0) return NL_OK;
   if (!values || !ids || !lse) return nl_set_error(NL_EINVAL, "top_logits: null output");
-  launch_top((hipStream_t)stream, M, V, logits, ld, k, kLog2e / temperature, values, ids, lse);
+  launch_top((hipStream_t)stream, M, V, logits, ld, k, temperature, values, ids, lse);
   return nl_check_launch("nl_top_logits");
 }
 
