@@ -460,7 +460,7 @@ struct DistillArgs {
   const void* values;
   int values_f32;
   const float* lse;  // null: softmax over the row's entries
-  double cd;         // log2(e) / T
+  double inv_t;      // 1 / T
   float c;           // the same in 32 bits: the temperature that the student's row is taken at
   float t2ln2;       // T^2 ln 2
   float grad;        // scale T
@@ -484,12 +484,14 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
   Row<NT, NVEC> r;
   r.load(zrow, a.V, tid);
   // The first wave takes the teacher's entries, up to 4 a lane. They count in 64
-  // bits: the loss is a difference of logarithms that may nearly cancel.
+  // bits: the loss is a difference of logarithms that may nearly cancel. v / T - lse is
+  // rounded once: of two rounded products, 1.4e30 each, the rest would be 1e14.
   if (tid < kWave) {
     double lp[kMaxK / kWave];
     bool bad = false;
     double mx = -INFINITY;
-    const double sub = a.lse ? (double)a.lse[row] * 1.4426950408889634074 : 0.0;
+    constexpr double kLog2e64 = 1.4426950408889634074;
+    const double sub = a.lse ? (double)a.lse[row] : 0.0;
 #pragma unroll
     for (int e = 0; e < kMaxK / kWave; ++e) {
       const int j = e * kWave + lane;
@@ -503,7 +505,7 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       if (id >= 0) {
         const float v = a.values_f32 ? reinterpret_cast<const float*>(a.values)[at]
                                      : bf16_to_f32(reinterpret_cast<const uint16_t*>(a.values)[at]);
-        lp[e] = (double)v * a.cd - sub;
+        lp[e] = __builtin_fma((double)v, a.inv_t, -sub);
         if (id < a.V) z = bf16_to_f32(zrow[id]);
         else lp[e] = __builtin_nan("");
         bad |= lp[e] != lp[e];
@@ -518,12 +520,15 @@ __global__ __launch_bounds__(NT) void distill_kernel(DistillArgs a) {
       float s = 0.f;
 #pragma unroll
       for (int e = 0; e < kMaxK / kWave; ++e)
-        if (e * kWave < a.k) s += exp2_split(lp[e] - at);
+        if (e * kWave < a.k) s += exp2_split((lp[e] - at) * kLog2e64);
       s = wave_sum(s);
       // (the largest comes off first: beside a value of 1e17 the logarithm would be lost)
       const double l = s == 0.f ? 0.0 : log2((double)s);
 #pragma unroll
-      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] = (lp[e] - at) - l;
+      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] = (lp[e] - at) * kLog2e64 - l;
+    } else {
+#pragma unroll
+      for (int e = 0; e < kMaxK / kWave; ++e) lp[e] *= kLog2e64;
     }
     float S = 0.f;
 #pragma unroll
@@ -696,7 +701,7 @@ extern "C" int nl_distill_fwd_bwd(void* stream, int M, int V, const nl_bf16* log
       return nl_set_error(NL_EINVAL, "distill: dlogits over the logits need ld_dlogits == ld");
   }
   DistillArgs a{V, k, logits, ld, ids, ids_64 != 0, values, values_dtype == NL_DTYPE_F32, lse,
-                1.4426950408889634074 / temperature, kLog2e / temperature,
+                1.0 / temperature, kLog2e / temperature,
                 temperature * temperature * kLn2, scale * temperature, loss, dlogits, ld_dlogits,
                 (((uintptr_t)logits ^ (uintptr_t)dlogits) & 15) == 0 && (M == 1 || (ld - ld_dlogits) % 8 == 0)};
   if (dlogits) launch_distill<true>((hipStream_t)stream, M, a);

@@ -209,3 +209,30 @@ def test_lse_far_from_zero(dev, V, T):
     fine = np.isfinite(want32)
     np.testing.assert_array_equal(got[~fine], want32[~fine])  # X / T past fp32
     assert (np.abs(got[fine].astype(np.float64) - want[fine]) <= 2.0 ** -16 + U * np.abs(want[fine])).all()
+
+
+@pytest.mark.parametrize("T", [1.0, 2.0 ** -7, 1024.0])
+def test_teacher_far_from_zero(dev, T):
+    """p = exp(v / T - lse) where both are large: their difference, and none of their products' roundings."""
+    import torch
+    from nlearn_amd.kernels.distill import distill_cross_entropy, top_logits
+
+    rng = np.random.default_rng(77)
+    V, k = 700, 4
+    far = [a for a in MASKS + [3e4, 1e6, 1e10, 1e20, 1e30] if abs(a / T) < 3e38]
+    a = torch.tensor(far, dtype=torch.float64).to(torch.bfloat16)[:, None]
+    v = a.float().expand(-1, k).contiguous()
+    z = _normal(rng, len(far), V)
+    ids = _teacher(rng, len(far), V, k)[0]
+    lse = (a.double()[:, 0] / T).float()  # exact: T is a power of two
+    loss, d = _distill(z, ids, v, lse, T, dev)
+    ones, none = torch.zeros_like(v), torch.zeros_like(lse)  # every p is 1
+    _check_loss(loss, z, ids, ones, none, T)
+    _check_gradient(d, z, ids, ones, none, T)
+    if T == 1.0:  # a teacher whose mask leaves nothing: its logsumexp rounds to the mask itself
+        t = a[a[:, 0].abs().double() >= 1e9].expand(-1, V)
+        values, ids, lse = top_logits(t.to(dev), k)
+        y = z[:t.shape[0]].to(dev).requires_grad_(True)
+        loss = distill_cross_entropy(y, ids, values, lse)
+        loss.backward()
+        assert torch.isfinite(loss) and torch.isfinite(y.grad).all()
