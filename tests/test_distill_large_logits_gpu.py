@@ -79,9 +79,10 @@ def _check_loss(got, x, ids, v, lse, T):
     z, i = _from_max(x), ids.numpy()
     want, _, mass, spread = orc.distill(z, i, v.double().numpy(), None if lse is None else lse.double().numpy(), T, 1.0)
     on = i >= 0
-    with np.errstate(divide="ignore"):
+    with np.errstate(divide="ignore", invalid="ignore"):
         w = np.where(on, v.double().numpy() / T, -np.inf)
         p = np.exp(w - (orc.lse(w) if lse is None else lse.double().numpy())[:, None])
+        p = np.where(w > -np.inf, p, 0)
     e = np.where(p > 0, np.abs(np.take_along_axis(z, np.where(on, i, 0), 1)) / T, 0)
     lim = T * T * (2.0 ** -16 * mass + 2.0 ** -22 * (p * e).sum(1) + 2.0 ** -21 * spread) + U * np.abs(want)
     assert (np.abs(got - want) <= lim).all(), (got, want, lim)
@@ -236,3 +237,32 @@ def test_teacher_far_from_zero(dev, T):
         loss = distill_cross_entropy(y, ids, values, lse)
         loss.backward()
         assert torch.isfinite(loss) and torch.isfinite(y.grad).all()
+
+
+@pytest.mark.parametrize("T", [1.0, 2.5])
+@pytest.mark.parametrize("V", [90, 700, 9000, 60000, 120000])
+def test_loss_by_row_of_padding_repeats_and_odd_values(dev, V, T):
+    """Each row's loss within its own bound: padding, repeated ids, no weight, masks on either side."""
+    rng = np.random.default_rng(V)
+    x = _normal(rng, 12, V)
+    ids, v, lse = _entries(rng, x, 9, T)
+    ids[0, 4:] = -1
+    ids[1] = -7
+    ids[2] = -1
+    x[2] = float("nan")                    # a student's row that no entry reads
+    ids[3] = 5                             # one id, nine times
+    ids[4, 1::2] = ids[4, 0].item()
+    v[5, 3:] = float("-inf")
+    v[6] = float("-inf")                   # entries without weight
+    ids[7, 2:] = ids[7, :1]
+    ids[7, 6:8] = -1
+    x[8, 10:] = float("-inf")              # a masked vocabulary; the entries are inside
+    ids[8] = _teacher(rng, 1, 10, 9)[0][0]
+    x[9] = MASKS[-1]
+    x[9, ids[9, 0].item()] = 0.0
+    v[9, 1:] = float("-inf")
+    x[10] = 3.0
+    for l in (lse, None):
+        loss, d = _distill(x, ids, v, l, T, dev)
+        _check_loss(loss, x, ids, v, l, T)
+        assert (loss[[1, 2, 6]] == 0).all() and (d[[1, 2, 6]] == 0).all()
