@@ -448,9 +448,10 @@ __device__ __forceinline__ F8Item f8_item(const GemmF8Args& g, int item) {
   t.sb = g.sb + (int64_t)(t.n0 >> g.shb) * g.ldsb + t.kb0;
   t.ba = (uint32_t)((int64_t)(ra - 1) * g.lda + g.Kp);
   t.bb = (uint32_t)((int64_t)(rb - 1) * g.ldb + g.Kp);
-  // whole dwords of scales where rows hold them (the last one may end in padding)
-  t.bsa = (uint32_t)(((ra - 1) >> g.sha) * g.ldsa + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
-  t.bsb = (uint32_t)(((rb - 1) >> g.shb) * g.ldsb + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
+  // whole dwords of scales where rows hold them (the last one may end in padding); none
+  // without a block (K == 0, where the operands' pointers may be null)
+  t.bsa = t.nkb == 0 ? 0 : (uint32_t)(((ra - 1) >> g.sha) * g.ldsa + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
+  t.bsb = t.nkb == 0 ? 0 : (uint32_t)(((rb - 1) >> g.shb) * g.ldsb + (g.dw ? (t.nkb + 3) / 4 * 4 : t.nkb));
   return t;
 }
 

@@ -443,3 +443,24 @@ def test_linear_is_its_parts(dev, M, K, N, xdtype, wdtype):
     assert torch.equal(y, gemm_fp8(qx, wf, x.dtype))
     assert torch.equal(x.grad, gemm_fp8(qd, wb, x.dtype))
     assert torch.equal(W.grad, gemm_fp8(qxt, qdt, W.dtype))
+
+
+@pytest.mark.parametrize("M,N", [(1, 1), (5, 300), (300, 130), (4096, 4104)])
+def test_gemm_without_a_sum_reads_nothing(dev, M, N):
+    """K == 0 writes zeros whatever the operands' strides are, without reading them: their pointers may be null."""
+    import torch
+    from nlearn_amd import _lib
+    from nlearn_amd.kernels.fp8 import Fp8Blocks, gemm_fp8
+
+    for dt, code in ((torch.float32, 0), (torch.bfloat16, 1)):
+        for lds in (0, 1, 4, 8):
+            for ga, gb in ((1, 1), (1, 128), (128, 128)):
+                out = torch.full((M, (N + 7) // 8 * 8), 7.0, dtype=dt, device=dev)
+                _lib.call("nl_gemm_fp8", _lib.stream_of(out), M, N, 0, None, 128, None, lds, ga, None, 128, None, lds, gb,
+                          out.data_ptr(), code, out.stride(0), None, 0)
+                assert (out[:, :N] == 0).all() and (out[:, N:] == 7).all()
+        # rows of eight scale bytes of which none belongs to the operand
+        blocks = [Fp8Blocks(torch.empty((rows, 128), dtype=torch.float8_e4m3fn, device=dev)[:, :0],
+                            torch.empty((rows, 8), dtype=torch.float8_e8m0fnu, device=dev)[:, :0], (rows, 0))
+                  for rows in (M, N)]
+        assert (gemm_fp8(*blocks, dt) == 0).all()
