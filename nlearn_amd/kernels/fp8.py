@@ -213,6 +213,15 @@ def _rows(t: torch.Tensor):
     return t, s0 if rows > 1 else cols
 
 
+def _main_grad(W: torch.Tensor):
+    """W's gradient buffer (or None), which the product is written into as an array of W's shape."""
+    mg = grad_buffer(W)
+    if mg is not None and (mg.shape != W.shape or mg.device != W.device):
+        raise ValueError(f"linear_fp8: main_grad {tuple(mg.shape)} on {mg.device} is not laid out like the weight "
+                         f"{tuple(W.shape)} on {W.device}")
+    return mg
+
+
 class _LinearFp8(torch.autograd.Function):
     """Both directions are one call of the library each: the host's share of a small
     product is what it costs (15 us against 55 for a forward pass call by call)."""
@@ -241,7 +250,7 @@ class _LinearFp8(torch.autograd.Function):
         (W,) = ctx.saved_tensors
         need_dx, need_dW = ctx.need
         M, K, N, x_dtype = ctx.sizes
-        mg = grad_buffer(W) if need_dW else None
+        mg = _main_grad(W) if need_dW else None
         dev = dy.device
         dx = _result(M, K, x_dtype, dev) if need_dx else None                  # dY . W^T
         # X^T . dY, straight into main_grad where its rows are aligned for the product's stores

@@ -217,3 +217,21 @@ def test_sizes_past_32_bits_are_refused():
         distill.top_logits(x, 3)
     with pytest.raises(ValueError, match=r"2\^31"):
         distill.distill_cross_entropy(x, torch.zeros((1, 3), dtype=torch.int32).expand(n, 3), torch.zeros((1, 3)).expand(n, 3))
+
+
+def test_main_grad_of_another_shape_is_refused():
+    """The weight gradient is written with the buffer's row stride: a buffer that is not W's shape would be overrun."""
+    import torch
+    from nlearn_amd.kernels import fp8
+
+    W = torch.zeros((128, 40), requires_grad=True)
+    assert fp8._main_grad(W) is None
+    W.main_grad = torch.zeros((128, 40))
+    assert fp8._main_grad(W) is W.main_grad
+    for shape in ((40, 128), (128, 41), (127, 40), (5120,), (128, 40, 1)):
+        W.main_grad = torch.zeros(shape)
+        with pytest.raises(ValueError, match="main_grad"):
+            fp8._main_grad(W)
+    W.main_grad = torch.zeros((128, 40), device="meta")
+    with pytest.raises(ValueError, match="main_grad"):
+        fp8._main_grad(W)

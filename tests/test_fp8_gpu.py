@@ -464,3 +464,16 @@ def test_gemm_without_a_sum_reads_nothing(dev, M, N):
                             torch.empty((rows, 8), dtype=torch.float8_e8m0fnu, device=dev)[:, :0], (rows, 0))
                   for rows in (M, N)]
         assert (gemm_fp8(*blocks, dt) == 0).all()
+
+
+def test_linear_main_grad_of_another_shape_is_refused(dev):
+    import torch
+    from nlearn_amd.kernels.fp8 import linear_fp8
+
+    x = torch.ones((8, 128), dtype=torch.bfloat16, device=dev)
+    W = torch.ones((128, 40), device=dev, requires_grad=True)
+    for buf in (torch.full((40, 128), 7.0, device=dev), torch.full((5120,), 7.0, device=dev), torch.full((128, 40), 7.0)):
+        W.main_grad = buf
+        with pytest.raises(ValueError, match="main_grad"):
+            linear_fp8(x, W).sum().backward()
+        assert (buf == 7).all()
