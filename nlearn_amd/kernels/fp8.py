@@ -230,27 +230,31 @@ class _LinearFp8(torch.autograd.Function):
     def forward(ctx, x2, W, need_dx, need_dW):
         ctx.need = need_dx, need_dW
         (M, K), N = x2.shape, W.shape[1]
-        ctx.save_for_backward(W)
-        ctx.sizes = (M, K, N, x2.dtype)
+        ctx.sizes = (M, K, N, x2.dtype, W.dtype, W.is_contiguous())
+        # for its main_grad alone, so not by a saved tensor, which a hook or a checkpoint hands back as another object
+        ctx.W = W if need_dW and (W.is_leaf or grad_buffer(W) is not None) else None
         y = _result(M, N, x2.dtype, x2.device)
         if M == 0 or K == 0 or N == 0:
+            ctx.save_for_backward(None)
             return y.zero_()
         saved_bytes, wsb, _ = _linear_bytes(M, K, N, need_dx, need_dW)
-        ctx.saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x2.device)
+        saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x2.device)
+        # with autograd, which frees it after the backward pass and shows it to hooks and checkpoints
+        ctx.save_for_backward(saved)
         ws = torch.empty(wsb, dtype=torch.uint8, device=x2.device)
         (x2, ldx), (Wr, ldw) = _rows(x2), _rows(W)
         _lib.call_on(x2, "nl_linear_fp8_fwd", M, K, N, x2.data_ptr(), _code(x2), ldx, Wr.data_ptr(), _code(Wr), ldw,
-                     y.data_ptr(), _code(y), _ld(y), need_dx, need_dW, ctx.saved.data_ptr(), saved_bytes,
+                     y.data_ptr(), _code(y), _ld(y), need_dx, need_dW, saved.data_ptr(), saved_bytes,
                      ws.data_ptr(), wsb)
         return y
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        (W,) = ctx.saved_tensors
+        (saved,) = ctx.saved_tensors
         need_dx, need_dW = ctx.need
-        M, K, N, x_dtype = ctx.sizes
-        mg = _main_grad(W) if need_dW else None
+        M, K, N, x_dtype, w_dtype, w_dense = ctx.sizes
+        mg = _main_grad(ctx.W) if ctx.W is not None else None
         dev = dy.device
         dx = _result(M, K, x_dtype, dev) if need_dx else None                  # dY . W^T
         # X^T . dY, straight into main_grad where its rows are aligned for the product's stores
@@ -258,10 +262,11 @@ class _LinearFp8(torch.autograd.Function):
         dW = None
         if direct:
             dW = mg
-        elif mg is None and need_dW and W.is_contiguous() and N % 8 == 0:
-            dW = torch.empty_like(W)  # laid out like W: autograd keeps it as W.grad without a copy
+        elif mg is None and need_dW and w_dense and N % 8 == 0:
+            # laid out like W: autograd keeps it as W.grad without a copy
+            dW = torch.empty((K, N), dtype=w_dtype, device=dev)
         elif need_dW:
-            dW = _result(K, N, W.dtype if mg is None else _F32, dev)
+            dW = _result(K, N, w_dtype if mg is None else _F32, dev)
         if M == 0 or K == 0 or N == 0:
             for t in (dx, mg if mg is not None else dW):
                 if t is not None:
@@ -270,7 +275,7 @@ class _LinearFp8(torch.autograd.Function):
         dy, lddy = _rows(dy if dy.dtype in (_BF16, _F32) else dy.to(_F32))
         saved_bytes, _, wsb = _linear_bytes(M, K, N, need_dx, need_dW)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-        _lib.call_on(dy, "nl_linear_fp8_bwd", M, K, N, dy.data_ptr(), _code(dy), lddy, ctx.saved.data_ptr(), saved_bytes,
+        _lib.call_on(dy, "nl_linear_fp8_bwd", M, K, N, dy.data_ptr(), _code(dy), lddy, saved.data_ptr(), saved_bytes,
                      need_dx, need_dW,
                      *((dx.data_ptr(), _code(dx), _ld(dx)) if need_dx else (None, 0, 0)),
                      *((dW.data_ptr(), _code(dW), _ld(dW)) if need_dW else (None, 0, 0)), ws.data_ptr(), wsb)

@@ -477,3 +477,58 @@ def test_linear_main_grad_of_another_shape_is_refused(dev):
         with pytest.raises(ValueError, match="main_grad"):
             linear_fp8(x, W).sum().backward()
         assert (buf == 7).all()
+
+
+def test_linear_keeps_its_operands_with_autograd(dev):
+    """What the backward reads is freed by it though the loss lives on, passes through saved-tensor hooks,
+    and is not kept by a checkpoint."""
+    import torch
+    from torch.utils.checkpoint import checkpoint
+    from nlearn_amd.kernels.fp8 import linear_fp8
+
+    rng = _rng(51)
+    M, K, N = 4096, 512, 256
+    x = torch.from_numpy(_matrix(rng, M, K)).to(dev).to(torch.bfloat16).requires_grad_(True)
+    W = torch.from_numpy(_matrix(rng, K, N)).to(dev).requires_grad_(True)
+    dy = torch.from_numpy(_matrix(rng, M, N)).to(dev).to(torch.bfloat16)
+    linear_fp8(x, W).backward(dy)
+    want = x.grad.clone(), W.grad.clone()
+    kept = M * K + K * N  # bytes of X^T and W in 8 bits
+
+    def grown(call):
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated(dev)
+        out = call()
+        return out, torch.cuda.memory_allocated(dev) - before
+
+    x.grad = W.grad = None
+    y, more = grown(lambda: linear_fp8(x, W))
+    assert more >= M * N * 2 + kept
+    def back():
+        y.backward(dy, retain_graph=False)
+        grads, x.grad, W.grad = (x.grad, W.grad), None, None
+        return [torch.equal(g, w) for g, w in zip(grads, want)]
+    same, less = grown(back)
+    assert all(same) and less <= -kept  # y itself is still held
+
+    packed = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: packed.append(t.numel() * t.element_size()) or t.cpu(),
+                                                  lambda t: t.to(dev)):
+        y = linear_fp8(x, W)
+    assert any(n >= kept for n in packed)
+    y.backward(dy)
+    assert torch.equal(x.grad, want[0]) and torch.equal(W.grad, want[1])
+
+    x.grad = W.grad = None
+    y, more = grown(lambda: checkpoint(linear_fp8, x, W, use_reentrant=False))
+    assert more < M * N * 2 + kept
+    y.backward(dy)
+    assert torch.equal(x.grad, want[0]) and torch.equal(W.grad, want[1])
+    x.grad = W.grad = None
+    W.main_grad = torch.full((K, N), float("nan"), device=dev)
+    checkpoint(linear_fp8, x, W, use_reentrant=False).backward(dy)
+    assert W.grad is None and torch.equal(W.main_grad, want[1])
+    # nothing kept where nothing is summed
+    e = torch.empty((0, K), dtype=torch.bfloat16, device=dev, requires_grad=True)
+    linear_fp8(e, W).sum().backward()
+    assert e.grad.shape == (0, K)
