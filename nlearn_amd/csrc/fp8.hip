@@ -936,14 +936,14 @@ int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t l
 }
 
 int64_t blocks_of(int64_t n) { return (n + kB - 1) / kB; }
-// a launch has fewer than 2^32 threads: 16 a block of 128 by rows, 512 a tile
-constexpr int64_t kMaxBlocks = (int64_t)1 << 28, kMaxTiles = (int64_t)1 << 23;
+// a launch has fewer than 2^32 threads: 16 a block of 128 by rows in whole groups of 256, 512 a tile
+constexpr int64_t kMaxBlocks = ((int64_t)1 << 28) - 16, kMaxTiles = ((int64_t)1 << 23) - 1;
 
 int quantize_one(hipStream_t st, const QuantArgs& a, int dtype) {
   const int64_t rb = blocks_of(a.rows), cb = blocks_of(a.cols);
   if (!a.qt && a.group == 1) {
     const int64_t blocks = a.rows * cb;
-    if (blocks >= kMaxBlocks) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^28 blocks and more");
+    if (blocks > kMaxBlocks) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: more than 2^28 - 16 blocks");
     const dim3 grid((unsigned)((blocks + 15) / 16));
     if (dtype == NL_DTYPE_BF16)
       hipLaunchKernelGGL((quantize_rows_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
@@ -951,7 +951,7 @@ int quantize_one(hipStream_t st, const QuantArgs& a, int dtype) {
       hipLaunchKernelGGL((quantize_rows_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     return nl_check_launch("nl_quantize_fp8");
   }
-  if (rb * cb >= kMaxTiles) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
+  if (rb * cb > kMaxTiles) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
   const dim3 grid((unsigned)(rb * cb));
   if (dtype == NL_DTYPE_BF16)
     hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(512), 0, st, a, (uint32_t)cb);
@@ -964,7 +964,7 @@ int quantize_one(hipStream_t st, const QuantArgs& a, int dtype) {
 int quantize_two(hipStream_t st, const QuantArgs& a, int a_dtype, const QuantArgs& b, int b_dtype) {
   const int64_t ca = blocks_of(a.cols), cb = blocks_of(b.cols);
   const int64_t na = blocks_of(a.rows) * ca, nb = blocks_of(b.rows) * cb;
-  if ((!a.qt && a.group == 1) || (!b.qt && b.group == 1) || na + nb >= kMaxTiles) {
+  if ((!a.qt && a.group == 1) || (!b.qt && b.group == 1) || na + nb > kMaxTiles) {
     if (int rc = quantize_one(st, a, a_dtype)) return rc;
     return quantize_one(st, b, b_dtype);
   }

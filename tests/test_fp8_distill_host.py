@@ -235,3 +235,16 @@ def test_main_grad_of_another_shape_is_refused():
     W.main_grad = torch.zeros((128, 40), device="meta")
     with pytest.raises(ValueError, match="main_grad"):
         fp8._main_grad(W)
+
+
+def test_launches_of_2_to_the_32_threads_are_refused():
+    """16 blocks of 128 a workgroup of 256: the last count below 2^28 that fits is 2^28 - 16."""
+    from nlearn_amd import _lib
+
+    L = _lib.load()
+    for rows in ((1 << 28) - 15, (1 << 28) - 1, 1 << 28):
+        assert L.nl_quantize_fp8(None, rows, 8, 256, 1, 8, 1, 512, 128, 1024, 1, None, 0, None, 0) == _lib.NL_EUNSUPPORTED
+        assert b"blocks" in L.nl_last_error()
+    # tiles of 128 x 128 and 512 threads: 2^23 of them
+    assert L.nl_quantize_fp8(None, 1 << 29, 256, 256, 1, 256, 128, 512, 256, 1024, 2, None, 0, None, 0) == _lib.NL_EUNSUPPORTED
+    assert b"tiles" in L.nl_last_error()
