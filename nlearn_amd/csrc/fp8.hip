@@ -891,6 +891,9 @@ void launch_f8(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
                        dim3(256), 0, st, g, p.splits);
 }
 
+// 256 rows of a tile are addressed with 31-bit offsets: bytes of an operand's row, elements of a result's
+constexpr int64_t kMaxLd = INT32_MAX / 256, kMaxLdc = INT32_MAX / 256 / 4;
+
 // The checks of one quantised operand: rows x K, group rows per scale.
 int check_operand(const char* what, int64_t rows, int64_t K, const void* q, int64_t ld, const void* s, int64_t lds,
                   int group) {
@@ -1014,9 +1017,8 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
   if (ldc < N) return nl_set_error(NL_EINVAL, "gemm_fp8: ldc < N");
   if (((uintptr_t)C & 15) || ldc % 8) return nl_set_error(NL_EALIGN, "gemm_fp8: C needs 16-byte aligned rows");
   const int64_t Kp = ((int64_t)K + kB - 1) / kB * kB;
-  // 256 rows of a tile are addressed with 31-bit offsets
-  if (ldc > INT32_MAX / 256 / 4) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of C of 2 million elements and more");
-  if (lda > INT32_MAX / 256 || ldb > INT32_MAX / 256 || ldsa > INT32_MAX / 256 || ldsb > INT32_MAX / 256)
+  if (ldc > kMaxLdc) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of C of 2 million elements and more");
+  if (lda > kMaxLd || ldb > kMaxLd || ldsa > kMaxLd || ldsb > kMaxLd)
     return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of 8 MiB and more");
   F8Plan p = f8_plan(M, N, K);
   if (p.tiles < 0 || (int64_t)p.tiles * p.splits > INT32_MAX) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: too many tiles");
@@ -1110,6 +1112,18 @@ int check_linear(const char* what, int M, int K, int N, const void* buf, size_t 
   return NL_OK;
 }
 
+// What the backward of a forward pass would refuse is refused before it: X^T's rows of M bytes,
+// dX's of K elements (128 columns of padding at most), dY by rows.
+int check_gradients(int M, int K, int N, bool dx, bool dw) {
+  if (dw && blocks_of(M) * kB > kMaxLd)
+    return nl_set_error(NL_EUNSUPPORTED, "linear_fp8_fwd: a weight gradient over more than 8388480 rows");
+  if (dx && K > kMaxLdc - kB)
+    return nl_set_error(NL_EUNSUPPORTED, "linear_fp8_fwd: an input gradient of more than 2 million columns");
+  if (dx && !dw && M * blocks_of(N) > kMaxBlocks)
+    return nl_set_error(NL_EUNSUPPORTED, "linear_fp8_fwd: an output gradient of more than 2^28 - 16 blocks");
+  return NL_OK;
+}
+
 }  // namespace
 }  // namespace nl
 
@@ -1129,6 +1143,7 @@ extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* 
                                  int need_dx, int need_dw, void* saved, size_t saved_bytes, void* ws,
                                  size_t ws_bytes) {
   if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_fwd: need M, K, N > 0");
+  if (int rc = check_gradients(M, K, N, need_dx != 0, need_dw != 0)) return rc;
   const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
   if (int rc = check_linear("linear_fp8_fwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
   if (int rc = check_linear("linear_fp8_fwd", M, K, N, ws, ws_bytes, p.fwd + (int64_t)p.ws_fwd, "workspace")) return rc;

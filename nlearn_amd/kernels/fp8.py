@@ -27,6 +27,8 @@ _E4M3 = torch.float8_e4m3fn
 _E8M0 = torch.float8_e8m0fnu
 _NONE = (None, 0, None, 0)  # an output that is not wanted
 BLOCK = 128
+MAX_COLUMNS = ((1 << 31) - 1) // 1024  # of a product's result: 256 rows of them within 31-bit offsets
+MAX_BLOCKS = (1 << 28) - 16            # of a matrix quantised by rows: a launch has fewer than 2^32 threads
 
 
 def _check_sizes(what: str, *sizes: int) -> None:
@@ -319,6 +321,10 @@ def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     _check_sizes("linear_fp8", *x2.shape, W.shape[1])
     if frozen is not None:
+        if x2.requires_grad and torch.is_grad_enabled():  # what the product of dY would refuse
+            M, (K, N) = x2.shape[0], W.shape
+            if K > MAX_COLUMNS - BLOCK or M * ((N + BLOCK - 1) // BLOCK) > MAX_BLOCKS:
+                raise ValueError(f"linear_fp8: no input gradient of ({M}, {K}) from an output gradient of ({M}, {N})")
         y = _LinearFp8Frozen.apply(x2, frozen)
     else:
         if W.dtype not in (_BF16, _F32):

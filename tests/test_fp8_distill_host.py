@@ -248,3 +248,29 @@ def test_launches_of_2_to_the_32_threads_are_refused():
     # tiles of 128 x 128 and 512 threads: 2^23 of them
     assert L.nl_quantize_fp8(None, 1 << 29, 256, 256, 1, 256, 128, 512, 256, 1024, 2, None, 0, None, 0) == _lib.NL_EUNSUPPORTED
     assert b"tiles" in L.nl_last_error()
+
+
+def test_forward_refuses_what_its_backward_would():
+    import torch
+    from nlearn_amd import _lib
+    from nlearn_amd.kernels import fp8
+
+    L = _lib.load()
+
+    def forward(M, K, N, dx, dw):
+        saved, ws = L.nl_linear_fp8_saved_bytes(M, K, N, dx, dw), L.nl_linear_fp8_ws_bytes(M, K, N, 0, dx, dw)
+        return L.nl_linear_fp8_fwd(None, M, K, N, 256, 1, K, 512, 0, N, 1024, 1, (N + 7) // 8 * 8, dx, dw, 2048, saved, 4096,
+                                   ws)
+
+    for M, K, N, dx, dw, what in ((8388481, 16, 8, 0, 1, b"8388480 rows"), (8388608, 16, 8, 1, 1, b"8388480 rows"),
+                                  (4, 2097024, 8, 1, 0, b"columns"), (1 << 27, 16, 256, 1, 0, b"blocks")):
+        assert forward(M, K, N, dx, dw) == _lib.NL_EUNSUPPORTED and what in L.nl_last_error(), (M, K, N)
+
+    def frozen(M, K, N):
+        W = fp8.Fp8Weight.__new__(fp8.Fp8Weight)
+        W.shape = (K, N)
+        return fp8.linear_fp8(torch.zeros((1, 1), dtype=torch.bfloat16).expand(M, K).requires_grad_(True), W)
+
+    for shape in ((4, 2097024, 8), (1 << 27, 16, 256)):
+        with pytest.raises(ValueError, match="no input gradient"):
+            frozen(*shape)
