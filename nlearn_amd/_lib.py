@@ -186,41 +186,23 @@ def stream_of(t) -> int:
 
 
 _cuda = None   # (torch.cuda, current device, current raw stream of a device), looked up once
-_held = None   # the library through calls that keep Python's lock
-
-
-def _load_held():
-    """The library loaded for ``call_on``: a launch returns in a few microseconds,
-    less than handing Python's lock over and back costs on autograd's thread."""
-    global _cuda, _held
-    import torch
-
-    load()
-    _cuda = (torch.cuda, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
-    held = ctypes.PyDLL(str(LIB_PATH))
-    for name, argtypes in _SIGNATURES.items():
-        fn = getattr(held, name)
-        fn.argtypes = argtypes
-        fn.restype = _RESTYPES.get(name, ctypes.c_int)
-    _held = held
 
 
 def call_on(t, name: str, *args) -> None:
     """``call(name, stream, *args)`` on the current stream of the tensor ``t``'s
-    device, with that device current for the launch."""
-    if _held is None:
-        _load_held()
+    device, with that device current for the launch (and for a probe's events)."""
+    global _cuda
+    if _cuda is None:
+        import torch
+
+        _cuda = (torch.cuda, torch._C._cuda_getDevice, torch._C._cuda_getCurrentRawStream)
     index = t.get_device()
-    if index < 0 or _probe is not None:
+    if index < 0:
         return call(name, stream_of(t), *args)
     if index == _cuda[1]():
-        rc = getattr(_held, name)(_cuda[2](index), *args)
-    else:
-        with _cuda[0].device(index):
-            rc = getattr(_held, name)(_cuda[2](index), *args)
-    if rc != NL_OK:
-        msg = _held.nl_last_error().decode() or _held.nl_strerror(rc).decode()
-        raise NlError(name, rc, msg)
+        return call(name, _cuda[2](index), *args)
+    with _cuda[0].device(index):
+        return call(name, _cuda[2](index), *args)
 
 
 def ws_bytes(batch: int, heads: int, seq: int) -> int:
