@@ -532,3 +532,24 @@ def test_linear_keeps_its_operands_with_autograd(dev):
     e = torch.empty((0, K), dtype=torch.bfloat16, device=dev, requires_grad=True)
     linear_fp8(e, W).sum().backward()
     assert e.grad.shape == (0, K)
+
+
+@pytest.mark.parametrize("ga,gb", [(1, 1), (1, 128), (128, 128)])
+@pytest.mark.parametrize("M,N,K", [(4097, 4099, 300), (4095, 4352, 1100), (4096, 4608, 128), (130, 200, 640)])
+def test_gemm_with_compact_scale_rows(dev, M, N, K, ga, gb):
+    """Scale rows that are no whole dwords, on large tiles (several a workgroup) and small ones: against float64,
+    and bit for bit what the same scales in padded rows give."""
+    import torch
+    from nlearn_amd.kernels.fp8 import gemm_fp8
+
+    results = []
+    for padded in ((False, False), (True, True), (False, True)):
+        rng = _rng(M, N, K, 61)
+        a, a64 = _operand(rng, M, K, ga, dev, padded[0])
+        b, b64 = _operand(rng, N, K, gb, dev, padded[1])
+        assert (a.scale.stride(0) % 4 == 0) == padded[0] or a.scale.shape[0] == 1
+        results.append([gemm_fp8(a, b, dt) for dt in (torch.float32, torch.bfloat16)])
+    for out in results[0]:
+        _check_product(out, a64, b64, K)
+    for other in results[1:]:
+        assert all(torch.equal(p, q) for p, q in zip(results[0], other))
