@@ -462,7 +462,8 @@ int nl_embedding_bwd(void* stream, int batch, int seq, int D, int vocab, const i
  * up to 128; the bytes past K of the last block are zero), and scale, one e8m0
  * byte s for each block of 128 along K and each `group` rows (group 1 or 128;
  * row r's scales are row r / group, lds bytes apart):
- *     value[r][k] = q[r][k] * 2^(scale[r / group][k / 128] - 127).
+ *     value[r][k] = q[r][k] * 2^(scale[r / group][k / 128] - 127)
+ * for scale bytes 0 to 254; byte 255 makes the block's values NaN.
  * q needs 16-byte aligned rows; scale rows that are a multiple of 4 bytes and
  * start on 4 bytes are read four blocks at a time.
  */
@@ -482,8 +483,10 @@ int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const void* x, int
                     uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst);
 
 /* C[M][N] = A . B^T for A of M x K and B of N x K values as above, summed in
- * fp32, written as fp32 or bf16 (to nearest even). C: 16-byte aligned, ldc a
- * multiple of 8. K == 0 writes zeros. Rows of A and B are below 8 MiB. A small C
+ * fp32, written as fp32 or bf16 (to nearest even). An fp32 result holds for scale
+ * bytes 3 to 246: its operands are widened to bf16, on whose grid (multiples of
+ * 2^-133) and below 2^128 their values must lie.
+ * C: 16-byte aligned, ldc a multiple of 8. K == 0 writes zeros. Rows of A and B are below 8 MiB. A small C
  * with a long K is split over K into fp32 partials in the caller's workspace
  * (nl_gemm_fp8_ws_bytes(); 0: none), summed in a fixed order; a NULL or smaller
  * workspace just disables the split. */

@@ -349,8 +349,11 @@ __device__ __forceinline__ uint32_t scales4(__amdgpu_buffer_rsrc_t rs, uint32_t 
   }
 }
 
-// 16 e4m3 bytes times a power of two (given as the float it is) to two fragments
-// of 8 bf16. Exact: 4 significant bits in 8, and bf16 has the range of the scales.
+// 16 e4m3 bytes times a power of two (given as its scale byte in a float's exponent) to two
+// fragments of 8 bf16: 4 significant bits in 8. Exact for scale bytes 3 to 246, with which
+// 2^-9 is at bf16's least subnormal, 2^-133, and 448 below its largest value. Below, values of
+// e4m3's subnormals lose bits; above, values of 2^128 and more are infinite. No share of the
+// exponent can be moved to the result: a lane's rows have scales of their own in every block.
 __device__ __forceinline__ void widen(const u32x4& v, float scale, bf16x8 out[2]) {
   uint32_t w[8];
 #pragma unroll

@@ -149,7 +149,8 @@ def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:
 
 def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | None = None,
              ws: torch.Tensor | None = None) -> torch.Tensor:
-    """a (M, K) . b (N, K)^T -> (M, N), summed in fp32, on the current stream.
+    """a (M, K) . b (N, K)^T -> (M, N), summed in fp32, on the current stream. An fp32
+    result holds for scale bytes 3 to 246.
     out: fp32 or bf16 with 16-byte aligned rows. ws: as ``gemm_fp8_ws`` gives it
     (allocated here if None; too small a one is not used and K is summed in one piece)."""
     (M, K), (N, Kb) = a.shape, b.shape

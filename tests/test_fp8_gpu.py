@@ -553,3 +553,32 @@ def test_gemm_with_compact_scale_rows(dev, M, N, K, ga, gb):
         _check_product(out, a64, b64, K)
     for other in results[1:]:
         assert all(torch.equal(p, q) for p, q in zip(results[0], other))
+
+
+@pytest.mark.parametrize("dtype,least,largest", [("float32", 3, 246), ("bfloat16", 0, 254)])
+def test_gemm_scale_bytes_of_the_whole_range(dev, dtype, least, largest):
+    """Every e4m3 value at scale bytes from end to end of the range that holds for a result's type, times values
+    whose scale makes the products ordinary: single products, exact in fp32 and rounded once in bf16."""
+    import torch
+    from nlearn_amd.kernels.fp8 import Fp8Blocks, gemm_fp8
+
+    table = orc.e4m3_table()
+    each = np.array([b for b in range(256) if np.isfinite(table[b])], np.uint8)
+
+    def operand(values, byte):
+        q = np.zeros((len(values), 128), np.uint8)
+        q[:, 77] = values
+        s = np.full((len(values), 1), byte, np.uint8)
+        return Fp8Blocks(torch.from_numpy(q).to(dev).view(torch.float8_e4m3fn),
+                         torch.from_numpy(s).to(dev).view(torch.float8_e8m0fnu), (len(values), 128))
+
+    few = np.array([0x01, 0x38, 0x7e, 0xb8], np.uint8)  # 2^-9, 1, 448, -1
+    want = torch.from_numpy(table[each][:, None] * table[few][None]).to(dev, getattr(torch, dtype))
+    for byte in sorted({least, least + 1, least + 5, 64, 127, 190, largest - 5, largest - 1, largest}):
+        against = min(max(254 - byte, least), largest)
+        f = 2.0 ** (byte + against - 254)  # 1 but where the ranges' ends are not alike
+        a, b = operand(each, byte), operand(few, against)
+        assert torch.equal(gemm_fp8(a, b, want.dtype), want * f), byte
+        assert torch.equal(gemm_fp8(b, a, want.dtype), want.t() * f), byte
+    # byte 255 is e8m0's NaN
+    assert torch.isnan(gemm_fp8(operand(few, 255), operand(few, 127), want.dtype)).all()
