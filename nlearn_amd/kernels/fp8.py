@@ -3,7 +3,7 @@
 * ``quantize_fp8(x)`` / ``quantize_fp8_both(x)``: a matrix to e4m3 values with one
   power-of-two scale for each block of 128 along the summed axis, per row
   (``group=1``: activations, gradients) or per 128 rows (``group=128``: weights).
-* ``gemm_fp8(a, b)``: a . b^T of two such operands, fp32 sums, bf16 or fp32 out.
+* ``gemm_fp8(a, b)``: a . b^T of two such operands, bf16 or fp32 out.
 * ``linear_fp8(x, W)``: ``linear(x, W)`` with all three products in 8 bits: y = x W,
   dX = dY W^T and dW = X^T dY, every operand quantised along the axis that its
   product sums over. ``fp8_weight(W)`` lays a frozen weight out once.
@@ -149,8 +149,10 @@ def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:
 
 def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | None = None,
              ws: torch.Tensor | None = None) -> torch.Tensor:
-    """a (M, K) . b (N, K)^T -> (M, N), summed in fp32, on the current stream. An fp32
-    result holds for scale bytes 3 to 246.
+    """a (M, K) . b (N, K)^T -> (M, N) on the current stream. An fp32 result is summed in
+    fp32 (scale bytes 3 to 246). A bf16 result is summed by the 8-bit matrix instruction,
+    which cuts 8 products at a time to 2^-13 of the largest of them: beside a bf16 rounding
+    that does not count, unless products cancel to a small part of their size.
     out: fp32 or bf16 with 16-byte aligned rows. ws: as ``gemm_fp8_ws`` gives it
     (allocated here if None; too small a one is not used and K is summed in one piece)."""
     (M, K), (N, Kb) = a.shape, b.shape
@@ -304,7 +306,8 @@ class _LinearFp8Frozen(torch.autograd.Function):
 
 
 def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
-    """x[..., K] @ W[K, N] -> [..., N] in x's dtype, with 8-bit products.
+    """x[..., K] @ W[K, N] -> [..., N] in x's dtype, with 8-bit products (as ``gemm_fp8``
+    sums them for that dtype; dW's go by W's, or by main_grad's).
 
     W: an fp32 or bf16 weight, quantised here, or an ``Fp8Weight`` (frozen: it gets
     no gradient). The gradients are those of the product of the quantised

@@ -582,3 +582,26 @@ def test_gemm_scale_bytes_of_the_whole_range(dev, dtype, least, largest):
         assert torch.equal(gemm_fp8(b, a, want.dtype), want.t() * f), byte
     # byte 255 is e8m0's NaN
     assert torch.isnan(gemm_fp8(operand(few, 255), operand(few, 127), want.dtype)).all()
+
+
+def test_gemm_of_cancelling_products(dev):
+    """Large products that cancel and a small one beside them: an fp32 result is the small one, a bf16 result is
+    within the cut that the header states."""
+    import torch
+    from nlearn_amd.kernels.fp8 import Fp8Blocks, gemm_fp8
+
+    rng = _rng(71)
+    M, N, K = 40, 24, 512
+    a, b = np.zeros((M, K)), np.zeros((N, K))
+    at = np.stack([rng.permutation(K)[:3] for _ in range(M)])
+    for m in range(M):
+        a[m, at[m]] = 256.0, -256.0, 2.0 ** rng.integers(-6, 1)
+        b[:, at[m]] = 1.0
+    operands = []
+    for x in (a, b):
+        q, s = orc.e4m3_bytes(x), np.full((x.shape[0], K // 128), 127, np.uint8)
+        operands.append((Fp8Blocks(torch.from_numpy(q).to(dev).view(torch.float8_e4m3fn),
+                                   torch.from_numpy(s).to(dev).view(torch.float8_e8m0fnu), x.shape), _values(q, s, 1, K, dev)))
+    (qa, a64), (qb, b64) = operands
+    assert torch.equal(gemm_fp8(qa, qb, torch.float32).double(), a64[0] @ b64[0].t())
+    _check_product(gemm_fp8(qa, qb, torch.bfloat16), a64, b64, K)
