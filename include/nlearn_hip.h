@@ -506,10 +506,12 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
  * 128 along K, W of 128 x 128), and its gradients from dy[M][N]: dx = dy . W^T (dy in
  * blocks along N) and dW = x^T . dy (x^T and dy^T in blocks along M), each the product
  * of the quantised operands. x, W, dy are fp32 or bf16 as nl_quantize_fp8 takes them,
- * the results fp32 or bf16 as nl_gemm_fp8 writes them. M, K, N > 0.
+ * the results fp32 or bf16 as nl_gemm_fp8 sums and writes them. M, K, N > 0; sizes whose
+ * wanted gradients the backward could not form (more than 8388480 rows for dW, 2 million
+ * columns or 2^28 - 16 blocks of dy for dx) are refused by the forward.
  * The forward leaves what the wanted gradients (need_dx, need_dw) read of x and W in
  * `saved`, in 8 bits; the backward gets the same need_dx, need_dw and, for a gradient
- * that is not wanted, NULL. One call launches 3 (forward) to 5 kernels; the workspaces
+ * that is not wanted, NULL. One call launches 2 (forward) to 5 kernels; the workspaces
  * are not needed behind them. saved and ws: 16-byte aligned, of the sizes given here. */
 size_t nl_linear_fp8_saved_bytes(int M, int K, int N, int need_dx, int need_dw);
 size_t nl_linear_fp8_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw);
@@ -529,7 +531,8 @@ int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_
  * largest first, equal ones by the lower id, and lse = log sum_v exp(logit_v / T).
  *   values[M][k] bf16 (the logits as stored), ids[M][k], lse[M].
  * NaN counts as larger than any number and -0 as equal to 0; a row with a NaN
- * has lse NaN. 1 <= k <= min(V, NL_TOP_MAX_K), T > 0 and finite. */
+ * has lse NaN. lse is rounded once, to fp32: half a step of it, 2^-24 |lse|, is the
+ * error of an exponent values / T - lse. 1 <= k <= min(V, NL_TOP_MAX_K), T > 0 and finite. */
 #define NL_TOP_MAX_K 256
 int nl_top_logits(void* stream, int M, int V, const nl_bf16* logits, int64_t ld, int k, float temperature,
                   nl_bf16* values, int32_t* ids, float* lse);

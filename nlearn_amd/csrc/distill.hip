@@ -9,8 +9,11 @@
 // Both are bound by HBM: a row of logits is read once into registers by one
 // workgroup (as the cross-entropy does), and every pass over it runs from there.
 // Rows that no workgroup's registers hold (beyond 106503 logits) are read twice.
-// Measured at 16384 x 50257, k = 64: the loss with its gradient 642 us (5.1 TB/s; a copy
-// reaches 4.7), the loss alone 328 us (5.0 TB/s), the top logits 406 us (4.1 TB/s).
+// Measured at 16384 x 50257, k = 64: the loss with its gradient 646 us (5.1 TB/s; a copy
+// reaches 4.7), the loss alone 327 us (5.0 TB/s), the top logits 410 us (4.0 TB/s). At 4096 x
+// 106503, in registers, 380, 173 and 297 us; at 4096 x 128256, read twice, 478, 183 and 432.
+// Every difference from a row's largest value is formed before a logarithm is added to it:
+// logits may be masks of any finite size, and a row may stand far from zero.
 #include "common.h"
 
 namespace nl {
@@ -183,8 +186,8 @@ __device__ __forceinline__ void row_sums(Row<NT, NVEC>& r, float c, int tid, Row
 // all their elements instead.) Those go to LDS as (key, index), a list for each wave,
 // and their rank among each other is their place. A row with more of them than fit
 // (ties, mostly), or with a NaN, goes over the row in memory again.
-// At 16384 x 50257: 391 us for k = 1, 406 for 64, 564 for 256, of which the sums of the
-// row take 328. (Every candidate ranked against all others, and each vector looked
+// At 16384 x 50257: 341 us for k = 1, 410 for 64, 566 for 256, of which the sums of the
+// row take 327. (Before: every candidate ranked against all others, and each vector looked
 // through where it was found: 397, 482 and 1112 us.)
 
 // bf16 bits as an ordered 16-bit number: -0 as 0, every NaN above infinity

@@ -303,10 +303,12 @@ __global__ __launch_bounds__(512) void quantize_two_kernel(QuantArgs a, uint32_t
 //     and two sets of fragments (128) in the 512 it has, and two thirds of the LDS
 //     reads of 8 waves of 128 x 64, which with the DMA's writes would take as long as
 //     the MFMAs.
-// Measured: 8192^3 to bf16 410 us, 2.68 PFLOP/s (a library's product with one scale a
-// tensor 3.03): the MFMAs are busy 71% of the cycles, at the 1.57 GHz that the part
-// holds under them; the rest is the meeting of the waves at each stage and the tiles'
-// stores. To fp32 (widened) 727 us, 1.51 PFLOP/s. 16384 x 50257 x 512, four stages a
+// Measured: 8192^3 to bf16 374 us over the same operands again and 409 over new ones each
+// time, 2.94 and 2.69 PFLOP/s (a library's product with one scale a tensor 3.03): the MFMAs
+// are busy 72 to 77% of the cycles, at the 1.55 to 1.62 GHz that the part holds under them;
+// the rest is the meeting of the waves at each stage and the tiles' stores. To fp32 (widened)
+// 725 us, 1.52 PFLOP/s. Scale rows that are no whole dwords cost 2% (4096 x 4096 x 4992: 68.9
+// us for 67.3; to fp32 122.6 for 122.4). 16384 x 50257 x 512, four stages a
 // tile: 466 to 491 us by card, some 100 fewer without its stores: 1.65 GB go out in bursts
 // between K loops that the next tile's first two stages hide in part. The stores pass
 // the caches by (not so, 16384 x 50257 x 512 took 569 us for 489, and the products of a
@@ -433,7 +435,7 @@ __device__ __forceinline__ F8Item f8_item(const GemmF8Args& g, int item) {
   t.split = item / g.tiles;
   const int tile = item - t.split * g.tiles;
   // tile rows that neighbours share a column of B over (16384 x 50257 x 512 and 8192^3, us on
-  // one card: 1 row 554 and 523, 4 520 and 487, 8 507 and 491, 16 503 and 507)
+  // one card: 1 row 516 and 411, 4 464 and 367, 8 464 and 372, 16 464 and 382)
   constexpr int GM = 8;
   const int in_group = GM * tiles_n;
   const int first_m = (tile / in_group) * GM;
@@ -851,7 +853,9 @@ F8Plan f8_plan(int M, int N, int K) {
   F8Plan p;
   // 256 x 256 tiles where there is one for every CU (4096^3 55.8 us against 70.1 with 128 x
   // 128); with 128 of them half the CUs stand idle (16384 x 512 x 2048 26.5 against 22.8,
-  // 4096 x 2048 x 2048 25.5 against 19.9).
+  // 4096 x 2048 x 2048 25.5 against 19.9). That is measured on tiles that rows fill; the rule
+  // counts them however full they are, and 8 x 131072 x 512 takes 22.7 for 14.7, 64 rows 24.7
+  // for 16.0.
   p.huge = tiles(256) >= 256;
   const int64_t t = tiles(p.huge ? 256 : 128);
   // A split of K shortens the walk over it (0.39 us a block with a bf16 result, 0.69 with

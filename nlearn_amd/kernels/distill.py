@@ -56,7 +56,8 @@ def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0):
     first and equal ones by the lower id, as bf16 [..., k] and int32 [..., k], and
     lse = logsumexp(logits / temperature) over the whole row, fp32 [...].
 
-    exp(values / temperature - lse) are the row's probabilities. NaN counts as
+    exp(values / temperature - lse) are the row's probabilities, to 2^-24 of |lse|: rows
+    1e5 and more away from zero are better moved to their maximum first. NaN counts as
     larger than any number. 1 <= k <= min(V, 256). Not differentiable."""
     x = _rows("top_logits", logits)
     T = _temperature("top_logits", temperature)
@@ -111,7 +112,8 @@ def distill_cross_entropy(logits: torch.Tensor, ids: torch.Tensor, values: torch
     logits [..., V] bf16 (the student's), ids [..., k] int32 or int64, values
     [..., k] bf16 or fp32 (the teacher's logits), T the temperature. With ``lse``
     [...] (the teacher's logsumexp at T, as ``top_logits`` gives it) p_j =
-    exp(values_j / T - lse); without it p is the softmax of the row's k values / T.
+    exp(values_j / T - lse); without it p is the softmax of the row's k values / T,
+    wherever they stand.
 
     An entry with a negative id is padding. An id may stand in a row more than
     once: its probabilities add up (a hard target can ride along as an entry of

@@ -229,7 +229,7 @@ def _main_grad(W: torch.Tensor):
 
 class _LinearFp8(torch.autograd.Function):
     """Both directions are one call of the library each: the host's share of a small
-    product is what it costs (15 us against 55 for a forward pass call by call)."""
+    product is what it costs (20 us against 42 for a forward pass call by call)."""
 
     @staticmethod
     def forward(ctx, x2, W, need_dx, need_dW):
@@ -311,7 +311,8 @@ def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
 
     W: an fp32 or bf16 weight, quantised here, or an ``Fp8Weight`` (frozen: it gets
     no gradient). The gradients are those of the product of the quantised
-    operands, with dY quantised too and the rounding taken as the identity."""
+    operands, with dY quantised too and the rounding taken as the identity. Both run
+    on the current stream: dW is not forked within ``overlap_weight_grads()``."""
     if x.dim() < 2:
         raise ValueError("linear_fp8: x needs >= 2 dims")
     frozen = W if isinstance(W, Fp8Weight) else None
