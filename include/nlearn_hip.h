@@ -524,6 +524,40 @@ int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_
                       void* ws, size_t ws_bytes);
 
 /* ======================================================================== */
+/* Root-mean-square norm                                                      */
+/* ======================================================================== */
+/*
+ * Rows of D elements, fp32 or bf16 (dtype; x, residual, sum_out, y and the
+ * gradients alike), any row stride >= D and any alignment of the type;
+ * 1 <= D <= 16384, fp32 gamma and statistics, 0 < eps <= 1:
+ *   s = x (+ residual, rounded to the type and written to sum_out; residual NULL: s = x)
+ *   y = s * rstd * gamma,   rstd = 1 / sqrt(mean(s^2) + eps)
+ * rstd[rows] is kept for the backward (NULL: not wanted). Squares may pass fp32;
+ * a row with an infinity has rstd 0, one with a NaN is NaN. Outputs may not overlap
+ * inputs. Replaces the RMSNorm of model.py:228-241 and the residual adds of model.py:315-324.
+ */
+int nl_rms_norm_fwd(void* stream, int rows, int D, int dtype, const void* x, int64_t ldx,
+                    const void* residual, int64_t ldr, void* sum_out, int64_t ld_sum,
+                    const float* gamma, float eps, void* y, int64_t ldy, float* rstd);
+
+/* The same with y in 8 bits, quantised along D as nl_quantize_fp8 does it (group 1),
+ * from the fp32 values (y is not rounded to the type of x first). */
+int nl_rms_norm_fp8(void* stream, int rows, int D, int dtype, const void* x, int64_t ldx,
+                    const void* residual, int64_t ldr, void* sum_out, int64_t ld_sum,
+                    const float* gamma, float eps, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds);
+
+/* Backward of nl_rms_norm_fwd, x the normalised rows (sum_out when there was a residual):
+ *   dx = rstd * (g - xh * mean(g * xh)) (+ dres),   g = dy * gamma,  xh = x * rstd
+ *   dgamma[c] (+)= sum_rows dy * xh    (accumulate != 0 adds; NULL: not wanted)
+ * dres (may be NULL) is the gradient arriving through sum_out. dgamma is summed in a fixed
+ * order, over a workspace of nl_rms_norm_bwd_ws_bytes() bytes. */
+size_t nl_rms_norm_bwd_ws_bytes(int rows, int D);
+int nl_rms_norm_bwd(void* stream, int rows, int D, int dtype, const void* dy, int64_t lddy,
+                    const void* x, int64_t ldx, const float* rstd, const float* gamma,
+                    const void* dres, int64_t lddres, void* dx, int64_t lddx, float* dgamma,
+                    int accumulate, void* ws, size_t ws_bytes);
+
+/* ======================================================================== */
 /* Distillation from a teacher's top logits                                   */
 /* ======================================================================== */
 /*

@@ -93,6 +93,10 @@ _SIGNATURES = {
     "nl_quantize_fp8": [_P, _I64, _I64, _P, _I, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64],
     "nl_gemm_fp8_ws_bytes": [_I, _I, _I],
     "nl_gemm_fp8": [_P, _I, _I, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I, _I64, _P, ctypes.c_size_t],
+    "nl_rms_norm_fwd": [_P, _I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P],
+    "nl_rms_norm_fp8": [_P, _I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I64],
+    "nl_rms_norm_bwd_ws_bytes": [_I, _I],
+    "nl_rms_norm_bwd": [_P, _I, _I, _I, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I, _P, ctypes.c_size_t],
     "nl_top_logits": [_P, _I, _I, _P, _I64, _I, _F, _P, _P, _P],
     "nl_linear_fp8_saved_bytes": [_I, _I, _I, _I, _I],
     "nl_linear_fp8_ws_bytes": [_I, _I, _I, _I, _I, _I],
@@ -116,6 +120,7 @@ _RESTYPES = {
     "nl_embedding_bwd_ws_bytes": ctypes.c_size_t,
     "nl_gemm_fp8_ws_bytes": ctypes.c_size_t,
     "nl_linear_fp8_saved_bytes": ctypes.c_size_t,
+    "nl_rms_norm_bwd_ws_bytes": ctypes.c_size_t,
     "nl_linear_fp8_ws_bytes": ctypes.c_size_t,
 }
 

@@ -1,0 +1,48 @@
+// fp8.h — e4m3 blocks of 128 with an e8m0 scale, as the kernels that write them form them.
+#pragma once
+
+#include "common.h"
+
+namespace nl {
+
+constexpr int kB = 128;  // elements per scale
+
+// |x| as ordered bits, and with 0 for a value that is not finite (it has no part in the scale).
+constexpr uint32_t kInfBits = 0x7f800000u;
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t finite_abs_bits(float x) {
+  const uint32_t u = abs_bits(x);
+  return u < kInfBits ? u : 0u;
+}
+
+// The e8m0 byte (e + 127) of a block whose largest |x| has these bits: with |x| =
+// 1.f * 2^(E-127), 448 = 1.75 * 2^8 gives e = E - 135, one more above 1.75.
+// Blocks below 2^-119 stay at 2^-127, a block of zeros is at 1.
+__device__ __forceinline__ int scale_byte(uint32_t amax) {
+  const int b = (int)(amax >> 23) - 8 + ((amax & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return amax == 0 ? 127 : (b > 0 ? b : 0);
+}
+
+// 2^-e, e in [-127, 120]: always a normal number, so the product with it is exact
+// wherever e4m3 keeps anything of it.
+__device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
+
+// Four scaled values to four e4m3 bytes (an infinity or a NaN gives NaN).
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
+  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+}
+
+template <int CTRL>
+__device__ __forceinline__ uint32_t dpp_u(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xf, 0xf, true);
+}
+// max over the 16 lanes of a row of lanes (the exchanges of wave_sum in common.h)
+__device__ __forceinline__ uint32_t max16(uint32_t v) {
+  v = max(v, dpp_u<0xB1>(v));
+  v = max(v, dpp_u<0x4E>(v));
+  v = max(v, dpp_u<0x141>(v));
+  return max(v, dpp_u<0x140>(v));
+}
+
+}  // namespace nl

@@ -3,6 +3,8 @@
 * ``quantize_fp8(x)`` / ``quantize_fp8_both(x)``: a matrix to e4m3 values with one
   power-of-two scale for each block of 128 along the summed axis, per row
   (``group=1``: activations, gradients) or per 128 rows (``group=128``: weights).
+* ``rms_norm_fp8(x, gamma)`` / ``add_rms_norm_fp8(x, r, gamma)``: the norm in front of a product,
+  written as such an operand.
 * ``gemm_fp8(a, b)``: a . b^T of two such operands, bf16 or fp32 out.
 * ``linear_fp8(x, W)``: ``linear(x, W)`` with all three products in 8 bits: y = x W,
   dX = dY W^T and dW = X^T dY, every operand quantised along the axis that its
@@ -21,6 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
+from .fused import _check_rms, _param, _strided_rows
 from .gemm import _BF16, _F32, _aligned, _check_device, _ld, grad_buffer, padded_ld
 
 _E4M3 = torch.float8_e4m3fn
@@ -139,6 +142,33 @@ def quantize_fp8(x: torch.Tensor, group: int = 1, transpose: bool = False) -> Fp
 def quantize_fp8_both(x: torch.Tensor, group: int = 1):
     """(quantize_fp8(x), quantize_fp8(x, transpose=True)) from one read of x."""
     return _quantize(x, group, True, True)
+
+
+def _rms_norm_fp8(what: str, x, r, gamma, eps):
+    eps = _check_rms(what, x, r, gamma, eps)
+    with torch.no_grad():
+        (x2, ldx), g = _strided_rows(x), _param(gamma)
+        rows, D = x2.shape
+        out = Fp8Blocks.empty(rows, D, 1, x.device)
+        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r is not None else None
+        if rows:
+            r2, ldr = _strided_rows(r) if r is not None else (None, 0)
+            _lib.call_on(x2, "nl_rms_norm_fp8", rows, D, _code(x2), x2.data_ptr(), ldx,
+                         r2.data_ptr() if r is not None else None, ldr, s.data_ptr() if r is not None else None, D,
+                         g.data_ptr(), eps, *out._abi())
+    return out, s
+
+
+def rms_norm_fp8(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-5) -> Fp8Blocks:
+    """``rms_norm(x, gamma, eps)`` quantised along its last dimension (one scale for each block
+    of 128 and row; leading dimensions are flattened), from fp32 values that were not rounded to
+    x's dtype before. What ``gemm_fp8`` reads; not differentiable, as ``quantize_fp8``."""
+    return _rms_norm_fp8("rms_norm_fp8", x, None, gamma, eps)[0]
+
+
+def add_rms_norm_fp8(x: torch.Tensor, r: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-5):
+    """(rms_norm_fp8(s, gamma, eps), s) with s = x + r rounded to their dtype, in one pass."""
+    return _rms_norm_fp8("add_rms_norm_fp8", x, r, gamma, eps)
 
 
 def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:

@@ -4,6 +4,9 @@
   LayerNorm with fp32 statistics (nlearn/model.py:228-241), the second one
   with the residual add of the block folded in (model.py:315-324): it returns
   both LN(x + r) and the new residual stream x + r, reading x and r once.
+* ``rms_norm(x, gamma)`` and ``add_rms_norm(x, r, gamma)``: the same pair without
+  the mean, as the reference's own blocks have it (model.py:228-241); bf16 or fp32
+  rows of any stride. ``fp8.rms_norm_fp8`` writes the result in 8 bits.
 * ``ffn(x, W1, b1, W2, b2)``: the FFN (model.py:266-277, with the benchmark's
   tanh-GELU and biases) as two GEMMs whose epilogues add the biases and apply
   the GELU; the backward's dX GEMM applies the GELU derivative in its
@@ -19,6 +22,7 @@ from __future__ import annotations
 import contextlib
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from .. import _lib
 from . import wgrad
@@ -192,6 +196,149 @@ def add_layer_norm(x: torch.Tensor, r: torch.Tensor, gamma: torch.Tensor, beta: 
                    eps: float = 1e-5):
     """(LN(s), s) with s = bf16(x + r): the residual add and the next LayerNorm in one pass."""
     return _AddLayerNorm.apply(x, r, gamma, beta, eps)
+
+
+# ---------------------------------------------------------------------------
+# RMS norm
+# ---------------------------------------------------------------------------
+
+MAX_RMS_COLUMNS = 16384
+
+
+def _strided_rows(t: torch.Tensor):
+    """(t as rows with a unit column stride that share no memory, their stride); copies only if it must."""
+    x = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    (rows, D), (s0, s1) = x.shape, x.stride()
+    if (D > 1 and s1 != 1) or (rows > 1 and s0 < D):
+        return x.contiguous(), D
+    return x, s0 if rows > 1 else D
+
+
+def _check_rms(what: str, x: torch.Tensor, r, gamma: torch.Tensor, eps: float) -> float:
+    if x.dim() < 1 or x.dtype not in (_BF16, _F32):
+        raise ValueError(f"{what}: rows must be bfloat16 or float32, got {x.dtype} {tuple(x.shape)}")
+    D = x.shape[-1]
+    if not 1 <= D <= MAX_RMS_COLUMNS:
+        raise ValueError(f"{what}: rows of 1 to {MAX_RMS_COLUMNS} elements, got {D}")
+    if x.numel() // D >= 1 << 31:
+        raise ValueError(f"{what}: fewer than 2^31 rows, got {x.numel() // D}")
+    if r is not None and (r.shape != x.shape or r.dtype is not x.dtype):
+        raise ValueError(f"{what}: x is {x.dtype} {tuple(x.shape)}, the residual {r.dtype} {tuple(r.shape)}")
+    if gamma.shape != (D,) or gamma.dtype not in (_BF16, _F32):
+        raise ValueError(f"{what}: gamma must be bfloat16 or float32 of shape {(D,)}, got {gamma.dtype} "
+                         f"{tuple(gamma.shape)}")
+    eps = float(eps)
+    if not 1e-30 <= eps <= 1.0:  # NaN fails too
+        raise ValueError(f"{what}: eps must lie in [1e-30, 1], got {eps}")
+    for t in (gamma,) if r is None else (gamma, r):
+        if t.device != x.device:
+            raise ValueError(f"{what}: all tensors must be on one device, got {x.device} and {t.device}")
+    _check_device(x)
+    return eps
+
+
+def _rms_code(t: torch.Tensor) -> int:
+    return _lib.NL_DTYPE_F32 if t.dtype is _F32 else _lib.NL_DTYPE_BF16
+
+
+def _rms_fwd(x, r, gamma, eps, keep: bool):
+    """(y, s or None, rstd or None), y and s dense of x's shape."""
+    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r is not None else None
+    x2, ldx = _strided_rows(x)
+    rows, D = x2.shape
+    rstd = torch.empty(rows, dtype=_F32, device=x.device) if keep else None
+    if rows:
+        r2, ldr = _strided_rows(r) if r is not None else (None, 0)
+        g = _param(gamma)
+        _lib.call_on(x2, "nl_rms_norm_fwd", rows, D, _rms_code(x2), x2.data_ptr(), ldx,
+                     r2.data_ptr() if r is not None else None, ldr, s.data_ptr() if r is not None else None, D,
+                     g.data_ptr(), eps, y.data_ptr(), D, rstd.data_ptr() if keep else None)
+    return y, s, rstd
+
+
+def _rms_grad_buffer(gamma: torch.Tensor):
+    mg = grad_buffer(gamma)
+    if mg is not None and (mg.shape != gamma.shape or mg.device != gamma.device or mg.dtype is not _F32
+                           or not mg.is_contiguous()):
+        raise ValueError(f"rms_norm: main_grad must be a dense float32 tensor of shape {tuple(gamma.shape)} on "
+                         f"{gamma.device}")
+    return mg
+
+
+def _rms_bwd(ctx, dy, ds, s, rstd, gamma):
+    """(dx, dgamma or None where a main_grad buffer took it)."""
+    mg = _rms_grad_buffer(ctx.gamma) if ctx.gamma is not None else None
+    need_dg = ctx.need_dgamma
+    dx = torch.empty(s.shape, dtype=s.dtype, device=s.device)
+    s2, lds = _strided_rows(s)
+    rows, D = s2.shape
+    dg = None
+    if need_dg:
+        dg = mg if mg is not None else torch.empty(D, dtype=_F32, device=s.device)
+    if rows == 0:
+        if dg is not None:
+            dg.zero_()
+    else:
+        d2, ldd = _strided_rows(dy.to(s.dtype))
+        r2, ldr = _strided_rows(ds.to(s.dtype)) if ds is not None else (None, 0)
+        g = _param(gamma)
+        wsb = _lib.load().nl_rms_norm_bwd_ws_bytes(rows, D) if need_dg else 0
+        ws = torch.empty(wsb // 4, dtype=_F32, device=s.device) if wsb else None
+        _lib.call_on(s2, "nl_rms_norm_bwd", rows, D, _rms_code(s2), d2.data_ptr(), ldd, s2.data_ptr(), lds,
+                     rstd.data_ptr(), g.data_ptr(), r2.data_ptr() if ds is not None else None, ldr, dx.data_ptr(), D,
+                     dg.data_ptr() if need_dg else None, 0, ws.data_ptr() if wsb else None, wsb)
+    return dx, dg.to(gamma.dtype) if need_dg and mg is None else None
+
+
+class _RMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, gamma, eps, keep):
+        y, _, rstd = _rms_fwd(x, None, gamma, eps, keep)
+        if keep:
+            ctx.save_for_backward(x, rstd, gamma)
+            ctx.need_dgamma = gamma.requires_grad
+            ctx.gamma = gamma if gamma.requires_grad else None  # for its main_grad
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        return *_rms_bwd(ctx, dy, None, *ctx.saved_tensors), None, None
+
+
+class _AddRMSNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, r, gamma, eps, keep):
+        ctx.set_materialize_grads(False)
+        y, s, rstd = _rms_fwd(x, r, gamma, eps, keep)
+        if keep:
+            ctx.save_for_backward(s, rstd, gamma)
+            ctx.need_dgamma = gamma.requires_grad
+            ctx.gamma = gamma if gamma.requires_grad else None
+        return y, s
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, ds):
+        if dy is None:
+            return ds, ds, None, None, None
+        dx, dg = _rms_bwd(ctx, dy, ds, *ctx.saved_tensors)
+        return dx, dx, dg, None, None
+
+
+def rms_norm(x: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-5) -> torch.Tensor:
+    """x / sqrt(mean(x^2) + eps) * gamma over the last dimension (up to 16384 elements),
+    in x's dtype, bf16 or fp32; statistics and gamma's gradient are fp32."""
+    eps = _check_rms("rms_norm", x, None, gamma, eps)
+    return _RMSNorm.apply(x, gamma, eps, torch.is_grad_enabled() and (x.requires_grad or gamma.requires_grad))
+
+
+def add_rms_norm(x: torch.Tensor, r: torch.Tensor, gamma: torch.Tensor, eps: float = 1e-5):
+    """(rms_norm(s), s) with s = x + r rounded to their dtype: the residual add and the next norm in one pass."""
+    eps = _check_rms("add_rms_norm", x, r, gamma, eps)
+    return _AddRMSNorm.apply(x, r, gamma, eps, torch.is_grad_enabled()
+                             and (x.requires_grad or r.requires_grad or gamma.requires_grad))
 
 
 # ---------------------------------------------------------------------------
