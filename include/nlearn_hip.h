@@ -361,6 +361,29 @@ int nl_adamw_multi_clip(void* stream, int n_tensors, const nl_adamw_tensor* tens
 size_t nl_global_norm_ws_bytes(int64_t n);
 int nl_global_norm(void* stream, int64_t n, const float* g, float* out, void* ws, size_t ws_bytes);
 
+/* The same over many tensors where they lie, and their clipping in the same call:
+ *   norm[0] = sqrt(sum of the squares of all elements)      (summed in fp64, in a fixed order)
+ *   out = g                        while norm[0] < max_norm, else (g / norm[0]) * max_norm
+ * Each tensor is `rows` rows of `cols` elements, fp32 or bf16, rows ld (of g) and ld_out (of
+ * out) elements apart, at any alignment of the type; a dense tensor is one row. out may be g
+ * (the same address and stride: written only where the norm reaches max_norm); no other two
+ * tensors of a clipping may overlap. An empty tensor adds nothing. The descriptions are read
+ * on the host before the call returns. ws: NL_GLOBAL_NORM_MULTI_WS bytes, 8-byte aligned,
+ * needed until the call's work has run. Up to 72 tensors take 2 launches, and 2 more for
+ * each further 72. */
+typedef struct nl_grad_tensor {
+  const void* g;
+  void* out;          /* not read by nl_global_norm_multi */
+  int64_t rows, cols;
+  int64_t ld, ld_out;
+  int64_t dtype;      /* NL_DTYPE_F32 or NL_DTYPE_BF16 */
+} nl_grad_tensor;
+#define NL_GLOBAL_NORM_MULTI_WS 8192
+int nl_global_norm_multi(void* stream, int n, const nl_grad_tensor* tensors, float* norm, void* ws,
+                         size_t ws_bytes);
+int nl_clip_by_global_norm(void* stream, int n, const nl_grad_tensor* tensors, float max_norm, float* norm,
+                           void* ws, size_t ws_bytes);
+
 /* Gradient accumulation over micro-steps, as optax.MultiSteps does it
  * (train.py:319-325,507-508 wrap the optimizer in MultiSteps(every_k_schedule=
  * NLEARN_GRAD_ACCUM)), with the loss-scale division of train_step

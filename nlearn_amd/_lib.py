@@ -78,6 +78,8 @@ _SIGNATURES = {
     "nl_adamw_multi_clip": [_P, _I, _P, _I64, _P, _D, _D, _F, _F, _P, _F],
     "nl_global_norm_ws_bytes": [_I64],
     "nl_global_norm": [_P, _I64, _P, _P, _P, ctypes.c_size_t],
+    "nl_global_norm_multi": [_P, _I, _P, _P, _P, ctypes.c_size_t],
+    "nl_clip_by_global_norm": [_P, _I, _P, _F, _P, _P, ctypes.c_size_t],
     "nl_grad_accumulate": [_P, _I64, _P, _P, _P],
     "nl_layernorm_fwd": [_P, _I, _I, _P, _P, _P, _P, _P, _F, _P, _P, _P],
     "nl_layernorm_bwd_ws_bytes": [_I, _I],

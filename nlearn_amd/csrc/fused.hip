@@ -726,11 +726,6 @@ int ln_bwd_blocks(int rows, int D) {
 }  // namespace
 }  // namespace nl
 
-void nl::launch_partial_sums(hipStream_t st, int P, int D, const float* part, float* out, int accumulate) {
-  hipLaunchKernelGGL(sum_partials_kernel, dim3((D + 15) / 16, 1), dim3(256), 0, st, P, D, part, out, nullptr, nullptr,
-                     accumulate);
-}
-
 using namespace nl;
 
 extern "C" int nl_layernorm_fwd(void* stream, int rows, int D, const nl_bf16* x, const nl_bf16* residual,

@@ -23,7 +23,7 @@ import torch
 from torch.autograd.function import once_differentiable
 
 from .. import _lib
-from .fused import _check_rms, _param, _strided_rows
+from .fused import _check_rms, _dense_like, _param, _strided_rows
 from .gemm import _BF16, _F32, _aligned, _check_device, _ld, grad_buffer, padded_ld
 
 _E4M3 = torch.float8_e4m3fn
@@ -146,16 +146,15 @@ def quantize_fp8_both(x: torch.Tensor, group: int = 1):
 
 def _rms_norm_fp8(what: str, x, r, gamma, eps):
     eps = _check_rms(what, x, r, gamma, eps)
-    with torch.no_grad():
-        (x2, ldx), g = _strided_rows(x), _param(gamma)
-        rows, D = x2.shape
-        out = Fp8Blocks.empty(rows, D, 1, x.device)
-        s = torch.empty(x.shape, dtype=x.dtype, device=x.device) if r is not None else None
-        if rows:
-            r2, ldr = _strided_rows(r) if r is not None else (None, 0)
-            _lib.call_on(x2, "nl_rms_norm_fp8", rows, D, _code(x2), x2.data_ptr(), ldx,
-                         r2.data_ptr() if r is not None else None, ldr, s.data_ptr() if r is not None else None, D,
-                         g.data_ptr(), eps, *out._abi())
+    (x2, ldx), g = _strided_rows(x.detach()), _param(gamma)
+    rows, D = x2.shape
+    out = Fp8Blocks.empty(rows, D, 1, x.device)
+    s = _dense_like(x2).view(x.shape) if r is not None else None
+    if rows:
+        r2, ldr = _strided_rows(r.detach()) if r is not None else (None, 0)
+        _lib.call_on(x2, "nl_rms_norm_fp8", rows, D, _code(x2), x2.data_ptr(), ldx,
+                     r2.data_ptr() if r is not None else None, ldr, s.data_ptr() if r is not None else None, D,
+                     g.data_ptr(), eps, *out._abi())
     return out, s
 
 

@@ -37,6 +37,7 @@ import torch
 from . import _lib
 from .checkpoint import load_checkpoint, load_resume_state, save_checkpoint, save_resume_state  # noqa: F401
 from .kernels import fused, wgrad
+from .kernels.clip import clip_by_global_norm, rows_of
 from .kernels.cross_entropy import cross_entropy, linear_cross_entropy, lm_head_cross_entropy  # noqa: F401
 from .model import (BASELINE, ModelConfig, count_params, init_model, model_forward, model_forward_features,
                     output_projection, tree_leaves)
@@ -178,7 +179,8 @@ class AdamW:
     ``prepare`` writes the device scalars for the coming step, ``apply`` launches
     the capturable work, ``finish`` runs what follows it outside a graph (nothing
     here), ``advance`` counts the step; ``update`` does all four. Leaves without
-    a buffer fall back to one launch per leaf on ``.grad`` (no clipping there)."""
+    a buffer fall back to one launch per leaf on ``.grad``, clipped in place before
+    (``kernels.clip``)."""
 
     def __init__(self, learning_rate, weight_decay: float = WEIGHT_DECAY, b1: float = 0.9, b2: float = 0.999,
                  eps: float = 1e-8, grad_buffers: bool = True, clip_norm: float = 0.0):
@@ -272,12 +274,15 @@ class AdamW:
                 _lib.call("nl_adamw_multi", stream, n, table.data_ptr(), n_chunks, state["hyper"].data_ptr(),
                           self.b1, self.b2, self.eps, self.wd)
             return
-        if self.clip_norm > 0 or loss_scale != 1.0:
-            raise RuntimeError("AdamW: clipping and loss scaling need the gradient buffers (grad_buffers=True)")
+        if loss_scale != 1.0:
+            raise RuntimeError("AdamW: loss scaling needs the gradient buffers (grad_buffers=True)")
         lr, bc1, bc2 = self.hyper_values(state["count"])
-        for p, m, v in zip(leaves, state["mu"], state["nu"]):
-            g = getattr(p, "main_grad", None)
-            g = p.grad if g is None else g
+        grads = [p.grad if getattr(p, "main_grad", None) is None else p.main_grad for p in leaves]
+        if self.clip_norm > 0 and any(g is not None for g in grads):
+            # a gradient whose rows have no one stride (a broadcast one) is copied first
+            grads = [g if g is None or rows_of(g) else g.contiguous() for g in grads]
+            _, state["gnorm"] = clip_by_global_norm([g for g in grads if g is not None], self.clip_norm, inplace=True)
+        for p, g, m, v in zip(leaves, grads, state["mu"], state["nu"]):
             if g is None:
                 continue
             if g.stride() != p.stride():

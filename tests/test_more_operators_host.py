@@ -1,4 +1,4 @@
-"""Refusals of the RMS norms, before anything reaches a GPU."""
+"""Refusals of the RMS norms, the global norm and the products, before anything reaches a GPU."""
 import pytest
 
 from nlearn_amd import _lib
@@ -57,3 +57,59 @@ def test_rms_norm_refusals_in_python():
             norm(x, torch.ones(64, device="meta"))
         with pytest.raises(ValueError, match="2\\^31"):
             norm(torch.zeros(1).expand(1 << 31, 1), torch.ones(1))
+
+
+def test_global_norm_refusals_of_the_library():
+    import ctypes
+
+    lib = _lib.load()
+
+    def leaf(g=256, out=256, rows=1, cols=8, ld=8, ldo=8, dtype=0):
+        return (ctypes.c_int64 * 7)(g or 0, out or 0, rows, cols, ld, ldo, dtype)
+
+    clip = lambda t=None, n=1, most=1.0, norm=512, ws=1024, wsb=8192: lib.nl_clip_by_global_norm(  # noqa: E731
+        None, n, t if t is not None else leaf(), most, norm, ws, wsb)
+    bad = [dict(n=-1), dict(most=0.0), dict(most=float("nan")), dict(norm=None), dict(ws=None), dict(wsb=8191),
+           dict(t=leaf(g=None)), dict(t=leaf(out=None)), dict(t=leaf(rows=-1)), dict(t=leaf(cols=-1)),
+           dict(t=leaf(dtype=2)), dict(t=leaf(rows=2, ld=7)), dict(t=leaf(rows=2, ldo=7)),
+           dict(t=leaf(rows=2, ld=8, ldo=9))]
+    for kw in bad:
+        assert clip(**kw) == _lib.NL_EINVAL, kw
+    for kw in (dict(t=leaf(g=258)), dict(t=leaf(out=257, dtype=1)), dict(ws=1028), dict(norm=514)):
+        assert clip(**kw) == _lib.NL_EALIGN, kw
+    for t in (leaf(rows=1 << 31), leaf(rows=2, cols=1 << 31, ld=1 << 31, ldo=1 << 31), leaf(cols=1 << 41)):
+        assert clip(t) == _lib.NL_EUNSUPPORTED
+    assert lib.nl_global_norm_multi(None, 1, leaf(g=None), 512, 1024, 8192) == _lib.NL_EINVAL
+    assert lib.nl_global_norm_multi(None, 1, None, 512, 1024, 8192) == _lib.NL_EINVAL
+    assert lib.nl_global_norm_multi(None, 1, leaf(out=None), None, 1024, 8192) == _lib.NL_EINVAL
+
+
+def test_global_norm_refusals_in_python():
+    import torch
+    from nlearn_amd.kernels.clip import clip_by_global_norm, global_norm, rows_of
+
+    x = torch.ones(8)
+    for most in (0.0, -1.0, float("nan"), float("inf"), 1e300):
+        with pytest.raises(ValueError, match="max_norm"):
+            clip_by_global_norm([x], most)
+    for call in (global_norm, lambda t: clip_by_global_norm(t, 1.0)):
+        with pytest.raises(ValueError, match="no "):
+            call([])
+        with pytest.raises(ValueError, match="float32 or bfloat16"):
+            call([x.double()])
+        with pytest.raises(RuntimeError, match="HIP device"):
+            call([x])
+    with pytest.raises(ValueError, match="twice"):
+        clip_by_global_norm([x, x], 1.0, inplace=True)
+    # how a tensor is walked: (rows, columns, row stride)
+    m = torch.zeros((6, 10))
+    assert rows_of(m) == (1, 60, 60) and rows_of(m.t()) == (1, 60, 60)
+    assert rows_of(m[:, :7]) == (6, 7, 10) and rows_of(m[:, :7].t()) == (6, 7, 10)
+    assert rows_of(m[:, 3]) == (6, 1, 10) and rows_of(m[2]) == (1, 10, 10)
+    assert rows_of(m[::2]) == (3, 10, 20) and rows_of(torch.zeros(())) == (1, 1, 1)
+    assert rows_of(m[1:2, 2:9:2]) == (4, 1, 2)
+    c = torch.zeros((4, 5, 8))
+    assert rows_of(c[..., :6]) == (20, 6, 8) and rows_of(c[:, :3, :6]) is None and rows_of(c[:, :3]) == (4, 24, 40)
+    assert rows_of(c.permute(1, 0, 2)) == (1, 160, 160)
+    assert rows_of(x.expand(3, 8)) is None and rows_of(x[:1].expand(4)) is None
+    assert rows_of(torch.as_strided(m, (4, 5), (3, 1))) is None
