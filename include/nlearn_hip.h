@@ -369,8 +369,8 @@ int nl_global_norm(void* stream, int64_t n, const float* g, float* out, void* ws
  * (the same address and stride: written only where the norm reaches max_norm); no other two
  * tensors of a clipping may overlap. An empty tensor adds nothing. The descriptions are read
  * on the host before the call returns. ws: NL_GLOBAL_NORM_MULTI_WS bytes, 8-byte aligned,
- * needed until the call's work has run. Up to 72 tensors take 2 launches, and 2 more for
- * each further 72. */
+ * needed until the call's work has run. Up to 64 tensors take 2 launches, and 2 more for
+ * each further 64. */
 typedef struct nl_grad_tensor {
   const void* g;
   void* out;          /* not read by nl_global_norm_multi */

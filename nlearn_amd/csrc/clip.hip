@@ -5,8 +5,8 @@
 //
 // Two passes over the gradients (the second needs the first one's sum), bound by
 // HBM; the second starts where the first ended, with what the 256 MB cache still
-// holds. The tensors' addresses travel as a kernel's arguments, 72 in a launch, so
-// nothing is copied to the device and a captured graph keeps them; up to 72 tensors
+// holds. The tensors' addresses travel as a kernel's arguments, 64 in a launch, so
+// nothing is copied to the device and a captured graph keeps them; up to 64 tensors
 // are two launches. The squares are summed in fp64 (a square passes fp32 at 2^64
 // and vanishes below 2^-75; at 4 elements a clock and CU the fp64 units wait for
 // HBM all the same), each workgroup's walk and the workgroups in a fixed order.
@@ -15,10 +15,10 @@
 namespace nl {
 namespace {
 
-constexpr int kMost = 72;       // tensors in a launch: their table and the rest fit the 4 KiB of arguments
+constexpr int kMost = 64;       // tensors in a launch: one a lane, and their table fits the 4 KiB of arguments
 constexpr int kGrid = 1024;     // workgroups of the sums, a partial sum each
-constexpr int kUnroll = 4;      // 16-byte vectors a thread has in flight
-constexpr int kChunk = 256 * kUnroll * 2;  // vectors of one tensor that a workgroup takes at a time
+constexpr int kVecs = 4;        // 16-byte vectors of a chunk that a thread takes, all in flight together
+constexpr int kChunk = 256 * kVecs;  // vectors of one tensor that a workgroup takes at a time
 
 typedef u32x4 __attribute__((aligned(2))) u32x4_any;
 
@@ -39,14 +39,12 @@ static_assert(sizeof(Table) <= 3700, "a kernel has 4 KiB of arguments");
 // Calls go(leaf, bf16, vectors of a row, first vector, vectors) for the chunks b, b + step, ... of the table.
 template <bool kBack, class F>
 __device__ __forceinline__ void walk(const Table& t, F&& go) {
+  // each lane knows a leaf's first chunk: one comparison finds a chunk's leaf
+  const int lane = threadIdx.x & 63;
+  const uint32_t start = lane < t.n ? t.leaf[lane].chunk0_bf16 >> 1 : 0xffffffffu;
   for (uint32_t b = blockIdx.x; b < t.chunks; b += gridDim.x) {
     const uint32_t chunk = kBack ? t.chunks - 1 - b : b;
-    int lo = 0, hi = t.n - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((t.leaf[mid].chunk0_bf16 >> 1) <= chunk) lo = mid;
-      else hi = mid - 1;
-    }
+    const int lo = __builtin_amdgcn_readfirstlane(__popcll(__ballot(start <= chunk)) - 1);
     const Leaf& f = t.leaf[lo];
     const bool bf16 = f.chunk0_bf16 & 1;
     const int64_t vpr = (f.cols + (bf16 ? 7 : 3)) / (bf16 ? 8 : 4);
@@ -56,31 +54,45 @@ __device__ __forceinline__ void walk(const Table& t, F&& go) {
   }
 }
 
-// Where vector i of a chunk lies: its row, its first column. Rows are counted from the chunk's first.
-struct Place {
-  int64_t row0, col0;  // of the chunk's first vector
-  uint32_t vpr;        // 0: one row
-};
-__device__ __forceinline__ Place place(const Leaf& f, int64_t vpr, int64_t first) {
-  if (f.rows == 1) return {0, first, 0};
-  const int64_t r = first / vpr;
-  return {r, first - r * vpr, (uint32_t)vpr};
-}
-__device__ __forceinline__ void at(const Place& p, int i, int64_t& row, int64_t& col) {
-  row = p.row0;
-  col = p.col0 + i;
-  if (p.vpr) {
-    const uint32_t d = (uint32_t)col / p.vpr;
-    row += d;
-    col = (uint32_t)col - d * p.vpr;
+// Where a thread's vectors of a chunk lie: their row and first column, and the elements of the row
+// from there on (0 or less: no such vector). go(k, row, column, left) for each.
+template <int V, class F>
+__device__ __forceinline__ void places(const Leaf& f, int64_t vpr, int64_t first, int n, F&& go) {
+  const uint32_t tid = threadIdx.x;
+  if (f.rows == 1) {
+#pragma unroll
+    for (int k = 0; k < kVecs; ++k) {
+      const int64_t col = (first + tid + k * 256) * V;
+      go(k, (int64_t)0, col, (int)(tid + k * 256) < n ? f.cols - col : 0);
+    }
+    return;
+  }
+  // rows and columns (in vectors) counted from the chunk's first row, where 32 bits hold them
+  const int64_t row0 = first / vpr;
+  const uint32_t w = (uint32_t)vpr;
+  const uint32_t at = (uint32_t)(first - row0 * vpr) + tid;
+  uint32_t row = at / w, col = at - row * w;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) {
+    go(k, row0 + row, (int64_t)col * V, (int)(tid + k * 256) < n ? f.cols - (int64_t)col * V : 0);
+    col += 256;
+    if (w >= 256) {  // the next row at most
+      if (col >= w) col -= w, ++row;
+    } else {
+      const uint32_t d = col / w;
+      row += d;
+      col -= d * w;
+    }
   }
 }
 
-// 16 bytes of a row's vector, zero past its end
+// 16 bytes at p, `left` elements of which are the row's (0 or less: none). `over`: what lies behind a
+// row may be read (it is the next row's): a load element by element waits for each, and where rows
+// are a few vectors long one of them ends in most waves' loads.
 template <typename T>
-__device__ __forceinline__ u32x4 load16(const T* p, int64_t left) {
+__device__ __forceinline__ u32x4 load16(const T* p, int64_t left, bool over) {
   constexpr int V = 16 / sizeof(T);
-  if (left >= V) return *reinterpret_cast<const u32x4_any*>(p);
+  if (left >= V || (over && left > 0)) return *reinterpret_cast<const u32x4_any*>(p);
   u32x4 v = {0u, 0u, 0u, 0u};
 #pragma unroll
   for (int k = 0; k < V - 1; ++k) {
@@ -94,7 +106,7 @@ template <typename T>
 __device__ __forceinline__ void store16(T* p, const u32x4& v, int64_t left) {
   constexpr int V = 16 / sizeof(T);
   if (left >= V) {
-    *reinterpret_cast<u32x4_any*>(p) = v;
+    __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(p));
     return;
   }
 #pragma unroll
@@ -102,6 +114,18 @@ __device__ __forceinline__ void store16(T* p, const u32x4& v, int64_t left) {
     if (k >= left) continue;
     if constexpr (sizeof(T) == 2) p[k] = (uint16_t)(v[k >> 1] >> (16 * (k & 1)));
     else p[k] = __uint_as_float(v[k]);
+  }
+}
+
+// zero past the row's last element
+template <typename T>
+__device__ __forceinline__ void mask16(u32x4& v, int left) {
+  constexpr int V = 16 / sizeof(T);
+  if (left >= V) return;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    if constexpr (sizeof(T) == 2) v[q] = left >= 2 * q + 2 ? v[q] : left == 2 * q + 1 ? v[q] & 0xffffu : 0u;
+    else v[q] = left > q ? v[q] : 0u;
   }
 }
 
@@ -122,24 +146,33 @@ __device__ __forceinline__ double squares(const u32x4& v) {
   return s;
 }
 
+// Whether a chunk is whole vectors of one row
+template <int V>
+__device__ __forceinline__ bool plain(const Leaf& f, int64_t first, int n) {
+  return f.rows == 1 && n == kChunk && (first + kChunk) * V <= f.cols;
+}
+
 template <typename T>
 __device__ __forceinline__ double chunk_squares(const Leaf& f, int64_t vpr, int64_t first, int n) {
-  const Place p = place(f, vpr, first);
+  constexpr int V = 16 / sizeof(T);
   const T* g = reinterpret_cast<const T*>(f.g);
-  double s = 0.0;
-  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * kUnroll) {
-    u32x4 v[kUnroll];
+  u32x4 v[kVecs];
+  if (plain<V>(f, first, n)) {
+    const T* p = g + first * V + threadIdx.x * V;
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int i = i0 + k * 256;
-      int64_t row, col;
-      at(p, i, row, col);
-      col *= 16 / (int)sizeof(T);
-      v[k] = i < n ? load16<T>(g + row * f.ld + col, f.cols - col) : u32x4{0u, 0u, 0u, 0u};
-    }
+    for (int k = 0; k < kVecs; ++k) v[k] = *reinterpret_cast<const u32x4_any*>(p + k * 256 * V);
+  } else {
+    int rest[kVecs];
+    places<V>(f, vpr, first, n, [&](int k, int64_t row, int64_t col, int64_t left) __attribute__((always_inline)) {
+      v[k] = load16<T>(g + row * f.ld + col, left, f.cols >= V && row + 1 < f.rows);
+      rest[k] = (int)(left < V ? left : V);
+    });
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) s += squares<T>(v[k]);
+    for (int k = 0; k < kVecs; ++k) mask16<T>(v[k], rest[k]);
   }
+  double s = 0.0;
+#pragma unroll
+  for (int k = 0; k < kVecs; ++k) s += squares<T>(v[k]);
   return s;
 }
 
@@ -179,32 +212,34 @@ __global__ __launch_bounds__(256) void norm_kernel(const double* __restrict__ pa
 template <typename T>
 __device__ __forceinline__ void chunk_clip(const Leaf& f, int64_t vpr, int64_t first, int n, bool clip, float norm,
                                            float most) {
-  const Place p = place(f, vpr, first);
+  constexpr int V = 16 / sizeof(T);
   const T* g = reinterpret_cast<const T*>(f.g);
   T* out = reinterpret_cast<T*>(f.out);
-  auto scaled = [&](float x) { return clip ? (x / norm) * most : x; };
-  for (int i0 = threadIdx.x; i0 < n; i0 += 256 * kUnroll) {
-    u32x4 v[kUnroll];
-    int64_t row[kUnroll], col[kUnroll];
+  auto scaled = [&](const u32x4& v) __attribute__((always_inline)) {
+    auto one = [&](float x) __attribute__((always_inline)) { return clip ? (x / norm) * most : x; };
+    u32x4 o;
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int i = i0 + k * 256;
-      at(p, i, row[k], col[k]);
-      col[k] *= 16 / (int)sizeof(T);
-      v[k] = i < n ? load16<T>(g + row[k] * f.ld + col[k], f.cols - col[k]) : u32x4{0u, 0u, 0u, 0u};
+    for (int q = 0; q < 4; ++q) {
+      if constexpr (sizeof(T) == 2) o[q] = pack_bf16x2(one(bf16_lo(v[q])), one(bf16_hi(v[q])));
+      else o[q] = __float_as_uint(one(__uint_as_float(v[q])));
     }
+    return o;
+  };
+  u32x4 v[kVecs];
+  if (plain<V>(f, first, n)) {
+    const int64_t at = first * V + threadIdx.x * V;
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (i0 + k * 256 >= n) continue;
-      u32x4 o;
+    for (int k = 0; k < kVecs; ++k) v[k] = *reinterpret_cast<const u32x4_any*>(g + at + k * 256 * V);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        if constexpr (sizeof(T) == 2) o[q] = pack_bf16x2(scaled(bf16_lo(v[k][q])), scaled(bf16_hi(v[k][q])));
-        else o[q] = __float_as_uint(scaled(__uint_as_float(v[k][q])));
-      }
-      store16<T>(out + row[k] * f.ldo + col[k], o, f.cols - col[k]);
-    }
+    for (int k = 0; k < kVecs; ++k) __builtin_nontemporal_store(scaled(v[k]), reinterpret_cast<u32x4_any*>(out + at + k * 256 * V));
+    return;
   }
+  places<V>(f, vpr, first, n, [&](int k, int64_t row, int64_t col, int64_t left) __attribute__((always_inline)) {
+    v[k] = load16<T>(g + row * f.ld + col, left, f.cols >= V && row + 1 < f.rows);
+  });
+  places<V>(f, vpr, first, n, [&](int k, int64_t row, int64_t col, int64_t left) __attribute__((always_inline)) {
+    store16<T>(out + row * f.ldo + col, scaled(v[k]), left);
+  });
 }
 
 __global__ __launch_bounds__(256) void clip_kernel(Table t, const double* __restrict__ part, int parts, float most,
