@@ -20,6 +20,7 @@ there is no framework fallback.
 from __future__ import annotations
 
 import contextlib
+import functools
 
 import torch
 from torch.autograd.function import once_differentiable
@@ -230,9 +231,9 @@ def _check_rms(what: str, x: torch.Tensor, r, gamma: torch.Tensor, eps: float) -
     eps = float(eps)
     if not 1e-30 <= eps <= 1.0:  # NaN fails too
         raise ValueError(f"{what}: eps must lie in [1e-30, 1], got {eps}")
-    for t in (gamma,) if r is None else (gamma, r):
-        if t.device != x.device:
-            raise ValueError(f"{what}: all tensors must be on one device, got {x.device} and {t.device}")
+    dev = x.get_device()
+    if gamma.get_device() != dev or (r is not None and r.get_device() != dev) or gamma.is_meta != x.is_meta:
+        raise ValueError(f"{what}: all tensors must be on one device, got {x.device}, gamma on {gamma.device}")
     _check_device(x)
     return eps
 
@@ -262,6 +263,11 @@ def _rms_fwd(x, r, gamma, eps, keep: bool):
     return y, s, rstd
 
 
+@functools.lru_cache(maxsize=1024)
+def _rms_ws_bytes(rows: int, D: int) -> int:
+    return int(_lib.load().nl_rms_norm_bwd_ws_bytes(rows, D))
+
+
 def _rms_grad_buffer(gamma: torch.Tensor):
     mg = grad_buffer(gamma)
     if mg is not None and (mg.shape != gamma.shape or mg.device != gamma.device or mg.dtype is not _F32
@@ -288,7 +294,7 @@ def _rms_bwd(ctx, dy, ds, s, rstd, gamma):
         d2, ldd = _strided_rows(dy if dy.dtype is s.dtype else dy.to(s.dtype))
         r2, ldr = _strided_rows(ds if ds.dtype is s.dtype else ds.to(s.dtype)) if ds is not None else (None, 0)
         g = _param(gamma)
-        wsb = _lib.load().nl_rms_norm_bwd_ws_bytes(rows, D) if need_dg else 0
+        wsb = _rms_ws_bytes(rows, D) if need_dg else 0
         ws = rstd.new_empty((wsb // 4,)) if wsb else None
         _lib.call_on(s2, "nl_rms_norm_bwd", rows, D, _rms_code(s2), d2.data_ptr(), ldd, s2.data_ptr(), lds,
                      rstd.data_ptr(), g.data_ptr(), r2.data_ptr() if ds is not None else None, ldr, dx.data_ptr(), D,
