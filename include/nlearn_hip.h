@@ -76,6 +76,7 @@ const char* nl_version(void);
 #define NL_OP_T 1
 #define NL_DTYPE_F32  0
 #define NL_DTYPE_BF16 1
+#define NL_DTYPE_E4M3 2  /* 8 bits with scales: results of nl_gemm_fp8_fused only */
 
 int nl_gemm(void* stream, int opA, int opB, int M, int N, int K,
             float alpha, const nl_bf16* A, int64_t lda,
@@ -525,6 +526,41 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
                 const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b,
                 void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes);
 
+/* nl_gemm_fp8 with what follows a layer's product in its epilogue, in fp32 behind the sum:
+ *   u = A . B^T + bias[n]      (bias NULL: none)
+ *   C = act(u) + residual      (residual NULL: none)
+ * act: gelu is the tanh form of nl_gemm_fused, silu u * sigmoid(u); NaN stays NaN.
+ * round_u: u is rounded to the type of C before act, as what a backward pass keeps; aux (the type
+ * of C, may be NULL): that u is written there (implies round_u). residual: the type of C (bf16 for
+ * C in 8 bits). C: fp32 or bf16, summed as nl_gemm_fp8 sums them; or NL_DTYPE_E4M3, summed as bf16
+ * is and quantised along N as nl_quantize_fp8 does it with group 1 (ldc bytes a row, whole blocks
+ * of 128, bytes past N zero; scale_c rows ldsc apart; no aux, no round_u). residual, aux: 16-byte
+ * aligned, rows a multiple of 8 elements apart. Every row of residual, aux and (fp32, bf16) C, the
+ * last one too, holds N rounded up to 8 elements: those past N are read, and overwritten in aux
+ * and C. residual may be C (the same address and stride); no other overlap. K == 0: the product is 0. Workspace as nl_gemm_fp8. */
+#define NL_ACT_NONE 0
+#define NL_ACT_RELU 1
+#define NL_ACT_GELU 2
+#define NL_ACT_SILU 3
+int nl_gemm_fp8_fused(void* stream, int M, int N, int K,
+                      const uint8_t* A, int64_t lda, const uint8_t* scale_a, int64_t ldsa, int group_a,
+                      const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b,
+                      const float* bias, int act, const void* residual, int64_t ldr, int round_u,
+                      void* aux, int64_t ldaux, void* C, int c_dtype, int64_t ldc,
+                      uint8_t* scale_c, int64_t ldsc, void* ws, size_t ws_bytes);
+
+/* A layer's output gradient behind an activation, quantised: d = dy * act'(u) (dy and u fp32 or
+ * bf16, of one type; act NL_ACT_NONE: d = dy, u is not read), formed in fp32.
+ *   q, scale; qt, scale_t:  d and its transpose as nl_quantize_fp8 gives them with group 1 (NULL: not wanted)
+ *   dbias[c] = sum_rows d   (NULL: not wanted), summed in a fixed order over a workspace of
+ *                           nl_quantize_fp8_dact_ws_bytes() bytes (4-byte aligned)
+ * relu'(0) is 0; a NaN in u gives NaN. */
+size_t nl_quantize_fp8_dact_ws_bytes(int64_t rows, int64_t cols);
+int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy,
+                         const void* u, int64_t ldu, int act, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
+                         uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, float* dbias, void* ws,
+                         size_t ws_bytes);
+
 /* y[M][N] = x[M][K] . W[K][N] with both operands quantised first (x in blocks of 1 x
  * 128 along K, W of 128 x 128), and its gradients from dy[M][N]: dx = dy . W^T (dy in
  * blocks along N) and dW = x^T . dy (x^T and dy^T in blocks along M), each the product
@@ -545,6 +581,24 @@ int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_
                       const void* saved, size_t saved_bytes, int need_dx, int need_dw,
                       void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw,
                       void* ws, size_t ws_bytes);
+
+/* The same pair with the epilogue of nl_gemm_fp8_fused: y = act(x . W + bias) + residual, with
+ * u = x . W + bias rounded to the type of y where there is an activation; u (may be NULL: not
+ * kept) is what the backward reads. The backward takes dy in the type of y and u, forms
+ * d = dy * act'(u) and its products, and dbias[N] = sum_rows d (NULL: not wanted). The residual's
+ * gradient is dy. residual, u: as nl_gemm_fp8_fused takes them; the workspace of the backward
+ * with dbias is larger. */
+size_t nl_linear_fp8_fused_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw, int need_db);
+int nl_linear_fp8_fused_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
+                            const void* W, int w_dtype, int64_t ldw, const float* bias, int act,
+                            const void* residual, int64_t ldr, void* u, int64_t ldu,
+                            void* y, int y_dtype, int64_t ldy, int need_dx, int need_dw,
+                            void* saved, size_t saved_bytes, void* ws, size_t ws_bytes);
+int nl_linear_fp8_fused_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
+                            const void* u, int64_t ldu, int act, float* dbias,
+                            const void* saved, size_t saved_bytes, int need_dx, int need_dw,
+                            void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw,
+                            void* ws, size_t ws_bytes);
 
 /* ======================================================================== */
 /* Root-mean-square norm                                                      */

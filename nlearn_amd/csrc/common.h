@@ -80,6 +80,17 @@ __device__ __forceinline__ float gelu_tanh_grad(float u) {
   return s * __builtin_fmaf(u * (1.f - s), q, 1.f);
 }
 
+// u * sigmoid(u) and its derivative s (1 + u (1 - s)), s = 1 / (1 + 2^(-u log2(e))); the derivative
+// clamps |u| <= 120, beyond which it is below 2^-166 or 1
+__device__ __forceinline__ float silu(float u) {
+  return u * __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.4426950408889634f * u));
+}
+__device__ __forceinline__ float silu_grad(float u) {
+  u = fminf(fmaxf(u, -120.f), 120.f);
+  const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.4426950408889634f * u));
+  return s * __builtin_fmaf(u, 1.f - s, 1.f);
+}
+
 // ---------------------------------------------------------------------------
 // wavefront reductions (butterfly over all 64 lanes)
 // ---------------------------------------------------------------------------
@@ -178,4 +189,6 @@ int nl_set_error(int code, const std::string& msg);
 int nl_check_launch(const char* what);
 namespace nl {
 int cu_count();  // compute units of the current device (256 where there is none)
+// out[c] (+)= sum over p < P of part[p][c], c < D, in a fixed order (rms.hip)
+void launch_partial_sums(hipStream_t st, int P, int D, const float* part, float* out, int accumulate);
 }

@@ -45,12 +45,23 @@ struct QuantArgs {
   int64_t ldqt;
   uint8_t* st;
   int64_t ldst;
+  // a layer's output gradient: x * act'(u) is quantised
+  const void* u = nullptr;  // in the type of x
+  int64_t ldu = 0;
+  int act = NL_ACT_NONE;
+  float* part = nullptr;    // column sums of each 128 rows, [ceil(rows / 128)][cols] (may be null)
 };
+
+// act'(u); NaN stays NaN
+__device__ __forceinline__ float act_grad(float u, int act) {
+  float d = act == NL_ACT_GELU ? gelu_tanh_grad(u) : act == NL_ACT_SILU ? silu_grad(u) : u > 0.f ? 1.f : 0.f;
+  return u == u ? d : u;
+}
 
 // x[row][c0 .. c0+7] as floats, zero past the last column
 template <typename T>
-__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
-  const T* p = reinterpret_cast<const T*>(a.x) + row * a.ldx + c0;
+__device__ __forceinline__ void load8_of(const T* x, int64_t ld, const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
+  const T* p = x + row * ld + c0;
   if (a.vec && c0 + 8 <= a.cols) {
     if constexpr (sizeof(T) == 2) {
       const u32x4 u = *reinterpret_cast<const u32x4*>(p);
@@ -80,9 +91,21 @@ __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c
   }
 }
 
+template <typename T, bool kAct = false>
+__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
+  load8_of<T>(reinterpret_cast<const T*>(a.x), a.ldx, a, row, c0, v);
+  if constexpr (kAct) {
+    if (a.act == NL_ACT_NONE) return;
+    float u[8];
+    load8_of<T>(reinterpret_cast<const T*>(a.u), a.ldu, a, row, c0, u);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + i < a.cols ? v[i] * act_grad(u[i], a.act) : 0.f;
+  }
+}
+
 // One row's block of 128 per 16 lanes, 8 elements a lane: one read, one write. Bound
 // by HBM: 16384 x 2048 bf16 17.8 us, 8192 x 8192 32.5 us (5.7 and 6.2 TB/s).
-template <typename T>
+template <typename T, bool kAct = false>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_t blocks, uint32_t kb) {
   const uint32_t id = blockIdx.x * 16u + (threadIdx.x >> 4);
   if (id >= blocks) return;  // whole groups of 16 lanes leave together
@@ -90,7 +113,7 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
   const int l = threadIdx.x & 15;
   const int64_t c0 = (int64_t)b * kB + l * 8;
   float v[8];
-  load8<T>(a, row, c0, v);
+  load8<T, kAct>(a, row, c0, v);
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
@@ -115,6 +138,16 @@ __device__ __forceinline__ uint32_t max_rows(uint32_t v) {
   return max((uint32_t)r32[0], (uint32_t)r32[1]);
 }
 
+// sum over the lanes l, l + 16, l + 32, l + 48
+__device__ __forceinline__ float sum_rows(float v) {
+  const uint32_t a = __float_as_uint(v);
+  const auto r16 = __builtin_amdgcn_permlane16_swap(a, a, false, false);
+  v = __uint_as_float(r16[0]) + __uint_as_float(r16[1]);
+  const uint32_t b = __float_as_uint(v);
+  const auto r32 = __builtin_amdgcn_permlane32_swap(b, b, false, false);
+  return __uint_as_float(r32[0]) + __uint_as_float(r32[1]);
+}
+
 // A 128 x 128 tile per workgroup: read once, written along the rows and, through
 // LDS, along the columns. Lane group g = tid / 16 holds rows 4g .. 4g+3, lane
 // l = tid % 16 columns 8l .. 8l+7, so a thread has 4 bytes of a column that lie
@@ -130,7 +163,7 @@ struct QuantTile {
   uint32_t colmax[8][kB];
   uint8_t colbyte[kB];
 };
-template <typename T>
+template <typename T, bool kAct = false>
 __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block, uint32_t cb, QuantTile& sm) {
   auto& tile = sm.tile;
   auto& colmax = sm.colmax;
@@ -144,10 +177,27 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   for (int i = 0; i < 4; ++i) {
     const int64_t r = r0 + g * 4 + i;
     if (r < a.rows) {
-      load8<T>(a, r, cl, v[i]);
+      load8<T, kAct>(a, r, cl, v[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+    }
+  }
+  if constexpr (kAct) {
+    if (a.part) {  // the tile's column sums: a thread's 4 rows, a wave's 4 groups, then the 8 waves
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float t = sum_rows((v[0][j] + v[1][j]) + (v[2][j] + v[3][j]));
+        if ((tid & 63) < 16) colmax[tid >> 6][l * 8 + j] = __float_as_uint(t);
+      }
+      __syncthreads();
+      if (tid < kB && c0 + tid < a.cols) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) t += __uint_as_float(colmax[i][tid]);
+        a.part[(int64_t)by * a.cols + c0 + tid] = t;
+      }
+      __syncthreads();
     }
   }
   uint32_t rm[4], cm[8];
@@ -229,10 +279,10 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   }
 }
 
-template <typename T>
+template <typename T, bool kAct = false>
 __global__ __launch_bounds__(512) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
   __shared__ __attribute__((aligned(16))) QuantTile sm;
-  quantize_tile<T>(a, blockIdx.x, cb, sm);
+  quantize_tile<T, kAct>(a, blockIdx.x, cb, sm);
 }
 
 // Two matrices in one launch, the first one's tiles (na of them) before the second's.
@@ -294,7 +344,20 @@ struct GemmF8Args {
   int tiles;     // output tiles
   int items;     // tiles * splits
   int kb_chunk;  // blocks per split (a multiple of 4 when there is more than one)
+  // the epilogue's, of the kernels that have one
+  const float* bias;  // may be null
+  int act;            // NL_ACT_*
+  const void* res;    // in the type of C (bf16 beside 8 bits), may be null
+  int64_t ldres;
+  void* aux;          // u in the type of C, may be null
+  int64_t ldaux;
+  uint8_t* sc;        // scales of C in 8 bits
+  int64_t ldsc;
 };
+
+// Epilogues of a product: none; u = acc + bias, C = act(u) + res; and that with u rounded to
+// the type of C before, and kept where it is asked for (what a backward pass reads).
+enum { kPlain = 0, kEpi = 1, kEpiKeep = 2 };
 
 // Four scale bytes of one row from byte `off` (n of them there): one dword where
 // rows are whole, aligned dwords, else byte by byte.
@@ -420,8 +483,23 @@ __device__ __forceinline__ F8Item f8_item(const GemmF8Args& g, int item) {
   return t;
 }
 
+// act(u) of 8 values; NaN stays NaN
+__device__ __forceinline__ void activate(float (&v)[8], int act) {
+  if (act == NL_ACT_GELU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = gelu_tanh(v[k]);
+  } else if (act == NL_ACT_SILU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = silu(v[k]);
+  } else if (act == NL_ACT_RELU) {
+#pragma unroll
+    for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+  }
+}
+
 // kDw: scale rows are whole, aligned dwords. Else a scale dword is four byte loads.
-template <int BM, int BN, int WTM, int WTN, typename OutT, bool kDw>
+// OutT: float, uint16_t (bf16) or, with an epilogue, uint8_t (e4m3 with its scales).
+template <int BM, int BN, int WTM, int WTN, typename OutT, bool kDw, int EPI = kPlain>
 __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 1 : 2) void gemm_f8_kernel(
     GemmF8Args g) {
   constexpr int WNW = BN / WTN, NWV = (BM / WTM) * WNW;
@@ -432,7 +510,9 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   constexpr bool kWide = sizeof(OutT) == 4;            // widened to bf16 for fp32 sums
   constexpr int NS = kWide ? 4 : 2;                    // fragment steps of a stage: 16 or 32 bytes of k a lane
   constexpr int CH = kWide ? 1 : 2;                    // 16-byte chunks of a fragment
-  constexpr int PITCH = 2 * WTN;                       // bytes of a slab row: WTN bf16 or half as many fp32
+  // bytes of a slab row: WTN bf16 or half as many fp32
+  constexpr int PITCH = BM * BN >= 65536 || 2 * WTN < 128 ? 2 * WTN : 128;
+  static_assert(PITCH == 2 * WTN || EPI != kPlain, "an item without an epilogue leaves in slabs of whole rows");
   // Each stage is an LDS object of its own: the compiler then knows that the DMA into
   // one does not alias the reads of the other.
   __shared__ __attribute__((aligned(16))) uint8_t st0[STAGE];
@@ -610,7 +690,21 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     load_scales(t, own ? (kt >> 2) + 1 : 0);
   };
   constexpr int kScales = (FM + FN) * (kDw ? 1 : 4);       // loads of one set of scales
-  constexpr int kStores = FM * (sizeof(OutT) / 2) * PITCH / 32;  // stores of a whole tile, 64 lanes of 16 bytes each
+  // stores of a whole tile, 64 lanes of 16 bytes each
+  constexpr int kStores = FM * 32 * WTN * (int)sizeof(OutT) / 1024;
+
+  // bias of this wave's columns, one of each 64 a lane (0 past the last column, or without a bias)
+  constexpr int kBias = EPI != kPlain ? WTN / 64 : 1;
+  float bias1[kBias];
+  auto load_bias = [&](const F8Item& t) __attribute__((always_inline)) {
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(g.bias ? (const void*)g.bias : (const void*)g.C, kNowhere);
+    const int n = g.bias ? g.N : 0;
+#pragma unroll
+    for (int k = 0; k < kBias; ++k) {
+      const int c = t.n0 + wn * WTN + k * 64 + lane;
+      bias1[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rb, c < n ? (uint32_t)c * 4u : kNowhere, 0, 0));
+    }
+  };
 
   load_scales(cur, 0);
   issue(st0, cur, 0);
@@ -631,6 +725,7 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     // Behind this stage's DMA lie the last item's stores and this set of scales (a tile
     // at an edge has waited for its stores itself).
     scales_ahead(0);
+    if constexpr (EPI != kPlain) load_bias(cur);
     stage(0, P0{}, std::true_type{}, std::integral_constant<int, (kScales + kStores < 63 ? kScales + kStores : 63)>{});
     stage(1, P1{}, No{}, P0{});
     if (stages > 2) {
@@ -662,6 +757,171 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     int ln = lane;
     asm volatile("" : "+v"(ln));
     const int fr = ln & 31, g4 = (ln >> 5) * 4;
+    if constexpr (EPI != kPlain) {
+      // The slab holds fp32 here, SC columns at a time, and a lane takes 8 columns of a row (the same
+      // ones in every row: its bias stays in registers), so that residual and result are whole 16-byte
+      // pieces. Every store is made, with an offset out of range where the matrix ends.
+      constexpr int SC = PITCH / 4, NH = WTN / SC;            // NH slabs side by side
+      constexpr int LPR = SC / 8, RPI = 64 / LPR;             // lanes of a row, rows at a time
+      constexpr int kReads = 32 / RPI, kPieces = SC / 8, CPR = PITCH / 16;
+      constexpr int kRes = sizeof(OutT) == 4 ? 2 : 1;         // 16-byte pieces of 8 residuals
+      constexpr int RE = sizeof(OutT) == 4 ? 4 : 2;           // bytes of one
+      constexpr bool k8 = sizeof(OutT) == 1;
+      const int rr = ln / LPR, gg = ln % LPR;
+      float bias[NH][8];
+#pragma unroll
+      for (int h = 0; h < NH; ++h)
+#pragma unroll
+        for (int k = 0; k < 8; ++k) bias[h][k] = __shfl(bias1[h * SC / 64], h * SC % 64 + gg * 8 + k, 64);
+      // One of the matrices that C's tile lies over: a descriptor from the tile's first element, this
+      // lane's offset from there, the rows there are (none of a matrix that is not given).
+      struct Mat {
+        __amdgpu_buffer_rsrc_t rs;
+        uint32_t lane, ld;
+        int rows;
+      };
+      const int cols = g.N - cur.n0;  // of the tile that are there (or more)
+      auto mat = [&](const void* p, int64_t ld) __attribute__((always_inline)) {
+        const uint8_t* base = reinterpret_cast<const uint8_t*>(p ? p : g.C);
+        return Mat{make_rsrc(uniform(base + (p ? ((int64_t)cur.m0 * ld + cur.n0) * RE : 0)), kNowhere),
+                   (uint32_t)(rr * (int)ld + gg * 8) * RE, (uint32_t)ld, p ? g.M - cur.m0 : 0};
+      };
+      // element `add` of the lane's 8 in rows `it` of slab (i, h): its offset; where `there` is false
+      // one out of every range
+      auto off = [&](const Mat& m, int i, int h, int it, int add, bool there) __attribute__((always_inline)) {
+        const int row = wm * WTM + i * 32 + it * RPI, col = wn * WTN + h * SC;
+        return there && rr < m.rows - row ? m.lane + ((uint32_t)row * m.ld + col + add) * RE : kNowhere;
+      };
+      // whether these 8 columns are there: a piece that N cuts is read and written whole, its matrices'
+      // rows hold N rounded up to 8
+      auto in8 = [&](int h) __attribute__((always_inline)) { return wn * WTN + h * SC + gg * 8 < cols; };
+      const Mat mres = mat(g.res, g.ldres), maux = mat(EPI == kEpiKeep ? g.aux : nullptr, g.ldaux),
+                mc = mat(k8 ? nullptr : g.C, g.ldc);
+      auto load_res = [&](int i, int h, u32x4 (&r)[kReads][kRes]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int it = 0; it < kReads; ++it) {
+#pragma unroll
+          for (int k = 0; k < kRes; ++k)
+            r[it][k] = __builtin_amdgcn_raw_buffer_load_b128(mres.rs, off(mres, i, h, it, 4 * k, in8(h)), 0, 0);
+        }
+      };
+      auto put8 = [&](const Mat& m, int i, int h, int it, const float (&v)[8]) __attribute__((always_inline)) {
+        u32x4 w[kRes];
+        if constexpr (RE == 2) {
+          w[0] = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
+        } else {
+          w[0] = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
+          w[kRes - 1] = __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]});
+        }
+#pragma unroll
+        for (int k = 0; k < kRes; ++k)
+          __builtin_amdgcn_raw_buffer_store_b128(w[k], m.rs, off(m, i, h, it, 4 * k, in8(h)), 0, 2 /* nt */);
+      };
+      auto put_slab = [&](int i, int h) __attribute__((always_inline)) {
+#pragma unroll
+        for (int p = 0; p < kPieces; ++p) {
+          const int j = h * (SC / 32) + p / 4, q = p % 4;
+          if (q == 0) asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
+          *reinterpret_cast<f32x4*>(wl + fr * PITCH + (((p * 2 + (ln >> 5)) ^ (fr & (CPR - 1))) << 4)) =
+              f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
+        }
+      };
+      auto get8 = [&](int it, float (&v)[8]) __attribute__((always_inline)) {
+        const int r = it * RPI + rr;
+        const f32x4 a = *reinterpret_cast<const f32x4*>(wl + r * PITCH + (((2 * gg) ^ (r & (CPR - 1))) << 4));
+        const f32x4 b = *reinterpret_cast<const f32x4*>(wl + r * PITCH + (((2 * gg + 1) ^ (r & (CPR - 1))) << 4));
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
+      };
+      // u, act(u) and the residual of 8 columns
+      auto finish = [&](int i, int h, int it, float (&v)[8], const u32x4 (&r)[kRes]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) v[k] += bias[h][k];
+        if constexpr (EPI == kEpiKeep) {
+          put8(maux, i, h, it, v);
+          if constexpr (RE == 2) {
+#pragma unroll
+            for (int k = 0; k < 8; k += 2) {
+              const uint32_t w = pack_bf16x2(v[k], v[k + 1]);
+              v[k] = bf16_lo(w);
+              v[k + 1] = bf16_hi(w);
+            }
+          }
+        }
+        activate(v, g.act);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          if constexpr (RE == 2) v[k] += k & 1 ? bf16_hi(r[0][k >> 1]) : bf16_lo(r[0][k >> 1]);
+          else v[k] += __uint_as_float(r[k >> 2][k & 3]);
+        }
+      };
+      u32x4 res[2][kReads][kRes];
+      float v[k8 ? NH : 1][kReads][8];
+      load_res(0, 0, res[0]);
+      put_slab(0, 0);
+#pragma unroll
+      for (int s = 0; s < FM * NH; ++s) {
+        const int i = s / NH, h = s % NH, hv = k8 ? h : 0;
+        if (s + 1 < FM * NH) load_res((s + 1) / NH, (s + 1) % NH, res[(s + 1) & 1]);
+#pragma unroll
+        for (int it = 0; it < kReads; ++it) get8(it, v[hv][it]);
+        if (s + 1 < FM * NH && !(k8 && h == NH - 1)) put_slab((s + 1) / NH, (s + 1) % NH);
+#pragma unroll
+        for (int it = 0; it < kReads; ++it) {
+          finish(i, h, it, v[hv][it], res[s & 1][it]);
+          if constexpr (!k8) put8(mc, i, h, it, v[0][it]);
+        }
+        if constexpr (k8) {
+          if (h < NH - 1) continue;
+          // a wave's columns are one block of 128: its largest value over the lanes of a row, then the
+          // bytes through the slab into whole rows
+          static_assert(WTN == kB, "a wave holds whole blocks of C");
+          const int n = cur.n0 + wn * WTN;
+          const bool there = n < g.N;
+          const __amdgpu_buffer_rsrc_t rc8 = make_rsrc(
+              uniform(reinterpret_cast<const uint8_t*>(g.C) + (there ? (int64_t)cur.m0 * g.ldc + n : 0)), kNowhere);
+          if (cols < BN) {  // nothing past N has a part in the scale, and its bytes are zero
+#pragma unroll
+            for (int it = 0; it < kReads; ++it)
+#pragma unroll
+              for (int x = 0; x < NH; ++x)
+#pragma unroll
+                for (int k = 0; k < 8; ++k)
+                  if (wn * WTN + x * SC + gg * 8 + k >= cols) v[x][it][k] = 0.f;
+          }
+#pragma unroll
+          for (int it = 0; it < kReads; ++it) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int x = 0; x < NH; ++x)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) m = max(m, finite_abs_bits(v[x][it][k]));
+            m = max(m, dpp_u<0xB1>(m));
+            m = max(m, dpp_u<0x4E>(m));
+            if constexpr (LPR == 8) m = max(m, dpp_u<0x141>(m));
+            const int byte = scale_byte(m), r = it * RPI + rr;
+            const float inv = inv_scale(byte);
+#pragma unroll
+            for (int x = 0; x < NH; ++x) {
+              const float(&w)[8] = v[x][it];
+              *reinterpret_cast<u32x2*>(wl + r * 128 + ((((x * SC + gg * 8) >> 4) ^ (r & 7)) << 4) + (gg & 1) * 8) =
+                  u32x2{pack_e4m3x4(w[0] * inv, w[1] * inv, w[2] * inv, w[3] * inv),
+                        pack_e4m3x4(w[4] * inv, w[5] * inv, w[6] * inv, w[7] * inv)};
+            }
+            const int row = wm * WTM + i * 32 + r;
+            if (gg == 0 && row < g.M - cur.m0 && there) g.sc[(int64_t)(cur.m0 + row) * g.ldsc + n / kB] = (uint8_t)byte;
+          }
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const int r = it * 8 + ln / 8, row = wm * WTM + i * 32 + r;
+            const u32x4 w = *reinterpret_cast<const u32x4*>(wl + r * 128 + (((ln % 8) ^ (r & 7)) << 4));
+            __builtin_amdgcn_raw_buffer_store_b128(
+                w, rc8, row < g.M - cur.m0 && there ? (uint32_t)row * (uint32_t)g.ldc + (uint32_t)(ln % 8 * 16) : kNowhere, 0, 0);
+          }
+          if (s + 1 < FM * NH) put_slab((s + 1) / NH, 0);
+        }
+      }
+    } else {
     const bool whole = cur.m0 + BM <= g.M && cur.n0 + BN <= g.N;
     using T = OutT;
     constexpr int SC = PITCH / (int)sizeof(T);                 // columns of a slab
@@ -767,6 +1027,7 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
       put_edge();
       wait_vm<0>();
     }
+    }
     if (next >= last) wait_vm<0>();  // no DMA is in flight when the workgroup ends
     if (next >= last) break;
     item = next;
@@ -799,6 +1060,85 @@ __global__ __launch_bounds__(256) void f8_reduce_kernel(GemmF8Args g, int splits
         if constexpr (sizeof(OutT) == 2) dst[k] = f32_to_bf16(s[k]);
         else dst[k] = s[k];
       }
+  }
+}
+
+// The same with an epilogue. Of C in 8 bits a block of 128 is 32 lanes' columns.
+template <typename OutT, int EPI>
+__global__ __launch_bounds__(256) void f8_reduce_epi_kernel(GemmF8Args g, int splits) {
+  using RT = typename std::conditional<sizeof(OutT) == 4, float, uint16_t>::type;  // of residual and u
+  const int n = (blockIdx.x * 64 + (threadIdx.x & 63)) * 4;
+  if (sizeof(OutT) != 1 && n >= g.N) return;
+  auto load4 = [&](const RT* p, float (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      v[k] = 0.f;
+      if (n + k < g.N) {
+        if constexpr (sizeof(RT) == 2) v[k] = bf16_to_f32(p[k]);
+        else v[k] = p[k];
+      }
+    }
+  };
+  auto store4 = [&](RT* p, const float (&v)[4]) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      if (n + k < g.N) {
+        if constexpr (sizeof(RT) == 2) p[k] = f32_to_bf16(v[k]);
+        else p[k] = v[k];
+      }
+  };
+  float bias[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) bias[k] = g.bias && n + k < g.N ? g.bias[n + k] : 0.f;
+  for (int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); m < g.M; m += (int64_t)gridDim.y * 4) {
+    const float* p = g.ws + m * g.ldw + n;
+    const int64_t step = (int64_t)g.M * g.ldw;
+    float res[4] = {0.f, 0.f, 0.f, 0.f};
+    if (g.res) load4(reinterpret_cast<const RT*>(g.res) + m * g.ldres + n, res);
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    if (n < g.N) {  // (partial rows are whole vectors)
+      for (int k0 = 0; k0 < splits; k0 += 8) {
+        f32x4 v[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k0 + k < splits) v[k] = *reinterpret_cast<const f32x4*>(p + (k0 + k) * step);
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+          if (k0 + k < splits) s += v[k];
+      }
+    }
+    float u[8], o[4];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) u[k] = k < 4 && n + k < g.N ? s[k & 3] + bias[k & 3] : 0.f;
+    if constexpr (EPI == kEpiKeep) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        if constexpr (sizeof(RT) == 2) u[k] = bf16_to_f32(f32_to_bf16(u[k]));
+        o[k] = u[k];
+      }
+      if (g.aux) store4(reinterpret_cast<RT*>(g.aux) + m * g.ldaux + n, o);
+    }
+    activate(u, g.act);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) o[k] = u[k] + res[k];
+    if constexpr (sizeof(OutT) == 1) {
+      uint32_t x = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) x = max(x, n + k < g.N ? finite_abs_bits(o[k]) : 0u);
+      x = max16(x);
+      const auto r16 = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+      x = max((uint32_t)r16[0], (uint32_t)r16[1]);
+      const int byte = scale_byte(x);
+      const float inv = inv_scale(byte);
+      if (n < (g.N + kB - 1) / kB * kB) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[k] = n + k < g.N ? o[k] * inv : 0.f;
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(g.C) + m * g.ldc + n) = pack_e4m3x4(o[0], o[1], o[2], o[3]);
+        if ((threadIdx.x & 31) == 0) g.sc[m * g.ldsc + n / kB] = (uint8_t)byte;
+      }
+    } else {
+      store4(reinterpret_cast<RT*>(g.C) + m * g.ldc + n, o);
+    }
   }
 }
 
@@ -840,22 +1180,39 @@ F8Plan f8_plan(int M, int N, int K) {
 
 int64_t f8_ldw(int N) { return ((int64_t)N + 3) / 4 * 4; }
 
+template <int BM, int BN, int WTM, int WTN, typename OutT, int EPI>
+void launch_tiles(hipStream_t st, const GemmF8Args& g) {
+  const dim3 grid((unsigned)std::min(g.items, (BM * BN >= 65536 ? 1 : 2) * cu_count()));
+  if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, true, EPI>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, false, EPI>), grid, dim3(256), 0, st, g);
+}
+
 template <typename OutT>
 void launch_f8(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
-  const int cus = cu_count();
-  if (p.huge) {
-    const dim3 grid((unsigned)std::min(g.items, cus));
-    if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT, true>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((gemm_f8_kernel<256, 256, 128, 128, OutT, false>), grid, dim3(256), 0, st, g);
-  } else {
-    const dim3 grid((unsigned)std::min(g.items, 2 * cus));
-    if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT, true>), grid, dim3(256), 0, st, g);
-    else hipLaunchKernelGGL((gemm_f8_kernel<128, 128, 64, 64, OutT, false>), grid, dim3(256), 0, st, g);
-  }
+  if (p.huge) launch_tiles<256, 256, 128, 128, OutT, kPlain>(st, g);
+  else launch_tiles<128, 128, 64, 64, OutT, kPlain>(st, g);
   if (p.splits > 1)
     hipLaunchKernelGGL((f8_reduce_kernel<OutT>),
                        dim3((unsigned)((g.N + 255) / 256), (unsigned)std::min<int64_t>(((int64_t)g.M + 3) / 4, 65535)),
                        dim3(256), 0, st, g, p.splits);
+}
+
+template <typename OutT, int EPI>
+void launch_f8_epi(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
+  if (p.splits > 1) {
+    // partials as the same result without an epilogue has them
+    using PT = typename std::conditional<sizeof(OutT) == 4, float, uint16_t>::type;
+    launch_tiles<128, 128, 64, 64, PT, kPlain>(st, g);
+    hipLaunchKernelGGL((f8_reduce_epi_kernel<OutT, EPI>),
+                       dim3((unsigned)((g.N + 255) / 256), (unsigned)std::min<int64_t>(((int64_t)g.M + 3) / 4, 65535)),
+                       dim3(256), 0, st, g, p.splits);
+  } else if (p.huge) {
+    launch_tiles<256, 256, 128, 128, OutT, EPI>(st, g);
+  } else if constexpr (sizeof(OutT) == 1) {
+    launch_tiles<128, 128, 32, 128, OutT, EPI>(st, g);
+  } else {
+    launch_tiles<128, 128, 64, 64, OutT, EPI>(st, g);
+  }
 }
 
 // 256 rows of a tile are addressed with 31-bit offsets: bytes of an operand's row, elements of a result's
@@ -884,13 +1241,15 @@ namespace nl {
 namespace {
 
 // The checks of nl_quantize_fp8, and its kernel's arguments (rows or cols 0: nothing to do).
+// sums: what is written is the column sums (too).
 int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t ldx, int group, uint8_t* q, int64_t ldq,
-               uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, QuantArgs* out) {
+               uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, QuantArgs* out,
+               bool sums = false) {
   if (rows < 0 || cols < 0 || rows > INT32_MAX || cols > INT32_MAX)
     return nl_set_error(NL_EINVAL, "quantize_fp8: need 0 <= rows, cols < 2^31");
   if (x_dtype != NL_DTYPE_F32 && x_dtype != NL_DTYPE_BF16)
     return nl_set_error(NL_EINVAL, "quantize_fp8: x is fp32 or bf16");
-  if (!q && !qt) return nl_set_error(NL_EINVAL, "quantize_fp8: no output");
+  if (!q && !qt && !sums) return nl_set_error(NL_EINVAL, "quantize_fp8: no output");
   if (q)
     if (int rc = check_operand("quantize_fp8", rows, cols, q, ldq, scale, lds, group)) return rc;
   if (qt)
@@ -905,28 +1264,53 @@ int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t l
   return NL_OK;
 }
 
+// The same of dy * act'(u), with its column sums: dbias, over partial rows in ws.
+int dact_args(int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy, const void* u, int64_t ldu, int act,
+              uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t,
+              int64_t ldst, float* dbias, float* part, QuantArgs* out) {
+  const char* what = "quantize_fp8_dact";
+  if (act < NL_ACT_NONE || act > NL_ACT_SILU) return nl_set_error(NL_EINVAL, std::string(what) + ": unknown activation");
+  if (int rc = quant_args(rows, cols, dy, dtype, lddy, 1, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, out,
+                          dbias != nullptr))
+    return rc;
+  if (dbias && cols > 1 << 25) return nl_set_error(NL_EUNSUPPORTED, std::string(what) + ": a bias of more than 2^25");
+  if (rows == 0 || cols == 0) return NL_OK;
+  if (act != NL_ACT_NONE) {
+    const int esz = dtype == NL_DTYPE_BF16 ? 2 : 4;
+    if (!u) return nl_set_error(NL_EINVAL, std::string(what) + ": null u");
+    if (rows > 1 && ldu < cols) return nl_set_error(NL_EINVAL, std::string(what) + ": ldu < cols");
+    if ((uintptr_t)u % esz) return nl_set_error(NL_EALIGN, std::string(what) + ": u is not aligned to its type");
+    out->vec = out->vec && ((uintptr_t)u & 15) == 0 && (rows == 1 || ldu * esz % 16 == 0);
+  }
+  if (dbias && !part) return nl_set_error(NL_EINVAL, std::string(what) + ": workspace too small");
+  if ((uintptr_t)dbias & 3) return nl_set_error(NL_EALIGN, std::string(what) + ": dbias is not aligned");
+  out->u = u, out->ldu = ldu, out->act = act, out->part = dbias ? part : nullptr;
+  return NL_OK;
+}
+
 int64_t blocks_of(int64_t n) { return (n + kB - 1) / kB; }
 // a launch has fewer than 2^32 threads: 16 a block of 128 by rows in whole groups of 256, 512 a tile
 constexpr int64_t kMaxBlocks = ((int64_t)1 << 28) - 16, kMaxTiles = ((int64_t)1 << 23) - 1;
 
+template <bool kAct>
 int quantize_one(hipStream_t st, const QuantArgs& a, int dtype) {
   const int64_t rb = blocks_of(a.rows), cb = blocks_of(a.cols);
-  if (!a.qt && a.group == 1) {
+  if (!a.qt && a.group == 1 && !a.part) {
     const int64_t blocks = a.rows * cb;
     if (blocks > kMaxBlocks) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: more than 2^28 - 16 blocks");
     const dim3 grid((unsigned)((blocks + 15) / 16));
     if (dtype == NL_DTYPE_BF16)
-      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
+      hipLaunchKernelGGL((quantize_rows_kernel<uint16_t, kAct>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     else
-      hipLaunchKernelGGL((quantize_rows_kernel<float>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
+      hipLaunchKernelGGL((quantize_rows_kernel<float, kAct>), grid, dim3(256), 0, st, a, (uint32_t)blocks, (uint32_t)cb);
     return nl_check_launch("nl_quantize_fp8");
   }
   if (rb * cb > kMaxTiles) return nl_set_error(NL_EUNSUPPORTED, "quantize_fp8: 2^23 tiles of 128 x 128 and more");
   const dim3 grid((unsigned)(rb * cb));
   if (dtype == NL_DTYPE_BF16)
-    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t>), grid, dim3(512), 0, st, a, (uint32_t)cb);
+    hipLaunchKernelGGL((quantize_tile_kernel<uint16_t, kAct>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   else
-    hipLaunchKernelGGL((quantize_tile_kernel<float>), grid, dim3(512), 0, st, a, (uint32_t)cb);
+    hipLaunchKernelGGL((quantize_tile_kernel<float, kAct>), grid, dim3(512), 0, st, a, (uint32_t)cb);
   return nl_check_launch("nl_quantize_fp8");
 }
 
@@ -935,8 +1319,8 @@ int quantize_two(hipStream_t st, const QuantArgs& a, int a_dtype, const QuantArg
   const int64_t ca = blocks_of(a.cols), cb = blocks_of(b.cols);
   const int64_t na = blocks_of(a.rows) * ca, nb = blocks_of(b.rows) * cb;
   if ((!a.qt && a.group == 1) || (!b.qt && b.group == 1) || na + nb > kMaxTiles) {
-    if (int rc = quantize_one(st, a, a_dtype)) return rc;
-    return quantize_one(st, b, b_dtype);
+    if (int rc = quantize_one<false>(st, a, a_dtype)) return rc;
+    return quantize_one<false>(st, b, b_dtype);
   }
   const dim3 grid((unsigned)(na + nb));
 #define NL_QUANT_TWO(TA, TB)                                                                                  \
@@ -962,7 +1346,42 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
   QuantArgs a;
   if (int rc = quant_args(rows, cols, x, x_dtype, ldx, group, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, &a))
     return rc;
-  return rows == 0 || cols == 0 ? NL_OK : quantize_one((hipStream_t)stream, a, x_dtype);
+  return rows == 0 || cols == 0 ? NL_OK : quantize_one<false>((hipStream_t)stream, a, x_dtype);
+}
+
+namespace nl {
+namespace {
+
+int quantize_dact(hipStream_t st, const QuantArgs& a, int dtype, float* dbias) {
+  const int rc = a.act == NL_ACT_NONE && !a.part ? quantize_one<false>(st, a, dtype) : quantize_one<true>(st, a, dtype);
+  if (rc || !a.part) return rc;
+  launch_partial_sums(st, (int)blocks_of(a.rows), (int)a.cols, a.part, dbias, 0);
+  return nl_check_launch("nl_quantize_fp8_dact");
+}
+
+}  // namespace
+}  // namespace nl
+
+extern "C" size_t nl_quantize_fp8_dact_ws_bytes(int64_t rows, int64_t cols) {
+  return rows <= 0 || cols <= 0 ? 0 : (size_t)blocks_of(rows) * cols * sizeof(float);
+}
+
+extern "C" int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy,
+                                    const void* u, int64_t ldu, int act, uint8_t* q, int64_t ldq, uint8_t* scale,
+                                    int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst,
+                                    float* dbias, void* ws, size_t ws_bytes) {
+  QuantArgs a;
+  if ((uintptr_t)ws & 3) return nl_set_error(NL_EALIGN, "quantize_fp8_dact: workspace not aligned");
+  float* part = ws && ws_bytes >= nl_quantize_fp8_dact_ws_bytes(rows, cols) ? (float*)ws : nullptr;
+  if (int rc = dact_args(rows, cols, dy, dtype, lddy, u, ldu, act, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, dbias,
+                         part, &a))
+    return rc;
+  if (cols == 0) return NL_OK;
+  if (rows == 0) {
+    if (dbias) launch_partial_sums((hipStream_t)stream, 0, (int)cols, part, dbias, 0);
+    return nl_check_launch("nl_quantize_fp8_dact");
+  }
+  return quantize_dact((hipStream_t)stream, a, dtype, dbias);
 }
 
 extern "C" size_t nl_gemm_fp8_ws_bytes(int M, int N, int K) {
@@ -971,18 +1390,54 @@ extern "C" size_t nl_gemm_fp8_ws_bytes(int M, int N, int K) {
   return p.splits > 1 ? (size_t)p.splits * M * f8_ldw(N) * sizeof(float) : 0;
 }
 
-extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, const uint8_t* scale_a,
-                           int64_t ldsa, int group_a, const uint8_t* B, int64_t ldb, const uint8_t* scale_b,
-                           int64_t ldsb, int group_b, void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes) {
+namespace nl {
+namespace {
+
+// The epilogue of a product as its callers give it; none: all as below.
+struct F8Epilogue {
+  int kind = kPlain;
+  const float* bias = nullptr;
+  int act = NL_ACT_NONE;
+  const void* res = nullptr;
+  int64_t ldres = 0;
+  void* aux = nullptr;
+  int64_t ldaux = 0;
+  uint8_t* sc = nullptr;
+  int64_t ldsc = 0;
+};
+
+// A matrix over C of the epilogue's: rows that 16-byte pieces divide.
+int check_over_c(const char* name, const void* p, int64_t ld, int N) {
+  if (!p) return NL_OK;
+  if (ld < N) return nl_set_error(NL_EINVAL, std::string("gemm_fp8: rows of ") + name + " are shorter than N");
+  if (((uintptr_t)p & 15) || ld % 8)
+    return nl_set_error(NL_EALIGN, std::string("gemm_fp8: ") + name + " needs 16-byte aligned rows");
+  if (ld > kMaxLdc) return nl_set_error(NL_EUNSUPPORTED, std::string("gemm_fp8: rows of ") + name + " of 2 million elements and more");
+  return NL_OK;
+}
+
+int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, const uint8_t* scale_a, int64_t ldsa,
+             int group_a, const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b, void* C,
+             int c_dtype, int64_t ldc, const F8Epilogue& e, void* ws, size_t ws_bytes) {
   if (M < 0 || N < 0 || K < 0) return nl_set_error(NL_EINVAL, "gemm_fp8: need M, N, K >= 0");
-  if (c_dtype != NL_DTYPE_F32 && c_dtype != NL_DTYPE_BF16)
+  const bool c8 = c_dtype == NL_DTYPE_E4M3;
+  if (c_dtype != NL_DTYPE_F32 && c_dtype != NL_DTYPE_BF16 && !(c8 && e.kind != kPlain))
     return nl_set_error(NL_EINVAL, "gemm_fp8: C is fp32 or bf16");
+  if (e.act < NL_ACT_NONE || e.act > NL_ACT_SILU) return nl_set_error(NL_EINVAL, "gemm_fp8: unknown activation");
   if (int rc = check_operand("gemm_fp8 A", M, K, A, lda, scale_a, ldsa, group_a)) return rc;
   if (int rc = check_operand("gemm_fp8 B", N, K, B, ldb, scale_b, ldsb, group_b)) return rc;
   if (M == 0 || N == 0) return NL_OK;
   if (!C) return nl_set_error(NL_EINVAL, "gemm_fp8: null C");
-  if (ldc < N) return nl_set_error(NL_EINVAL, "gemm_fp8: ldc < N");
-  if (((uintptr_t)C & 15) || ldc % 8) return nl_set_error(NL_EALIGN, "gemm_fp8: C needs 16-byte aligned rows");
+  if (c8) {
+    if (e.aux) return nl_set_error(NL_EINVAL, "gemm_fp8: a result in 8 bits keeps no u");
+    if (int rc = check_operand("gemm_fp8 C", M, N, C, ldc, e.sc, e.ldsc, 1)) return rc;
+  } else {
+    if (ldc < N) return nl_set_error(NL_EINVAL, "gemm_fp8: ldc < N");
+    if (((uintptr_t)C & 15) || ldc % 8) return nl_set_error(NL_EALIGN, "gemm_fp8: C needs 16-byte aligned rows");
+  }
+  if ((uintptr_t)e.bias & 3) return nl_set_error(NL_EALIGN, "gemm_fp8: bias is not aligned");
+  if (int rc = check_over_c("the residual", e.res, e.ldres, N)) return rc;
+  if (int rc = check_over_c("aux", e.aux, e.ldaux, N)) return rc;
   const int64_t Kp = ((int64_t)K + kB - 1) / kB * kB;
   if (ldc > kMaxLdc) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of C of 2 million elements and more");
   if (lda > kMaxLd || ldb > kMaxLd || ldsa > kMaxLd || ldsb > kMaxLd)
@@ -994,7 +1449,8 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
                A, lda, scale_a, ldsa, group_a == kB ? 7 : 0,
                B, ldb, scale_b, ldsb, group_b == kB ? 7 : 0,
                dwords(scale_a, ldsa) && dwords(scale_b, ldsb) ? 1 : 0,
-               C, ldc, nullptr, f8_ldw(N), p.tiles, 0, p.kb_chunk};
+               C, ldc, nullptr, f8_ldw(N), p.tiles, 0, p.kb_chunk,
+               e.bias, e.act, e.res, e.ldres, e.aux, e.ldaux, e.sc, e.ldsc};
   if (p.splits > 1) {
     if (ws && ws_bytes >= nl_gemm_fp8_ws_bytes(M, N, K)) {
       if ((uintptr_t)ws & 15) return nl_set_error(NL_EALIGN, "gemm_fp8: workspace not 16-byte aligned");
@@ -1005,9 +1461,43 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
     }
   }
   g.items = p.tiles * p.splits;
-  if (c_dtype == NL_DTYPE_F32) launch_f8<float>((hipStream_t)stream, p, g);
-  else launch_f8<uint16_t>((hipStream_t)stream, p, g);
+  const hipStream_t st = (hipStream_t)stream;
+  if (e.kind == kPlain) {
+    if (c_dtype == NL_DTYPE_F32) launch_f8<float>(st, p, g);
+    else launch_f8<uint16_t>(st, p, g);
+  } else if (c8) {
+    launch_f8_epi<uint8_t, kEpi>(st, p, g);
+  } else if (c_dtype == NL_DTYPE_F32) {
+    if (e.aux) launch_f8_epi<float, kEpiKeep>(st, p, g);  // (in fp32 u is not rounded)
+    else launch_f8_epi<float, kEpi>(st, p, g);
+  } else {
+    if (e.kind == kEpiKeep) launch_f8_epi<uint16_t, kEpiKeep>(st, p, g);
+    else launch_f8_epi<uint16_t, kEpi>(st, p, g);
+  }
   return nl_check_launch("nl_gemm_fp8");
+}
+
+}  // namespace
+}  // namespace nl
+
+extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, const uint8_t* scale_a,
+                           int64_t ldsa, int group_a, const uint8_t* B, int64_t ldb, const uint8_t* scale_b,
+                           int64_t ldsb, int group_b, void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes) {
+  return gemm_fp8(stream, M, N, K, A, lda, scale_a, ldsa, group_a, B, ldb, scale_b, ldsb, group_b, C, c_dtype, ldc,
+                  F8Epilogue{}, ws, ws_bytes);
+}
+
+extern "C" int nl_gemm_fp8_fused(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda,
+                                 const uint8_t* scale_a, int64_t ldsa, int group_a, const uint8_t* B, int64_t ldb,
+                                 const uint8_t* scale_b, int64_t ldsb, int group_b, const float* bias, int act,
+                                 const void* residual, int64_t ldr, int round_u, void* aux, int64_t ldaux, void* C,
+                                 int c_dtype, int64_t ldc, uint8_t* scale_c, int64_t ldsc, void* ws, size_t ws_bytes) {
+  F8Epilogue e;
+  e.kind = round_u || aux ? kEpiKeep : kEpi;
+  e.bias = bias, e.act = act, e.res = residual, e.ldres = ldr, e.aux = aux, e.ldaux = ldaux, e.sc = scale_c, e.ldsc = ldsc;
+  if (c_dtype == NL_DTYPE_E4M3 && round_u) return nl_set_error(NL_EINVAL, "gemm_fp8: a result in 8 bits does not round u");
+  return gemm_fp8(stream, M, N, K, A, lda, scale_a, ldsa, group_a, B, ldb, scale_b, ldsb, group_b, C, c_dtype, ldc, e,
+                  ws, ws_bytes);
 }
 
 // ===========================================================================
@@ -1066,9 +1556,9 @@ int part_args(const void* x, int dtype, int64_t ldx, int64_t rows, int64_t cols,
 }
 
 int product(void* st, const uint8_t* abuf, const Part& a, const uint8_t* bbuf, const Part& b, void* C, int dtype,
-            int64_t ldc, void* ws, size_t wsb) {
-  return nl_gemm_fp8(st, (int)a.rows, (int)b.rows, (int)a.cols, abuf + a.at, a.ld(), abuf + a.sat, a.lds(), a.group,
-                     bbuf + b.at, b.ld(), bbuf + b.sat, b.lds(), b.group, C, dtype, ldc, wsb ? ws : nullptr, wsb);
+            int64_t ldc, void* ws, size_t wsb, const F8Epilogue& e = F8Epilogue{}) {
+  return gemm_fp8(st, (int)a.rows, (int)b.rows, (int)a.cols, abuf + a.at, a.ld(), abuf + a.sat, a.lds(), a.group,
+                  bbuf + b.at, b.ld(), bbuf + b.sat, b.lds(), b.group, C, dtype, ldc, e, wsb ? ws : nullptr, wsb);
 }
 
 int check_linear(const char* what, int M, int K, int N, const void* buf, size_t have, int64_t want, const char* name) {
@@ -1105,10 +1595,12 @@ extern "C" size_t nl_linear_fp8_ws_bytes(int M, int K, int N, int backward, int 
   return backward ? (size_t)p.bwd + std::max(p.ws_dx, p.ws_dw) : (size_t)p.fwd + p.ws_fwd;
 }
 
-extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
-                                 const void* W, int w_dtype, int64_t ldw, void* y, int y_dtype, int64_t ldy,
-                                 int need_dx, int need_dw, void* saved, size_t saved_bytes, void* ws,
-                                 size_t ws_bytes) {
+namespace nl {
+namespace {
+
+int linear_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx, const void* W, int w_dtype,
+               int64_t ldw, const F8Epilogue& e, void* y, int y_dtype, int64_t ldy, int need_dx, int need_dw,
+               void* saved, size_t saved_bytes, void* ws, size_t ws_bytes) {
   if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_fwd: need M, K, N > 0");
   if (int rc = check_gradients(M, K, N, need_dx != 0, need_dw != 0)) return rc;
   const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
@@ -1119,29 +1611,77 @@ extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* 
   if (int rc = part_args(W, w_dtype, ldw, K, N, sv, need_dx ? &p.wb : nullptr, b, &p.wf, &qw)) return rc;
   if (int rc = part_args(x, x_dtype, ldx, M, K, b, &p.x, sv, need_dw ? &p.xt : nullptr, &qx)) return rc;
   if (int rc = quantize_two((hipStream_t)stream, qx, x_dtype, qw, w_dtype)) return rc;
-  return product(stream, b, p.x, b, p.wf, y, y_dtype, ldy, b + p.fwd, p.ws_fwd);
+  return product(stream, b, p.x, b, p.wf, y, y_dtype, ldy, b + p.fwd, p.ws_fwd, e);
+}
+
+// dy * act'(u) quantised for the wanted gradients; dbias (may be null) over partial rows behind
+// what else the workspace holds.
+int linear_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy, const void* u,
+               int64_t ldu, int act, float* dbias, const void* saved, size_t saved_bytes, int need_dx, int need_dw,
+               void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws, size_t ws_bytes) {
+  if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_bwd: need M, K, N > 0");
+  if (!need_dx && !need_dw && !dbias) return NL_OK;
+  const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
+  const int64_t behind = p.bwd + (int64_t)std::max(p.ws_dx, p.ws_dw);
+  const int64_t sums = dbias ? (int64_t)nl_quantize_fp8_dact_ws_bytes(M, N) : 0;
+  if (int rc = check_linear("linear_fp8_bwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
+  if (int rc = check_linear("linear_fp8_bwd", M, K, N, ws, ws_bytes, behind + sums, "workspace")) return rc;
+  const uint8_t* sv = (const uint8_t*)saved;
+  uint8_t* b = (uint8_t*)ws;
+  QuantArgs q;
+  if (int rc = dact_args(M, N, dy, dy_dtype, lddy, u, ldu, act, need_dx ? b + p.dy.at : nullptr, p.dy.ld(),
+                         need_dx ? b + p.dy.sat : nullptr, p.dy.lds(), need_dw ? b + p.dyt.at : nullptr, p.dyt.ld(),
+                         need_dw ? b + p.dyt.sat : nullptr, p.dyt.lds(), dbias, (float*)(b + behind), &q))
+    return rc;
+  if (int rc = quantize_dact((hipStream_t)stream, q, dy_dtype, dbias)) return rc;
+  if (need_dx)
+    if (int rc = product(stream, b, p.dy, sv, p.wb, dx, dx_dtype, lddx, b + p.bwd, p.ws_dx)) return rc;
+  if (need_dw)
+    if (int rc = product(stream, sv, p.xt, b, p.dyt, dW, dw_dtype, lddw, b + p.bwd, p.ws_dw)) return rc;
+  return NL_OK;
+}
+
+}  // namespace
+}  // namespace nl
+
+extern "C" int nl_linear_fp8_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
+                                 const void* W, int w_dtype, int64_t ldw, void* y, int y_dtype, int64_t ldy,
+                                 int need_dx, int need_dw, void* saved, size_t saved_bytes, void* ws,
+                                 size_t ws_bytes) {
+  return linear_fwd(stream, M, K, N, x, x_dtype, ldx, W, w_dtype, ldw, F8Epilogue{}, y, y_dtype, ldy, need_dx, need_dw,
+                    saved, saved_bytes, ws, ws_bytes);
 }
 
 extern "C" int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
                                  const void* saved, size_t saved_bytes, int need_dx, int need_dw, void* dx,
                                  int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws,
                                  size_t ws_bytes) {
-  if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_bwd: need M, K, N > 0");
-  if (!need_dx && !need_dw) return NL_OK;
-  const LinearParts p = linear_parts(M, K, N, need_dx != 0, need_dw != 0);
-  if (int rc = check_linear("linear_fp8_bwd", M, K, N, saved, saved_bytes, p.saved, "saved buffer")) return rc;
-  if (int rc = check_linear("linear_fp8_bwd", M, K, N, ws, ws_bytes, p.bwd + (int64_t)std::max(p.ws_dx, p.ws_dw),
-                            "workspace"))
-    return rc;
-  const uint8_t* sv = (const uint8_t*)saved;
-  uint8_t* b = (uint8_t*)ws;
-  QuantArgs qdy;
-  if (int rc = part_args(dy, dy_dtype, lddy, M, N, b, need_dx ? &p.dy : nullptr, b, need_dw ? &p.dyt : nullptr, &qdy))
-    return rc;
-  if (int rc = quantize_one((hipStream_t)stream, qdy, dy_dtype)) return rc;
-  if (need_dx)
-    if (int rc = product(stream, b, p.dy, sv, p.wb, dx, dx_dtype, lddx, b + p.bwd, p.ws_dx)) return rc;
-  if (need_dw)
-    if (int rc = product(stream, sv, p.xt, b, p.dyt, dW, dw_dtype, lddw, b + p.bwd, p.ws_dw)) return rc;
-  return NL_OK;
+  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, nullptr, 0, NL_ACT_NONE, nullptr, saved, saved_bytes, need_dx,
+                    need_dw, dx, dx_dtype, lddx, dW, dw_dtype, lddw, ws, ws_bytes);
+}
+
+extern "C" size_t nl_linear_fp8_fused_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw,
+                                               int need_db) {
+  return nl_linear_fp8_ws_bytes(M, K, N, backward, need_dx, need_dw) +
+         (backward && need_db ? nl_quantize_fp8_dact_ws_bytes(M, N) : 0);
+}
+
+extern "C" int nl_linear_fp8_fused_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
+                                       const void* W, int w_dtype, int64_t ldw, const float* bias, int act,
+                                       const void* residual, int64_t ldr, void* u, int64_t ldu, void* y, int y_dtype,
+                                       int64_t ldy, int need_dx, int need_dw, void* saved, size_t saved_bytes,
+                                       void* ws, size_t ws_bytes) {
+  F8Epilogue e;
+  e.kind = act != NL_ACT_NONE ? kEpiKeep : kEpi;
+  e.bias = bias, e.act = act, e.res = residual, e.ldres = ldr, e.aux = act != NL_ACT_NONE ? u : nullptr, e.ldaux = ldu;
+  return linear_fwd(stream, M, K, N, x, x_dtype, ldx, W, w_dtype, ldw, e, y, y_dtype, ldy, need_dx, need_dw, saved,
+                    saved_bytes, ws, ws_bytes);
+}
+
+extern "C" int nl_linear_fp8_fused_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
+                                       const void* u, int64_t ldu, int act, float* dbias, const void* saved,
+                                       size_t saved_bytes, int need_dx, int need_dw, void* dx, int dx_dtype,
+                                       int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws, size_t ws_bytes) {
+  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, u, ldu, act, dbias, saved, saved_bytes, need_dx, need_dw, dx,
+                    dx_dtype, lddx, dW, dw_dtype, lddw, ws, ws_bytes);
 }

@@ -389,9 +389,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsBwdAr
   }
 }
 
-// dgamma (+)= the partial rows, in a fixed order: a workgroup takes 16 columns, thread (ph, q) the
+// out (+)= the sum of P partial rows (of dgamma, of a bias gradient), in a fixed order: a workgroup takes 16 columns, thread (ph, q) the
 // rows ph, ph + 256, ... of columns 4q .. 4q+3; then the 16 phases of a wave, then the 16 waves.
-__global__ __launch_bounds__(1024) void rms_sum_kernel(int P, int D, const float* __restrict__ part,
+__global__ __launch_bounds__(1024) void row_sums_kernel(int P, int D, const float* __restrict__ part,
                                                        float* __restrict__ out, int accumulate) {
   __shared__ float sums[16][17];
   const int q = threadIdx.x & 3, ph = threadIdx.x >> 2, c = blockIdx.x * 16 + q * 4, n = D - c;
@@ -510,6 +510,11 @@ int rms_forward(const char* what, void* stream, int dtype, bool f8, const RmsArg
 }  // namespace
 }  // namespace nl
 
+void nl::launch_partial_sums(hipStream_t st, int P, int D, const float* part, float* out, int accumulate) {
+  hipLaunchKernelGGL(row_sums_kernel, dim3((unsigned)(((int64_t)D + 15) / 16)), dim3(1024), 0, st, P, D, part, out,
+                     accumulate);
+}
+
 using namespace nl;
 
 extern "C" int nl_rms_norm_fwd(void* stream, int rows, int D, int dtype, const void* x, int64_t ldx,
@@ -563,7 +568,6 @@ extern "C" int nl_rms_norm_bwd(void* stream, int rows, int D, int dtype, const v
     });
   }
   if (dgamma && (rows > 0 || !accumulate)) 
-    hipLaunchKernelGGL(rms_sum_kernel, dim3((D + 15) / 16), dim3(1024), 0, st, blocks, D, (const float*)ws, dgamma,
-                       accumulate);
+    launch_partial_sums(st, blocks, D, (const float*)ws, dgamma, accumulate);
   return nl_check_launch(what);
 }

@@ -5,7 +5,8 @@
   (``group=1``: activations, gradients) or per 128 rows (``group=128``: weights).
 * ``rms_norm_fp8(x, gamma)`` / ``add_rms_norm_fp8(x, r, gamma)``: the norm in front of a product,
   written as such an operand.
-* ``gemm_fp8(a, b)``: a . b^T of two such operands, bf16 or fp32 out.
+* ``gemm_fp8(a, b)``: a . b^T of two such operands, bf16 or fp32 out; with bias, activation
+  and residual in its epilogue, also in 8 bits for the next product.
 * ``linear_fp8(x, W)``: ``linear(x, W)`` with all three products in 8 bits: y = x W,
   dX = dY W^T and dW = X^T dY, every operand quantised along the axis that its
   product sums over. ``fp8_weight(W)`` lays a frozen weight out once.
@@ -176,14 +177,108 @@ def gemm_fp8_ws(a: Fp8Blocks, b: Fp8Blocks) -> torch.Tensor | None:
     return torch.empty(wsb // 4, dtype=_F32, device=a.q.device) if wsb else None
 
 
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "silu": 3}  # NL_ACT_*; gelu in the tanh form of ``ffn``
+
+
+def _act_code(what: str, activation) -> int:
+    if activation not in ACTIVATIONS:
+        raise ValueError(f"{what}: activation must be one of {', '.join(map(repr, ACTIVATIONS))}, got {activation!r}")
+    return ACTIVATIONS[activation]
+
+
+def _check_bias(what: str, bias, N: int, like: torch.Tensor):
+    if bias.shape != (N,) or bias.dtype not in (_F32, _BF16) or bias.get_device() != like.get_device():
+        raise ValueError(f"{what}: bias must be float32 or bfloat16 of shape {(N,)} on {like.device}, got {bias.dtype} "
+                         f"{tuple(bias.shape)} on {bias.device}")
+
+
+def _whole_rows(rows: int, cols: int, dtype, device) -> torch.Tensor:
+    """``_result`` whose last row, too, holds ``cols`` rounded up to 8 elements."""
+    if cols % 8 == 0:
+        return _result(rows, cols, dtype, device)
+    return torch.empty((rows, padded_ld(cols)), dtype=dtype, device=device)[:, :cols]
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """t with 16-byte aligned rows that all hold their length rounded up to 8; copies only if it must."""
+    rows, cols = t.shape
+    s0, s1 = t.stride()
+    if (s1 == 1 or cols == 1) and (rows <= 1 or s0 >= cols) and t.data_ptr() % 16 == 0 and (rows <= 1 or s0 % 8 == 0):
+        need = t.storage_offset() + max(rows - 1, 0) * s0 + (cols + 7) // 8 * 8
+        if cols % 8 == 0 or need * t.element_size() <= t.untyped_storage().nbytes():
+            return t
+    out = _whole_rows(rows, cols, t.dtype, t.device)
+    out.copy_(t)
+    return out
+
+
+def _fused_product(a: Fp8Blocks, b: Fp8Blocks, out, ws, bias, act: int, residual, round_u: bool, u) -> None:
+    """nl_gemm_fp8_fused into ``out``, a tensor whose rows hold N rounded up to 8 or an Fp8Blocks."""
+    (M, K), N = a.shape, b.shape[0]
+    if ws is None:
+        ws = gemm_fp8_ws(a, b)
+    qa, lda, sa, ldsa = a._abi()
+    qb, ldb, sb, ldsb = b._abi()
+    if isinstance(out, Fp8Blocks):
+        c, ldc, sc, ldsc = out._abi()
+        code = _lib.NL_DTYPE_E4M3
+    else:
+        c, ldc, sc, ldsc = out.data_ptr(), _ld(out), None, 0
+        code = _code(out)
+    _lib.call_on(a.q, "nl_gemm_fp8_fused", M, N, K, qa, lda, sa, ldsa, a.group, qb, ldb, sb, ldsb, b.group,
+                 bias.data_ptr() if bias is not None else None, act,
+                 residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
+                 round_u, u.data_ptr() if u is not None else None, _ld(u) if u is not None else 0, c, code, ldc, sc, ldsc,
+                 ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
+
+
+def _gemm_fp8_fused(a, b, out_dtype, out, ws, bias, activation, residual):
+    (M, _), N = a.shape, b.shape[0]
+    act = _act_code("gemm_fp8", activation)
+    if out is not None:
+        out_dtype = out.dtype
+    if out_dtype not in (_F32, _BF16, _E4M3) or (out is not None and out_dtype is _E4M3):
+        raise ValueError("gemm_fp8: a result is float32, bfloat16 or (a new one) float8_e4m3fn, got "
+                         f"{out_dtype}")
+    dt = _BF16 if out_dtype is _E4M3 else out_dtype
+    if bias is not None:
+        _check_bias("gemm_fp8", bias, N, a.q)
+        bias = _param(bias)
+    if residual is not None and (residual.dtype is not dt or tuple(residual.shape) != (M, N)
+                                 or residual.get_device() != a.q.get_device()):
+        raise ValueError(f"gemm_fp8: the residual must be {dt} of shape {(M, N)} on {a.q.device}, got "
+                         f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
+    if out is not None:
+        _ld(out)  # refuses rows that overlap
+    if ws is not None and (ws.get_device() != a.q.get_device() or not ws.is_contiguous()):
+        raise ValueError(f"gemm_fp8: the workspace must be contiguous and on {a.q.device}")
+    if out_dtype is _E4M3:
+        into = Fp8Blocks.empty(M, N, 1, a.q.device)
+    elif out is not None and N % 8 == 0:
+        into = out
+    else:  # (rows of the caller's own are not written past N)
+        into = _whole_rows(M, N, out_dtype, a.q.device)
+    if M and N:
+        residual = _readable(residual.detach()) if residual is not None else None
+        _fused_product(a, b, into, ws, bias, act, residual, False, None)
+    return into if out is None else out if into is out else out.copy_(into)
+
+
 def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | None = None,
-             ws: torch.Tensor | None = None) -> torch.Tensor:
-    """a (M, K) . b (N, K)^T -> (M, N) on the current stream. An fp32 result is summed in
-    fp32 (scale bytes 3 to 246). A bf16 result is summed by the 8-bit matrix instruction,
-    which cuts 8 products at a time to 2^-13 of the largest of them: beside a bf16 rounding
-    that does not count, unless products cancel to a small part of their size.
-    out: fp32 or bf16 with 16-byte aligned rows. ws: as ``gemm_fp8_ws`` gives it
-    (allocated here if None; too small a one is not used and K is summed in one piece)."""
+             ws: torch.Tensor | None = None, bias: torch.Tensor | None = None, activation: str | None = None,
+             residual: torch.Tensor | None = None):
+    """act(a (M, K) . b (N, K)^T + bias) + residual -> (M, N) on the current stream. An fp32
+    result is summed in fp32 (scale bytes 3 to 246). A bf16 result is summed by the 8-bit matrix
+    instruction, which cuts 8 products at a time to 2^-13 of the largest of them: beside a bf16
+    rounding that does not count, unless products cancel to a small part of their size.
+
+    bias (N,) fp32 or bf16, activation "relu", "gelu" (tanh form) or "silu" and residual (M, N) in
+    the result's dtype are applied in fp32 behind the sum. ``out_dtype=torch.float8_e4m3fn`` gives
+    ``Fp8Blocks``, quantised along N, for the next product (summed as bf16 is; a bf16 residual).
+    Not differentiable (``linear_fp8`` is).
+
+    out: fp32 or bf16 with 16-byte aligned rows (it may be the residual). ws: as ``gemm_fp8_ws`` gives
+    it (allocated here if None; too small a one is not used and K is summed in one piece)."""
     (M, K), (N, Kb) = a.shape, b.shape
     if K != Kb:
         raise ValueError(f"gemm_fp8: inner dimensions differ ({K} vs {Kb})")
@@ -191,6 +286,10 @@ def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | No
     _check_device(a.q, b.q)
     if a.q.get_device() != b.q.get_device():
         raise ValueError(f"gemm_fp8: operands on {a.q.device} and {b.q.device}")
+    if bias is not None or activation is not None or residual is not None or out_dtype is _E4M3:
+        if out is not None and (tuple(out.shape) != (M, N) or out.device != a.q.device):
+            raise ValueError(f"gemm_fp8: output must be of shape {(M, N)} on {a.q.device}")
+        return _gemm_fp8_fused(a, b, out_dtype, out, ws, bias, activation, residual)
     if out is None:
         if out_dtype is not _F32 and out_dtype is not _BF16:
             raise ValueError("gemm_fp8: output must be float32 or bfloat16")
@@ -334,14 +433,136 @@ class _LinearFp8Frozen(torch.autograd.Function):
         return gemm_fp8(_quantize(dy, 1, True, False)[0], ctx.W.bwd, ctx.x_dtype), None      # dY . W^T
 
 
-def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
-    """x[..., K] @ W[K, N] -> [..., N] in x's dtype, with 8-bit products (as ``gemm_fp8``
-    sums them for that dtype; dW's go by W's, or by main_grad's).
+@functools.lru_cache(maxsize=1024)
+def _linear_fused_bytes(M: int, K: int, N: int, need_dx: bool, need_dW: bool, need_db: bool):
+    lib = _lib.load()
+    return (lib.nl_linear_fp8_saved_bytes(M, K, N, need_dx, need_dW),
+            lib.nl_linear_fp8_fused_ws_bytes(M, K, N, 0, need_dx, need_dW, need_db),
+            lib.nl_linear_fp8_fused_ws_bytes(M, K, N, 1, need_dx, need_dW, need_db))
+
+
+def _bias_grad(bias: torch.Tensor):
+    """(what dbias is written to, whether that is bias's main_grad)."""
+    mg = grad_buffer(bias)
+    if mg is None:
+        return torch.empty(bias.shape, dtype=_F32, device=bias.device), False
+    if mg.shape != bias.shape or mg.device != bias.device or mg.dtype is not _F32 or not mg.is_contiguous():
+        raise ValueError(f"linear_fp8: the bias's main_grad must be a dense float32 tensor of shape {tuple(bias.shape)} "
+                         f"on {bias.device}")
+    return mg, True
+
+
+class _LinearFp8Fused(torch.autograd.Function):
+    """act(x W + bias) + residual, W a tensor or (``frozen``) an Fp8Weight; each direction is one
+    call of the library, or for a frozen weight a quantisation and a product."""
+
+    @staticmethod
+    def forward(ctx, x2, W, bias, res2, frozen, act, need):
+        (M, K), N = x2.shape, (W if frozen is None else frozen).shape[1]
+        need_dx, need_dW, need_db, _ = need
+        ctx.sizes, ctx.need, ctx.act, ctx.frozen = (M, K, N, x2.dtype), need, act, frozen
+        # for their main_grad alone
+        ctx.W = W if need_dW and (W.is_leaf or grad_buffer(W) is not None) else None
+        ctx.w_like = None if W is None else (W.dtype, W.is_contiguous())
+        ctx.bias = bias if need_db else None
+        ctx.res_dtype = None if res2 is None else res2.dtype
+        y = _whole_rows(M, N, x2.dtype, x2.device)
+        # what act'(u) is formed from, in the dtype of y as the activation itself sees it
+        u = _whole_rows(M, N, x2.dtype, x2.device) if act and (need_dx or need_dW or need_db) else None
+        saved = None
+        if M and N:
+            b32 = _param(bias) if bias is not None else None
+            r = _readable(res2) if res2 is not None else None
+            if frozen is not None:
+                _fused_product(_quantize(x2, 1, True, False)[0], frozen.fwd, y, None, b32, act, r, bool(act), u)
+            elif K == 0:  # no product to quantise for
+                none = Fp8Blocks.empty
+                _fused_product(none(M, 0, 1, x2.device), none(N, 0, BLOCK, x2.device), y, None, b32, act, r, bool(act), u)
+            else:
+                saved_bytes, wsb, _ = _linear_fused_bytes(M, K, N, need_dx, need_dW, need_db)
+                saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x2.device)
+                ws = torch.empty(wsb, dtype=torch.uint8, device=x2.device)
+                (x2, ldx), (Wr, ldw) = _rows(x2), _rows(W)
+                _lib.call_on(x2, "nl_linear_fp8_fused_fwd", M, K, N, x2.data_ptr(), _code(x2), ldx, Wr.data_ptr(),
+                             _code(Wr), ldw, b32.data_ptr() if b32 is not None else None, act,
+                             r.data_ptr() if r is not None else None, _ld(r) if r is not None else 0,
+                             u.data_ptr() if u is not None else None, _ld(u) if u is not None else 0,
+                             y.data_ptr(), _code(y), _ld(y), need_dx, need_dW, saved.data_ptr(), saved_bytes,
+                             ws.data_ptr(), wsb)
+        ctx.save_for_backward(saved, u)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        saved, u = ctx.saved_tensors
+        M, K, N, x_dtype = ctx.sizes
+        need_dx, need_dW, need_db, need_dr = ctx.need
+        act, frozen = ctx.act, ctx.frozen
+        dr = dy.to(ctx.res_dtype) if need_dr else None
+        if not (need_dx or need_dW or need_db):
+            return None, None, None, dr, None, None, None
+        dev = dy.device
+        mg = _main_grad(ctx.W) if ctx.W is not None else None
+        db, db_taken = _bias_grad(ctx.bias) if need_db else (None, False)
+        dx = _result(M, K, x_dtype, dev) if need_dx else None
+        direct = mg is not None and mg.dtype in (_BF16, _F32) and _aligned(mg)
+        dW = None
+        if need_dW:
+            w_dtype, w_dense = ctx.w_like
+            if direct:
+                dW = mg
+            elif mg is None and w_dense and N % 8 == 0:
+                dW = torch.empty((K, N), dtype=w_dtype, device=dev)  # laid out like W: kept as W.grad without a copy
+            else:
+                dW = _result(K, N, w_dtype if mg is None else _F32, dev)
+        if M == 0 or N == 0:
+            for t in (dx, dW, db):
+                if t is not None:
+                    t.zero_()
+        else:
+            dy2, lddy = _rows(dy if dy.dtype is x_dtype else dy.to(x_dtype))
+            up, ldu = (u.data_ptr(), _ld(u)) if u is not None else (None, 0)
+            dbp = db.data_ptr() if need_db else None
+            if frozen is not None or K == 0:
+                want_dx = need_dx and K > 0
+                q = Fp8Blocks.empty(M, N, 1, dev) if want_dx else None
+                wsb = _lib.load().nl_quantize_fp8_dact_ws_bytes(M, N) if need_db else 0
+                ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+                if want_dx or need_db:
+                    _lib.call_on(dy2, "nl_quantize_fp8_dact", M, N, dy2.data_ptr(), _code(dy2), lddy, up, ldu, act,
+                                 *(q._abi() if want_dx else _NONE), *_NONE, dbp, ws.data_ptr() if wsb else None, wsb)
+                if want_dx:
+                    dx = gemm_fp8(q, frozen.bwd, x_dtype, out=dx)                           # dU . W^T
+            else:
+                saved_bytes, _, wsb = _linear_fused_bytes(M, K, N, need_dx, need_dW, need_db)
+                ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+                _lib.call_on(dy2, "nl_linear_fp8_fused_bwd", M, K, N, dy2.data_ptr(), _code(dy2), lddy, up, ldu, act, dbp,
+                             saved.data_ptr(), saved_bytes, need_dx, need_dW,
+                             *((dx.data_ptr(), _code(dx), _ld(dx)) if need_dx else (None, 0, 0)),
+                             *((dW.data_ptr(), _code(dW), _ld(dW)) if need_dW else (None, 0, 0)), ws.data_ptr(), wsb)
+        if mg is not None:
+            if not direct:
+                mg.copy_(dW)
+            dW = None
+        if need_db:
+            db = None if db_taken else db.to(ctx.bias.dtype)
+        return dx, dW, db, dr, None, None, None
+
+
+def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation: str | None = None,
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(x[..., K] @ W[K, N] + bias) + residual -> [..., N] in x's dtype, with 8-bit products (as
+    ``gemm_fp8`` sums them for that dtype; dW's go by W's, or by main_grad's).
 
     W: an fp32 or bf16 weight, quantised here, or an ``Fp8Weight`` (frozen: it gets
     no gradient). The gradients are those of the product of the quantised
-    operands, with dY quantised too and the rounding taken as the identity. Both run
-    on the current stream: dW is not forked within ``overlap_weight_grads()``."""
+    operands, with the output's gradient quantised too and the rounding taken as the identity. Both run
+    on the current stream: dW is not forked within ``overlap_weight_grads()``.
+
+    bias (N,) fp32 or bf16, activation "relu", "gelu" (tanh form) or "silu", residual [..., N] in x's
+    dtype: in the product's epilogue. With an activation u = x W + bias is rounded to x's dtype before
+    it, as ``ffn`` does it: that u is kept for the backward, which quantises dY act'(u)."""
     if x.dim() < 2:
         raise ValueError("linear_fp8: x needs >= 2 dims")
     frozen = W if isinstance(W, Fp8Weight) else None
@@ -351,21 +572,40 @@ def linear_fp8(x: torch.Tensor, W) -> torch.Tensor:
         raise ValueError(f"linear_fp8: x has {x.shape[-1]} features, W has {W.shape[0]} rows")
     if x.dtype not in (_BF16, _F32):
         raise ValueError(f"linear_fp8: x must be bfloat16 or float32, got {x.dtype}")
+    N = W.shape[1]
+    act = _act_code("linear_fp8", activation)
+    if bias is not None:
+        _check_bias("linear_fp8", bias, N, x)
+    if residual is not None and (residual.dtype is not x.dtype or residual.shape != (*x.shape[:-1], N)
+                                 or residual.get_device() != x.get_device()):
+        raise ValueError(f"linear_fp8: the residual must be {x.dtype} of shape {(*x.shape[:-1], N)} on {x.device}, got "
+                         f"{residual.dtype} {tuple(residual.shape)} on {residual.device}")
+    fused = bias is not None or act or residual is not None
     lead = x.shape[:-1]
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-    _check_sizes("linear_fp8", *x2.shape, W.shape[1])
+    _check_sizes("linear_fp8", *x2.shape, N)
+    grads = torch.is_grad_enabled()
     if frozen is not None:
-        if x2.requires_grad and torch.is_grad_enabled():  # what the product of dY would refuse
+        if x2.requires_grad and grads:  # what the product of dY would refuse
             M, (K, N) = x2.shape[0], W.shape
             if K > MAX_COLUMNS - BLOCK or M * ((N + BLOCK - 1) // BLOCK) > MAX_BLOCKS:
                 raise ValueError(f"linear_fp8: no input gradient of ({M}, {K}) from an output gradient of ({M}, {N})")
-        y = _LinearFp8Frozen.apply(x2, frozen)
+        if not fused:
+            y = _LinearFp8Frozen.apply(x2, frozen)
+        else:
+            _check_device(x2, frozen.fwd.q)
+            if x2.get_device() != frozen.fwd.q.get_device():
+                raise ValueError(f"linear_fp8: x on {x.device}, W on {frozen.fwd.q.device}")
     else:
         if W.dtype not in (_BF16, _F32):
             raise ValueError(f"linear_fp8: W must be bfloat16 or float32, got {W.dtype}")
         _check_device(x2, W)
         if x2.get_device() != W.get_device():
             raise ValueError(f"linear_fp8: x on {x.device}, W on {W.device}")
-        grads = torch.is_grad_enabled()
-        y = _LinearFp8.apply(x2, W, grads and x2.requires_grad, grads and W.requires_grad)
-    return y if x.dim() == 2 else y.reshape(*lead, W.shape[1])
+        if not fused:
+            y = _LinearFp8.apply(x2, W, grads and x2.requires_grad, grads and W.requires_grad)
+    if fused:
+        res2 = None if residual is None else residual if x.dim() == 2 else residual.reshape(-1, N)
+        need = tuple(grads and t is not None and t.requires_grad for t in (x2, None if frozen else W, bias, res2))
+        y = _LinearFp8Fused.apply(x2, None if frozen else W, bias, res2, frozen, act, need)
+    return y if x.dim() == 2 else y.reshape(*lead, N)
