@@ -355,9 +355,10 @@ struct GemmF8Args {
   int64_t ldsc;
 };
 
-// Epilogues of a product: none; u = acc + bias, C = act(u) + res; and that with u rounded to
-// the type of C before, and kept where it is asked for (what a backward pass reads).
-enum { kPlain = 0, kEpi = 1, kEpiKeep = 2 };
+// Epilogues of a product: none; u = acc + bias, C = act(u); that with u rounded to the type of C
+// before, and kept where it is asked for (what a backward pass reads); each with a residual.
+enum { kPlain = 0, kEpi = 1, kEpiKeep = 2, kEpiRes = 3, kEpiResKeep = 4 };
+constexpr bool keeps(int epi) { return epi == kEpiKeep || epi == kEpiResKeep; }
 
 // Four scale bytes of one row from byte `off` (n of them there): one dword where
 // rows are whole, aligned dwords, else byte by byte.
@@ -483,17 +484,18 @@ __device__ __forceinline__ F8Item f8_item(const GemmF8Args& g, int item) {
   return t;
 }
 
-// act(u) of 8 values; NaN stays NaN
-__device__ __forceinline__ void activate(float (&v)[8], int act) {
+// act(u) of some values; NaN stays NaN
+template <int N>
+__device__ __forceinline__ void activate(float (&v)[N], int act) {
   if (act == NL_ACT_GELU) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = gelu_tanh(v[k]);
+    for (int k = 0; k < N; ++k) v[k] = gelu_tanh(v[k]);
   } else if (act == NL_ACT_SILU) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = silu(v[k]);
+    for (int k = 0; k < N; ++k) v[k] = silu(v[k]);
   } else if (act == NL_ACT_RELU) {
 #pragma unroll
-    for (int k = 0; k < 8; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
+    for (int k = 0; k < N; ++k) v[k] = v[k] < 0.f ? 0.f : v[k];
   }
 }
 
@@ -757,168 +759,280 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
     int ln = lane;
     asm volatile("" : "+v"(ln));
     const int fr = ln & 31, g4 = (ln >> 5) * 4;
-    if constexpr (EPI != kPlain) {
-      // The slab holds fp32 here, SC columns at a time, and a lane takes 8 columns of a row (the same
-      // ones in every row: its bias stays in registers), so that residual and result are whole 16-byte
-      // pieces. Every store is made, with an offset out of range where the matrix ends.
+    // 32 rows of 64 bf16 columns of a matrix over C, at `row` and `col` of the tile, as whole 16-byte
+    // pieces: 8 lanes a row. Rows and columns that are not there are out of every range (a piece that
+    // N cuts is whole: rows hold N rounded up to 8).
+    const int rr = ln / 8, gg = ln % 8;
+    auto piece_off = [&](uint32_t ld, int rows, int cols, int row, int col) __attribute__((always_inline)) {
+      return rr < rows - row && gg * 8 < cols - col ? (((uint32_t)rr + row) * ld + gg * 8 + col) * 2 : kNowhere;
+    };
+    auto load_rows = [&](__amdgpu_buffer_rsrc_t rs, uint32_t ld, int rows, int cols, int row, int col, u32x4 (&r)[4])
+        __attribute__((always_inline)) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        r[it] = __builtin_amdgcn_raw_buffer_load_b128(rs, piece_off(ld, rows, cols, row + it * 8, col), 0, 0);
+    };
+    // ... added to the lanes' own values of them, through the slab
+    auto add_rows = [&](const u32x4 (&r)[4], float (&v0)[16], float (&v1)[16]) __attribute__((always_inline)) {
+#pragma unroll
+      for (int it = 0; it < 4; ++it)
+        *reinterpret_cast<u32x4*>(wl + (it * 8 + rr) * 128 + ((gg ^ rr) << 4)) = r[it];
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const u32x2 w = *reinterpret_cast<const u32x2*>(wl + fr * 128 + (((j * 4 + q) ^ (fr & 7)) << 4) + g4 * 2);
+          float* v = (j ? v1 : v0) + 4 * q;
+          v[0] += bf16_lo(w[0]), v[1] += bf16_hi(w[0]), v[2] += bf16_lo(w[1]), v[3] += bf16_hi(w[1]);
+        }
+    };
+    if constexpr (sizeof(OutT) == 1) {
+      // C in 8 bits. A wave's columns are one block of 128, and a lane pair (l, l + 32) has a whole row
+      // of it: bias, activation, residual and the row's largest value in the lanes as they are, and
+      // the bytes through the slab into whole rows.
+      static_assert(WTN == kB && (PITCH == 256 || FM == 1), "a wave holds whole blocks of C");
+      uint8_t* wb = wl + (PITCH == 256 ? 4096 : 0);  // the bias, behind the bytes or (one group of rows) before them
+#pragma unroll
+      for (int k = 0; k < kBias; ++k) reinterpret_cast<float*>(wb)[k * 64 + ln] = bias1[k];
+      const int n = cur.n0 + wn * WTN, cols = g.N - n, rows = g.M - cur.m0;
+      const bool there = cols > 0;
+      const __amdgpu_buffer_rsrc_t rc = make_rsrc(
+          uniform(reinterpret_cast<const uint8_t*>(g.C) + (there ? (int64_t)cur.m0 * g.ldc + n : 0)), kNowhere);
+      const __amdgpu_buffer_rsrc_t rres = make_rsrc(
+          uniform(reinterpret_cast<const uint8_t*>(g.res ? g.res : g.C) +
+                  (g.res && there ? ((int64_t)cur.m0 * g.ldres + n) * 2 : 0)), kNowhere);
+      constexpr bool kHasRes = EPI == kEpiRes;
+      u32x4 res[4];
+      auto load_res = [&](int i, int h) __attribute__((always_inline)) {
+        load_rows(rres, (uint32_t)g.ldres, there ? rows : 0, cols, wm * WTM + i * 32, h * 64, res);
+      };
+      if constexpr (kHasRes) load_res(0, 0);
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int row = wm * WTM + i * 32 + fr;
+        float v[FN][16];
+#pragma unroll
+        for (int j = 0; j < FN; ++j) {
+          asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            const f32x4 b = *reinterpret_cast<const f32x4*>(wb + (j * 32 + q * 8 + g4) * 4);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[j][4 * q + k] = acc[i][j][4 * q + k] + b[k];
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < FN; ++j) activate(v[j], g.act);
+        if constexpr (kHasRes) {
+          add_rows(res, v[0], v[1]);
+          load_res(i, 1);
+          add_rows(res, v[2], v[3]);
+          if (i + 1 < FM) load_res(i + 1, 0);
+        }
+        if (cols < kB) {  // nothing past N has a part in the scale, and its bytes are zero
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k)
+              if (j * 32 + k / 4 * 8 + g4 + k % 4 >= cols) v[j][k] = 0.f;
+        }
+        // (the hardware's maximum passes a NaN over)
+        float top = 0.f;
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int k = 0; k < 16; ++k) top = fmaxf(top, fabsf(v[j][k]));
+        uint32_t m = __float_as_uint(top);
+        if (__builtin_expect(__any(m >= kInfBits), 0)) {  // look again for what is finite
+          m = 0;
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int k = 0; k < 16; ++k) m = max(m, finite_abs_bits(v[j][k]));
+        }
+        const auto r32 = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        m = max((uint32_t)r32[0], (uint32_t)r32[1]);
+        const int byte = scale_byte(m);
+        const float inv = inv_scale(byte);
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<uint32_t*>(wl + fr * 128 + (((2 * j + (q >> 1)) ^ (fr & 7)) << 4) + (q & 1) * 8 + g4) =
+                pack_e4m3x4(v[j][4 * q] * inv, v[j][4 * q + 1] * inv, v[j][4 * q + 2] * inv, v[j][4 * q + 3] * inv);
+        if (ln < 32 && row < rows && there) g.sc[(int64_t)(cur.m0 + row) * g.ldsc + n / kB] = (uint8_t)byte;
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int r = it * 8 + ln / 8, at = wm * WTM + i * 32 + r;
+          const u32x4 w = *reinterpret_cast<const u32x4*>(wl + r * 128 + (((ln % 8) ^ (r & 7)) << 4));
+          __builtin_amdgcn_raw_buffer_store_b128(
+              w, rc, at < rows && there ? (uint32_t)at * (uint32_t)g.ldc + (uint32_t)(ln % 8 * 16) : kNowhere, 0, 0);
+        }
+      }
+    } else if constexpr (sizeof(OutT) == 2 && EPI != kPlain) {
+      // bf16: bias, activation and residual in the lanes as they are, and rows of 64 columns through
+      // the slab, u before C. The residual's rows are loaded kDepth slabs ahead.
+      constexpr bool kRoom = PITCH == 256;  // the bias has a place behind the slab's rows; else in registers
+      constexpr int NH = WTN / 64;
+      float* wb = reinterpret_cast<float*>(wl + (kRoom ? 4096 : 0));
+#pragma unroll
+      for (int k = 0; k < kBias; ++k) wb[k * 64 + ln] = bias1[k];
+      f32x4 bias[kRoom ? 1 : FN][4];
+      if constexpr (!kRoom) {
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q) bias[j][q] = *reinterpret_cast<const f32x4*>(wb + j * 32 + q * 8 + g4);
+      }
+      constexpr bool kHasRes = EPI == kEpiRes || EPI == kEpiResKeep;
+      constexpr int kSlabs = FM * NH, kDepth = kSlabs < 3 ? kSlabs : 3;
+      const int cols = g.N - cur.n0, rows = g.M - cur.m0;
+      const void* aux = keeps(EPI) ? g.aux : nullptr;
+      const __amdgpu_buffer_rsrc_t rc =
+          make_rsrc(uniform(reinterpret_cast<const uint8_t*>(g.C) + ((int64_t)cur.m0 * g.ldc + cur.n0) * 2), kNowhere);
+      const __amdgpu_buffer_rsrc_t raux =
+          make_rsrc(uniform(reinterpret_cast<const uint8_t*>(aux ? aux : g.C) +
+                            (aux ? ((int64_t)cur.m0 * g.ldaux + cur.n0) * 2 : 0)), kNowhere);
+      // 32 rows of 64 columns: packed, and out (a piece that N cuts whole: rows hold N rounded up to 8)
+      auto put = [&](const uint32_t (&w)[2][8], __amdgpu_buffer_rsrc_t rs, uint32_t ld, int there, int i, int h)
+          __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int q = 0; q < 4; ++q)
+            *reinterpret_cast<u32x2*>(wl + fr * 128 + (((j * 4 + q) ^ (fr & 7)) << 4) + g4 * 2) =
+                u32x2{w[j][2 * q], w[j][2 * q + 1]};
+        u32x4 val[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          val[it] = *reinterpret_cast<const u32x4*>(wl + (it * 8 + rr) * 128 + ((gg ^ rr) << 4));
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          __builtin_amdgcn_raw_buffer_store_b128(
+              val[it], rs, piece_off(ld, there, cols, wm * WTM + i * 32 + it * 8, wn * WTN + h * 64), 0, 2 /* nt */);
+      };
+      const __amdgpu_buffer_rsrc_t rres =
+          make_rsrc(uniform(reinterpret_cast<const uint8_t*>(kHasRes ? g.res : g.C) +
+                            (kHasRes ? ((int64_t)cur.m0 * g.ldres + cur.n0) * 2 : 0)), kNowhere);
+      u32x4 res[kHasRes ? kDepth : 1][4];
+      auto load_res = [&](int s) __attribute__((always_inline)) {
+        load_rows(rres, (uint32_t)g.ldres, rows, cols, wm * WTM + s / NH * 32, wn * WTN + s % NH * 64, res[s % kDepth]);
+      };
+      if constexpr (kHasRes) {
+#pragma unroll
+        for (int s = 0; s < kDepth; ++s) load_res(s);
+      }
+#pragma unroll
+      for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int h = 0; h < NH; ++h) {
+          float v[2][16];
+          uint32_t w[2][8];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            asm volatile("" : "+v"(acc[i][h * 2 + j]));  // out of the accumulators here and not before
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              f32x4 b;
+              if constexpr (kRoom) b = *reinterpret_cast<const f32x4*>(wb + h * 64 + j * 32 + q * 8 + g4);
+              else b = bias[h * 2 + j][q];
+#pragma unroll
+              for (int k = 0; k < 4; ++k) v[j][4 * q + k] = acc[i][h * 2 + j][4 * q + k] + b[k];
+            }
+          }
+          auto packed = [&]() __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) w[j][k] = pack_bf16x2(v[j][2 * k], v[j][2 * k + 1]);
+          };
+          if constexpr (keeps(EPI)) {
+            packed();
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int k = 0; k < 8; ++k) v[j][2 * k] = bf16_lo(w[j][k]), v[j][2 * k + 1] = bf16_hi(w[j][k]);
+            put(w, raux, (uint32_t)g.ldaux, aux ? rows : 0, i, h);
+          }
+#pragma unroll
+          for (int j = 0; j < 2; ++j) activate(v[j], g.act);
+          if constexpr (kHasRes) {
+            const int s = i * NH + h;
+            add_rows(res[s % kDepth], v[0], v[1]);
+            if (s + kDepth < kSlabs) load_res(s + kDepth);
+          }
+          packed();
+          put(w, rc, (uint32_t)g.ldc, rows, i, h);
+        }
+    } else if constexpr (EPI != kPlain) {
+      // fp32: a lane takes 4 columns of a row (the same ones in every row: its bias stays in registers)
+      // from the slab, SC columns at a time, so that residual, u and result are whole rows of pieces.
+      constexpr bool kHasRes = EPI == kEpiRes || EPI == kEpiResKeep;
       constexpr int SC = PITCH / 4, NH = WTN / SC;            // NH slabs side by side
-      constexpr int LPR = SC / 8, RPI = 64 / LPR;             // lanes of a row, rows at a time
-      constexpr int kReads = 32 / RPI, kPieces = SC / 8, CPR = PITCH / 16;
-      constexpr int kRes = sizeof(OutT) == 4 ? 2 : 1;         // 16-byte pieces of 8 residuals
-      constexpr int RE = sizeof(OutT) == 4 ? 4 : 2;           // bytes of one
-      constexpr bool k8 = sizeof(OutT) == 1;
-      const int rr = ln / LPR, gg = ln % LPR;
-      float bias[NH][8];
+      constexpr int LPR = SC / 4, RPI = 64 / LPR, kReads = 32 / RPI, kPieces = SC / 8;
+      const int r4 = ln / LPR, c4 = ln % LPR;
+      const int cols = g.N - cur.n0, rows = g.M - cur.m0;
+      float bias[NH][4];
 #pragma unroll
       for (int h = 0; h < NH; ++h)
 #pragma unroll
-        for (int k = 0; k < 8; ++k) bias[h][k] = __shfl(bias1[h * SC / 64], h * SC % 64 + gg * 8 + k, 64);
-      // One of the matrices that C's tile lies over: a descriptor from the tile's first element, this
-      // lane's offset from there, the rows there are (none of a matrix that is not given).
-      struct Mat {
-        __amdgpu_buffer_rsrc_t rs;
-        uint32_t lane, ld;
-        int rows;
+        for (int k = 0; k < 4; ++k) bias[h][k] = __shfl(bias1[h * SC / 64], h * SC % 64 + c4 * 4 + k, 64);
+      auto over_c = [&](const void* p, int64_t ld) __attribute__((always_inline)) {
+        return make_rsrc(uniform(reinterpret_cast<const uint8_t*>(p ? p : g.C) + (p ? ((int64_t)cur.m0 * ld + cur.n0) * 4 : 0)),
+                         kNowhere);
       };
-      const int cols = g.N - cur.n0;  // of the tile that are there (or more)
-      auto mat = [&](const void* p, int64_t ld) __attribute__((always_inline)) {
-        const uint8_t* base = reinterpret_cast<const uint8_t*>(p ? p : g.C);
-        return Mat{make_rsrc(uniform(base + (p ? ((int64_t)cur.m0 * ld + cur.n0) * RE : 0)), kNowhere),
-                   (uint32_t)(rr * (int)ld + gg * 8) * RE, (uint32_t)ld, p ? g.M - cur.m0 : 0};
-      };
-      // element `add` of the lane's 8 in rows `it` of slab (i, h): its offset; where `there` is false
-      // one out of every range
-      auto off = [&](const Mat& m, int i, int h, int it, int add, bool there) __attribute__((always_inline)) {
+      const void* aux = keeps(EPI) ? g.aux : nullptr;
+      const __amdgpu_buffer_rsrc_t rres = over_c(kHasRes ? g.res : nullptr, g.ldres), raux = over_c(aux, g.ldaux),
+                                   rc = over_c(g.C, g.ldc);
+      auto at = [&](int64_t ld, int there, int i, int h, int it) __attribute__((always_inline)) {
         const int row = wm * WTM + i * 32 + it * RPI, col = wn * WTN + h * SC;
-        return there && rr < m.rows - row ? m.lane + ((uint32_t)row * m.ld + col + add) * RE : kNowhere;
+        return r4 < there - row && c4 * 4 < cols - col ? (((uint32_t)r4 + row) * (uint32_t)ld + c4 * 4 + col) * 4 : kNowhere;
       };
-      // whether these 8 columns are there: a piece that N cuts is read and written whole, its matrices'
-      // rows hold N rounded up to 8
-      auto in8 = [&](int h) __attribute__((always_inline)) { return wn * WTN + h * SC + gg * 8 < cols; };
-      const Mat mres = mat(g.res, g.ldres), maux = mat(EPI == kEpiKeep ? g.aux : nullptr, g.ldaux),
-                mc = mat(k8 ? nullptr : g.C, g.ldc);
-      auto load_res = [&](int i, int h, u32x4 (&r)[kReads][kRes]) __attribute__((always_inline)) {
+      auto load_res = [&](int s, f32x4 (&r)[kReads]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int it = 0; it < kReads; ++it) {
-#pragma unroll
-          for (int k = 0; k < kRes; ++k)
-            r[it][k] = __builtin_amdgcn_raw_buffer_load_b128(mres.rs, off(mres, i, h, it, 4 * k, in8(h)), 0, 0);
-        }
-      };
-      auto put8 = [&](const Mat& m, int i, int h, int it, const float (&v)[8]) __attribute__((always_inline)) {
-        u32x4 w[kRes];
-        if constexpr (RE == 2) {
-          w[0] = u32x4{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7])};
-        } else {
-          w[0] = __builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]});
-          w[kRes - 1] = __builtin_bit_cast(u32x4, f32x4{v[4], v[5], v[6], v[7]});
-        }
-#pragma unroll
-        for (int k = 0; k < kRes; ++k)
-          __builtin_amdgcn_raw_buffer_store_b128(w[k], m.rs, off(m, i, h, it, 4 * k, in8(h)), 0, 2 /* nt */);
+        for (int it = 0; it < kReads; ++it)
+          r[it] = __builtin_bit_cast(
+              f32x4, __builtin_amdgcn_raw_buffer_load_b128(rres, at(g.ldres, rows, s / NH, s % NH, it), 0, 0));
       };
       auto put_slab = [&](int i, int h) __attribute__((always_inline)) {
 #pragma unroll
         for (int p = 0; p < kPieces; ++p) {
           const int j = h * (SC / 32) + p / 4, q = p % 4;
           if (q == 0) asm volatile("" : "+v"(acc[i][j]));  // out of the accumulators here and not before
-          *reinterpret_cast<f32x4*>(wl + fr * PITCH + (((p * 2 + (ln >> 5)) ^ (fr & (CPR - 1))) << 4)) =
+          *reinterpret_cast<f32x4*>(wl + fr * PITCH + (((p * 2 + (ln >> 5)) ^ (fr & (LPR - 1))) << 4)) =
               f32x4{acc[i][j][4 * q], acc[i][j][4 * q + 1], acc[i][j][4 * q + 2], acc[i][j][4 * q + 3]};
         }
       };
-      auto get8 = [&](int it, float (&v)[8]) __attribute__((always_inline)) {
-        const int r = it * RPI + rr;
-        const f32x4 a = *reinterpret_cast<const f32x4*>(wl + r * PITCH + (((2 * gg) ^ (r & (CPR - 1))) << 4));
-        const f32x4 b = *reinterpret_cast<const f32x4*>(wl + r * PITCH + (((2 * gg + 1) ^ (r & (CPR - 1))) << 4));
-#pragma unroll
-        for (int k = 0; k < 4; ++k) v[k] = a[k], v[4 + k] = b[k];
-      };
-      // u, act(u) and the residual of 8 columns
-      auto finish = [&](int i, int h, int it, float (&v)[8], const u32x4 (&r)[kRes]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int k = 0; k < 8; ++k) v[k] += bias[h][k];
-        if constexpr (EPI == kEpiKeep) {
-          put8(maux, i, h, it, v);
-          if constexpr (RE == 2) {
-#pragma unroll
-            for (int k = 0; k < 8; k += 2) {
-              const uint32_t w = pack_bf16x2(v[k], v[k + 1]);
-              v[k] = bf16_lo(w);
-              v[k + 1] = bf16_hi(w);
-            }
-          }
-        }
-        activate(v, g.act);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          if constexpr (RE == 2) v[k] += k & 1 ? bf16_hi(r[0][k >> 1]) : bf16_lo(r[0][k >> 1]);
-          else v[k] += __uint_as_float(r[k >> 2][k & 3]);
-        }
-      };
-      u32x4 res[2][kReads][kRes];
-      float v[k8 ? NH : 1][kReads][8];
-      load_res(0, 0, res[0]);
+      f32x4 res[kHasRes ? 2 : 1][kReads];
+      if constexpr (kHasRes) load_res(0, res[0]);
       put_slab(0, 0);
 #pragma unroll
       for (int s = 0; s < FM * NH; ++s) {
-        const int i = s / NH, h = s % NH, hv = k8 ? h : 0;
-        if (s + 1 < FM * NH) load_res((s + 1) / NH, (s + 1) % NH, res[(s + 1) & 1]);
-#pragma unroll
-        for (int it = 0; it < kReads; ++it) get8(it, v[hv][it]);
-        if (s + 1 < FM * NH && !(k8 && h == NH - 1)) put_slab((s + 1) / NH, (s + 1) % NH);
+        const int i = s / NH, h = s % NH;
+        if constexpr (kHasRes)
+          if (s + 1 < FM * NH) load_res(s + 1, res[(s + 1) & 1]);
+        f32x4 x[kReads];
 #pragma unroll
         for (int it = 0; it < kReads; ++it) {
-          finish(i, h, it, v[hv][it], res[s & 1][it]);
-          if constexpr (!k8) put8(mc, i, h, it, v[0][it]);
+          const int r = it * RPI + r4;
+          x[it] = *reinterpret_cast<const f32x4*>(wl + r * PITCH + ((c4 ^ (r & (LPR - 1))) << 4));
         }
-        if constexpr (k8) {
-          if (h < NH - 1) continue;
-          // a wave's columns are one block of 128: its largest value over the lanes of a row, then the
-          // bytes through the slab into whole rows
-          static_assert(WTN == kB, "a wave holds whole blocks of C");
-          const int n = cur.n0 + wn * WTN;
-          const bool there = n < g.N;
-          const __amdgpu_buffer_rsrc_t rc8 = make_rsrc(
-              uniform(reinterpret_cast<const uint8_t*>(g.C) + (there ? (int64_t)cur.m0 * g.ldc + n : 0)), kNowhere);
-          if (cols < BN) {  // nothing past N has a part in the scale, and its bytes are zero
+        if (s + 1 < FM * NH) put_slab((s + 1) / NH, (s + 1) % NH);
 #pragma unroll
-            for (int it = 0; it < kReads; ++it)
+        for (int it = 0; it < kReads; ++it) {
+          float v[4];
 #pragma unroll
-              for (int x = 0; x < NH; ++x)
+          for (int k = 0; k < 4; ++k) v[k] = x[it][k] + bias[h][k];
+          if constexpr (keeps(EPI))
+            __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}), raux,
+                                                   at(g.ldaux, aux ? rows : 0, i, h, it), 0, 2 /* nt */);
+          activate(v, g.act);
+          if constexpr (kHasRes) {
 #pragma unroll
-                for (int k = 0; k < 8; ++k)
-                  if (wn * WTN + x * SC + gg * 8 + k >= cols) v[x][it][k] = 0.f;
+            for (int k = 0; k < 4; ++k) v[k] += res[s & 1][it][k];
           }
-#pragma unroll
-          for (int it = 0; it < kReads; ++it) {
-            uint32_t m = 0;
-#pragma unroll
-            for (int x = 0; x < NH; ++x)
-#pragma unroll
-              for (int k = 0; k < 8; ++k) m = max(m, finite_abs_bits(v[x][it][k]));
-            m = max(m, dpp_u<0xB1>(m));
-            m = max(m, dpp_u<0x4E>(m));
-            if constexpr (LPR == 8) m = max(m, dpp_u<0x141>(m));
-            const int byte = scale_byte(m), r = it * RPI + rr;
-            const float inv = inv_scale(byte);
-#pragma unroll
-            for (int x = 0; x < NH; ++x) {
-              const float(&w)[8] = v[x][it];
-              *reinterpret_cast<u32x2*>(wl + r * 128 + ((((x * SC + gg * 8) >> 4) ^ (r & 7)) << 4) + (gg & 1) * 8) =
-                  u32x2{pack_e4m3x4(w[0] * inv, w[1] * inv, w[2] * inv, w[3] * inv),
-                        pack_e4m3x4(w[4] * inv, w[5] * inv, w[6] * inv, w[7] * inv)};
-            }
-            const int row = wm * WTM + i * 32 + r;
-            if (gg == 0 && row < g.M - cur.m0 && there) g.sc[(int64_t)(cur.m0 + row) * g.ldsc + n / kB] = (uint8_t)byte;
-          }
-#pragma unroll
-          for (int it = 0; it < 4; ++it) {
-            const int r = it * 8 + ln / 8, row = wm * WTM + i * 32 + r;
-            const u32x4 w = *reinterpret_cast<const u32x4*>(wl + r * 128 + (((ln % 8) ^ (r & 7)) << 4));
-            __builtin_amdgcn_raw_buffer_store_b128(
-                w, rc8, row < g.M - cur.m0 && there ? (uint32_t)row * (uint32_t)g.ldc + (uint32_t)(ln % 8 * 16) : kNowhere, 0, 0);
-          }
-          if (s + 1 < FM * NH) put_slab((s + 1) / NH, 0);
+          __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, f32x4{v[0], v[1], v[2], v[3]}), rc,
+                                                 at(g.ldc, rows, i, h, it), 0, 2 /* nt */);
         }
       }
     } else {
@@ -1110,7 +1224,7 @@ __global__ __launch_bounds__(256) void f8_reduce_epi_kernel(GemmF8Args g, int sp
     float u[8], o[4];
 #pragma unroll
     for (int k = 0; k < 8; ++k) u[k] = k < 4 && n + k < g.N ? s[k & 3] + bias[k & 3] : 0.f;
-    if constexpr (EPI == kEpiKeep) {
+    if constexpr (keeps(EPI)) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         if constexpr (sizeof(RT) == 2) u[k] = bf16_to_f32(f32_to_bf16(u[k]));
@@ -1203,7 +1317,7 @@ void launch_f8_epi(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
     // partials as the same result without an epilogue has them
     using PT = typename std::conditional<sizeof(OutT) == 4, float, uint16_t>::type;
     launch_tiles<128, 128, 64, 64, PT, kPlain>(st, g);
-    hipLaunchKernelGGL((f8_reduce_epi_kernel<OutT, EPI>),
+    hipLaunchKernelGGL((f8_reduce_epi_kernel<OutT, keeps(EPI) ? kEpiKeep : kEpi>),
                        dim3((unsigned)((g.N + 255) / 256), (unsigned)std::min<int64_t>(((int64_t)g.M + 3) / 4, 65535)),
                        dim3(256), 0, st, g, p.splits);
   } else if (p.huge) {
@@ -1443,6 +1557,17 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
   if (lda > kMaxLd || ldb > kMaxLd || ldsa > kMaxLd || ldsb > kMaxLd)
     return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of 8 MiB and more");
   F8Plan p = f8_plan(M, N, K);
+  // 128 x 128 tiles, two workgroups a CU, where the epilogue of one runs beside the other's walk over a
+  // short K, although each operand is read twice as often. Measured (us, against 256 x 256): C in 8 bits
+  // with gelu 16384 x 2048 x 512 33.2 and 39.2, 16384 x 8192 x 1024 169 and 183, 16384 x 2048 x 2048 72.5
+  // and 72.1, with a residual 82 and 89; u kept 41.8 and 49.5, 204 and 214, 82.6 and 83.2, 4096^3 77 and
+  // 65; a residual alone 36.3 and 40.0, 218 and 216; neither 33.6 and 34.4, 174 and 164.
+  const int64_t shallow = c8 ? (e.res ? 2048 : 1024) : e.kind == kEpiKeep && e.aux ? 2048 : e.res ? 512 : 0;
+  if (e.kind != kPlain && p.huge && Kp <= shallow) {
+    p.huge = false;
+    const int64_t t = (((int64_t)M + 127) / 128) * (((int64_t)N + 127) / 128);
+    p.tiles = t > INT32_MAX ? -1 : (int)t;
+  }
   if (p.tiles < 0 || (int64_t)p.tiles * p.splits > INT32_MAX) return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: too many tiles");
   auto dwords = [](const void* s, int64_t ld) { return ld % 4 == 0 && ((uintptr_t)s & 3) == 0; };
   GemmF8Args g{M, N, K, (int)Kp,
@@ -1466,13 +1591,13 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
     if (c_dtype == NL_DTYPE_F32) launch_f8<float>(st, p, g);
     else launch_f8<uint16_t>(st, p, g);
   } else if (c8) {
-    launch_f8_epi<uint8_t, kEpi>(st, p, g);
-  } else if (c_dtype == NL_DTYPE_F32) {
-    if (e.aux) launch_f8_epi<float, kEpiKeep>(st, p, g);  // (in fp32 u is not rounded)
-    else launch_f8_epi<float, kEpi>(st, p, g);
+    e.res ? launch_f8_epi<uint8_t, kEpiRes>(st, p, g) : launch_f8_epi<uint8_t, kEpi>(st, p, g);
+  } else if (c_dtype == NL_DTYPE_F32) {  // (in fp32 u is not rounded)
+    if (e.aux) e.res ? launch_f8_epi<float, kEpiResKeep>(st, p, g) : launch_f8_epi<float, kEpiKeep>(st, p, g);
+    else e.res ? launch_f8_epi<float, kEpiRes>(st, p, g) : launch_f8_epi<float, kEpi>(st, p, g);
   } else {
-    if (e.kind == kEpiKeep) launch_f8_epi<uint16_t, kEpiKeep>(st, p, g);
-    else launch_f8_epi<uint16_t, kEpi>(st, p, g);
+    if (e.kind == kEpiKeep) e.res ? launch_f8_epi<uint16_t, kEpiResKeep>(st, p, g) : launch_f8_epi<uint16_t, kEpiKeep>(st, p, g);
+    else e.res ? launch_f8_epi<uint16_t, kEpiRes>(st, p, g) : launch_f8_epi<uint16_t, kEpi>(st, p, g);
   }
   return nl_check_launch("nl_gemm_fp8");
 }
