@@ -52,16 +52,31 @@ struct QuantArgs {
   float* part = nullptr;    // column sums of each 128 rows, [ceil(rows / 128)][cols] (may be null)
 };
 
-// act'(u); NaN stays NaN
-__device__ __forceinline__ float act_grad(float u, int act) {
-  float d = act == NL_ACT_GELU ? gelu_tanh_grad(u) : act == NL_ACT_SILU ? silu_grad(u) : u > 0.f ? 1.f : 0.f;
-  return u == u ? d : u;
+// v *= act'(u); NaN stays NaN
+template <typename G>
+__device__ __forceinline__ void scale_by(float (&v)[8], const float (&u)[8], G grad) {
+#pragma unroll
+  for (int k = 0; k < 8; ++k) v[k] *= u[k] == u[k] ? grad(u[k]) : u[k];
+}
+template <typename T, int R>
+__device__ __forceinline__ void scale_by_act_grad(float (&v)[R][8], const Vec<T> (&u)[R], int act) {
+  auto rows = [&](auto grad) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+      float f[8];
+      unpack(u[i], f);
+      scale_by(v[i], f, grad);
+    }
+  };
+  if (act == NL_ACT_GELU) rows([](float x) { return gelu_tanh_grad(x); });
+  else if (act == NL_ACT_SILU) rows([](float x) { return silu_grad(x); });
+  else rows([](float x) { return x > 0.f ? 1.f : 0.f; });
 }
 
 // x[row][c0 .. c0+7] as floats, zero past the last column
 template <typename T>
-__device__ __forceinline__ void load8_of(const T* x, int64_t ld, const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
-  const T* p = x + row * ld + c0;
+__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
+  const T* p = reinterpret_cast<const T*>(a.x) + row * a.ldx + c0;
   if (a.vec && c0 + 8 <= a.cols) {
     if constexpr (sizeof(T) == 2) {
       const u32x4 u = *reinterpret_cast<const u32x4*>(p);
@@ -91,16 +106,11 @@ __device__ __forceinline__ void load8_of(const T* x, int64_t ld, const QuantArgs
   }
 }
 
-template <typename T, bool kAct = false>
-__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
-  load8_of<T>(reinterpret_cast<const T*>(a.x), a.ldx, a, row, c0, v);
-  if constexpr (kAct) {
-    if (a.act == NL_ACT_NONE) return;
-    float u[8];
-    load8_of<T>(reinterpret_cast<const T*>(a.u), a.ldu, a, row, c0, u);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = c0 + i < a.cols ? v[i] * act_grad(u[i], a.act) : 0.f;
-  }
+// u[row][c0 .. c0+7], zero past the last row and column (whose values stay +0)
+template <typename T>
+__device__ __forceinline__ Vec<T> load_u(const QuantArgs& a, int64_t row, int64_t c0) {
+  const int64_t left = row < a.rows ? a.cols - c0 : 0;
+  return load_vec(reinterpret_cast<const T*>(a.u) + row * a.ldu + c0, (int)(left < 8 ? left : 8));
 }
 
 // One row's block of 128 per 16 lanes, 8 elements a lane: one read, one write. Bound
@@ -112,8 +122,15 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
   const uint32_t row = id / kb, b = id - row * kb;
   const int l = threadIdx.x & 15;
   const int64_t c0 = (int64_t)b * kB + l * 8;
-  float v[8];
-  load8<T, kAct>(a, row, c0, v);
+  float x[1][8];
+  load8<T>(a, row, c0, x[0]);
+  if constexpr (kAct) {
+    if (a.act != NL_ACT_NONE) {
+      const Vec<T> u[1] = {load_u<T>(a, row, c0)};
+      scale_by_act_grad<T>(x, u, a.act);
+    }
+  }
+  const float(&v)[8] = x[0];
   uint32_t m = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) m = max(m, abs_bits(v[i]));
@@ -177,13 +194,19 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   for (int i = 0; i < 4; ++i) {
     const int64_t r = r0 + g * 4 + i;
     if (r < a.rows) {
-      load8<T, kAct>(a, r, cl, v[i]);
+      load8<T>(a, r, cl, v[i]);
     } else {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
     }
   }
   if constexpr (kAct) {
+    if (a.act != NL_ACT_NONE) {
+      Vec<T> u[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) u[i] = load_u<T>(a, r0 + g * 4 + i, cl);
+      scale_by_act_grad<T>(v, u, a.act);
+    }
     if (a.part) {  // the tile's column sums: a thread's 4 rows, a wave's 4 groups, then the 8 waves
 #pragma unroll
       for (int j = 0; j < 8; ++j) {

@@ -24,38 +24,6 @@ namespace {
 constexpr int kMaxRms = 16384;    // columns
 constexpr int kBwdBlocks = 1024;  // most workgroups of the backward, which leave a partial row of dgamma each
 
-typedef u32x4 __attribute__((aligned(2))) u32x4_any;  // 16 bytes at any address of an element
-typedef f32x4 __attribute__((aligned(4))) f32x4_any;
-
-// 8 elements as they are stored
-template <typename T>
-struct Vec {
-  u32x4 v[sizeof(T) / 2];
-};
-
-// elements p[0 .. n-1] of up to 8, zero behind them
-template <typename T>
-__device__ __forceinline__ Vec<T> load_vec(const T* p, int n) {
-  Vec<T> o;
-  constexpr int kParts = sizeof(T) / 2;
-  if (n >= 8) {
-#pragma unroll
-    for (int i = 0; i < kParts; ++i) o.v[i] = reinterpret_cast<const u32x4_any*>(p)[i];
-    return o;
-  }
-#pragma unroll
-  for (int i = 0; i < kParts; ++i) o.v[i] = u32x4{0u, 0u, 0u, 0u};
-  if (n > 0) {
-#pragma unroll
-    for (int k = 0; k < 7; ++k) {
-      if (k >= n) continue;
-      if constexpr (sizeof(T) == 2) o.v[0][k >> 1] |= (uint32_t)p[k] << (16 * (k & 1));
-      else o.v[k >> 2][k & 3] = __float_as_uint(p[k]);
-    }
-  }
-  return o;
-}
-
 template <typename T>
 __device__ __forceinline__ void store_vec(T* p, const Vec<T>& o, int n) {
   if (n >= 8) {
@@ -71,14 +39,6 @@ __device__ __forceinline__ void store_vec(T* p, const Vec<T>& o, int n) {
   }
 }
 
-template <typename T>
-__device__ __forceinline__ void unpack(const Vec<T>& o, float f[8]) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    if constexpr (sizeof(T) == 2) f[k] = k & 1 ? bf16_hi(o.v[0][k >> 1]) : bf16_lo(o.v[0][k >> 1]);
-    else f[k] = __uint_as_float(o.v[k >> 2][k & 3]);
-  }
-}
 template <typename T>
 __device__ __forceinline__ Vec<T> pack(const float f[8]) {
   Vec<T> o;
