@@ -1513,9 +1513,9 @@ extern "C" int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, co
   if (int rc = dact_args(rows, cols, dy, dtype, lddy, u, ldu, act, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, dbias,
                          part, &a))
     return rc;
-  if (cols == 0) return NL_OK;
+  if (cols == 0 || (rows == 0 && !dbias)) return NL_OK;
   if (rows == 0) {
-    if (dbias) launch_partial_sums((hipStream_t)stream, 0, (int)cols, part, dbias, 0);
+    launch_partial_sums((hipStream_t)stream, 0, (int)cols, part, dbias, 0);
     return nl_check_launch("nl_quantize_fp8_dact");
   }
   return quantize_dact((hipStream_t)stream, a, dtype, dbias);

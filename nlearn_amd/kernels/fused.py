@@ -239,7 +239,7 @@ def _check_rms(what: str, x: torch.Tensor, r, gamma: torch.Tensor, eps: float) -
 
 
 def _dense_like(t: torch.Tensor) -> torch.Tensor:
-    """An empty dense tensor like t (the first form costs half of torch.empty's 2 us)."""
+    """An empty dense tensor like t, without a gradient (the first form costs half of torch.empty's 2 us)."""
     return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 

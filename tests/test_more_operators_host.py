@@ -113,3 +113,100 @@ def test_global_norm_refusals_in_python():
     assert rows_of(c.permute(1, 0, 2)) == (1, 160, 160)
     assert rows_of(x.expand(3, 8)) is None and rows_of(x[:1].expand(4)) is None
     assert rows_of(torch.as_strided(m, (4, 5), (3, 1))) is None
+
+
+def test_fused_product_refusals_of_the_library():
+    lib = _lib.load()
+
+    def product(M=4, N=16, K=128, bias=None, act=0, res=None, ldr=16, rnd=0, aux=None, ldaux=16, C=1024, dt=1, ldc=16,
+                sc=None, ldsc=0):
+        return lib.nl_gemm_fp8_fused(None, M, N, K, 256, 128, 512, 4, 1, 4096, 128, 768, 4, 128, bias, act, res, ldr, rnd,
+                                     aux, ldaux, C, dt, ldc, sc, ldsc, None, 0)
+
+    assert product(M=0) == product(N=0) == _lib.NL_OK
+    for bad in (dict(M=-1), dict(act=4), dict(act=-1), dict(C=None), dict(ldc=8), dict(dt=3), dict(res=2048, ldr=8),
+                dict(aux=2048, ldaux=8), dict(dt=2, ldc=128, sc=None), dict(dt=2, ldc=64, sc=64, ldsc=1),
+                dict(dt=2, ldc=128, sc=64, ldsc=0), dict(dt=2, ldc=128, sc=64, ldsc=1, aux=2048),
+                dict(dt=2, ldc=128, sc=64, ldsc=1, rnd=1)):
+        assert product(**bad) == _lib.NL_EINVAL, bad
+        assert lib.nl_last_error()
+    for bad in (dict(bias=258), dict(res=2056), dict(res=2048, ldr=20), dict(aux=2056), dict(C=1032), dict(ldc=20),
+                dict(dt=2, ldc=136, sc=64, ldsc=1)):
+        assert product(**bad) == _lib.NL_EALIGN, bad
+    for bad in (dict(res=2048, ldr=1 << 22), dict(aux=2048, ldaux=1 << 22), dict(ldc=1 << 22)):
+        assert product(**bad) == _lib.NL_EUNSUPPORTED, bad
+    # the plain product has no 8-bit result
+    assert lib.nl_gemm_fp8(None, 4, 16, 128, 256, 128, 512, 4, 1, 4096, 128, 768, 4, 128, 1024, 2, 128, None,
+                           0) == _lib.NL_EINVAL
+
+
+def test_output_gradient_refusals_of_the_library():
+    lib = _lib.load()
+
+    def dact(rows=4, cols=16, dy=256, dt=1, ld=16, u=512, ldu=16, act=2, q=1024, ldq=128, s=64, lds=1, db=None, ws=None,
+             wsb=0):
+        return lib.nl_quantize_fp8_dact(None, rows, cols, dy, dt, ld, u, ldu, act, q, ldq, s, lds, None, 0, None, 0, db, ws,
+                                        wsb)
+
+    assert dact(rows=0) == dact(cols=0) == _lib.NL_OK
+    need = lib.nl_quantize_fp8_dact_ws_bytes(4, 16)
+    assert need == 64 and lib.nl_quantize_fp8_dact_ws_bytes(0, 16) == 0
+    for bad in (dict(act=4), dict(u=None), dict(ldu=8), dict(dy=None), dict(q=None), dict(dt=2), dict(ld=8), dict(s=None),
+                dict(db=2048), dict(db=2048, ws=4096, wsb=need - 1)):
+        assert dact(**bad) == _lib.NL_EINVAL, bad
+    for bad in (dict(u=513), dict(dy=257), dict(db=2050, ws=4096, wsb=need), dict(ws=4098), dict(q=1032)):
+        assert dact(**bad) == _lib.NL_EALIGN, bad
+    assert dact(cols=(1 << 25) + 1, ld=1 << 26, ldu=1 << 26, ldq=1 << 26, lds=1 << 19, db=2048, ws=4096,
+                wsb=1 << 60) == _lib.NL_EUNSUPPORTED
+    # a layer: the same checks, and its buffers
+    assert lib.nl_linear_fp8_fused_ws_bytes(64, 32, 16, 1, 1, 1, 1) == (
+        lib.nl_linear_fp8_ws_bytes(64, 32, 16, 1, 1, 1) + lib.nl_quantize_fp8_dact_ws_bytes(64, 16))
+    fwd = lambda act=2, ws=4096, bias=None: lib.nl_linear_fp8_fused_fwd(  # noqa: E731
+        None, 64, 32, 16, 256, 1, 32, 512, 0, 16, bias, act, None, 0, 8192, 16, 1024, 1, 16, 0, 0, None, 0, ws, 1 << 20)
+    assert fwd(ws=None) == _lib.NL_EINVAL and fwd(ws=4104) == _lib.NL_EALIGN
+    bwd = lambda act=2, u=512, wsb=1 << 20, db=2048: lib.nl_linear_fp8_fused_bwd(  # noqa: E731
+        None, 64, 32, 16, 256, 1, 16, u, 16, act, db, 4096, 1 << 20, 1, 0, 1024, 1, 32, None, 0, 0, 8192, wsb)
+    assert bwd(act=7) == bwd(u=None) == bwd(wsb=64) == _lib.NL_EINVAL
+    assert bwd(db=2050) == _lib.NL_EALIGN
+
+
+def test_fused_product_refusals_in_python():
+    import torch
+    from nlearn_amd.kernels.fp8 import Fp8Blocks, Fp8Weight, _gemm_fp8_fused, _readable, gemm_fp8, linear_fp8
+
+    x, W = torch.zeros((3, 64), dtype=torch.bfloat16), torch.zeros((64, 20))
+    bias, res = torch.zeros(20), torch.zeros((3, 20), dtype=torch.bfloat16)
+    with pytest.raises(RuntimeError, match="HIP device"):
+        linear_fp8(x, W, bias=bias, activation="gelu", residual=res)
+    for kw, what in ((dict(activation="tanh"), "activation"), (dict(activation=True), "activation"),
+                     (dict(bias=bias[:19]), "bias"), (dict(bias=bias.double()), "bias"), (dict(bias=bias[None]), "bias"),
+                     (dict(residual=res.float()), "residual"), (dict(residual=res[:2]), "residual"),
+                     (dict(residual=res[:1].expand(3, 20)[:, :19]), "residual")):
+        for w in (W, Fp8Weight(Fp8Blocks.empty(20, 64, 128, "cpu"), Fp8Blocks.empty(64, 20, 128, "cpu"))):
+            with pytest.raises(ValueError, match=what):
+                linear_fp8(x, w, **kw)
+    a, b = Fp8Blocks.empty(3, 64, 1, "cpu"), Fp8Blocks.empty(20, 64, 1, "cpu")
+    with pytest.raises(RuntimeError, match="HIP device"):
+        gemm_fp8(a, b, bias=bias)
+    bf, e4 = torch.bfloat16, torch.float8_e4m3fn
+    for args, what in (((bf, None, None, None, "swish", None), "activation"), ((bf, None, None, bias[:3], None, None), "bias"),
+                       ((torch.float16, None, None, None, None, None), "result"),
+                       ((bf, None, None, None, None, res.float()), "residual"), ((e4, None, None, None, None, res.float()), "residual"),
+                       ((torch.float32, None, None, None, None, res), "residual"),
+                       ((bf, None, None, None, None, res[:2]), "residual"),
+                       ((bf, torch.zeros((3, 20), dtype=e4), None, bias, None, None), "result"),
+                       ((bf, res[:1].expand(3, 20), None, bias, None, None), "overlap"),
+                       ((bf, None, torch.zeros((4, 4))[:, :2], bias, None, None), "workspace")):
+        with pytest.raises(ValueError, match=what):
+            _gemm_fp8_fused(a, b, *args)
+    # what the epilogue may read of a matrix over C: whole rows of 8, the last one's too
+    t = torch.zeros((5, 24))
+    assert _readable(t) is t and _readable(t[:, :16]).data_ptr() == t.data_ptr()
+    assert _readable(t[:, :20]).data_ptr() == t.data_ptr()
+    tight = torch.zeros(4 * 24 + 20).as_strided((5, 20), (24, 1))
+    copy = _readable(tight)
+    assert copy.data_ptr() != tight.data_ptr() and copy.stride(0) % 8 == 0 and torch.equal(copy, tight)
+    assert copy.untyped_storage().nbytes() >= 4 * (4 * copy.stride(0) + 24)
+    for odd in (t[:, 1:17], t[:, ::2], t.t(), t[:1].expand(5, 24)):
+        copy = _readable(odd)
+        assert copy.data_ptr() % 16 == 0 and copy.stride(1) == 1 and torch.equal(copy, odd)
