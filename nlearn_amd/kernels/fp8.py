@@ -197,7 +197,10 @@ def _whole_rows(rows: int, cols: int, dtype, device) -> torch.Tensor:
     """``_result`` whose last row, too, holds ``cols`` rounded up to 8 elements."""
     if cols % 8 == 0:
         return _result(rows, cols, dtype, device)
-    return torch.empty((rows, padded_ld(cols)), dtype=dtype, device=device)[:, :cols]
+    # a tensor of its own over that storage: as a view it could not be written in place behind an autograd Function
+    ld = padded_ld(cols)
+    base = torch.empty_strided((rows, ld), (ld, 1), dtype=dtype, device=device)
+    return base.new_empty((0,)).set_(base.untyped_storage(), 0, (rows, cols), (ld, 1))
 
 
 def _readable(t: torch.Tensor) -> torch.Tensor:
@@ -586,6 +589,9 @@ def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation:
     x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
     _check_sizes("linear_fp8", *x2.shape, N)
     grads = torch.is_grad_enabled()
+    if bias is not None and grads and bias.requires_grad:
+        if (x2.shape[0] + BLOCK - 1) // BLOCK * ((N + BLOCK - 1) // BLOCK) >= 1 << 23:
+            raise ValueError(f"linear_fp8: no bias gradient over ({x2.shape[0]}, {N}): 2^23 tiles of 128 x 128 and more")
     if frozen is not None:
         if x2.requires_grad and grads:  # what the product of dY would refuse
             M, (K, N) = x2.shape[0], W.shape

@@ -389,6 +389,32 @@ def test_layer_leading_dimensions_strides_and_nothing(dev):
         assert torch.equal(b.grad, (b.detach() > 0).float() * shape[0])
 
 
+def test_layer_outputs_written_in_place_and_broadcast_residuals(dev):
+    import torch
+    from nlearn_amd.kernels.fp8 import fp8_weight, gemm_fp8, linear_fp8, quantize_fp8
+
+    g = torch.Generator(device=dev).manual_seed(13)
+    for N in (40, 37):
+        x = torch.randn((30, 64), generator=g, device=dev, dtype=torch.bfloat16)
+        W = torch.randn((64, N), generator=g, device=dev).requires_grad_(True)
+        row = torch.randn((1, N), generator=g, device=dev, dtype=torch.bfloat16).requires_grad_(True)
+        y = linear_fp8(x, W, activation="relu", residual=row.expand(30, N))
+        want = y.detach() + 1
+        y += 1
+        assert torch.equal(y, want)
+        dW, dr = torch.autograd.grad(y, (W, row), torch.ones_like(y))
+        assert torch.equal(dr, torch.full_like(dr, 30)) and torch.isfinite(dW).all()
+        # one tensor as input and residual: its gradients add up
+        V = torch.randn((64, 64), generator=g, device=dev)
+        z = x.clone().requires_grad_(True)
+        (both,) = torch.autograd.grad(linear_fp8(z, V, residual=z), z, torch.ones_like(z))
+        (one,) = torch.autograd.grad(linear_fp8(z, V, residual=x), z, torch.ones_like(z))
+        assert torch.equal(both, one + 1)
+        f = fp8_weight(W.detach())
+        r = torch.randn((30, N), generator=g, device=dev, dtype=torch.bfloat16)
+        assert torch.equal(linear_fp8(x, f, residual=r), gemm_fp8(quantize_fp8(x), f.fwd, residual=r))
+
+
 def test_bias_gradient_against_differences(dev):
     """The bias is not quantised: d(sum dY y)/db against central differences of the fp32 layer itself."""
     import torch

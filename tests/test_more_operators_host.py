@@ -185,6 +185,9 @@ def test_fused_product_refusals_in_python():
         for w in (W, Fp8Weight(Fp8Blocks.empty(20, 64, 128, "cpu"), Fp8Blocks.empty(64, 20, 128, "cpu"))):
             with pytest.raises(ValueError, match=what):
                 linear_fp8(x, w, **kw)
+    many = torch.zeros((1, 1), dtype=torch.bfloat16).expand((1 << 30) + 1, 1)
+    with pytest.raises(ValueError, match="bias gradient"):
+        linear_fp8(many, torch.zeros((1, 1)), bias=torch.zeros(1, requires_grad=True))
     a, b = Fp8Blocks.empty(3, 64, 1, "cpu"), Fp8Blocks.empty(20, 64, 1, "cpu")
     with pytest.raises(RuntimeError, match="HIP device"):
         gemm_fp8(a, b, bias=bias)
