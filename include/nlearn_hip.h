@@ -527,7 +527,7 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
                 void* C, int c_dtype, int64_t ldc, void* ws, size_t ws_bytes);
 
 /* nl_gemm_fp8 with what follows a layer's product in its epilogue, in fp32 behind the sum:
- *   u = A . B^T + bias[n]      (bias NULL: none)
+ *   u = A . B^T + bias[n]      (bias fp32 or bf16; NULL: none)
  *   C = act(u) + residual      (residual NULL: none)
  * act: gelu is the tanh form of nl_gemm_fused, silu u * sigmoid(u); NaN stays NaN.
  * round_u: u is rounded to the type of C before act, as what a backward pass keeps; aux (the type
@@ -545,21 +545,21 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
 int nl_gemm_fp8_fused(void* stream, int M, int N, int K,
                       const uint8_t* A, int64_t lda, const uint8_t* scale_a, int64_t ldsa, int group_a,
                       const uint8_t* B, int64_t ldb, const uint8_t* scale_b, int64_t ldsb, int group_b,
-                      const float* bias, int act, const void* residual, int64_t ldr, int round_u,
+                      const void* bias, int bias_dtype, int act, const void* residual, int64_t ldr, int round_u,
                       void* aux, int64_t ldaux, void* C, int c_dtype, int64_t ldc,
                       uint8_t* scale_c, int64_t ldsc, void* ws, size_t ws_bytes);
 
 /* A layer's output gradient behind an activation, quantised: d = dy * act'(u) (dy and u fp32 or
  * bf16, of one type; act NL_ACT_NONE: d = dy, u is not read), formed in fp32.
  *   q, scale; qt, scale_t:  d and its transpose as nl_quantize_fp8 gives them with group 1 (NULL: not wanted)
- *   dbias[c] = sum_rows d   (NULL: not wanted), summed in a fixed order over a workspace of
- *                           nl_quantize_fp8_dact_ws_bytes() bytes (4-byte aligned)
+ *   dbias[c] = sum_rows d   (fp32 or bf16; NULL: not wanted), summed in fp32 in a fixed order over a
+ *                           workspace of nl_quantize_fp8_dact_ws_bytes() bytes (4-byte aligned)
  * relu'(0) is 0; a NaN in u gives NaN. */
 size_t nl_quantize_fp8_dact_ws_bytes(int64_t rows, int64_t cols);
 int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy,
                          const void* u, int64_t ldu, int act, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,
-                         uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, float* dbias, void* ws,
-                         size_t ws_bytes);
+                         uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst, void* dbias, int db_dtype,
+                         void* ws, size_t ws_bytes);
 
 /* y[M][N] = x[M][K] . W[K][N] with both operands quantised first (x in blocks of 1 x
  * 128 along K, W of 128 x 128), and its gradients from dy[M][N]: dx = dy . W^T (dy in
@@ -590,12 +590,12 @@ int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* dy, int dy_
  * with dbias is larger. */
 size_t nl_linear_fp8_fused_ws_bytes(int M, int K, int N, int backward, int need_dx, int need_dw, int need_db);
 int nl_linear_fp8_fused_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
-                            const void* W, int w_dtype, int64_t ldw, const float* bias, int act,
+                            const void* W, int w_dtype, int64_t ldw, const void* bias, int bias_dtype, int act,
                             const void* residual, int64_t ldr, void* u, int64_t ldu,
                             void* y, int y_dtype, int64_t ldy, int need_dx, int need_dw,
                             void* saved, size_t saved_bytes, void* ws, size_t ws_bytes);
 int nl_linear_fp8_fused_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
-                            const void* u, int64_t ldu, int act, float* dbias,
+                            const void* u, int64_t ldu, int act, void* dbias, int db_dtype,
                             const void* saved, size_t saved_bytes, int need_dx, int need_dw,
                             void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw,
                             void* ws, size_t ws_bytes);

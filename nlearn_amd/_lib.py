@@ -99,16 +99,16 @@ _SIGNATURES = {
     "nl_rms_norm_fp8": [_P, _I, _I, _I, _P, _I64, _P, _I64, _P, _I64, _P, _F, _P, _I64, _P, _I64],
     "nl_rms_norm_bwd_ws_bytes": [_I, _I],
     "nl_rms_norm_bwd": [_P, _I, _I, _I, _P, _I64, _P, _I64, _P, _P, _P, _I64, _P, _I64, _P, _I, _P, ctypes.c_size_t],
-    "nl_gemm_fp8_fused": [_P, _I, _I, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I, _P, _I64, _I, _P, _I64,
-                          _P, _I, _I64, _P, _I64, _P, ctypes.c_size_t],
+    "nl_gemm_fp8_fused": [_P, _I, _I, _I, _P, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _I, _P, _I, _I, _P, _I64, _I, _P,
+                          _I64, _P, _I, _I64, _P, _I64, _P, ctypes.c_size_t],
     "nl_quantize_fp8_dact_ws_bytes": [_I64, _I64],
-    "nl_quantize_fp8_dact": [_P, _I64, _I64, _P, _I, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _P,
-                             ctypes.c_size_t],
+    "nl_quantize_fp8_dact": [_P, _I64, _I64, _P, _I, _I64, _P, _I64, _I, _P, _I64, _P, _I64, _P, _I64, _P, _I64, _P, _I,
+                             _P, ctypes.c_size_t],
     "nl_linear_fp8_fused_ws_bytes": [_I, _I, _I, _I, _I, _I, _I],
-    "nl_linear_fp8_fused_fwd": [_P, _I, _I, _I, _P, _I, _I64, _P, _I, _I64, _P, _I, _P, _I64, _P, _I64, _P, _I, _I64, _I,
-                                _I, _P, ctypes.c_size_t, _P, ctypes.c_size_t],
-    "nl_linear_fp8_fused_bwd": [_P, _I, _I, _I, _P, _I, _I64, _P, _I64, _I, _P, _P, ctypes.c_size_t, _I, _I, _P, _I, _I64,
-                                _P, _I, _I64, _P, ctypes.c_size_t],
+    "nl_linear_fp8_fused_fwd": [_P, _I, _I, _I, _P, _I, _I64, _P, _I, _I64, _P, _I, _I, _P, _I64, _P, _I64, _P, _I, _I64,
+                                _I, _I, _P, ctypes.c_size_t, _P, ctypes.c_size_t],
+    "nl_linear_fp8_fused_bwd": [_P, _I, _I, _I, _P, _I, _I64, _P, _I64, _I, _P, _I, _P, ctypes.c_size_t, _I, _I, _P, _I,
+                                _I64, _P, _I, _I64, _P, ctypes.c_size_t],
     "nl_top_logits": [_P, _I, _I, _P, _I64, _I, _F, _P, _P, _P],
     "nl_linear_fp8_saved_bytes": [_I, _I, _I, _I, _I],
     "nl_linear_fp8_ws_bytes": [_I, _I, _I, _I, _I, _I],

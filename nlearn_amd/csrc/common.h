@@ -189,6 +189,7 @@ int nl_set_error(int code, const std::string& msg);
 int nl_check_launch(const char* what);
 namespace nl {
 int cu_count();  // compute units of the current device (256 where there is none)
-// out[c] (+)= sum over p < P of part[p][c], c < D, in a fixed order (rms.hip)
-void launch_partial_sums(hipStream_t st, int P, int D, const float* part, float* out, int accumulate);
+// out[c] (+)= sum over p < P of part[p][c], c < D, in a fixed order (rms.hip); dtype: of out (bf16 is
+// not accumulated)
+void launch_partial_sums(hipStream_t st, int P, int D, const float* part, void* out, int dtype, int accumulate);
 }

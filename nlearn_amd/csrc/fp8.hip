@@ -368,7 +368,8 @@ struct GemmF8Args {
   int items;     // tiles * splits
   int kb_chunk;  // blocks per split (a multiple of 4 when there is more than one)
   // the epilogue's, of the kernels that have one
-  const float* bias;  // may be null
+  const void* bias;   // fp32 or (bias16) bf16, may be null
+  int bias16;
   int act;            // NL_ACT_*
   const void* res;    // in the type of C (bf16 beside 8 bits), may be null
   int64_t ldres;
@@ -722,12 +723,15 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   constexpr int kBias = EPI != kPlain ? WTN / 64 : 1;
   float bias1[kBias];
   auto load_bias = [&](const F8Item& t) __attribute__((always_inline)) {
-    const __amdgpu_buffer_rsrc_t rb = make_rsrc(g.bias ? (const void*)g.bias : (const void*)g.C, kNowhere);
+    const __amdgpu_buffer_rsrc_t rb = make_rsrc(g.bias ? g.bias : g.C, kNowhere);
     const int n = g.bias ? g.N : 0;
 #pragma unroll
     for (int k = 0; k < kBias; ++k) {
       const int c = t.n0 + wn * WTN + k * 64 + lane;
-      bias1[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rb, c < n ? (uint32_t)c * 4u : kNowhere, 0, 0));
+      if (g.bias16)
+        bias1[k] = bf16_to_f32(__builtin_amdgcn_raw_buffer_load_b16(rb, c < n ? (uint32_t)c * 2u : kNowhere, 0, 0));
+      else
+        bias1[k] = __uint_as_float(__builtin_amdgcn_raw_buffer_load_b32(rb, c < n ? (uint32_t)c * 4u : kNowhere, 0, 0));
     }
   };
 
@@ -1226,7 +1230,12 @@ __global__ __launch_bounds__(256) void f8_reduce_epi_kernel(GemmF8Args g, int sp
   };
   float bias[4];
 #pragma unroll
-  for (int k = 0; k < 4; ++k) bias[k] = g.bias && n + k < g.N ? g.bias[n + k] : 0.f;
+  for (int k = 0; k < 4; ++k) {
+    bias[k] = 0.f;
+    if (g.bias && n + k < g.N)
+      bias[k] = g.bias16 ? bf16_to_f32(reinterpret_cast<const uint16_t*>(g.bias)[n + k])
+                         : reinterpret_cast<const float*>(g.bias)[n + k];
+  }
   for (int64_t m = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6); m < g.M; m += (int64_t)gridDim.y * 4) {
     const float* p = g.ws + m * g.ldw + n;
     const int64_t step = (int64_t)g.M * g.ldw;
@@ -1404,7 +1413,7 @@ int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t l
 // The same of dy * act'(u), with its column sums: dbias, over partial rows in ws.
 int dact_args(int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy, const void* u, int64_t ldu, int act,
               uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t,
-              int64_t ldst, float* dbias, float* part, QuantArgs* out) {
+              int64_t ldst, const void* dbias, int db_dtype, float* part, QuantArgs* out) {
   const char* what = "quantize_fp8_dact";
   if (act < NL_ACT_NONE || act > NL_ACT_SILU) return nl_set_error(NL_EINVAL, std::string(what) + ": unknown activation");
   if (int rc = quant_args(rows, cols, dy, dtype, lddy, 1, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, out,
@@ -1420,7 +1429,10 @@ int dact_args(int64_t rows, int64_t cols, const void* dy, int dtype, int64_t ldd
     out->vec = out->vec && ((uintptr_t)u & 15) == 0 && (rows == 1 || ldu * esz % 16 == 0);
   }
   if (dbias && !part) return nl_set_error(NL_EINVAL, std::string(what) + ": workspace too small");
-  if ((uintptr_t)dbias & 3) return nl_set_error(NL_EALIGN, std::string(what) + ": dbias is not aligned");
+  if (dbias && db_dtype != NL_DTYPE_F32 && db_dtype != NL_DTYPE_BF16)
+    return nl_set_error(NL_EINVAL, std::string(what) + ": dbias is fp32 or bf16");
+  if ((uintptr_t)dbias & (db_dtype == NL_DTYPE_BF16 ? 1 : 3))
+    return nl_set_error(NL_EALIGN, std::string(what) + ": dbias is not aligned to its type");
   out->u = u, out->ldu = ldu, out->act = act, out->part = dbias ? part : nullptr;
   return NL_OK;
 }
@@ -1489,10 +1501,10 @@ extern "C" int nl_quantize_fp8(void* stream, int64_t rows, int64_t cols, const v
 namespace nl {
 namespace {
 
-int quantize_dact(hipStream_t st, const QuantArgs& a, int dtype, float* dbias) {
+int quantize_dact(hipStream_t st, const QuantArgs& a, int dtype, void* dbias, int db_dtype) {
   const int rc = a.act == NL_ACT_NONE && !a.part ? quantize_one<false>(st, a, dtype) : quantize_one<true>(st, a, dtype);
   if (rc || !a.part) return rc;
-  launch_partial_sums(st, (int)blocks_of(a.rows), (int)a.cols, a.part, dbias, 0);
+  launch_partial_sums(st, (int)blocks_of(a.rows), (int)a.cols, a.part, dbias, db_dtype, 0);
   return nl_check_launch("nl_quantize_fp8_dact");
 }
 
@@ -1506,19 +1518,19 @@ extern "C" size_t nl_quantize_fp8_dact_ws_bytes(int64_t rows, int64_t cols) {
 extern "C" int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy,
                                     const void* u, int64_t ldu, int act, uint8_t* q, int64_t ldq, uint8_t* scale,
                                     int64_t lds, uint8_t* qt, int64_t ldqt, uint8_t* scale_t, int64_t ldst,
-                                    float* dbias, void* ws, size_t ws_bytes) {
+                                    void* dbias, int db_dtype, void* ws, size_t ws_bytes) {
   QuantArgs a;
   if ((uintptr_t)ws & 3) return nl_set_error(NL_EALIGN, "quantize_fp8_dact: workspace not aligned");
   float* part = ws && ws_bytes >= nl_quantize_fp8_dact_ws_bytes(rows, cols) ? (float*)ws : nullptr;
   if (int rc = dact_args(rows, cols, dy, dtype, lddy, u, ldu, act, q, ldq, scale, lds, qt, ldqt, scale_t, ldst, dbias,
-                         part, &a))
+                         db_dtype, part, &a))
     return rc;
   if (cols == 0 || (rows == 0 && !dbias)) return NL_OK;
   if (rows == 0) {
-    launch_partial_sums((hipStream_t)stream, 0, (int)cols, part, dbias, 0);
+    launch_partial_sums((hipStream_t)stream, 0, (int)cols, part, dbias, db_dtype, 0);
     return nl_check_launch("nl_quantize_fp8_dact");
   }
-  return quantize_dact((hipStream_t)stream, a, dtype, dbias);
+  return quantize_dact((hipStream_t)stream, a, dtype, dbias, db_dtype);
 }
 
 extern "C" size_t nl_gemm_fp8_ws_bytes(int M, int N, int K) {
@@ -1533,7 +1545,8 @@ namespace {
 // The epilogue of a product as its callers give it; none: all as below.
 struct F8Epilogue {
   int kind = kPlain;
-  const float* bias = nullptr;
+  const void* bias = nullptr;
+  int bias_dtype = NL_DTYPE_F32;
   int act = NL_ACT_NONE;
   const void* res = nullptr;
   int64_t ldres = 0;
@@ -1572,7 +1585,10 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
     if (ldc < N) return nl_set_error(NL_EINVAL, "gemm_fp8: ldc < N");
     if (((uintptr_t)C & 15) || ldc % 8) return nl_set_error(NL_EALIGN, "gemm_fp8: C needs 16-byte aligned rows");
   }
-  if ((uintptr_t)e.bias & 3) return nl_set_error(NL_EALIGN, "gemm_fp8: bias is not aligned");
+  if (e.bias && e.bias_dtype != NL_DTYPE_F32 && e.bias_dtype != NL_DTYPE_BF16)
+    return nl_set_error(NL_EINVAL, "gemm_fp8: bias is fp32 or bf16");
+  const int bias16 = e.bias_dtype == NL_DTYPE_BF16 ? 1 : 0;
+  if ((uintptr_t)e.bias & (bias16 ? 1 : 3)) return nl_set_error(NL_EALIGN, "gemm_fp8: bias is not aligned to its type");
   if (int rc = check_over_c("the residual", e.res, e.ldres, N)) return rc;
   if (int rc = check_over_c("aux", e.aux, e.ldaux, N)) return rc;
   const int64_t Kp = ((int64_t)K + kB - 1) / kB * kB;
@@ -1598,7 +1614,7 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
                B, ldb, scale_b, ldsb, group_b == kB ? 7 : 0,
                dwords(scale_a, ldsa) && dwords(scale_b, ldsb) ? 1 : 0,
                C, ldc, nullptr, f8_ldw(N), p.tiles, 0, p.kb_chunk,
-               e.bias, e.act, e.res, e.ldres, e.aux, e.ldaux, e.sc, e.ldsc};
+               e.bias, bias16, e.act, e.res, e.ldres, e.aux, e.ldaux, e.sc, e.ldsc};
   if (p.splits > 1) {
     if (ws && ws_bytes >= nl_gemm_fp8_ws_bytes(M, N, K)) {
       if ((uintptr_t)ws & 15) return nl_set_error(NL_EALIGN, "gemm_fp8: workspace not 16-byte aligned");
@@ -1637,12 +1653,13 @@ extern "C" int nl_gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, 
 
 extern "C" int nl_gemm_fp8_fused(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda,
                                  const uint8_t* scale_a, int64_t ldsa, int group_a, const uint8_t* B, int64_t ldb,
-                                 const uint8_t* scale_b, int64_t ldsb, int group_b, const float* bias, int act,
-                                 const void* residual, int64_t ldr, int round_u, void* aux, int64_t ldaux, void* C,
+                                 const uint8_t* scale_b, int64_t ldsb, int group_b, const void* bias, int bias_dtype,
+                                 int act, const void* residual, int64_t ldr, int round_u, void* aux, int64_t ldaux, void* C,
                                  int c_dtype, int64_t ldc, uint8_t* scale_c, int64_t ldsc, void* ws, size_t ws_bytes) {
   F8Epilogue e;
   e.kind = round_u || aux ? kEpiKeep : kEpi;
-  e.bias = bias, e.act = act, e.res = residual, e.ldres = ldr, e.aux = aux, e.ldaux = ldaux, e.sc = scale_c, e.ldsc = ldsc;
+  e.bias = bias, e.bias_dtype = bias_dtype, e.act = act, e.res = residual, e.ldres = ldr, e.aux = aux, e.ldaux = ldaux;
+  e.sc = scale_c, e.ldsc = ldsc;
   if (c_dtype == NL_DTYPE_E4M3 && round_u) return nl_set_error(NL_EINVAL, "gemm_fp8: a result in 8 bits does not round u");
   return gemm_fp8(stream, M, N, K, A, lda, scale_a, ldsa, group_a, B, ldb, scale_b, ldsb, group_b, C, c_dtype, ldc, e,
                   ws, ws_bytes);
@@ -1765,7 +1782,7 @@ int linear_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, in
 // dy * act'(u) quantised for the wanted gradients; dbias (may be null) over partial rows behind
 // what else the workspace holds.
 int linear_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy, const void* u,
-               int64_t ldu, int act, float* dbias, const void* saved, size_t saved_bytes, int need_dx, int need_dw,
+               int64_t ldu, int act, void* dbias, int db_dtype, const void* saved, size_t saved_bytes, int need_dx, int need_dw,
                void* dx, int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws, size_t ws_bytes) {
   if (M <= 0 || K <= 0 || N <= 0) return nl_set_error(NL_EINVAL, "linear_fp8_bwd: need M, K, N > 0");
   if (!need_dx && !need_dw && !dbias) return NL_OK;
@@ -1779,9 +1796,9 @@ int linear_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, 
   QuantArgs q;
   if (int rc = dact_args(M, N, dy, dy_dtype, lddy, u, ldu, act, need_dx ? b + p.dy.at : nullptr, p.dy.ld(),
                          need_dx ? b + p.dy.sat : nullptr, p.dy.lds(), need_dw ? b + p.dyt.at : nullptr, p.dyt.ld(),
-                         need_dw ? b + p.dyt.sat : nullptr, p.dyt.lds(), dbias, (float*)(b + behind), &q))
+                         need_dw ? b + p.dyt.sat : nullptr, p.dyt.lds(), dbias, db_dtype, (float*)(b + behind), &q))
     return rc;
-  if (int rc = quantize_dact((hipStream_t)stream, q, dy_dtype, dbias)) return rc;
+  if (int rc = quantize_dact((hipStream_t)stream, q, dy_dtype, dbias, db_dtype)) return rc;
   if (need_dx)
     if (int rc = product(stream, b, p.dy, sv, p.wb, dx, dx_dtype, lddx, b + p.bwd, p.ws_dx)) return rc;
   if (need_dw)
@@ -1804,7 +1821,7 @@ extern "C" int nl_linear_fp8_bwd(void* stream, int M, int K, int N, const void* 
                                  const void* saved, size_t saved_bytes, int need_dx, int need_dw, void* dx,
                                  int dx_dtype, int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws,
                                  size_t ws_bytes) {
-  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, nullptr, 0, NL_ACT_NONE, nullptr, saved, saved_bytes, need_dx,
+  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, nullptr, 0, NL_ACT_NONE, nullptr, 0, saved, saved_bytes, need_dx,
                     need_dw, dx, dx_dtype, lddx, dW, dw_dtype, lddw, ws, ws_bytes);
 }
 
@@ -1815,21 +1832,22 @@ extern "C" size_t nl_linear_fp8_fused_ws_bytes(int M, int K, int N, int backward
 }
 
 extern "C" int nl_linear_fp8_fused_fwd(void* stream, int M, int K, int N, const void* x, int x_dtype, int64_t ldx,
-                                       const void* W, int w_dtype, int64_t ldw, const float* bias, int act,
-                                       const void* residual, int64_t ldr, void* u, int64_t ldu, void* y, int y_dtype,
+                                       const void* W, int w_dtype, int64_t ldw, const void* bias, int bias_dtype,
+                                       int act, const void* residual, int64_t ldr, void* u, int64_t ldu, void* y, int y_dtype,
                                        int64_t ldy, int need_dx, int need_dw, void* saved, size_t saved_bytes,
                                        void* ws, size_t ws_bytes) {
   F8Epilogue e;
   e.kind = act != NL_ACT_NONE ? kEpiKeep : kEpi;
-  e.bias = bias, e.act = act, e.res = residual, e.ldres = ldr, e.aux = act != NL_ACT_NONE ? u : nullptr, e.ldaux = ldu;
+  e.bias = bias, e.bias_dtype = bias_dtype, e.act = act, e.res = residual, e.ldres = ldr;
+  e.aux = act != NL_ACT_NONE ? u : nullptr, e.ldaux = ldu;
   return linear_fwd(stream, M, K, N, x, x_dtype, ldx, W, w_dtype, ldw, e, y, y_dtype, ldy, need_dx, need_dw, saved,
                     saved_bytes, ws, ws_bytes);
 }
 
 extern "C" int nl_linear_fp8_fused_bwd(void* stream, int M, int K, int N, const void* dy, int dy_dtype, int64_t lddy,
-                                       const void* u, int64_t ldu, int act, float* dbias, const void* saved,
-                                       size_t saved_bytes, int need_dx, int need_dw, void* dx, int dx_dtype,
+                                       const void* u, int64_t ldu, int act, void* dbias, int db_dtype,
+                                       const void* saved, size_t saved_bytes, int need_dx, int need_dw, void* dx, int dx_dtype,
                                        int64_t lddx, void* dW, int dw_dtype, int64_t lddw, void* ws, size_t ws_bytes) {
-  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, u, ldu, act, dbias, saved, saved_bytes, need_dx, need_dw, dx,
+  return linear_bwd(stream, M, K, N, dy, dy_dtype, lddy, u, ldu, act, dbias, db_dtype, saved, saved_bytes, need_dx, need_dw, dx,
                     dx_dtype, lddx, dW, dw_dtype, lddw, ws, ws_bytes);
 }

@@ -352,7 +352,7 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsBwdAr
 // out (+)= the sum of P partial rows (of dgamma, of a bias gradient), in a fixed order: a workgroup takes 16 columns, thread (ph, q) the
 // rows ph, ph + 256, ... of columns 4q .. 4q+3; then the 16 phases of a wave, then the 16 waves.
 __global__ __launch_bounds__(1024) void row_sums_kernel(int P, int D, const float* __restrict__ part,
-                                                       float* __restrict__ out, int accumulate) {
+                                                       void* __restrict__ out, int bf16, int accumulate) {
   __shared__ float sums[16][17];
   const int q = threadIdx.x & 3, ph = threadIdx.x >> 2, c = blockIdx.x * 16 + q * 4, n = D - c;
   float a[4] = {0.f, 0.f, 0.f, 0.f};
@@ -380,7 +380,12 @@ __global__ __launch_bounds__(1024) void row_sums_kernel(int P, int D, const floa
     float t = 0.f;
 #pragma unroll
     for (int w = 0; w < 16; ++w) t += sums[w][threadIdx.x];
-    out[col] = accumulate ? out[col] + t : t;
+    if (bf16) {
+      reinterpret_cast<uint16_t*>(out)[col] = f32_to_bf16(t);
+    } else {
+      float* o = reinterpret_cast<float*>(out) + col;
+      *o = accumulate ? *o + t : t;
+    }
   }
 }
 
@@ -470,9 +475,9 @@ int rms_forward(const char* what, void* stream, int dtype, bool f8, const RmsArg
 }  // namespace
 }  // namespace nl
 
-void nl::launch_partial_sums(hipStream_t st, int P, int D, const float* part, float* out, int accumulate) {
+void nl::launch_partial_sums(hipStream_t st, int P, int D, const float* part, void* out, int dtype, int accumulate) {
   hipLaunchKernelGGL(row_sums_kernel, dim3((unsigned)(((int64_t)D + 15) / 16)), dim3(1024), 0, st, P, D, part, out,
-                     accumulate);
+                     dtype == NL_DTYPE_BF16 ? 1 : 0, accumulate);
 }
 
 using namespace nl;
@@ -528,6 +533,6 @@ extern "C" int nl_rms_norm_bwd(void* stream, int rows, int D, int dtype, const v
     });
   }
   if (dgamma && (rows > 0 || !accumulate)) 
-    launch_partial_sums(st, blocks, D, (const float*)ws, dgamma, accumulate);
+    launch_partial_sums(st, blocks, D, (const float*)ws, dgamma, NL_DTYPE_F32, accumulate);
   return nl_check_launch(what);
 }

@@ -216,6 +216,20 @@ def _readable(t: torch.Tensor) -> torch.Tensor:
     return out
 
 
+def _vector(t):
+    """(address, type) of a bias or its gradient."""
+    return (None, 0) if t is None else (t.data_ptr(), 0 if t.dtype is _F32 else 1)
+
+
+def _dense_vector(bias):
+    """bias with unit stride; copies only if it must."""
+    return bias if bias is None or bias.is_contiguous() else bias.detach().contiguous()
+
+
+def _bytes(n: int, device) -> torch.Tensor:
+    return torch.empty_strided((n,), (1,), dtype=torch.uint8, device=device)
+
+
 def _fused_product(a: Fp8Blocks, b: Fp8Blocks, out, ws, bias, act: int, residual, round_u: bool, u) -> None:
     """nl_gemm_fp8_fused into ``out``, a tensor whose rows hold N rounded up to 8 or an Fp8Blocks."""
     (M, K), N = a.shape, b.shape[0]
@@ -230,9 +244,9 @@ def _fused_product(a: Fp8Blocks, b: Fp8Blocks, out, ws, bias, act: int, residual
         c, ldc, sc, ldsc = out.data_ptr(), _ld(out), None, 0
         code = _code(out)
     _lib.call_on(a.q, "nl_gemm_fp8_fused", M, N, K, qa, lda, sa, ldsa, a.group, qb, ldb, sb, ldsb, b.group,
-                 bias.data_ptr() if bias is not None else None, act,
-                 residual.data_ptr() if residual is not None else None, _ld(residual) if residual is not None else 0,
-                 round_u, u.data_ptr() if u is not None else None, _ld(u) if u is not None else 0, c, code, ldc, sc, ldsc,
+                 *_vector(bias), act, residual.data_ptr() if residual is not None else None,
+                 _ld(residual) if residual is not None else 0, round_u, u.data_ptr() if u is not None else None,
+                 u.stride(0) if u is not None else 0, c, code, ldc, sc, ldsc,
                  ws.data_ptr() if ws is not None else None, ws.numel() * ws.element_size() if ws is not None else 0)
 
 
@@ -247,7 +261,7 @@ def _gemm_fp8_fused(a, b, out_dtype, out, ws, bias, activation, residual):
     dt = _BF16 if out_dtype is _E4M3 else out_dtype
     if bias is not None:
         _check_bias("gemm_fp8", bias, N, a.q)
-        bias = _param(bias)
+        bias = _dense_vector(bias)
     if residual is not None and (residual.dtype is not dt or tuple(residual.shape) != (M, N)
                                  or residual.get_device() != a.q.get_device()):
         raise ValueError(f"gemm_fp8: the residual must be {dt} of shape {(M, N)} on {a.q.device}, got "
@@ -449,10 +463,10 @@ def _bias_grad(bias: torch.Tensor):
     """(what dbias is written to, whether that is bias's main_grad)."""
     mg = grad_buffer(bias)
     if mg is None:
-        return torch.empty(bias.shape, dtype=_F32, device=bias.device), False
-    if mg.shape != bias.shape or mg.device != bias.device or mg.dtype is not _F32 or not mg.is_contiguous():
-        raise ValueError(f"linear_fp8: the bias's main_grad must be a dense float32 tensor of shape {tuple(bias.shape)} "
-                         f"on {bias.device}")
+        return torch.empty_strided(bias.shape, (1,), dtype=bias.dtype, device=bias.device), False
+    if mg.shape != bias.shape or mg.device != bias.device or mg.dtype not in (_F32, _BF16) or not mg.is_contiguous():
+        raise ValueError(f"linear_fp8: the bias's main_grad must be a dense tensor of shape {tuple(bias.shape)} on "
+                         f"{bias.device}")
     return mg, True
 
 
@@ -469,30 +483,28 @@ class _LinearFp8Fused(torch.autograd.Function):
         ctx.W = W if need_dW and (W.is_leaf or grad_buffer(W) is not None) else None
         ctx.w_like = None if W is None else (W.dtype, W.is_contiguous())
         ctx.bias = bias if need_db else None
-        ctx.res_dtype = None if res2 is None else res2.dtype
-        y = _whole_rows(M, N, x2.dtype, x2.device)
+        dev = x2.device
+        y = _whole_rows(M, N, x2.dtype, dev)
         # what act'(u) is formed from, in the dtype of y as the activation itself sees it
-        u = _whole_rows(M, N, x2.dtype, x2.device) if act and (need_dx or need_dW or need_db) else None
+        u = _whole_rows(M, N, x2.dtype, dev) if act and (need_dx or need_dW or need_db) else None
         saved = None
         if M and N:
-            b32 = _param(bias) if bias is not None else None
+            bias = _dense_vector(bias)
             r = _readable(res2) if res2 is not None else None
             if frozen is not None:
-                _fused_product(_quantize(x2, 1, True, False)[0], frozen.fwd, y, None, b32, act, r, bool(act), u)
+                _fused_product(_quantize(x2, 1, True, False)[0], frozen.fwd, y, None, bias, act, r, bool(act), u)
             elif K == 0:  # no product to quantise for
                 none = Fp8Blocks.empty
-                _fused_product(none(M, 0, 1, x2.device), none(N, 0, BLOCK, x2.device), y, None, b32, act, r, bool(act), u)
+                _fused_product(none(M, 0, 1, dev), none(N, 0, BLOCK, dev), y, None, bias, act, r, bool(act), u)
             else:
                 saved_bytes, wsb, _ = _linear_fused_bytes(M, K, N, need_dx, need_dW, need_db)
-                saved = torch.empty(saved_bytes, dtype=torch.uint8, device=x2.device)
-                ws = torch.empty(wsb, dtype=torch.uint8, device=x2.device)
+                saved, ws = _bytes(saved_bytes, dev), _bytes(wsb, dev)
                 (x2, ldx), (Wr, ldw) = _rows(x2), _rows(W)
                 _lib.call_on(x2, "nl_linear_fp8_fused_fwd", M, K, N, x2.data_ptr(), _code(x2), ldx, Wr.data_ptr(),
-                             _code(Wr), ldw, b32.data_ptr() if b32 is not None else None, act,
-                             r.data_ptr() if r is not None else None, _ld(r) if r is not None else 0,
-                             u.data_ptr() if u is not None else None, _ld(u) if u is not None else 0,
-                             y.data_ptr(), _code(y), _ld(y), need_dx, need_dW, saved.data_ptr(), saved_bytes,
-                             ws.data_ptr(), wsb)
+                             _code(Wr), ldw, *_vector(bias), act, r.data_ptr() if r is not None else None,
+                             _ld(r) if r is not None else 0, u.data_ptr() if u is not None else None,
+                             u.stride(0) if u is not None else 0, y.data_ptr(), _code(y), y.stride(0), need_dx, need_dW,
+                             saved.data_ptr(), saved_bytes, ws.data_ptr(), wsb)
         ctx.save_for_backward(saved, u)
         return y
 
@@ -503,7 +515,9 @@ class _LinearFp8Fused(torch.autograd.Function):
         M, K, N, x_dtype = ctx.sizes
         need_dx, need_dW, need_db, need_dr = ctx.need
         act, frozen = ctx.act, ctx.frozen
-        dr = dy.to(ctx.res_dtype) if need_dr else None
+        if dy.dtype is not x_dtype:
+            dy = dy.to(x_dtype)
+        dr = dy if need_dr else None   # (the residual has x's dtype)
         if not (need_dx or need_dW or need_db):
             return None, None, None, dr, None, None, None
         dev = dy.device
@@ -517,7 +531,8 @@ class _LinearFp8Fused(torch.autograd.Function):
             if direct:
                 dW = mg
             elif mg is None and w_dense and N % 8 == 0:
-                dW = torch.empty((K, N), dtype=w_dtype, device=dev)  # laid out like W: kept as W.grad without a copy
+                # laid out like W: kept as W.grad without a copy
+                dW = torch.empty_strided((K, N), (N, 1), dtype=w_dtype, device=dev)
             else:
                 dW = _result(K, N, w_dtype if mg is None else _F32, dev)
         if M == 0 or N == 0:
@@ -525,33 +540,33 @@ class _LinearFp8Fused(torch.autograd.Function):
                 if t is not None:
                     t.zero_()
         else:
-            dy2, lddy = _rows(dy if dy.dtype is x_dtype else dy.to(x_dtype))
-            up, ldu = (u.data_ptr(), _ld(u)) if u is not None else (None, 0)
-            dbp = db.data_ptr() if need_db else None
+            dy2, lddy = _rows(dy)
+            up, ldu = (u.data_ptr(), u.stride(0)) if u is not None else (None, 0)
+            dbp = _vector(db)
             if frozen is not None or K == 0:
                 want_dx = need_dx and K > 0
                 q = Fp8Blocks.empty(M, N, 1, dev) if want_dx else None
                 wsb = _lib.load().nl_quantize_fp8_dact_ws_bytes(M, N) if need_db else 0
-                ws = torch.empty(wsb, dtype=torch.uint8, device=dev) if wsb else None
+                ws = _bytes(wsb, dev) if wsb else None
                 if want_dx or need_db:
                     _lib.call_on(dy2, "nl_quantize_fp8_dact", M, N, dy2.data_ptr(), _code(dy2), lddy, up, ldu, act,
-                                 *(q._abi() if want_dx else _NONE), *_NONE, dbp, ws.data_ptr() if wsb else None, wsb)
+                                 *(q._abi() if want_dx else _NONE), *_NONE, *dbp, ws.data_ptr() if wsb else None, wsb)
                 if want_dx:
                     dx = gemm_fp8(q, frozen.bwd, x_dtype, out=dx)                           # dU . W^T
+                if need_dW:
+                    dW.zero_()  # of no rows
             else:
                 saved_bytes, _, wsb = _linear_fused_bytes(M, K, N, need_dx, need_dW, need_db)
-                ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
-                _lib.call_on(dy2, "nl_linear_fp8_fused_bwd", M, K, N, dy2.data_ptr(), _code(dy2), lddy, up, ldu, act, dbp,
+                ws = _bytes(wsb, dev)
+                _lib.call_on(dy2, "nl_linear_fp8_fused_bwd", M, K, N, dy2.data_ptr(), _code(dy2), lddy, up, ldu, act, *dbp,
                              saved.data_ptr(), saved_bytes, need_dx, need_dW,
-                             *((dx.data_ptr(), _code(dx), _ld(dx)) if need_dx else (None, 0, 0)),
+                             *((dx.data_ptr(), _code(dx), dx.stride(0)) if need_dx else (None, 0, 0)),
                              *((dW.data_ptr(), _code(dW), _ld(dW)) if need_dW else (None, 0, 0)), ws.data_ptr(), wsb)
         if mg is not None:
             if not direct:
                 mg.copy_(dW)
             dW = None
-        if need_db:
-            db = None if db_taken else db.to(ctx.bias.dtype)
-        return dx, dW, db, dr, None, None, None
+        return dx, dW, None if db_taken else db, dr, None, None, None
 
 
 def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation: str | None = None,

@@ -250,7 +250,7 @@ def test_output_gradient_behind_an_activation(dev, rows, cols, ld, dtype):
         wsb = _lib.load().nl_quantize_fp8_dact_ws_bytes(rows, cols)
         ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
         args = [dy.data_ptr(), code, ld, u.data_ptr(), ld, act]
-        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *q._abi(), *t._abi(), db.data_ptr(), ws.data_ptr(), wsb)
+        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *q._abi(), *t._abi(), db.data_ptr(), 0, ws.data_ptr(), wsb)
         z = _np(u)
         d = _np(dy) * _act(z, name)[1]
         e = np.abs(_np(dy)) * _slope_error(z, name)
@@ -261,10 +261,10 @@ def test_output_gradient_behind_an_activation(dev, rows, cols, ld, dtype):
         # one output at a time: the same
         q2, t2 = Fp8Blocks.empty(rows, cols, 1, dev), Fp8Blocks.empty(cols, rows, 1, dev)
         none = (None, 0, None, 0)
-        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *q2._abi(), *none, None, None, 0)
-        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *none, *t2._abi(), None, None, 0)
+        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *q2._abi(), *none, None, 0, None, 0)
+        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *none, *t2._abi(), None, 0, None, 0)
         db2 = torch.empty(cols, device=dev)
-        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *none, *none, db2.data_ptr(), ws.data_ptr(), wsb)
+        _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *none, *none, db2.data_ptr(), 0, ws.data_ptr(), wsb)
         for p, r in ((q, q2), (t, t2)):
             assert torch.equal(p.q.view(torch.uint8), r.q.view(torch.uint8))
             assert torch.equal(p.scale.contiguous().view(torch.uint8), r.scale.contiguous().view(torch.uint8))
@@ -274,7 +274,7 @@ def test_output_gradient_behind_an_activation(dev, rows, cols, ld, dtype):
     ws = torch.empty(64, dtype=torch.uint8, device=dev)
     for act in (1, 2, 3):
         _lib.call_on(one, "nl_quantize_fp8_dact", 1, 4, one.data_ptr(), code, 4, nan.data_ptr(), 4, act, None, 0, None, 0, None, 0,
-                     None, 0, db.data_ptr(), ws.data_ptr(), 64)
+                     None, 0, db.data_ptr(), 0, ws.data_ptr(), 64)
         assert torch.isnan(db).all()
 
 

@@ -118,19 +118,19 @@ def test_global_norm_refusals_in_python():
 def test_fused_product_refusals_of_the_library():
     lib = _lib.load()
 
-    def product(M=4, N=16, K=128, bias=None, act=0, res=None, ldr=16, rnd=0, aux=None, ldaux=16, C=1024, dt=1, ldc=16,
+    def product(M=4, N=16, K=128, bias=None, bdt=0, act=0, res=None, ldr=16, rnd=0, aux=None, ldaux=16, C=1024, dt=1, ldc=16,
                 sc=None, ldsc=0):
-        return lib.nl_gemm_fp8_fused(None, M, N, K, 256, 128, 512, 4, 1, 4096, 128, 768, 4, 128, bias, act, res, ldr, rnd,
+        return lib.nl_gemm_fp8_fused(None, M, N, K, 256, 128, 512, 4, 1, 4096, 128, 768, 4, 128, bias, bdt, act, res, ldr, rnd,
                                      aux, ldaux, C, dt, ldc, sc, ldsc, None, 0)
 
     assert product(M=0) == product(N=0) == _lib.NL_OK
     for bad in (dict(M=-1), dict(act=4), dict(act=-1), dict(C=None), dict(ldc=8), dict(dt=3), dict(res=2048, ldr=8),
                 dict(aux=2048, ldaux=8), dict(dt=2, ldc=128, sc=None), dict(dt=2, ldc=64, sc=64, ldsc=1),
                 dict(dt=2, ldc=128, sc=64, ldsc=0), dict(dt=2, ldc=128, sc=64, ldsc=1, aux=2048),
-                dict(dt=2, ldc=128, sc=64, ldsc=1, rnd=1)):
+                dict(dt=2, ldc=128, sc=64, ldsc=1, rnd=1), dict(bias=256, bdt=2)):
         assert product(**bad) == _lib.NL_EINVAL, bad
         assert lib.nl_last_error()
-    for bad in (dict(bias=258), dict(res=2056), dict(res=2048, ldr=20), dict(aux=2056), dict(C=1032), dict(ldc=20),
+    for bad in (dict(bias=258), dict(bias=257, bdt=1), dict(res=2056), dict(res=2048, ldr=20), dict(aux=2056), dict(C=1032), dict(ldc=20),
                 dict(dt=2, ldc=136, sc=64, ldsc=1)):
         assert product(**bad) == _lib.NL_EALIGN, bad
     for bad in (dict(res=2048, ldr=1 << 22), dict(aux=2048, ldaux=1 << 22), dict(ldc=1 << 22)):
@@ -143,18 +143,19 @@ def test_fused_product_refusals_of_the_library():
 def test_output_gradient_refusals_of_the_library():
     lib = _lib.load()
 
-    def dact(rows=4, cols=16, dy=256, dt=1, ld=16, u=512, ldu=16, act=2, q=1024, ldq=128, s=64, lds=1, db=None, ws=None,
-             wsb=0):
-        return lib.nl_quantize_fp8_dact(None, rows, cols, dy, dt, ld, u, ldu, act, q, ldq, s, lds, None, 0, None, 0, db, ws,
-                                        wsb)
+    def dact(rows=4, cols=16, dy=256, dt=1, ld=16, u=512, ldu=16, act=2, q=1024, ldq=128, s=64, lds=1, db=None, bdt=0,
+             ws=None, wsb=0):
+        return lib.nl_quantize_fp8_dact(None, rows, cols, dy, dt, ld, u, ldu, act, q, ldq, s, lds, None, 0, None, 0, db, bdt,
+                                        ws, wsb)
 
     assert dact(rows=0) == dact(cols=0) == _lib.NL_OK
     need = lib.nl_quantize_fp8_dact_ws_bytes(4, 16)
     assert need == 64 and lib.nl_quantize_fp8_dact_ws_bytes(0, 16) == 0
     for bad in (dict(act=4), dict(u=None), dict(ldu=8), dict(dy=None), dict(q=None), dict(dt=2), dict(ld=8), dict(s=None),
-                dict(db=2048), dict(db=2048, ws=4096, wsb=need - 1)):
+                dict(db=2048), dict(db=2048, ws=4096, wsb=need - 1), dict(db=2048, bdt=2, ws=4096, wsb=need)):
         assert dact(**bad) == _lib.NL_EINVAL, bad
-    for bad in (dict(u=513), dict(dy=257), dict(db=2050, ws=4096, wsb=need), dict(ws=4098), dict(q=1032)):
+    for bad in (dict(u=513), dict(dy=257), dict(db=2050, ws=4096, wsb=need),
+                dict(db=2049, bdt=1, ws=4096, wsb=need), dict(ws=4098), dict(q=1032)):
         assert dact(**bad) == _lib.NL_EALIGN, bad
     assert dact(cols=(1 << 25) + 1, ld=1 << 26, ldu=1 << 26, ldq=1 << 26, lds=1 << 19, db=2048, ws=4096,
                 wsb=1 << 60) == _lib.NL_EUNSUPPORTED
@@ -162,10 +163,10 @@ def test_output_gradient_refusals_of_the_library():
     assert lib.nl_linear_fp8_fused_ws_bytes(64, 32, 16, 1, 1, 1, 1) == (
         lib.nl_linear_fp8_ws_bytes(64, 32, 16, 1, 1, 1) + lib.nl_quantize_fp8_dact_ws_bytes(64, 16))
     fwd = lambda act=2, ws=4096, bias=None: lib.nl_linear_fp8_fused_fwd(  # noqa: E731
-        None, 64, 32, 16, 256, 1, 32, 512, 0, 16, bias, act, None, 0, 8192, 16, 1024, 1, 16, 0, 0, None, 0, ws, 1 << 20)
+        None, 64, 32, 16, 256, 1, 32, 512, 0, 16, bias, 0, act, None, 0, 8192, 16, 1024, 1, 16, 0, 0, None, 0, ws, 1 << 20)
     assert fwd(ws=None) == _lib.NL_EINVAL and fwd(ws=4104) == _lib.NL_EALIGN
     bwd = lambda act=2, u=512, wsb=1 << 20, db=2048: lib.nl_linear_fp8_fused_bwd(  # noqa: E731
-        None, 64, 32, 16, 256, 1, 16, u, 16, act, db, 4096, 1 << 20, 1, 0, 1024, 1, 32, None, 0, 0, 8192, wsb)
+        None, 64, 32, 16, 256, 1, 16, u, 16, act, db, 0, 4096, 1 << 20, 1, 0, 1024, 1, 32, None, 0, 0, 8192, wsb)
     assert bwd(act=7) == bwd(u=None) == bwd(wsb=64) == _lib.NL_EINVAL
     assert bwd(db=2050) == _lib.NL_EALIGN
 
