@@ -349,8 +349,9 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsBwdAr
   }
 }
 
-// out (+)= the sum of P partial rows (of dgamma, of a bias gradient), in a fixed order: a workgroup takes 16 columns, thread (ph, q) the
-// rows ph, ph + 256, ... of columns 4q .. 4q+3; then the 16 phases of a wave, then the 16 waves.
+// out (+)= the sum of P partial rows (of dgamma, of a bias gradient), in a fixed order: a workgroup
+// takes 16 columns, thread (ph, q) the rows ph, ph + 256, ... of columns 4q .. 4q+3; then the 16
+// phases of a wave, then the 16 waves.
 __global__ __launch_bounds__(1024) void row_sums_kernel(int P, int D, const float* __restrict__ part,
                                                        void* __restrict__ out, int bf16, int accumulate) {
   __shared__ float sums[16][17];
@@ -410,7 +411,7 @@ int bwd_blocks(int rows, int D) {
   // the partial rows) with 1024, 512 and 256 workgroups: 16384 x 512 bf16 10.9 + 4.3, 12.0 + 4.0,
   // 15.6 + 3.9; 16384 x 4096 92 + 7, 83 + 5, 110 + 5; 2048 x 8192 39 + 11, 28 + 7, 27 + 4.
   const int rpb = rows_per_block(D);
-  return std::min((rows + rpb - 1) / rpb, D <= 512 ? kBwdBlocks : D <= 4096 ? 512 : 256);
+  return std::min((rows - 1) / rpb + 1, D <= 512 ? kBwdBlocks : D <= 4096 ? 512 : 256);
 }
 
 int check_rows(const char* what, int rows, int D, int dtype) {
@@ -521,6 +522,7 @@ extern "C" int nl_rms_norm_bwd(void* stream, int rows, int D, int dtype, const v
     if ((uintptr_t)ws & 15) return nl_set_error(NL_EALIGN, "nl_rms_norm_bwd: workspace not 16-byte aligned");
   }
   if (dgamma && ((uintptr_t)dgamma & 3)) return nl_set_error(NL_EALIGN, "nl_rms_norm_bwd: dgamma is not aligned");
+  if (rows == 0 && (!dgamma || accumulate)) return NL_OK;
   const int blocks = rows > 0 ? bwd_blocks(rows, D) : 0;
   const hipStream_t st = (hipStream_t)stream;
   if (rows > 0) {
@@ -532,7 +534,7 @@ extern "C" int nl_rms_norm_bwd(void* stream, int rows, int D, int dtype, const v
       else hipLaunchKernelGGL((rms_bwd_kernel<float, TPR, VPL>), grid, block, 0, st, a);
     });
   }
-  if (dgamma && (rows > 0 || !accumulate)) 
+  if (dgamma)
     launch_partial_sums(st, blocks, D, (const float*)ws, dgamma, NL_DTYPE_F32, accumulate);
   return nl_check_launch(what);
 }

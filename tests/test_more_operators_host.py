@@ -25,6 +25,7 @@ def test_rms_norm_refusals_of_the_library():
     assert bwd(dy=257) == bwd(ws=4104) == bwd(dg=1026) == _lib.NL_EALIGN
     assert lib.nl_rms_norm_bwd_ws_bytes(4, 16) >= 64 and lib.nl_rms_norm_bwd_ws_bytes(0, 16) == 0
     assert lib.nl_rms_norm_bwd_ws_bytes(1 << 30, 16384) <= 1 << 26
+    assert lib.nl_rms_norm_bwd_ws_bytes((1 << 31) - 1, 1) == lib.nl_rms_norm_bwd_ws_bytes(1 << 20, 1) > 0
 
 
 def test_rms_norm_refusals_in_python():

@@ -318,3 +318,27 @@ def test_norm_in_8_bits_of_rows_that_are_not_finite(dev):
     np.testing.assert_allclose(v[0], 1.0, rtol=2.0 ** -4)
     assert np.isnan(v[1, 5]) and (np.delete(v[1], 5) == 0).all()
     assert np.isnan(v[2]).all() and (v[3] == 0).all()
+
+
+@pytest.mark.parametrize("rows,cols", [(0, 40), (1, 7), (300, 129), (90, 5000)])
+def test_gradient_added_to_what_is_there(dev, rows, cols):
+    """The library's accumulate: dgamma + what it held, by one addition."""
+    import torch
+    from nlearn_amd import _lib
+
+    g = torch.Generator(device=dev).manual_seed(rows + cols)
+    x, dy = (torch.randn((rows, cols), generator=g, device=dev) for _ in range(2))
+    gamma, held = (torch.randn((cols,), generator=g, device=dev) for _ in range(2))
+    rstd = torch.rand((rows,), generator=g, device=dev) + 0.5
+    wsb = _lib.load().nl_rms_norm_bwd_ws_bytes(rows, cols)
+    ws = torch.empty(max(wsb, 16), dtype=torch.uint8, device=dev)
+    got = []
+    for acc in (0, 1):
+        dx, dg = torch.empty_like(x), held.clone()
+        _lib.call_on(gamma, "nl_rms_norm_bwd", rows, cols, 0, dy.data_ptr(), cols, x.data_ptr(), cols, rstd.data_ptr(),
+                     gamma.data_ptr(), None, 0, dx.data_ptr(), cols, dg.data_ptr(), acc, ws.data_ptr(), wsb)
+        got.append((dx, dg))
+    assert torch.equal(got[0][0], got[1][0])
+    assert torch.equal(got[1][1], held + got[0][1])
+    if rows == 0:
+        assert (got[0][1] == 0).all()
