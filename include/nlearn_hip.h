@@ -537,7 +537,8 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
  * of 128, bytes past N zero; scale_c rows ldsc apart; no aux, no round_u). residual, aux: 16-byte
  * aligned, rows a multiple of 8 elements apart. Every row of residual, aux and (fp32, bf16) C, the
  * last one too, holds N rounded up to 8 elements: those past N are read, and overwritten in aux
- * and C. residual may be C (the same address and stride); no other overlap. K == 0: the product is 0. Workspace as nl_gemm_fp8. */
+ * and C. residual may be C (the same address and stride); no other overlap. K == 0: the product
+ * is 0. Workspace as nl_gemm_fp8. */
 #define NL_ACT_NONE 0
 #define NL_ACT_RELU 1
 #define NL_ACT_GELU 2
@@ -554,7 +555,7 @@ int nl_gemm_fp8_fused(void* stream, int M, int N, int K,
  *   q, scale; qt, scale_t:  d and its transpose as nl_quantize_fp8 gives them with group 1 (NULL: not wanted)
  *   dbias[c] = sum_rows d   (fp32 or bf16; NULL: not wanted), summed in fp32 in a fixed order over a
  *                           workspace of nl_quantize_fp8_dact_ws_bytes() bytes (4-byte aligned)
- * relu'(0) is 0; a NaN in u gives NaN. */
+ * relu gives dy where u > 0 and 0 elsewhere, whatever dy is; a NaN in u gives NaN. */
 size_t nl_quantize_fp8_dact_ws_bytes(int64_t rows, int64_t cols);
 int nl_quantize_fp8_dact(void* stream, int64_t rows, int64_t cols, const void* dy, int dtype, int64_t lddy,
                          const void* u, int64_t ldu, int act, uint8_t* q, int64_t ldq, uint8_t* scale, int64_t lds,

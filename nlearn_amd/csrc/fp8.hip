@@ -52,25 +52,21 @@ struct QuantArgs {
   float* part = nullptr;    // column sums of each 128 rows, [ceil(rows / 128)][cols] (may be null)
 };
 
-// v *= act'(u); NaN stays NaN
-template <typename G>
-__device__ __forceinline__ void scale_by(float (&v)[8], const float (&u)[8], G grad) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) v[k] *= u[k] == u[k] ? grad(u[k]) : u[k];
-}
+// v *= act'(u); a u that is NaN gives NaN, and relu passes or drops v whatever it is
 template <typename T, int R>
 __device__ __forceinline__ void scale_by_act_grad(float (&v)[R][8], const Vec<T> (&u)[R], int act) {
-  auto rows = [&](auto grad) __attribute__((always_inline)) {
+  auto each = [&](auto scaled) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       float f[8];
       unpack(u[i], f);
-      scale_by(v[i], f, grad);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) v[i][k] = scaled(v[i][k], f[k]);
     }
   };
-  if (act == NL_ACT_GELU) rows([](float x) { return gelu_tanh_grad(x); });
-  else if (act == NL_ACT_SILU) rows([](float x) { return silu_grad(x); });
-  else rows([](float x) { return x > 0.f ? 1.f : 0.f; });
+  if (act == NL_ACT_GELU) each([](float g, float x) { return g * (x == x ? gelu_tanh_grad(x) : x); });
+  else if (act == NL_ACT_SILU) each([](float g, float x) { return g * (x == x ? silu_grad(x) : x); });
+  else each([](float g, float x) { return x > 0.f ? g : x == x ? 0.f : x; });
 }
 
 // x[row][c0 .. c0+7] as floats, zero past the last column

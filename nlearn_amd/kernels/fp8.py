@@ -627,7 +627,7 @@ def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation:
         if not fused:
             y = _LinearFp8.apply(x2, W, grads and x2.requires_grad, grads and W.requires_grad)
     if fused:
-        res2 = None if residual is None else residual if x.dim() == 2 else residual.reshape(-1, N)
+        res2 = None if residual is None else residual if x.dim() == 2 else residual.reshape(x2.shape[0], N)
         need = tuple(grads and t is not None and t.requires_grad for t in (x2, None if frozen else W, bias, res2))
         y = _LinearFp8Fused.apply(x2, None if frozen else W, bias, res2, frozen, act, need)
     return y if x.dim() == 2 else y.reshape(*lead, N)

@@ -435,3 +435,43 @@ def test_bias_gradient_against_differences(dev):
             # |act'''| < 3 for both: h^2 / 2 each; a value's roundings (80 u of |y| + 1) over 2 h
             bound = dy.double().abs().sum(0) * (0.5 * h * h) + (dy.double().abs() * (y.double().abs() + 1)).sum(0) * 80 * U / h
         assert ((db.double() - slope).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+def test_relu_drops_gradients_that_are_not_finite(dev, dtype):
+    """Behind relu an output gradient counts where u > 0 and nowhere else, infinities and NaN among them."""
+    import torch
+    from nlearn_amd import _lib
+
+    dt = getattr(torch, dtype)
+    u = torch.tensor([[-1.0, 0.0, 2.0, -0.0, 3.0, float("-inf"), float("inf"), float("nan")]], device=dev)
+    u = u.repeat(130, 20).to(dt)
+    dy = torch.ones_like(u)
+    dy[:, 0::8], dy[:, 1::8], dy[:, 5::8] = float("inf"), float("nan"), float("-inf")
+    rows, cols = u.shape
+    from nlearn_amd.kernels.fp8 import Fp8Blocks
+
+    want = torch.where(u > 0, dy, torch.zeros_like(dy))
+    want[:, 7::8] = float("nan")
+    q, t = Fp8Blocks.empty(rows, cols, 1, dev), Fp8Blocks.empty(cols, rows, 1, dev)
+    only = Fp8Blocks.empty(rows, cols, 1, dev)
+    db = torch.empty(cols, device=dev)
+    wsb = _lib.load().nl_quantize_fp8_dact_ws_bytes(rows, cols)
+    ws = torch.empty(wsb, dtype=torch.uint8, device=dev)
+    args = [dy.data_ptr(), 0 if dt is torch.float32 else 1, cols, u.data_ptr(), cols, 1]
+    _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *q._abi(), *t._abi(), db.data_ptr(), 0, ws.data_ptr(), wsb)
+    _lib.call_on(dy, "nl_quantize_fp8_dact", rows, cols, *args, *only._abi(), None, 0, None, 0, None, 0, None, 0)
+    for got in (q.dequantize(), t.dequantize().T, only.dequantize()):
+        torch.testing.assert_close(got, want.float(), rtol=0, atol=0, equal_nan=True)
+    torch.testing.assert_close(db, want.float().sum(0), rtol=0, atol=0, equal_nan=True)
+
+
+def test_layer_without_outputs(dev):
+    import torch
+    from nlearn_amd.kernels.fp8 import linear_fp8
+
+    x = torch.ones((2, 3, 8), device=dev, requires_grad=True)
+    y = linear_fp8(x, torch.zeros((8, 0), device=dev), residual=torch.zeros((2, 3, 0), device=dev))
+    assert y.shape == (2, 3, 0)
+    y.sum().backward()
+    assert (x.grad == 0).all()
