@@ -531,7 +531,8 @@ int nl_gemm_fp8(void* stream, int M, int N, int K,
  *   C = act(u) + residual      (residual NULL: none)
  * act: gelu is the tanh form of nl_gemm_fused, silu u * sigmoid(u); NaN stays NaN.
  * round_u: u is rounded to the type of C before act, as what a backward pass keeps; aux (the type
- * of C, may be NULL): that u is written there (implies round_u). residual: the type of C (bf16 for
+ * of C, may be NULL): that u is written there (implies round_u). With round_u relu's u is summed as
+ * an fp32 result is, whatever the type of C: its sign decides what a gradient passes. residual: the type of C (bf16 for
  * C in 8 bits). C: fp32 or bf16, summed as nl_gemm_fp8 sums them; or NL_DTYPE_E4M3, summed as bf16
  * is and quantised along N as nl_quantize_fp8 does it with group 1 (ldc bytes a row, whole blocks
  * of 128, bytes past N zero; scale_c rows ldsc apart; no aux, no round_u). residual, aux: 16-byte

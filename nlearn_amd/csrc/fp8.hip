@@ -57,7 +57,7 @@ __device__ __forceinline__ float clamp_nan(float x, float c) {
   return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -c), c);
 }
 // The derivatives of gelu_tanh and silu from s (common.h), with u (1 - s) q multiplied out:
-// s + s (1 - s) u q, s (1 - s) = s - s^2 by one fma. 14 instructions an element for 19: a layer's gradient
+// s + s (1 - s) u q, s (1 - s) = s - s^2 by one fma.
 __device__ __forceinline__ float gelu_grad_of(float u) {
   const float s = __builtin_amdgcn_rcpf(gelu_sigmoid_arg(u));
   return __builtin_fmaf(__builtin_fmaf(-s, s, s), u * __builtin_fmaf(kGeluD2, u * u, kGeluD1), s);
@@ -312,7 +312,10 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   }
 }
 
-// (128 registers with an activation: two workgroups a CU; 138 were 71 us for 16384 x 2048 with gelu, 128 are 48)
+// With an activation 16384 x 2048 bf16 takes 48 us (gelu; relu 47, none 32), 52 with the column sums
+// and their own launch: 201 MB at the rate of the tile without one. 128 registers are two workgroups a
+// CU; with 138, one, it took 71, and held to 80, three, it spills (91). Stores past the caches gained 3
+// of the 32 here and lost 10 us in the layer, whose products read them next.
 template <typename T, bool kAct = false>
 __global__ __launch_bounds__(512, kAct ? 4 : 2) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
   __shared__ __attribute__((aligned(16))) QuantTile sm;
@@ -392,6 +395,14 @@ struct GemmF8Args {
 
 // Epilogues of a product: none; u = acc + bias, C = act(u); that with u rounded to the type of C
 // before, and kept where it is asked for (what a backward pass reads); each with a residual.
+// All of it is done in the lanes as the matrix unit leaves the sums, and only what is stored passes
+// the slab: bias and activation on rows read back from an fp32 slab took 39 us to bf16 and 51 to 8
+// bits for 16384 x 2048 x 512 with gelu. Measured (us; without an epilogue 27): bias to bf16 27, with
+// gelu 34, with u kept 39 (two results of 67 MB), a residual 36; to 8 bits 27, with gelu 33; to fp32
+// with gelu 50 (without an epilogue 46). 8192^3: 403 without, silu or gelu to bf16 410, to 8 bits
+// 424, a residual 430 to 444. With K = 512 a tile's sums take as long as its epilogue (gelu: 13
+// vector instructions an element to 8 bits, about 15 us of the chip's issue beside 13 us of the
+// matrix units), and two workgroups a CU hide half of that; starting them half a tile apart changed nothing.
 enum { kPlain = 0, kEpi = 1, kEpiKeep = 2, kEpiRes = 3, kEpiResKeep = 4 };
 constexpr bool keeps(int epi) { return epi == kEpiKeep || epi == kEpiResKeep; }
 
@@ -535,8 +546,9 @@ __device__ __forceinline__ void activate(float (&v)[N], int act) {
 }
 
 // kDw: scale rows are whole, aligned dwords. Else a scale dword is four byte loads.
-// OutT: float, uint16_t (bf16) or, with an epilogue, uint8_t (e4m3 with its scales).
-template <int BM, int BN, int WTM, int WTN, typename OutT, bool kDw, int EPI = kPlain>
+// OutT: float, uint16_t (bf16) or, with an epilogue, uint8_t (e4m3 with its scales). kWide: widened
+// to bf16 for fp32 sums.
+template <int BM, int BN, int WTM, int WTN, typename OutT, bool kDw, int EPI = kPlain, bool kWide = sizeof(OutT) == 4>
 __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 1 : 2) void gemm_f8_kernel(
     GemmF8Args g) {
   constexpr int WNW = BN / WTN, NWV = (BM / WTM) * WNW;
@@ -544,7 +556,6 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
   constexpr int STAGE = (BM + BN) * kB;
   constexpr int IA = BM / 8 / NWV, IB = BN / 8 / NWV;  // DMA instructions (8 rows each) per wave and stage
   static_assert(IA * 8 * NWV == BM && IB * 8 * NWV == BN, "a stage splits into whole DMA instructions");
-  constexpr bool kWide = sizeof(OutT) == 4;            // widened to bf16 for fp32 sums
   constexpr int NS = kWide ? 4 : 2;                    // fragment steps of a stage: 16 or 32 bytes of k a lane
   constexpr int CH = kWide ? 1 : 2;                    // 16-byte chunks of a fragment
   // bytes of a slab row: WTN bf16 or half as many fp32
@@ -1337,11 +1348,11 @@ F8Plan f8_plan(int M, int N, int K) {
 
 int64_t f8_ldw(int N) { return ((int64_t)N + 3) / 4 * 4; }
 
-template <int BM, int BN, int WTM, int WTN, typename OutT, int EPI>
+template <int BM, int BN, int WTM, int WTN, typename OutT, int EPI, bool kWide = sizeof(OutT) == 4>
 void launch_tiles(hipStream_t st, const GemmF8Args& g) {
   const dim3 grid((unsigned)std::min(g.items, (BM * BN >= 65536 ? 1 : 2) * cu_count()));
-  if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, true, EPI>), grid, dim3(256), 0, st, g);
-  else hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, false, EPI>), grid, dim3(256), 0, st, g);
+  if (g.dw) hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, true, EPI, kWide>), grid, dim3(256), 0, st, g);
+  else hipLaunchKernelGGL((gemm_f8_kernel<BM, BN, WTM, WTN, OutT, false, EPI, kWide>), grid, dim3(256), 0, st, g);
 }
 
 template <typename OutT>
@@ -1354,21 +1365,21 @@ void launch_f8(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
                        dim3(256), 0, st, g, p.splits);
 }
 
-template <typename OutT, int EPI>
+template <typename OutT, int EPI, bool kWide = sizeof(OutT) == 4>
 void launch_f8_epi(hipStream_t st, const F8Plan& p, const GemmF8Args& g) {
   if (p.splits > 1) {
     // partials as the same result without an epilogue has them
-    using PT = typename std::conditional<sizeof(OutT) == 4, float, uint16_t>::type;
+    using PT = typename std::conditional<kWide, float, uint16_t>::type;
     launch_tiles<128, 128, 64, 64, PT, kPlain>(st, g);
     hipLaunchKernelGGL((f8_reduce_epi_kernel<OutT, keeps(EPI) ? kEpiKeep : kEpi>),
                        dim3((unsigned)((g.N + 255) / 256), (unsigned)std::min<int64_t>(((int64_t)g.M + 3) / 4, 65535)),
                        dim3(256), 0, st, g, p.splits);
   } else if (p.huge) {
-    launch_tiles<256, 256, 128, 128, OutT, EPI>(st, g);
+    launch_tiles<256, 256, 128, 128, OutT, EPI, kWide>(st, g);
   } else if constexpr (sizeof(OutT) == 1) {
     launch_tiles<128, 128, 32, 128, OutT, EPI>(st, g);
   } else {
-    launch_tiles<128, 128, 64, 64, OutT, EPI>(st, g);
+    launch_tiles<128, 128, 64, 64, OutT, EPI, kWide>(st, g);
   }
 }
 
@@ -1607,6 +1618,11 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
   if (lda > kMaxLd || ldb > kMaxLd || ldsa > kMaxLd || ldsb > kMaxLd)
     return nl_set_error(NL_EUNSUPPORTED, "gemm_fp8: rows of 8 MiB and more");
   F8Plan p = f8_plan(M, N, K);
+  // relu in front of a backward pass: the sign of u decides whether a gradient passes, and sums cut at
+  // 2^-13 of a product had it wrong for one u in 100000 (an error of 0.6% in dx): fp32 sums, whatever
+  // the result's type. That costs a layer's forward (us, with its quantisers) 60 for 52 with gelu's sums
+  // at 16384 x 512 x 2048, 142 for 92 at 4096^3; with 256 x 256 tiles 66 and 144.
+  const bool fine = c_dtype == NL_DTYPE_F32 || (e.kind == kEpiKeep && e.act == NL_ACT_RELU);
   // 128 x 128 tiles, two workgroups a CU, where the epilogue of one runs beside the other's walk over a
   // short K, although each operand is read twice as often. Measured (us, against 256 x 256): C in 8 bits
   // with gelu 16384 x 2048 x 512 33.2 and 39.2, 16384 x 8192 x 1024 169 and 183, 16384 x 2048 x 2048 72.5
@@ -1646,7 +1662,8 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
     if (e.aux) e.res ? launch_f8_epi<float, kEpiResKeep>(st, p, g) : launch_f8_epi<float, kEpiKeep>(st, p, g);
     else e.res ? launch_f8_epi<float, kEpiRes>(st, p, g) : launch_f8_epi<float, kEpi>(st, p, g);
   } else {
-    if (e.kind == kEpiKeep) e.res ? launch_f8_epi<uint16_t, kEpiResKeep>(st, p, g) : launch_f8_epi<uint16_t, kEpiKeep>(st, p, g);
+    if (fine) e.res ? launch_f8_epi<uint16_t, kEpiResKeep, true>(st, p, g) : launch_f8_epi<uint16_t, kEpiKeep, true>(st, p, g);
+    else if (e.kind == kEpiKeep) e.res ? launch_f8_epi<uint16_t, kEpiResKeep>(st, p, g) : launch_f8_epi<uint16_t, kEpiKeep>(st, p, g);
     else e.res ? launch_f8_epi<uint16_t, kEpiRes>(st, p, g) : launch_f8_epi<uint16_t, kEpi>(st, p, g);
   }
   return nl_check_launch("nl_gemm_fp8");

@@ -11,9 +11,15 @@
 //
 // A row is read once and kept in registers, 8 columns a lane and vector, by 16
 // lanes up to 128 columns, a wave up to 2048, 256 threads up to 8192 and 512 up to
-// 16384. All of it is bound by HBM where there are many rows, and by the chain load
-// -> sum -> store where there are few. Vectors are loaded and stored at whatever
-// alignment the rows have (the hardware takes any multiple of the element).
+// 16384 (1024 threads of two vectors spilled registers). Vectors are loaded and stored
+// at whatever alignment the rows have (the hardware takes any multiple of the element).
+// Bound by HBM where there are many rows: with the residual 16384 x 512 bf16 12.0 us
+// (67 MB, 5.6 TB/s; a large copy reaches 5.1), its gradients 10.9 us (67 MB) and 4.3 us
+// for the sum of dgamma's partial rows; 16384 x 2048 bf16 to 8 bits 45 us (235 MB, 5.2
+// TB/s). By the chain load -> sum -> store where there are few: one row of 512 1.8 us,
+// 8 rows of 2048 to 8 bits 4.8 us, 777 x 1001 fp32 4.3 us and 5.7 + 3.5 us. A backward in
+// one launch for few rows, each workgroup summing dgamma of its own columns over all rows,
+// took 17 us there.
 #include <type_traits>
 
 #include "fp8.h"

@@ -581,7 +581,8 @@ def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation:
 
     bias (N,) fp32 or bf16, activation "relu", "gelu" (tanh form) or "silu", residual [..., N] in x's
     dtype: in the product's epilogue. With an activation u = x W + bias is rounded to x's dtype before
-    it, as ``ffn`` does it: that u is kept for the backward, which quantises dY act'(u)."""
+    it, as ``ffn`` does it: that u is kept for the backward, which quantises dY act'(u). In front of relu u is
+    summed in fp32 whatever x's dtype (scale bytes 3 to 246): its sign decides what a gradient passes."""
     if x.dim() < 2:
         raise ValueError("linear_fp8: x needs >= 2 dims")
     frozen = W if isinstance(W, Fp8Weight) else None

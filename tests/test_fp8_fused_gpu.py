@@ -475,3 +475,29 @@ def test_layer_without_outputs(dev):
     assert y.shape == (2, 3, 0)
     y.sum().backward()
     assert (x.grad == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(3, 20, 16), (200, 136, 24), (300, 300, 260), (40, 500, 2100), (4096, 4100, 130)])
+def test_relu_passes_gradients_where_the_exact_sum_is_positive(dev, M, N, K, dtype):
+    """Products of 2^16 that cancel beside small ones: the sum is a small whole number (every partial sum is one below
+    2^24, exact in fp32 in any order), and its sign decides whether a gradient passes."""
+    import torch
+    from nlearn_amd.kernels.fp8 import fp8_weight, linear_fp8
+
+    g = torch.Generator(device=dev).manual_seed(M + N)
+    x = torch.randint(-2, 3, (M, K), generator=g, device=dev).float()
+    W = torch.randint(-1, 2, (K, N), generator=g, device=dev).float()
+    for k in range(0, K - 1, 16):
+        x[:, k] = x[:, k + 1] = 256
+        W[k], W[k + 1] = 256, -256
+    u = (x.double() @ W.double()).float()
+    assert u.abs().max() <= 256  # whole numbers in bf16
+    x = x.to(getattr(torch, dtype))
+    bias = torch.zeros((N,), device=dev).requires_grad_(True)
+    for weight in (W, fp8_weight(W)):
+        for res in (None, torch.ones((M, N), device=dev, dtype=x.dtype)):
+            y = linear_fp8(x, weight, bias=bias, activation="relu", residual=res)
+            assert torch.equal(y.float(), u.clamp(min=0) + (0 if res is None else 1))
+            (db,) = torch.autograd.grad(y, bias, torch.ones_like(y))
+            assert torch.equal(db, (u > 0).float().sum(0))
