@@ -80,15 +80,9 @@ __device__ __forceinline__ float gelu_tanh_grad(float u) {
   return s * __builtin_fmaf(u * (1.f - s), q, 1.f);
 }
 
-// u * sigmoid(u) and its derivative s (1 + u (1 - s)), s = 1 / (1 + 2^(-u log2(e))); the derivative
-// clamps |u| <= 120, beyond which it is below 2^-166 or 1
+// u * sigmoid(u), sigmoid(u) = 1 / (1 + 2^(-u log2(e)))
 __device__ __forceinline__ float silu(float u) {
-  return u * __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.4426950408889634f * u));
-}
-__device__ __forceinline__ float silu_grad(float u) {
-  u = fminf(fmaxf(u, -120.f), 120.f);
-  const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.4426950408889634f * u));
-  return s * __builtin_fmaf(u, 1.f - s, 1.f);
+  return u * __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * u));
 }
 
 // ---------------------------------------------------------------------------

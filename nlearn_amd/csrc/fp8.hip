@@ -56,14 +56,14 @@ struct QuantArgs {
 __device__ __forceinline__ float clamp_nan(float x, float c) {
   return __builtin_elementwise_minimum(__builtin_elementwise_maximum(x, -c), c);
 }
-// The derivatives of gelu_tanh and silu from s (common.h), with u (1 - s) q multiplied out:
-// s + s (1 - s) u q, s (1 - s) = s - s^2 by one fma.
+// The derivatives of gelu_tanh and silu from their sigmoid s (common.h), s + s (1 - s) u q with s (1 - s) =
+// s - s^2 by one fma (q = 1 of silu, which beyond |u| = 120 is below 2^-166 or 1).
 __device__ __forceinline__ float gelu_grad_of(float u) {
   const float s = __builtin_amdgcn_rcpf(gelu_sigmoid_arg(u));
   return __builtin_fmaf(__builtin_fmaf(-s, s, s), u * __builtin_fmaf(kGeluD2, u * u, kGeluD1), s);
 }
 __device__ __forceinline__ float silu_grad_of(float u) {
-  const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-1.4426950408889634f * u));
+  const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * u));
   return __builtin_fmaf(__builtin_fmaf(-s, s, s), u, s);
 }
 // v *= act'(u); a u that is NaN gives NaN, and relu passes or drops v whatever it is
