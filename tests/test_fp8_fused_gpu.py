@@ -501,3 +501,71 @@ def test_relu_passes_gradients_where_the_exact_sum_is_positive(dev, M, N, K, dty
             assert torch.equal(y.float(), u.clamp(min=0) + (0 if res is None else 1))
             (db,) = torch.autograd.grad(y, bias, torch.ones_like(y))
             assert torch.equal(db, (u > 0).float().sum(0))
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("M,N,K", [(4096, 4100, 24), (4200, 4096, 2200)])
+def test_relu_on_large_tiles(dev, M, N, K, dtype):
+    """The same with u kept and not, with a residual and without: whole numbers, exact in fp32, on 256 x 256 tiles too."""
+    import torch
+    from nlearn_amd.kernels.fp8 import fp8_weight, linear_fp8
+
+    g = torch.Generator(device=dev).manual_seed(M + N)
+    x = torch.randint(-2, 3, (M, K), generator=g, device=dev).float()
+    W = torch.randint(-1, 2, (K, N), generator=g, device=dev).float()
+    W *= torch.rand((K, N), generator=g, device=dev) < 0.1
+    for k in range(0, K - 1, 16):
+        x[:, k] = x[:, k + 1] = 256
+        W[k], W[k + 1] = 256, -256
+    u = (x.double() @ W.double()).float()
+    assert u.abs().max() <= 255  # whole numbers in bf16, with the residual too
+    x = x.to(getattr(torch, dtype))
+    bias = torch.zeros((N,), device=dev)
+    for res in (None, torch.ones((M, N), device=dev, dtype=x.dtype)):
+        want = u.clamp(min=0) + (0 if res is None else 1)
+        for weight in (W, fp8_weight(W)):
+            assert torch.equal(linear_fp8(x, weight, bias=bias, activation="relu", residual=res).float(), want)
+            leaf = bias.clone().requires_grad_(True)
+            y = linear_fp8(x, weight, bias=leaf, activation="relu", residual=res)
+            assert torch.equal(y.float(), want)
+            (db,) = torch.autograd.grad(y, leaf, torch.ones_like(y))
+            assert torch.equal(db, (u > 0).float().sum(0))
+
+
+@pytest.mark.parametrize("M,N,K", [(1, 300, 300), (130, 260, 77), (64, 512, 4000), (300, 133, 700), (4096, 4100, 300)])
+def test_scale_rows_of_any_length(dev, M, N, K):
+    """Scales whose rows are no whole dwords: the bits that padded ones give, in every form of the epilogue."""
+    import torch
+    from nlearn_amd.kernels.fp8 import Fp8Blocks, Fp8Weight, fp8_weight, gemm_fp8, linear_fp8
+
+    def compact(b):
+        kb = b.scale.shape[1]
+        rows = torch.empty((b.scale.shape[0], kb + 1 - kb % 2), dtype=torch.uint8, device=dev)  # an odd stride
+        rows[:, :kb] = b.scale.contiguous().view(torch.uint8)
+        return Fp8Blocks(b.q, rows.view(torch.float8_e8m0fnu)[:, :kb], b.shape, b.group)
+
+    rng = _rng(M, N, K, 9)
+    a, _ = _blocks(rng, M, K, 1, dev)
+    b, _ = _blocks(rng, N, K, 1, dev)
+    odd = compact(a), compact(b)
+    assert odd[0].scale.stride(0) % 2 == 1 or M == 1
+    bias = torch.from_numpy(rng.standard_normal(N).astype(np.float32)).to(dev)
+    bytes_ = lambda t: t if torch.is_tensor(t) else torch.cat([t.q.view(torch.uint8).flatten(),  # noqa: E731
+                                                               t.scale.contiguous().view(torch.uint8).flatten()])
+    for dt in (torch.bfloat16, torch.float32, torch.float8_e4m3fn):
+        rt = torch.bfloat16 if dt is torch.float8_e4m3fn else dt
+        res = torch.from_numpy(rng.standard_normal((M, N)).astype(np.float32)).to(dev).to(rt)
+        for r in (None, res):
+            want, got = (gemm_fp8(*ab, out_dtype=dt, bias=bias, activation="gelu", residual=r) for ab in ((a, b), odd))
+            assert torch.equal(bytes_(want), bytes_(got)), (dt, r is None)
+    # a frozen weight's, with u kept
+    W = torch.from_numpy(rng.standard_normal((K, N)).astype(np.float32) / K ** 0.5).to(dev)
+    f = fp8_weight(W)
+    f2 = Fp8Weight(compact(f.fwd), compact(f.bwd))
+    for dt in (torch.bfloat16, torch.float32):
+        x = torch.from_numpy(rng.standard_normal((M, K)).astype(np.float32)).to(dev).to(dt).requires_grad_(True)
+        for name in ("gelu", "relu"):
+            for r in (None, torch.ones((M, N), device=dev, dtype=dt)):
+                y, y2 = (linear_fp8(x, w, bias=bias, activation=name, residual=r) for w in (f, f2))
+                assert torch.equal(y, y2)
+                assert torch.equal(*(torch.autograd.grad(v, x, torch.ones_like(v))[0] for v in (y, y2)))
