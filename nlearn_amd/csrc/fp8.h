@@ -24,14 +24,16 @@ __device__ __forceinline__ int scale_byte(uint32_t amax) {
   return amax == 0 ? 127 : (b > 0 ? b : 0);
 }
 
-// 2^-e, e in [-127, 120]: always a normal number, so the product with it is exact
-// wherever e4m3 keeps anything of it.
-__device__ __forceinline__ float inv_scale(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
-
-// Four scaled values to four e4m3 bytes (an infinity or a NaN gives NaN).
-__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d) {
-  int r = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, r, true);
+// Four values divided by 2^(byte - 127) to four e4m3 bytes (an infinity or a NaN gives NaN). The
+// conversion reads the scale from a float's exponent, 0 being 2^-127 (the same bytes as x * 2^-e
+// converted, for every byte up to 253 and subnormal x), and rounds once.
+__device__ __forceinline__ uint32_t pack_e4m3x4(float a, float b, float c, float d, int byte) {
+  typedef short s16x2 __attribute__((ext_vector_type(2)));
+  const float scale = __uint_as_float((uint32_t)byte << 23);
+  s16x2 r = {0, 0};
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, a, b, scale, false);
+  r = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(r, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, r);
 }
 
 template <int CTRL>

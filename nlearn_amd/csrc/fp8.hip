@@ -150,10 +150,8 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
     for (int i = 0; i < 8; ++i) m = max(m, finite_abs_bits(v[i]));
   }
   const int byte = scale_byte(max16(m));
-  const float inv = inv_scale(byte);
   *reinterpret_cast<u32x2*>(a.q + (int64_t)row * a.ldq + c0) =
-      u32x2{pack_e4m3x4(v[0] * inv, v[1] * inv, v[2] * inv, v[3] * inv),
-            pack_e4m3x4(v[4] * inv, v[5] * inv, v[6] * inv, v[7] * inv)};
+      u32x2{pack_e4m3x4(v[0], v[1], v[2], v[3], byte), pack_e4m3x4(v[4], v[5], v[6], v[7], byte)};
   if (l == 0) a.s[(int64_t)row * a.lds + b] = (uint8_t)byte;
 }
 
@@ -280,11 +278,9 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
       const int64_t r = r0 + g * 4 + i;
       const int byte = a.group != 1 ? one : scale_byte(max16(rm[i]));
       if (r >= a.rows) continue;
-      const float inv = inv_scale(byte);
       const float* w = v[i];
       *reinterpret_cast<u32x2*>(a.q + r * a.ldq + cl) =
-          u32x2{pack_e4m3x4(w[0] * inv, w[1] * inv, w[2] * inv, w[3] * inv),
-                pack_e4m3x4(w[4] * inv, w[5] * inv, w[6] * inv, w[7] * inv)};
+          u32x2{pack_e4m3x4(w[0], w[1], w[2], w[3], byte), pack_e4m3x4(w[4], w[5], w[6], w[7], byte)};
       if (l == 0 && a.group == 1) a.s[r * a.lds + bx] = (uint8_t)byte;
     }
     if (a.group != 1 && tid == 0) a.s[(int64_t)by * a.lds + bx] = (uint8_t)one;
@@ -293,8 +289,8 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
     const int c = l * 8 + j;
-    const float inv = inv_scale(a.group != 1 ? one : colbyte[c]);
-    tile[c * 32 + (g ^ ((l & 7) << 2))] = pack_e4m3x4(v[0][j] * inv, v[1][j] * inv, v[2][j] * inv, v[3][j] * inv);
+    tile[c * 32 + (g ^ ((l & 7) << 2))] =
+        pack_e4m3x4(v[0][j], v[1][j], v[2][j], v[3][j], a.group != 1 ? one : colbyte[c]);
   }
   __syncthreads();
   // 8 lanes write a column's 128 bytes, 16 a lane
@@ -902,13 +898,12 @@ __global__ __launch_bounds__((BM / WTM) * (BN / WTN) * 64, (BM * BN >= 65536) ? 
         const auto r32 = __builtin_amdgcn_permlane32_swap(m, m, false, false);
         m = max((uint32_t)r32[0], (uint32_t)r32[1]);
         const int byte = scale_byte(m);
-        const float inv = inv_scale(byte);
 #pragma unroll
         for (int j = 0; j < FN; ++j)
 #pragma unroll
           for (int q = 0; q < 4; ++q)
             *reinterpret_cast<uint32_t*>(wl + fr * 128 + (((2 * j + (q >> 1)) ^ (fr & 7)) << 4) + (q & 1) * 8 + g4) =
-                pack_e4m3x4(v[j][4 * q] * inv, v[j][4 * q + 1] * inv, v[j][4 * q + 2] * inv, v[j][4 * q + 3] * inv);
+                pack_e4m3x4(v[j][4 * q], v[j][4 * q + 1], v[j][4 * q + 2], v[j][4 * q + 3], byte);
         if (ln < 32 && row < rows && there) g.sc[(int64_t)(cur.m0 + row) * g.ldsc + n / kB] = (uint8_t)byte;
 #pragma unroll
         for (int it = 0; it < 4; ++it) {
@@ -1297,11 +1292,11 @@ __global__ __launch_bounds__(256) void f8_reduce_epi_kernel(GemmF8Args g, int sp
       const auto r16 = __builtin_amdgcn_permlane16_swap(x, x, false, false);
       x = max((uint32_t)r16[0], (uint32_t)r16[1]);
       const int byte = scale_byte(x);
-      const float inv = inv_scale(byte);
       if (n < (g.N + kB - 1) / kB * kB) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) o[k] = n + k < g.N ? o[k] * inv : 0.f;
-        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(g.C) + m * g.ldc + n) = pack_e4m3x4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < 4; ++k) o[k] = n + k < g.N ? o[k] : 0.f;
+        *reinterpret_cast<uint32_t*>(reinterpret_cast<uint8_t*>(g.C) + m * g.ldc + n) =
+            pack_e4m3x4(o[0], o[1], o[2], o[3], byte);
         if ((threadIdx.x & 31) == 0) g.sc[m * g.ldsc + n / kB] = (uint8_t)byte;
       }
     } else {

@@ -216,12 +216,11 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_fwd_kernel(RmsArgs 
 #pragma unroll
         for (int j = 0; j < 8; ++j) m = max(m, c + j < a.D ? finite_abs_bits(f[i][j]) : 0u);
         const int byte = scale_byte(max16(m));
-        const float inv = inv_scale(byte);
         if (c < (a.D + kB - 1) / kB * kB) {
 #pragma unroll
-          for (int j = 0; j < 8; ++j) f[i][j] = c + j < a.D ? f[i][j] * inv : 0.f;
-          *reinterpret_cast<u32x2*>(a.q + row * a.ldq + c) = u32x2{pack_e4m3x4(f[i][0], f[i][1], f[i][2], f[i][3]),
-                                                                   pack_e4m3x4(f[i][4], f[i][5], f[i][6], f[i][7])};
+          for (int j = 0; j < 8; ++j) f[i][j] = c + j < a.D ? f[i][j] : 0.f;
+          *reinterpret_cast<u32x2*>(a.q + row * a.ldq + c) = u32x2{
+              pack_e4m3x4(f[i][0], f[i][1], f[i][2], f[i][3], byte), pack_e4m3x4(f[i][4], f[i][5], f[i][6], f[i][7], byte)};
           if ((l & 15) == 0) a.sc[row * a.ldsc + c / kB] = (uint8_t)byte;
         }
       } else {
