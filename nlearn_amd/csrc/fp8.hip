@@ -116,6 +116,15 @@ __device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c
   }
 }
 
+// 8 elements at any address of one
+template <typename T>
+__device__ __forceinline__ Vec<T> load_whole(const T* p) {
+  Vec<T> o;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.v[i] = reinterpret_cast<const u32x4_any*>(p)[i];
+  return o;
+}
+
 // u[row][c0 .. c0+7], zero past the last row and column (whose values stay +0)
 template <typename T>
 __device__ __forceinline__ Vec<T> load_u(const QuantArgs& a, int64_t row, int64_t c0) {
@@ -198,23 +207,45 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   const int64_t r0 = (int64_t)by * kB, c0 = (int64_t)bx * kB;
   const int64_t cl = c0 + l * 8;
   float v[4][8];
+  const bool with_u = kAct && a.act != NL_ACT_NONE;
+  if (r0 + kB <= a.rows && c0 + kB <= a.cols) {
+    // a whole tile: every load is out before the first one is waited for
+    const T* x = reinterpret_cast<const T*>(a.x) + (r0 + g * 4) * a.ldx + cl;
+    Vec<T> w[4], u[kAct ? 4 : 1];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int64_t r = r0 + g * 4 + i;
-    if (r < a.rows) {
-      load8<T>(a, r, cl, v[i]);
-    } else {
+    for (int i = 0; i < 4; ++i) w[i] = load_whole(x + i * a.ldx);
+    if constexpr (kAct) {
+      if (with_u) {
+        const T* p = reinterpret_cast<const T*>(a.u) + (r0 + g * 4) * a.ldu + cl;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+        for (int i = 0; i < 4; ++i) u[i] = load_whole(p + i * a.ldu);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) unpack(w[i], v[i]);
+    if constexpr (kAct)
+      if (with_u) scale_by_act_grad<T>(v, u, a.act);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int64_t r = r0 + g * 4 + i;
+      if (r < a.rows) {
+        load8<T>(a, r, cl, v[i]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
+      }
+    }
+    if constexpr (kAct) {
+      if (with_u) {
+        Vec<T> u[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = load_u<T>(a, r0 + g * 4 + i, cl);
+        scale_by_act_grad<T>(v, u, a.act);
+      }
     }
   }
   if constexpr (kAct) {
-    if (a.act != NL_ACT_NONE) {
-      Vec<T> u[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) u[i] = load_u<T>(a, r0 + g * 4 + i, cl);
-      scale_by_act_grad<T>(v, u, a.act);
-    }
     if (a.part) {  // the tile's column sums: a thread's 4 rows, a wave's 4 groups, then the 8 waves
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
@@ -308,10 +339,11 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   }
 }
 
-// With an activation 16384 x 2048 bf16 takes 48 us (gelu; relu 47, none 32), 52 with the column sums
-// and their own launch: 201 MB at the rate of the tile without one. 128 registers are two workgroups a
-// CU; with 138, one, it took 71, and held to 80, three, it spills (91). Stores past the caches gained 3
-// of the 32 here and lost 10 us in the layer, whose products read them next.
+// With an activation 16384 x 2048 bf16 takes 41 us (gelu; relu 42, none 28), 45 with the column sums
+// and their own launch: 201 MB at 4.9 TB/s, the rate of the tile without one. Row by row, each row's load
+// waited for before the next one's, it was 47 and 31. 128 registers are two workgroups a CU; with 138,
+// one, it took 71, and held to 80, three, it spilled (91; without an activation 31 for 28). Stores past
+// the caches gained 3 alone and lost 10 us in the layer, whose products read them next.
 template <typename T, bool kAct = false>
 __global__ __launch_bounds__(512, kAct ? 4 : 2) void quantize_tile_kernel(QuantArgs a, uint32_t cb) {
   __shared__ __attribute__((aligned(16))) QuantTile sm;
