@@ -187,11 +187,11 @@ __device__ __forceinline__ float sum_rows(float v) {
 // l = tid % 16 columns 8l .. 8l+7, so a thread has 4 bytes of a column that lie
 // together in the transpose. Column c's dword g is at slot g ^ 4 (c / 8 % 8): 16-byte
 // pieces stay whole, and 8 lanes' columns fall on different banks.
-// Bound by HBM: 16384 x 2048 bf16 28.9 us (4.65 TB/s, where a copy reaches 4.66), an
-// fp32 weight of 512 x 50257 28.7 us; with 256 threads of twice the elements, each
-// looked at twice for values that are not finite, they took 33.1 and 31.9 us. A layer's x
-// and W go in one launch: 777 x 1000 x 333 forward 22.3 us, in two 26.7; 16384 x 2048 x 512
-// 48.2 and 52.5.
+// Bound by HBM: 16384 x 2048 bf16 27.7 us (4.85 TB/s), an fp32 weight of 512 x 50257 in
+// padded rows 31.7 us, in dense ones 37 (62 where each row's loads were waited for before
+// the next row's); with 256 threads of twice the elements, each looked at twice for values
+// that are not finite, the first two took 33.1 and 31.9 us. A layer's x and W go in one
+// launch: 777 x 1000 x 333 forward 22.3 us, in two 26.7; 16384 x 2048 x 512 48.2 and 52.5.
 struct QuantTile {
   uint32_t tile[kB * 32];
   uint32_t colmax[8][kB];
@@ -428,8 +428,8 @@ struct GemmF8Args {
 // bits for 16384 x 2048 x 512 with gelu. Measured (us; without an epilogue 27): bias to bf16 27, with
 // gelu 34, with u kept 39 (two results of 67 MB), a residual 36; to 8 bits 27, with gelu 33; to fp32
 // with gelu 50 (without an epilogue 46). 8192^3: 403 without, silu or gelu to bf16 410, to 8 bits
-// 424, a residual 430 to 444. With K = 512 a tile's sums take as long as its epilogue (gelu: 13
-// vector instructions an element to 8 bits, about 15 us of the chip's issue beside 13 us of the
+// 424, a residual 430 to 444. With K = 512 a tile's sums take as long as its epilogue (gelu: 12
+// vector instructions an element to 8 bits, about 14 us of the chip's issue beside 13 us of the
 // matrix units), and two workgroups a CU hide half of that; starting them half a tile apart changed nothing.
 enum { kPlain = 0, kEpi = 1, kEpiKeep = 2, kEpiRes = 3, kEpiResKeep = 4 };
 constexpr bool keeps(int epi) { return epi == kEpiKeep || epi == kEpiResKeep; }
