@@ -35,7 +35,6 @@ struct QuantArgs {
   int64_t rows, cols;
   const void* x;
   int64_t ldx;
-  int vec;      // rows start on 16 bytes
   int group;    // rows per scale: 1 or 128
   uint8_t* q;   // blocks along the columns (may be null)
   int64_t ldq;
@@ -66,9 +65,9 @@ __device__ __forceinline__ float silu_grad_of(float u) {
   const float s = __builtin_amdgcn_rcpf(1.f + fast_exp2(-kLog2e * u));
   return __builtin_fmaf(__builtin_fmaf(-s, s, s), u, s);
 }
-// v *= act'(u); a u that is NaN gives NaN, and relu passes or drops v whatever it is
+// v *= act'(u), u of a row's `left` elements; a u that is NaN gives NaN, and relu passes or drops v whatever it is
 template <typename T, int R>
-__device__ __forceinline__ void scale_by_act_grad(float (&v)[R][8], const Vec<T> (&u)[R], int act) {
+__device__ __forceinline__ void scale_by_act_grad(float (&v)[R][8], const Vec<T> (&u)[R], int left, int act) {
   auto each = [&](auto scaled) __attribute__((always_inline)) {
 #pragma unroll
     for (int i = 0; i < R; ++i) {
@@ -81,59 +80,33 @@ __device__ __forceinline__ void scale_by_act_grad(float (&v)[R][8], const Vec<T>
   if (act == NL_ACT_GELU) each([](float g, float x) { return g * gelu_grad_of(clamp_nan(x, 20.f)); });
   else if (act == NL_ACT_SILU) each([](float g, float x) { return g * silu_grad_of(clamp_nan(x, 120.f)); });
   else each([](float g, float x) { return x > 0.f ? g : x == x ? 0.f : x; });
-}
-
-// x[row][c0 .. c0+7] as floats, zero past the last column
-template <typename T>
-__device__ __forceinline__ void load8(const QuantArgs& a, int64_t row, int64_t c0, float v[8]) {
-  const T* p = reinterpret_cast<const T*>(a.x) + row * a.ldx + c0;
-  if (a.vec && c0 + 8 <= a.cols) {
-    if constexpr (sizeof(T) == 2) {
-      const u32x4 u = *reinterpret_cast<const u32x4*>(p);
+  if (left < 8) {  // (not by what u holds behind the row)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[2 * i] = bf16_lo(u[i]);
-        v[2 * i + 1] = bf16_hi(u[i]);
-      }
-    } else {
-      const f32x4 u0 = reinterpret_cast<const f32x4*>(p)[0], u1 = reinterpret_cast<const f32x4*>(p)[1];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        v[i] = u0[i];
-        v[4 + i] = u1[i];
-      }
-    }
-    return;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f = 0.f;
-    if (c0 + i < a.cols) {
-      if constexpr (sizeof(T) == 2) f = bf16_to_f32(p[i]);
-      else f = p[i];
-    }
-    v[i] = f;
+    for (int i = 0; i < R; ++i) clear_tail(v[i], left);
   }
 }
 
-// 8 elements at any address of one
+// row[c0 .. c0+7] of a matrix of a.rows x a.cols with rows of ld, as it is stored (what is not there: see load_row)
 template <typename T>
-__device__ __forceinline__ Vec<T> load_whole(const T* p) {
-  Vec<T> o;
-#pragma unroll
-  for (int i = 0; i < (int)sizeof(T) / 2; ++i) o.v[i] = reinterpret_cast<const u32x4_any*>(p)[i];
-  return o;
-}
-
-// u[row][c0 .. c0+7], zero past the last row and column (whose values stay +0)
-template <typename T>
-__device__ __forceinline__ Vec<T> load_u(const QuantArgs& a, int64_t row, int64_t c0) {
+__device__ __forceinline__ Vec<T> load8(const QuantArgs& a, const void* x, int64_t ld, int64_t row, int64_t c0) {
   const int64_t left = row < a.rows ? a.cols - c0 : 0;
-  return load_vec(reinterpret_cast<const T*>(a.u) + row * a.ldu + c0, (int)(left < 8 ? left : 8));
+  return load_row(reinterpret_cast<const T*>(x) + row * ld + c0, (int)(left < 8 ? left : 8),
+                  a.cols >= 8 && row + 1 < a.rows);
+}
+// ... as floats, zero past the last row and column
+template <typename T, int R>
+__device__ __forceinline__ void values8(const QuantArgs& a, const Vec<T> (&w)[R], int64_t c0, float (&v)[R][8]) {
+  const int64_t left = a.cols - c0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    unpack(w[i], v[i]);
+    if (a.cols & 7) clear_tail(v[i], (int)(left < 8 ? left : 8));
+  }
 }
 
 // One row's block of 128 per 16 lanes, 8 elements a lane: one read, one write. Bound
-// by HBM: 16384 x 2048 bf16 17.8 us, 8192 x 8192 32.5 us (5.7 and 6.2 TB/s).
+// by HBM: 16384 x 2048 bf16 18 us, 8192 x 8192 32.5 us (5.7 and 6.2 TB/s), rows of 2047
+// 19 (40 where rows off 16 bytes were read element by element).
 template <typename T, bool kAct = false>
 __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_t blocks, uint32_t kb) {
   const uint32_t id = blockIdx.x * 16u + (threadIdx.x >> 4);
@@ -142,12 +115,13 @@ __global__ __launch_bounds__(256) void quantize_rows_kernel(QuantArgs a, uint32_
   const int l = threadIdx.x & 15;
   const int64_t c0 = (int64_t)b * kB + l * 8;
   float x[1][8];
-  load8<T>(a, row, c0, x[0]);
-  if constexpr (kAct) {
-    if (a.act != NL_ACT_NONE) {
-      const Vec<T> u[1] = {load_u<T>(a, row, c0)};
-      scale_by_act_grad<T>(x, u, a.act);
-    }
+  const Vec<T> w[1] = {load8<T>(a, a.x, a.ldx, row, c0)};
+  if (kAct && a.act != NL_ACT_NONE) {
+    const Vec<T> u[1] = {load8<T>(a, a.u, a.ldu, row, c0)};
+    values8<T>(a, w, c0, x);
+    scale_by_act_grad(x, u, (int)(a.cols - c0 < 8 ? a.cols - c0 : 8), a.act);
+  } else {
+    values8<T>(a, w, c0, x);
   }
   const float(&v)[8] = x[0];
   uint32_t m = 0;
@@ -187,11 +161,12 @@ __device__ __forceinline__ float sum_rows(float v) {
 // l = tid % 16 columns 8l .. 8l+7, so a thread has 4 bytes of a column that lie
 // together in the transpose. Column c's dword g is at slot g ^ 4 (c / 8 % 8): 16-byte
 // pieces stay whole, and 8 lanes' columns fall on different banks.
-// Bound by HBM: 16384 x 2048 bf16 27.7 us (4.85 TB/s), an fp32 weight of 512 x 50257 in
-// padded rows 31.7 us, in dense ones 37 (62 where each row's loads were waited for before
-// the next row's); with 256 threads of twice the elements, each looked at twice for values
-// that are not finite, the first two took 33.1 and 31.9 us. A layer's x and W go in one
-// launch: 777 x 1000 x 333 forward 22.3 us, in two 26.7; 16384 x 2048 x 512 48.2 and 52.5.
+// Bound by HBM: 16384 x 2048 bf16 26.5 us (5.1 TB/s), 16384 x 2047 29, an fp32 weight of
+// 512 x 50257 in padded rows 31.7 us, in dense ones 35 (31, 53 and 62 where each row's loads
+// were waited for before the next row's, those off 16 bytes element by element); with 256
+// threads of twice the elements, each looked at twice for values that are not finite, whole
+// and padded rows took 33.1 and 31.9 us. A layer's x and W go in one launch: 777 x 1000 x 333
+// forward 22.3 us, in two 26.7; 16384 x 2048 x 512 48.2 and 52.5.
 struct QuantTile {
   uint32_t tile[kB * 32];
   uint32_t colmax[8][kB];
@@ -208,42 +183,32 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   const int64_t cl = c0 + l * 8;
   float v[4][8];
   const bool with_u = kAct && a.act != NL_ACT_NONE;
-  if (r0 + kB <= a.rows && c0 + kB <= a.cols) {
-    // a whole tile: every load is out before the first one is waited for
-    const T* x = reinterpret_cast<const T*>(a.x) + (r0 + g * 4) * a.ldx + cl;
-    Vec<T> w[4], u[kAct ? 4 : 1];
+  Vec<T> w[4], u[kAct ? 4 : 1];
+  if (r0 + kB <= a.rows && c0 + kB <= a.cols) {  // a whole tile
+    // every load is out before the first one is waited for
+    auto load4 = [&](const void* x, int64_t ld, Vec<T> (&o)[4]) __attribute__((always_inline)) {
+      const T* p = reinterpret_cast<const T*>(x) + (r0 + g * 4) * ld + cl;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = load_whole(x + i * a.ldx);
-    if constexpr (kAct) {
-      if (with_u) {
-        const T* p = reinterpret_cast<const T*>(a.u) + (r0 + g * 4) * a.ldu + cl;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = load_whole(p + i * a.ldu);
-      }
-    }
+      for (int i = 0; i < 4; ++i) o[i] = load_vec(p + i * ld, 8);
+    };
+    load4(a.x, a.ldx, w);
+    if constexpr (kAct)
+      if (with_u) load4(a.u, a.ldu, u);
 #pragma unroll
     for (int i = 0; i < 4; ++i) unpack(w[i], v[i]);
     if constexpr (kAct)
-      if (with_u) scale_by_act_grad<T>(v, u, a.act);
+      if (with_u) scale_by_act_grad(v, u, 8, a.act);
   } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t r = r0 + g * 4 + i;
-      if (r < a.rows) {
-        load8<T>(a, r, cl, v[i]);
-      } else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) v[i][j] = 0.f;
-      }
-    }
-    if constexpr (kAct) {
+    for (int i = 0; i < 4; ++i) w[i] = load8<T>(a, a.x, a.ldx, r0 + g * 4 + i, cl);
+    if constexpr (kAct)
       if (with_u) {
-        Vec<T> u[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) u[i] = load_u<T>(a, r0 + g * 4 + i, cl);
-        scale_by_act_grad<T>(v, u, a.act);
+        for (int i = 0; i < 4; ++i) u[i] = load8<T>(a, a.u, a.ldu, r0 + g * 4 + i, cl);
       }
-    }
+    values8<T>(a, w, cl, v);
+    if constexpr (kAct)
+      if (with_u) scale_by_act_grad(v, u, (int)(a.cols - cl < 8 ? a.cols - cl : 8), a.act);
   }
   if constexpr (kAct) {
     if (a.part) {  // the tile's column sums: a thread's 4 rows, a wave's 4 groups, then the 8 waves
@@ -339,8 +304,8 @@ __device__ __forceinline__ void quantize_tile(const QuantArgs& a, uint32_t block
   }
 }
 
-// With an activation 16384 x 2048 bf16 takes 41 us (gelu; relu 42, none 28), 45 with the column sums
-// and their own launch: 201 MB at 4.9 TB/s, the rate of the tile without one. Row by row, each row's load
+// With an activation 16384 x 2048 bf16 takes 43 us (gelu; relu 42, none 26.5), 46 with the column sums
+// and their own launch: 201 MB at 4.7 TB/s, near the rate of the tile without one. Row by row, each row's load
 // waited for before the next one's, it was 47 and 31. 128 registers are two workgroups a CU; with 138,
 // one, it took 71, and held to 80, three, it spilled (91; without an activation 31 for 28). Stores past
 // the caches gained 3 alone and lost 10 us in the layer, whose products read them next.
@@ -1454,8 +1419,7 @@ int quant_args(int64_t rows, int64_t cols, const void* x, int x_dtype, int64_t l
   if (!x) return nl_set_error(NL_EINVAL, "quantize_fp8: null x");
   if (rows > 1 && ldx < cols) return nl_set_error(NL_EINVAL, "quantize_fp8: ldx < cols");
   if ((uintptr_t)x % esz) return nl_set_error(NL_EALIGN, "quantize_fp8: x is not aligned to its type");
-  *out = QuantArgs{rows, cols, x, ldx, (((uintptr_t)x & 15) == 0 && (rows == 1 || ldx * esz % 16 == 0)) ? 1 : 0, group,
-                   q, ldq, scale, lds, qt, ldqt, scale_t, ldst};
+  *out = QuantArgs{rows, cols, x, ldx, group, q, ldq, scale, lds, qt, ldqt, scale_t, ldst};
   return NL_OK;
 }
 
@@ -1475,7 +1439,6 @@ int dact_args(int64_t rows, int64_t cols, const void* dy, int dtype, int64_t ldd
     if (!u) return nl_set_error(NL_EINVAL, std::string(what) + ": null u");
     if (rows > 1 && ldu < cols) return nl_set_error(NL_EINVAL, std::string(what) + ": ldu < cols");
     if ((uintptr_t)u % esz) return nl_set_error(NL_EALIGN, std::string(what) + ": u is not aligned to its type");
-    out->vec = out->vec && ((uintptr_t)u & 15) == 0 && (rows == 1 || ldu * esz % 16 == 0);
   }
   if (dbias && !part) return nl_set_error(NL_EINVAL, std::string(what) + ": workspace too small");
   if (dbias && db_dtype != NL_DTYPE_F32 && db_dtype != NL_DTYPE_BF16)

@@ -60,19 +60,6 @@ __device__ __forceinline__ Vec<T> pack(const float f[8]) {
   return o;
 }
 
-// The vector of a row from p on, `n` elements of which are the row's (0 or less: none). `over`: what
-// lies behind the row may be read (the next row, of 8 elements at least): one load then, and what is
-// not the row's is cleared by clear_tail; element by element (zero behind them) a row's last vector
-// waited for each, and 100,663 rows of 333 bf16 took 99 us with the residual for 58.
-template <typename T>
-__device__ __forceinline__ Vec<T> load_row(const T* p, int n, bool over) {
-  return load_vec(p, over && n > 0 ? 8 : n);
-}
-__device__ __forceinline__ void clear_tail(float (&f)[8], int n) {
-#pragma unroll
-  for (int k = 0; k < 8; ++k) f[k] = k < n ? f[k] : 0.f;
-}
-
 // gamma[c .. c+7], zero past the last column (any alignment of a float)
 __device__ __forceinline__ void load_gamma(const float* p, int n, float f[8]) {
   if (n >= 8) {

@@ -342,3 +342,38 @@ def test_gradient_added_to_what_is_there(dev, rows, cols):
     assert torch.equal(got[1][1], held + got[0][1])
     if rows == 0:
         assert (got[0][1] == 0).all()
+
+
+@pytest.mark.parametrize("dtype", ["bfloat16", "float32"])
+@pytest.mark.parametrize("cols", [9, 101, 333, 1001, 4099])
+def test_rows_keep_to_themselves(dev, cols, dtype):
+    """Rows that end inside a vector, beside rows of NaN and infinities: the bits that finite neighbours leave."""
+    import torch
+    from nlearn_amd.kernels.fp8 import add_rms_norm_fp8, linear_fp8, quantize_fp8, quantize_fp8_both
+    from nlearn_amd.kernels.fused import add_rms_norm
+
+    dt = getattr(torch, dtype)
+    rng = _rng(cols, 77)
+    clean = [torch.from_numpy(_matrix(rng, 140, cols)).to(dev).to(dt) for _ in range(4)]
+    bad = [t.clone() for t in clean]
+    for t in bad:
+        t[1::2] = float("nan")
+        t[3::4] = float("inf")
+    gamma = torch.from_numpy(1 + 0.1 * rng.standard_normal(cols).astype(np.float32)).to(dev)
+    W = torch.from_numpy(rng.standard_normal((16, cols)).astype(np.float32)).to(dev)
+    bits = lambda b: (b.q.view(torch.uint8), b.scale.contiguous().view(torch.uint8))  # noqa: E731
+
+    def everything(x, r, dy, ds):
+        x, r = x.clone().requires_grad_(True), r.clone().requires_grad_(True)
+        y, s = add_rms_norm(x, r, gamma, EPS)
+        (dx,) = torch.autograd.grad((y, s), x, (dy, ds))
+        b, t = add_rms_norm_fp8(x.detach(), r.detach(), gamma, EPS)
+        h = torch.ones((140, 16), device=dev, dtype=dt).requires_grad_(True)
+        outs = [y, s, dx, t, *bits(b), *bits(quantize_fp8(dy)), *bits(quantize_fp8_both(dy)[0])]
+        for name in ("gelu", "silu", "relu"):
+            z = linear_fp8(h, W, activation=name, residual=r.detach())
+            outs += [z, torch.autograd.grad(z, h, dy)[0]]
+        return outs
+
+    for a, b in zip(everything(*clean), everything(*bad)):
+        assert torch.equal(a[0::2], b[0::2])
