@@ -113,9 +113,9 @@ __device__ __forceinline__ uint32_t row_max(uint32_t v, float* red) {
 }
 
 // The sum of a thread's squares, those of a vector by pairs, then the vectors: at most VPL + 3 roundings stand
-// behind a square. (In one chain 31 squares below half a step of a first one were all lost: 15 units of the
-// result's last place for 2. 8 sums side by side are as good, and 2 registers more cost 2048 columns to 8 bits
-// a wave a SIMD.)
+// behind a square. (In one chain 31 squares below half a step of a first one were all lost: y off by 16 u, u = 2^-24,
+// for 1.2. 8 sums side by side are as good, but with 129 registers for 127 the norm of 2048 columns to 8 bits
+// would run 3 waves a SIMD for 4.)
 template <int VPL, class F>
 __device__ __forceinline__ float thread_squares(const float (&f)[VPL][8], F&& scaled) {
   float s = 0.f;
@@ -321,13 +321,15 @@ __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void rms_bwd_kernel(RmsBwdAr
         clear_tail(g[i], a.D - (i * TPR + l) * 8);
         clear_tail(xh[i], a.D - (i * TPR + l) * 8);
       }
+      float p[4];  // by pairs, as a row's squares are
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         xh[i][j] *= w.rs;
         ag[i][j] = __builtin_fmaf(g[i][j], xh[i][j], ag[i][j]);
         g[i][j] *= gam[i][j];
-        m = __builtin_fmaf(g[i][j], xh[i][j], m);
+        p[j >> 1] = j & 1 ? __builtin_fmaf(g[i][j], xh[i][j], p[j >> 1]) : g[i][j] * xh[i][j];
       }
+      m += (p[0] + p[1]) + (p[2] + p[3]);
     }
     m = row_sum<TPR>(m, red) / (float)a.D;
     T* dx = reinterpret_cast<T*>(a.dx) + row * a.lddx;
