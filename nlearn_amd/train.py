@@ -180,7 +180,8 @@ class AdamW:
     the capturable work, ``finish`` runs what follows it outside a graph (nothing
     here), ``advance`` counts the step; ``update`` does all four. Leaves without
     a buffer fall back to one launch per leaf on ``.grad``, clipped in place before
-    (``kernels.clip``)."""
+    (``kernels.clip``; a ``.grad`` without rows of one stride, as a broadcast one, is
+    replaced by a dense, clipped one)."""
 
     def __init__(self, learning_rate, weight_decay: float = WEIGHT_DECAY, b1: float = 0.9, b2: float = 0.999,
                  eps: float = 1e-8, grad_buffers: bool = True, clip_norm: float = 0.0):
@@ -279,8 +280,12 @@ class AdamW:
         lr, bc1, bc2 = self.hyper_values(state["count"])
         grads = [p.grad if getattr(p, "main_grad", None) is None else p.main_grad for p in leaves]
         if self.clip_norm > 0 and any(g is not None for g in grads):
-            # a gradient whose rows have no one stride (a broadcast one) is copied first
-            grads = [g if g is None or rows_of(g) else g.contiguous() for g in grads]
+            for i, g in enumerate(grads):
+                if g is not None and rows_of(g) is None:
+                    # rows of no one stride (a broadcast gradient) cannot be written over: a dense copy takes their place
+                    grads[i] = g.contiguous()
+                    if g is leaves[i].grad:
+                        leaves[i].grad = grads[i]
             _, state["gnorm"] = clip_by_global_norm([g for g in grads if g is not None], self.clip_norm, inplace=True)
         for p, g, m, v in zip(leaves, grads, state["mu"], state["nu"]):
             if g is None:
