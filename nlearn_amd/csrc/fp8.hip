@@ -1267,9 +1267,9 @@ __global__ __launch_bounds__(256) void f8_reduce_epi_kernel(GemmF8Args g, int sp
           if (k0 + k < splits) s += v[k];
       }
     }
-    float u[8], o[4];
+    float u[4], o[4];
 #pragma unroll
-    for (int k = 0; k < 8; ++k) u[k] = k < 4 && n + k < g.N ? s[k & 3] + bias[k & 3] : 0.f;
+    for (int k = 0; k < 4; ++k) u[k] = n + k < g.N ? s[k] + bias[k] : 0.f;
     if constexpr (keeps(EPI)) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
