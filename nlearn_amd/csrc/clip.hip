@@ -4,9 +4,10 @@
 //   n = sqrt(sum over all elements of g^2),   g -> g while n < max_norm, else (g / n) * max_norm
 //
 // Two passes over the gradients (the second needs the first one's sum), bound by
-// HBM: 46 tensors of 263 MB, fp32 and bf16, 47 us for the sums (5.6 TB/s) and 82 us
-// for the second pass (527 MB, 6.4 TB/s with what the 256 MB cache still holds of
-// them: it starts where the first ended). Results are stored past the caches: the
+// HBM (medians of a kernel trace over three sets of tensors in turn): 46 tensors of 263 MB,
+// fp32 and bf16, 50 us for the sums (5.2 TB/s; at least 47) and 85 us for the second pass
+// (527 MB, 6.2 TB/s with what the 256 MB cache still holds of them: it starts where the
+// first ended; at least 82). Results are stored past the caches: the
 // sums of the next call took 99 us, not 72, beside the write-back of dirty lines.
 // Rows that end inside a vector read into the next row: element by element the sums
 // took 70 us. The tensors' addresses travel as a kernel's arguments, 64 in a launch,

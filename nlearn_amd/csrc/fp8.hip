@@ -396,6 +396,9 @@ struct GemmF8Args {
 // 424, a residual 430 to 444. With K = 512 a tile's sums take as long as its epilogue (gelu: 12
 // vector instructions an element to 8 bits, about 14 us of the chip's issue beside 13 us of the
 // matrix units), and two workgroups a CU hide half of that; starting them half a tile apart changed nothing.
+// On 256 x 256 tiles a group's values, the residual's pieces and the next item's first fragments live beside the
+// sums, and registers go to scratch: with a residual 52 to 54 of a result in 8 bits, 3 to 11 of bf16 and up to 1 of
+// fp32; fp32 with u kept 28 to 34, 8 bits without a residual 6. The other forms and all of 128 x 128 keep theirs.
 enum { kPlain = 0, kEpi = 1, kEpiKeep = 2, kEpiRes = 3, kEpiResKeep = 4 };
 constexpr bool keeps(int epi) { return epi == kEpiKeep || epi == kEpiResKeep; }
 
@@ -1611,7 +1614,11 @@ int gemm_fp8(void* stream, int M, int N, int K, const uint8_t* A, int64_t lda, c
   // relu in front of a backward pass: the sign of u decides whether a gradient passes, and sums cut at
   // 2^-13 of a product had it wrong for one u in 100000 (an error of 0.6% in dx): fp32 sums, whatever
   // the result's type. That costs a layer's forward (us, with its quantisers) 60 for 52 with gelu's sums
-  // at 16384 x 512 x 2048, 142 for 92 at 4096^3; with 256 x 256 tiles 66 and 144.
+  // at 16384 x 512 x 2048, 142 for 92 at 4096^3; with 256 x 256 tiles 66 and 144. It is paid where no gradient
+  // is wanted, too: a layer's output does not depend on that.
+  // A result in 8 bits is summed with the cut. Of normal operands it leaves 9e-4 of the bytes a step beside
+  // those of fp32 sums: 9e-4 of the result's norm, where the rounding to 8 bits is 2.7e-2. With fp32 sums (us, gelu):
+  // 16384 x 2048 x 512 49 for 34, 16384 x 512 x 2048 36 for 23, 16384 x 8192 x 1024 275 for 170, 8192^3 760 for 415.
   const bool fine = c_dtype == NL_DTYPE_F32 || (e.kind == kEpiKeep && e.act == NL_ACT_RELU);
   // 128 x 128 tiles, two workgroups a CU, where the epilogue of one runs beside the other's walk over a
   // short K, although each operand is read twice as often. Measured (us, against 256 x 256): C in 8 bits

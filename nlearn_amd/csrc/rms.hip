@@ -13,11 +13,13 @@
 // lanes up to 128 columns, a wave up to 2048, 256 threads up to 8192 and 512 up to
 // 16384 (1024 threads of two vectors spilled registers). Vectors are loaded and stored
 // at whatever alignment the rows have (the hardware takes any multiple of the element).
-// Bound by HBM where there are many rows: with the residual 16384 x 512 bf16 12.0 us
-// (67 MB, 5.6 TB/s; a large copy reaches 5.1), its gradients 10.9 us (67 MB) and 4.3 us
-// for the sum of dgamma's partial rows; 16384 x 2048 bf16 to 8 bits 45 us (235 MB, 5.2
-// TB/s). By the chain load -> sum -> store where there are few: one row of 512 1.8 us,
-// 8 rows of 2048 to 8 bits 4.8 us, 777 x 1001 fp32 4.3 us and 5.7 + 3.5 us. A backward in
+// Bound by HBM where there are many rows (medians of a kernel trace over three sets of
+// inputs in turn; a large copy reaches 5.1 TB/s): with the residual 16384 x 512 bf16 14.9 us
+// (67 MB, 4.5 TB/s), its gradients 13.9 us (67 MB) and 3.9 us for the sum of dgamma's
+// partial rows (over the same rows again, which the 256 MB cache holds, 12.0, 10.9 and 4.3);
+// 16384 x 2048 bf16 to 8 bits 46 us (235 MB, 5.1 TB/s). By the chain load -> sum -> store
+// where there are few: one row of 512 2.0 us, 8 rows of 2048 to 8 bits 5.0 us, 777 x 1001
+// fp32 4.0 us and 5.1 + 3.3 us. A backward in
 // one launch for few rows, each workgroup summing dgamma of its own columns over all rows,
 // took 17 us there.
 #include <type_traits>
@@ -417,7 +419,8 @@ __global__ __launch_bounds__(1024) void row_sums_kernel(int P, int D, const floa
   }
 }
 
-// Threads and vectors a row takes: the fewest threads that hold it in 4 vectors each.
+// Threads and vectors a row takes: 16 lanes up to 128 columns, a wave of as few vectors a lane as hold
+// it up to 2048, beyond that 256 and from 8193 on 512 threads of up to 4.
 template <class F>
 void by_width(int D, F&& go) {
 #define NL_W(TPR, VPL) go(std::integral_constant<int, TPR>{}, std::integral_constant<int, VPL>{})

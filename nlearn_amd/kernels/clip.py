@@ -87,6 +87,9 @@ def global_norm(tensors) -> torch.Tensor:
 def clip_by_global_norm(grads, max_norm: float, inplace: bool = False):
     """(clipped, norm): every gradient g as it is while norm = global_norm(grads) < max_norm,
     else as (g / norm) * max_norm, in g's dtype and layout. The norm stays on the device.
+    A new tensor keeps g's strides and so spans as much memory as g does: the result of a
+    narrow slice of a wide matrix has nearly that matrix's size (clip a dense copy, or in
+    place, where that is too much).
 
     ``inplace=True`` writes the results over the gradients (which may not overlap) and only
     where the norm reaches max_norm; otherwise they are new tensors. With a norm that is

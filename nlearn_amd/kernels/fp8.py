@@ -292,8 +292,9 @@ def gemm_fp8(a: Fp8Blocks, b: Fp8Blocks, out_dtype=_BF16, out: torch.Tensor | No
 
     bias (N,) fp32 or bf16, activation "relu", "gelu" (tanh form) or "silu" and residual (M, N) in
     the result's dtype are applied in fp32 behind the sum. ``out_dtype=torch.float8_e4m3fn`` gives
-    ``Fp8Blocks``, quantised along N, for the next product (summed as bf16 is; a bf16 residual).
-    Not differentiable (``linear_fp8`` is).
+    ``Fp8Blocks``, quantised along N, for the next product (a bf16 residual). It is summed as bf16
+    is, which leaves about one value in 1000 a step beside that of fp32 sums; where that matters,
+    quantise an fp32 result with ``quantize_fp8``. Not differentiable (``linear_fp8`` is).
 
     out: fp32 or bf16 with 16-byte aligned rows (it may be the residual). ws: as ``gemm_fp8_ws`` gives
     it (allocated here if None; too small a one is not used and K is summed in one piece)."""
@@ -582,7 +583,8 @@ def linear_fp8(x: torch.Tensor, W, bias: torch.Tensor | None = None, activation:
     bias (N,) fp32 or bf16, activation "relu", "gelu" (tanh form) or "silu", residual [..., N] in x's
     dtype: in the product's epilogue. With an activation u = x W + bias is rounded to x's dtype before
     it, as ``ffn`` does it: that u is kept for the backward, which quantises dY act'(u). In front of relu u is
-    summed in fp32 whatever x's dtype (scale bytes 3 to 246): its sign decides what a gradient passes."""
+    summed in fp32 whatever x's dtype (scale bytes 3 to 246): its sign decides what a gradient passes. The
+    output is the same where no gradient is wanted."""
     if x.dim() < 2:
         raise ValueError("linear_fp8: x needs >= 2 dims")
     frozen = W if isinstance(W, Fp8Weight) else None
